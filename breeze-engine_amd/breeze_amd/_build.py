@@ -13,7 +13,9 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(PKG), "csrc")
 # Host code and small kernels; the decode and prefill kernels, one unit per
 # (bits, activation mode) so the device passes run side by side.
-SOURCES = ["qmm.hip", "pf16_w4.hip", "pf16_w8.hip", "pf_w4_i8.hip"] + [f"{k}_w{b}_{m}.hip" for k in ("dec", "pf") for b in (4, 8) for m in ("hp", "lp")]
+# Then the token mixers (the paged cache, attention over it).
+MIXERS = ["kv_cache.hip", "paged_attn.hip"]
+SOURCES = ["qmm.hip", "pf16_w4.hip", "pf16_w8.hip", "pf_w4_i8.hip", *MIXERS] + [f"{k}_w{b}_{m}.hip" for k in ("dec", "pf") for b in (4, 8) for m in ("hp", "lp")]
 LIB_NAME = "libbreeze_qmm.so"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -46,6 +48,9 @@ DEVICE_FLAGS = [
     # kernel's first loads do not wait for a kernarg fetch.
     "-mllvm", "-amdgpu-kernarg-preload-count=14",
 ]
+# The token mixers': their accumulators may take the accumulation registers, and
+# their arguments are one structure.
+MIXER_FLAGS = DEVICE_FLAGS[:4]
 
 
 def lib_path():
@@ -78,8 +83,9 @@ def build(verbose=False):
         fatbins = [os.path.join(work, f"{i}.hipfb") for i in range(len(srcs))]
         objs = [os.path.join(work, f"{i}.o") for i in range(len(srcs))]
         try:
-            running = [(_run([HIPCC, "-x", "hip", *FLAGS, *DEVICE_FLAGS, "--offload-device-only", "-c", s, "-o", fb],
-                             verbose), s) for s, fb in zip(srcs, fatbins)]
+            running = [(_run([HIPCC, "-x", "hip", *FLAGS,
+                              *(MIXER_FLAGS if os.path.basename(s) in MIXERS else DEVICE_FLAGS),
+                              "--offload-device-only", "-c", s, "-o", fb], verbose), s) for s, fb in zip(srcs, fatbins)]
             finish(running, "device pass")
             running = [(_run([HIPCC, "-x", "hip", *FLAGS, "--offload-host-only", "-Xclang",
                               "-fcuda-include-gpubinary", "-Xclang", fb, "-c", s, "-o", o], verbose), s)

@@ -1,0 +1,272 @@
+"""The decoder's token mixers on GPU tensors: what runs between a layer's
+quantized projections (``hip_backend``).
+
+- ``KVCache`` holds one layer's keys and values in pages, as INT8 or e4m3 with
+  one scale for each token and head; ``kv_write`` quantizes new tokens into it
+  and ``kv_read`` reads tokens back.
+- ``paged_attention``: causal attention of new tokens (one a sequence, or a
+  chunk) over that cache, in place of the decoder's full attention
+  (kernel/qwen35_decoder.cpp:334-395, which keeps fp32 keys and values).
+
+Tensors are fp32, bf16 or fp16 on one gfx950 GPU.  Calls are asynchronous on
+the current stream, own no memory between calls (a workspace comes from
+torch's allocator) and can be captured into graphs.  Shapes, types and strides
+are checked here and raise ``ValueError``; what lies on the GPU (lengths,
+offsets, page and slot numbers) is checked by the kernels, which skip what is
+out of range.  There is no CPU fallback.
+"""
+import ctypes
+
+from . import hip_backend as hb
+
+_dtypes = None  # torch dtype -> the library's number for it
+
+
+class _CCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("num_pages", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int), ("kind", ctypes.c_int)]
+
+
+def _torch():
+    global _dtypes
+    torch = hb._import_torch()
+    if _dtypes is None:
+        _dtypes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    return torch
+
+
+def _type(t, what):
+    n = _dtypes.get(t.dtype)
+    if n is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return n
+
+
+def _rows(t, what):
+    """`t` [T, heads, D] with its last dimension contiguous and rows that the
+    kernels' wide loads can read: itself, or a copy."""
+    st = t.stride()
+    if st[2] == 1 and not (st[0] | st[1]) & 3 and not t.data_ptr() & 15:
+        return t
+    return t.contiguous() if st[2] != 1 or (st[0] | st[1]) & 3 else t.clone()
+
+
+def _ints(t, shape, what):
+    torch = hb._torch
+    if t.dtype is not torch.int32 or tuple(t.shape) != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what} must be int32 of shape {shape} with a contiguous last dimension, "
+                         f"got {t.dtype} {tuple(t.shape)} (strides {t.stride()})")
+    return t
+
+
+def _same_device(device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors lie on {t.device} and {device}: all must be on one GPU")
+    if device.type != "cuda":
+        raise ValueError(f"tensors lie on {device}: they must be on a GPU")
+    hb._require_lib()
+
+
+class _Current:
+    """Makes a tensor's device the current one for a call, where it is another."""
+
+    def __init__(self, device):
+        torch = hb._torch
+        self._other = None
+        if device.index != torch.cuda.current_device():
+            self._other = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._other is not None:
+            self._other.__enter__()
+
+    def __exit__(self, *e):
+        if self._other is not None:
+            self._other.__exit__(*e)
+
+
+class KVCache:
+    """One layer's keys and values in pages.
+
+    ``k``, ``v``: ``[pages, kv_heads, page_size, head_dim]``, int8 or
+    float8_e4m3fn; ``k_scale``, ``v_scale``: fp32 ``[pages, kv_heads,
+    page_size]``.  A value is the stored number times its token's and head's
+    scale.  ``head_dim`` is 64, 128 or 256; ``page_size`` a power of two from 16
+    to 1024.  The tensors are kept as given and written in place."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        torch = _torch()
+        kinds = {torch.int8: 0, torch.float8_e4m3fn: 1}
+        if k.dtype not in kinds or v.dtype is not k.dtype:
+            raise ValueError(f"cache pages must be int8 or float8_e4m3fn, both alike, got {k.dtype} and {v.dtype}")
+        if k.dim() != 4 or k.shape != v.shape:
+            raise ValueError(f"cache pages must be [pages, kv_heads, page_size, head_dim], both alike, got "
+                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        P, H, page, D = k.shape
+        if D not in (64, 128, 256):
+            raise ValueError(f"head_dim must be 64, 128 or 256, got {D}")
+        if page & (page - 1) or not 16 <= page <= 1024:
+            raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page}")
+        if P < 1 or not 1 <= H <= 4096 or P * page >= 1 << 31:
+            raise ValueError(f"a cache needs a page, 1 to 4096 heads and fewer than 2^31 slots, got {tuple(k.shape)}")
+        for t in (k_scale, v_scale):
+            if t.dtype is not torch.float32 or tuple(t.shape) != (P, H, page):
+                raise ValueError(f"cache scales must be float32 {(P, H, page)}, got {t.dtype} {tuple(t.shape)}")
+        for t in (k, v, k_scale, v_scale):
+            if not t.is_contiguous() or t.data_ptr() & 15:
+                raise ValueError("cache tensors must be contiguous and 16-byte aligned")
+            if t.device != k.device:
+                raise ValueError(f"cache tensors lie on {t.device} and {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = P, H, page, D
+        self.device = k.device
+        self._c = _CCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, H, page, D,
+                          kinds[k.dtype])
+        self._p = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, num_pages, page_size, kv_heads, head_dim, kind="int8", device="cuda"):
+        """A cache of zeros; ``kind`` is "int8" or "fp8" (e4m3)."""
+        torch = _torch()
+        if kind not in ("int8", "fp8"):
+            raise ValueError(f"kind must be 'int8' or 'fp8', got {kind!r}")
+        shape = (int(num_pages), int(kv_heads), int(page_size))
+        pages = [torch.zeros((*shape, int(head_dim)), dtype=torch.int8, device=device) for _ in range(2)]
+        if kind == "fp8":
+            pages = [p.view(torch.float8_e4m3fn) for p in pages]
+        return cls(*pages, *(torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def kv_write(cache, k, v, slots):
+    """Quantize new tokens' keys and values into the cache.
+
+    ``k``, ``v``: ``[T, kv_heads, head_dim]`` of one type (views of a wider
+    projection are read in place); ``slots``: int32 ``[T]``, a token's page
+    times the page size plus its place in the page.  A slot outside the cache
+    (-1, say) skips its token; no slot may occur twice in a call.
+
+    INT8: the scale is max|x| / 127 in fp32, the value the whole number nearest
+    to x / scale, ties to even.  e4m3: the scale is the smallest power of two
+    that brings the row within 448.  A row that holds an infinity or NaN reads
+    back as NaN."""
+    _torch()
+    shape = (k.shape[0] if k.dim() else 0, cache.kv_heads, cache.head_dim)
+    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+        raise ValueError(f"k and v must be [T, {cache.kv_heads}, {cache.head_dim}], got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    dt = _type(k, "k")
+    if v.dtype is not k.dtype:
+        raise ValueError(f"k and v must have one type, got {k.dtype} and {v.dtype}")
+    _ints(slots, (shape[0],), "slots")
+    _same_device(cache.device, k, v, slots)
+    if shape[0] == 0:
+        return
+    with _Current(cache.device):
+        k, v = _rows(k, "k"), _rows(v, "v")
+        hb._check_rc(hb._lib.i4_kv_write_dev(cache._p, k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2],
+                                             shape[0], dt, slots.data_ptr(), hb._torch_stream(k)), "i4_kv_write_dev")
+
+
+def kv_read(cache, slots, dtype):
+    """The tokens of int32 ``slots`` [T] as (k, v), each ``[T, kv_heads,
+    head_dim]`` of ``dtype``: value times scale, rounded once.  Zeros where a
+    slot is outside the cache."""
+    torch = _torch()
+    if dtype not in _dtypes:
+        raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+    T = slots.shape[0] if slots.dim() else 0
+    _ints(slots, (T,), "slots")
+    _same_device(cache.device, slots)
+    k, v = (torch.empty((T, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device) for _ in range(2))
+    if T:
+        with _Current(cache.device):
+            hb._check_rc(hb._lib.i4_kv_read_dev(cache._p, k.data_ptr(), v.data_ptr(), T, _dtypes[dtype],
+                                                slots.data_ptr(), hb._torch_stream(k)), "i4_kv_read_dev")
+    return k, v
+
+
+def _output(out, like, shape, what):
+    torch = hb._torch
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    st = out.stride()
+    if out.dtype is not like.dtype or tuple(out.shape) != shape or out.device != like.device:
+        raise ValueError(f"{what} must be {like.dtype} {shape} on {like.device}, got {out.dtype} {tuple(out.shape)} on "
+                         f"{out.device}")
+    if st[2] != 1 or (st[0] | st[1]) & 3 or out.data_ptr() & 15 or st[1] < shape[2] or st[0] < shape[1] * st[1]:
+        raise ValueError(f"{what} needs a contiguous last dimension, strides of multiples of four elements, rows that "
+                         f"do not overlap and 16-byte alignment, got strides {st}")
+    return out
+
+
+def _span(t):
+    n = sum((s - 1) * d for s, d in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _no_overlap(out, t, what):
+    """`out` is apart from `t`, or the same rows at the same places."""
+    a, b = _span(out), _span(t)
+    if a[0] < b[1] and b[0] < a[1] and not (a == b and out.stride() == t.stride()):
+        raise ValueError(f"out overlaps {what}: it may be {what} itself, or apart from it")
+
+
+def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=None):
+    """Causal attention of new tokens over the cache; ``[T, heads, head_dim]``
+    of q's type.
+
+    ``q``: ``[T, heads, head_dim]``, the sequences' new tokens one after another
+    (heads a multiple of the cache's; query head i reads key-value head i //
+    (heads // kv_heads)).  ``block_table``: int32 ``[B, columns]``, each
+    sequence's pages in order.  ``kv_lens``: int32 ``[B]``, each sequence's keys
+    in the cache, its new tokens' included (``kv_write`` comes first).
+    ``cu_q``: int32 ``[B + 1]``, where each sequence's new tokens begin and the
+    last one's end; None: one token a sequence, T = B.  New token i of n sees
+    the keys up to kv_len - n + i.  ``scale`` > 0 is the softmax scale
+    (head_dim ** -0.5).
+
+    A row that sees no key is zero; keys in pages outside the cache or past the
+    table's columns are not seen; rows outside every sequence are not written.
+    ``out`` may be given, q itself included.
+
+    Sums and softmax statistics are fp32 and the cache's values enter the
+    products exactly.  fp32 queries and their probabilities keep 22 bits; with
+    bf16 and fp16 the probabilities are rounded to fp16's 11."""
+    torch = _torch()
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.kv_heads or not q.shape[1]:
+        raise ValueError(f"q must be [T, a multiple of {cache.kv_heads} heads, {cache.head_dim}], got {tuple(q.shape)}")
+    T, heads, D = q.shape
+    dt = _type(q, "q")
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [B, columns], got {tuple(block_table.shape)}")
+    B, cols = block_table.shape
+    _ints(block_table, (B, cols), "block_table")
+    _ints(kv_lens, (B,), "kv_lens")
+    if cu_q is not None:
+        _ints(cu_q, (B + 1,), "cu_q")
+    elif T != B:
+        raise ValueError(f"{T} tokens in {B} sequences: cu_q says where each begins")
+    if scale is None:
+        scale = D ** -0.5
+    elif not 0 < scale < 1e30:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    _same_device(cache.device, q, block_table, kv_lens, cu_q, out)
+    given = out is not None
+    out = _output(out, q, (T, heads, D), "out")
+    if T == 0 or B == 0:
+        return out
+    with _Current(cache.device):
+        q = _rows(q, "q")
+        if given:
+            _no_overlap(out, q, "q")
+        n = hb._lib.i4_paged_attention_workspace(cache._p, T, B, heads, cols, cu_q is not None)
+        if n < 0:
+            raise ValueError(hb.last_error())
+        work = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None
+        hb._check_rc(hb._lib.i4_paged_attention_dev(
+            cache._p, q.data_ptr(), *q.stride()[:2], T, heads, dt, block_table.data_ptr(), block_table.stride(0), cols,
+            kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, scale, out.data_ptr(), *out.stride()[:2],
+            None if work is None else work.data_ptr(), n, hb._torch_stream(q)), "i4_paged_attention_dev")
+    return out

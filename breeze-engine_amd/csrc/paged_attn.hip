@@ -1,0 +1,793 @@
+// Attention of new tokens over the quantized paged cache.
+//
+//   o_i = sum_j softmax_j(scale * q_i . k_j) v_j,   j <= kv_len - q_len + i
+//
+// for the q_len new tokens i of each sequence, whose keys and values are in
+// the cache already; k_j = ks_j * (what the page holds), v_j alike.
+//
+// Numerics.  A page's INT8 or e4m3 values are exact in fp16, so both products
+// run on the fp16 matrix instructions with exact cache operands and fp32 sums.
+// q is scaled by a power of two for each row (its largest magnitude lands in
+// [2^13, 2^14)), which bf16 and fp16 queries survive exactly; fp32 queries are
+// split into two fp16 terms (22 bits), as are their probabilities.  bf16 and
+// fp16 calls round the probabilities once to fp16's 11 bits, three more than
+// a bf16 output keeps and as many as an fp16 one.  The key scales multiply the
+// scores and the value scales the probabilities; the latter are held relative
+// to a power of two `nu` near the tile's largest value scale, so that the fp16
+// range covers them whatever the values' size.  Running maxima and sums are fp32.
+//
+// Both kernels compute S^T = K Q^T and O^T = V^T P^T: a lane then holds one
+// query row's scores, and the first product's result is the second one's
+// operand as it stands, with the keys in the order that the result layout
+// gives them; V's operand is read from LDS in that order, transposed by the
+// LDS unit.
+#include "mix_common.h"
+
+#include <algorithm>
+
+#include "../../include/breeze_qmm.h"
+
+using namespace mx;
+
+namespace {
+
+struct AttnArgs {
+    const void* q;
+    void* out;
+    int64_t q_token, q_head, o_token, o_head;  // element strides
+    const uint8_t* kp;
+    const uint8_t* vp;
+    const float* ks;
+    const float* vs;
+    const int32_t* table;
+    const int32_t* kv_lens;
+    const int32_t* cu;  // null: one token a sequence
+    float* part;        // [nsplit][T * Hq][D] when nsplit > 1
+    f2* ml;             // [nsplit][T * Hq] (maximum, sum)
+    int64_t table_row;
+    int T, B, Hq, H, G, P, pshift, table_w, nsplit, nslots, dt;
+    float scale;  // softmax scale * log2(e)
+};
+
+// The weights of the second product are p * vs * 2^12 / nu: at most 2^15 while
+// the tile's value scales are at most 8 nu.
+constexpr float kPScale = 4096.0f;
+
+typedef __attribute__((address_space(3))) s4* lds_s4;
+
+__device__ inline h4 read_tr(const _Float16* p) {
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p)));
+}
+__device__ inline h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// The power of two that a tile's value scales are taken relative to: kept
+// while the largest is within (nu / 256, 8 nu].
+__device__ inline float next_nu(float nu, float vmax) {
+    if (!(vmax > 0.0f) || vmax > 3e38f) return nu;
+    if (vmax <= nu * 8.0f && vmax > nu * 0x1p-8f) return nu;
+    const float want = bits_f(max(f_bits(vmax) & 0x7F800000u, 1u << 23));
+    return nu > 0.0f ? fmaxf(want, nu * 0x1p-100f) : want;
+}
+__device__ inline float nu_ratio(float was, float now) { return was > 0.0f ? was / now : 1.0f; }
+
+struct Seq {
+    int q0, n, kv;  // first token, new tokens, keys
+};
+
+__device__ inline Seq sequence(const AttnArgs& a, int b) {
+    Seq s;
+    int q0 = b, q1 = b + 1;
+    if (a.cu) {
+        q0 = min(max(a.cu[b], 0), a.T);
+        q1 = min(max(a.cu[b + 1], q0), a.T);
+    }
+    s.q0 = q0;
+    s.n = q1 - q0;
+    s.kv = (int)min((int64_t)max(a.kv_lens[b], 0), (int64_t)a.table_w << a.pshift);
+    return s;
+}
+
+// Cache row (in rows of D) of the 16 keys from `key` on for head h; -1 where
+// the sequence or its table has none.
+__device__ inline int64_t group_row(const AttnArgs& a, const int32_t* table, int h, int key, int kv) {
+    if (key >= kv) return -1;
+    const int page = table[key >> a.pshift];
+    if (page < 0 || page >= a.P) return -1;
+    return (((int64_t)page * a.H + h) << a.pshift) + (key & ((1 << a.pshift) - 1));
+}
+
+__device__ inline uint32_t lane_max_u32(uint32_t x, int step) { return max(x, (uint32_t)__shfl_xor((int)x, step)); }
+
+// The power of two that brings a row whose largest magnitude has these bits to [2^13, 2^14).
+__device__ inline float row_scale(uint32_t top) {
+    if (top >= 0x7F800000u) return __builtin_nanf("");
+    const int e = 13 - ((int)(top >> 23) - 127);
+    return top == 0 ? 1.0f : bits_f((uint32_t)(min(max(e, -126), 100) + 127) << 23);
+}
+
+// Splits w into fp16 terms: hi, and what hi leaves.
+__device__ inline void split8(const float* w, h8& hi, h8& lo) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const h2 a = to_h2(w[j], w[j + 1]);
+        const h2 b = to_h2(w[j] - (float)a[0], w[j + 1] - (float)a[1]);
+        hi[j] = a[0];
+        hi[j + 1] = a[1];
+        lo[j] = b[0];
+        lo[j + 1] = b[1];
+    }
+}
+__device__ inline h8 round8(const float* w) {
+    h8 r;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const h2 a = to_h2(w[j], w[j + 1]);
+        r[j] = a[0];
+        r[j + 1] = a[1];
+    }
+    return r;
+}
+
+// ------------------------------------------------------------------ few rows: the keys shared out
+//
+// One workgroup for a sequence's up to 16 rows (new tokens times the query
+// heads of one key-value head), one key-value head and one split of the keys;
+// its four waves take tiles of 32 keys in turn.  Bound by HBM: the next tile's
+// keys and values are on their way while this one is computed, 16 KB a wave
+// (D = 256), and no wave waits for another before the end.
+
+template <int D, int KIND, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
+    constexpr int KC = D / 64;        // 16-byte chunks of a key a lane takes (a quarter of each 64 values)
+    constexpr int VC = D / 32;        // 16-byte chunks of a tile's values a lane takes
+    constexpr int VS = D + 16;        // LDS row of a key's values: the transposed reads' four rows fall on unlike banks
+    constexpr int OS = D + 4;
+    constexpr int kLds = 4 * 32 * VS * 2 > 4 * 16 * OS * 4 ? 4 * 32 * VS * 2 : 4 * 16 * OS * 4;
+    __shared__ __align__(16) uint8_t lds[kLds];
+    __shared__ float sm[4][16], sl[4][16], snu[4];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % a.H, bs = blockIdx.x / a.H, split = bs % a.nsplit, b = bs / a.nsplit;
+    const Seq sq = sequence(a, b);
+    const int rows = sq.n * a.G;
+    if (rows <= 0 || rows > 16) return;
+    const int r16 = lane & 15, c = lane >> 4;
+    const int32_t* table = a.table + b * a.table_row;
+
+    // The query operand: row r16, values 64 i + 16 c + 8 half + 0..7 for slab 2 i + half.
+    const bool has_row = r16 < rows;
+    const int tok = sq.q0 + (has_row ? r16 / a.G : 0), head = h * a.G + (has_row ? r16 % a.G : 0);
+    const int last = has_row ? sq.kv - sq.n + r16 / a.G : -1;  // the last key that the row sees
+    h8 qh[D / 32], ql[SPLIT ? D / 32 : 1];
+    float rowf;
+    {
+        float x[D / 4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                f4 v = {0, 0, 0, 0};
+                if (has_row) v = load4(a.q, a.dt, tok * a.q_token + head * a.q_head + 64 * i + 16 * c + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[16 * i + j + e] = v[e];
+                    top = max(top, f_bits(v[e]) & 0x7FFFFFFFu);
+                }
+            }
+        top = lane_max_u32(lane_max_u32(top, 16), 32);
+        const float up = row_scale(top);
+        rowf = a.scale / up;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = x[8 * s + j] * up;
+            if constexpr (SPLIT) split8(w, qh[s], ql[s]);
+            else qh[s] = round8(w);
+        }
+    }
+
+    const int ntile = (sq.kv + 31) >> 5, per = (ntile + a.nsplit - 1) / a.nsplit;
+    const int t1 = min((split + 1) * per, ntile);
+    int t = split * per + wave;
+
+    f4 o[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i] = (f4){0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f, nu = 0.0f;
+
+    u4 kraw[2][KC], vraw[VC];
+    f4 ksc[2], vsc[2];
+    _Float16* vt = reinterpret_cast<_Float16*>(lds) + wave * (32 * VS);
+
+    int64_t row[2];
+    const auto rows_of = [&](int tile, int64_t* r) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) r[u] = tile < t1 ? group_row(a, table, h, 32 * tile + 16 * u, sq.kv) : -1;
+    };
+    const auto load = [&](const int64_t* r) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t at = r[u] < 0 ? 0 : r[u];  // a masked group reads the cache's first rows
+            const uint8_t* kp = a.kp + (at + r16) * D + 16 * c;
+#pragma unroll
+            for (int i = 0; i < KC; ++i) kraw[u][i] = *reinterpret_cast<const u4*>(kp + 64 * i);
+            ksc[u] = *reinterpret_cast<const f4*>(a.ks + at + 4 * c);
+            vsc[u] = *reinterpret_cast<const f4*>(a.vs + at + 4 * c);
+        }
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+            constexpr int per_row = D / 16;
+            const int chunk = lane + 64 * i, kr = chunk / per_row;  // kr / 16 does not depend on the lane
+            const int64_t at = r[(64 * i / per_row) >> 4] < 0 ? 0 : r[(64 * i / per_row) >> 4];
+            vraw[i] = *reinterpret_cast<const u4*>(a.vp + (at + (kr & 15)) * D + 16 * (chunk % per_row));
+        }
+    };
+    rows_of(t, row);
+    if (t < t1) load(row);
+    int64_t next[2];
+    rows_of(t + 4, next);
+
+    for (; t < t1; t += 4) {
+        const int key0 = 32 * t;
+        const bool tail = key0 + 32 > sq.kv || row[0] < 0 || row[1] < 0;
+        // Values to LDS, [key][d] in fp16.
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+            constexpr int per_row = D / 16;
+            const int chunk = lane + 64 * i, kr = chunk / per_row;
+            u4 w = vraw[i];
+            if (KIND == kFp8 && tail && (key0 + kr >= sq.kv || row[kr >> 4] < 0)) w = (u4){0, 0, 0, 0};
+            h8* dst = reinterpret_cast<h8*>(vt + kr * VS + 16 * (chunk % per_row));
+            dst[0] = unpack8<KIND>(w.x, w.y);
+            dst[1] = unpack8<KIND>(w.z, w.w);
+        }
+        f4 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u] = (f4){0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < KC; ++i) {
+                const h8 k0 = unpack8<KIND>(kraw[u][i].x, kraw[u][i].y), k1 = unpack8<KIND>(kraw[u][i].z, kraw[u][i].w);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * i], s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * i + 1], s[u], 0, 0, 0);
+                if constexpr (SPLIT) {
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[2 * i], s[u], 0, 0, 0);
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[2 * i + 1], s[u], 0, 0, 0);
+                }
+            }
+        }
+        float x[8], vw[8];
+        bool see[8];
+        float top = -INFINITY, vmax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int u = j >> 2, key = key0 + 16 * u + 4 * c + (j & 3);
+            see[j] = key <= last && row[u] >= 0;
+            x[j] = see[j] ? s[u][j & 3] * ksc[u][j & 3] : -INFINITY;
+            vw[j] = see[j] ? vsc[u][j & 3] : 0.0f;
+            top = fmaxf(top, x[j]);
+            vmax = fmaxf(vmax, vw[j]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) row[u] = next[u];
+        if (t + 4 < t1) load(row);
+        rows_of(t + 8, next);
+
+        top = max_halves(max_rows16(top));
+        vmax = max_halves(max_rows16(vmax));
+#pragma unroll
+        for (int st = 1; st < 16; st *= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, st));  // rows see unlike keys
+        const float now = next_nu(nu, vmax), was = nu;
+        nu = now;
+        const float mn = fmaxf(m, top), safe = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = fast_exp2((m - safe) * rowf) * nu_ratio(was, now);
+        const float lalpha = fast_exp2((m - safe) * rowf);
+        m = mn;
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
+        }
+        l *= lalpha;
+        const float up = nu > 0.0f ? kPScale / nu : 0.0f;
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float p = fast_exp2((x[j] - safe) * rowf);
+            l += p;
+            w[j] = vw[j] == 0.0f ? 0.0f : p * (vw[j] * up);
+        }
+        h8 ph, pl;
+        if constexpr (SPLIT) split8(w, ph, pl);
+        else ph = round8(w);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const _Float16* p = vt + (4 * c + (r16 >> 2)) * VS + 16 * i + 4 * (r16 & 3);
+            const h8 v = join(read_tr(p), read_tr(p + 16 * VS));
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[i], 0, 0, 0);
+            if constexpr (SPLIT) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[i], 0, 0, 0);
+        }
+    }
+
+    // The four waves' sums, joined in wave order.
+    l = sum_halves(sum_rows16(l));
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(lds);
+    if (c == 0) {
+        sm[wave][r16] = m * rowf;  // in units of log2
+        sl[wave][r16] = l;
+    }
+    if (lane == 0) snu[wave] = nu * (1.0f / kPScale);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+        *reinterpret_cast<f4*>(so + (wave * 16 + r16) * OS + 16 * i + 4 * c) = o[i];
+    __syncthreads();
+    const int r = threadIdx.x >> 4, part = threadIdx.x & 15;
+    if (r >= rows) return;
+    float top = -INFINITY, sum = 0.0f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w][r]);
+    const float safe = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = fast_exp2(sm[w][r] - safe);
+        sum += f[w] * sl[w][r];
+        f[w] *= snu[w];
+    }
+    const int ot = sq.q0 + r / a.G, oh = h * a.G + r % a.G;
+    const int64_t orow = (int64_t)ot * a.Hq + oh, prow = (int64_t)split * a.T * a.Hq + orow;
+    const float inv = a.nsplit > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    if (a.nsplit > 1 && part == 0) a.ml[prow] = (f2){top, sum};
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const int d = 64 * i + 4 * part;
+        f4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(so + (w * 16 + r) * OS + d) * f[w];
+        v *= inv;
+        if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+        else store4(a.out, a.dt, ot * a.o_token + oh * a.o_head + d, v);
+    }
+}
+
+// ------------------------------------------------------------------ many rows: the rows shared out
+//
+// One workgroup for 128 rows of a sequence, one key-value head and one split
+// of the keys; each of its four waves holds 32 rows' queries and sums, and
+// tiles of 64 keys pass through LDS, unpacked to fp16 on the way in.  The next
+// tile's bytes are loaded while this one is computed.  Sequences of up to 16
+// rows are the other kernel's.
+
+constexpr int kRowTile = 128, kKeyTile = 64;
+
+template <int D, int KIND, bool SPLIT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnArgs a) {
+    constexpr int KS = D + 8, VS = D + 16;  // LDS rows of a key: reads of one instruction fall on unlike banks
+    constexpr int NC = D / 64;              // 16-byte chunks a thread loads of a tile's keys (and of its values)
+    constexpr int per_row = D / 16;
+    __shared__ __align__(16) _Float16 sk[kKeyTile * KS], sv[kKeyTile * VS];
+    __shared__ __align__(16) float sks[kKeyTile], svs[kKeyTile];
+    __shared__ float sbad[kKeyTile], snu;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r32 = lane & 31, hf = lane >> 5;
+    const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.nsplit;
+    const int slot = a.nslots - 1 - ss / a.nsplit;  // a prompt's last rows see the most keys: first
+    // Sequence b's tiles take the slots from cu[b] * G / 128 + b on, which leaves
+    // room for all of them without a pass over the lengths.
+    int b = 0;
+    if (a.cu) {
+        int hi = a.B;
+        while (hi - b > 1) {
+            const int mid = (b + hi) >> 1;
+            const int64_t start = (int64_t)min(max(a.cu[mid], 0), a.T) * a.G / kRowTile + mid;
+            if (start <= slot) b = mid;
+            else hi = mid;
+        }
+    } else {
+        b = slot / ((a.G + kRowTile - 1) / kRowTile);
+    }
+    const Seq sq = sequence(a, b);
+    const int64_t rows = (int64_t)sq.n * a.G;
+    const int64_t before = a.cu ? (int64_t)sq.q0 * a.G / kRowTile + b : (int64_t)b * ((a.G + kRowTile - 1) / kRowTile);
+    const int64_t first = (slot - before) * kRowTile;
+    if (rows <= 16 || first < 0 || first >= rows) return;
+    const int64_t row = first + 32 * wave + r32;
+    const bool has_row = row < rows;
+    const int tok_in = has_row ? (int)(row / a.G) : 0;
+    const int tok = sq.q0 + tok_in, head = h * a.G + (has_row ? (int)(row % a.G) : 0);
+    const int last = has_row ? sq.kv - sq.n + tok_in : -1;
+    // Keys that the workgroup's, and this wave's, last row sees; keys that all of the wave's rows see.
+    const auto seen_by = [&](int64_t r) { return max(sq.kv - sq.n + (int)(min(r, rows - 1) / a.G) + 1, 0); };
+    const int wg_end = seen_by(first + kRowTile - 1);
+    const bool wave_rows = first + 32 * wave < rows;
+    const int wave_end = wave_rows ? seen_by(first + 32 * wave + 31) : 0;
+    const int wave_all = seen_by(first + 32 * wave);
+
+    h8 qh[D / 16], ql[SPLIT ? D / 16 : 1];
+    float rowf;
+    {
+        uint32_t top = 0;
+        const int64_t at = tok * a.q_token + head * a.q_head + 8 * hf;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const f4 v = load4(a.q, a.dt, at + 16 * s + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, f_bits(v[e]) & 0x7FFFFFFFu);
+            }
+        top = lane_max_u32(top, 32);
+        const float up = row_scale(top);
+        rowf = a.scale / up;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const f4 v = load4(a.q, a.dt, at + 16 * s + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[j + e] = v[e] * up;
+            }
+            if constexpr (SPLIT) split8(w, qh[s], ql[s]);
+            else qh[s] = round8(w);
+        }
+    }
+
+    const int ntile = (min(wg_end, sq.kv) + kKeyTile - 1) / kKeyTile, per = (ntile + a.nsplit - 1) / a.nsplit;
+    const int t1 = min((split + 1) * per, ntile);
+    int t = split * per;
+    const int32_t* table = a.table + b * a.table_row;
+
+    f16 o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    float m = -INFINITY, l = 0.0f, nu = 0.0f;
+
+    u4 kraw[NC], vraw[NC];
+    int64_t grow[NC];    // cache rows of the groups of 16 keys that this wave's chunks belong to
+    float ksc = 0.0f, vsc = 0.0f;  // wave 0: a key's two scales
+    bool sc_bad = true;
+    const auto load = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int kr = (wave * 64 + 256 * i) / per_row;  // the wave's first row of this pass
+            grow[i] = group_row(a, table, h, kKeyTile * tile + (kr & ~15), sq.kv);
+            const int64_t at = (grow[i] < 0 ? 0 : grow[i]) + ((tid + 256 * i) / per_row & 15);
+            kraw[i] = *reinterpret_cast<const u4*>(a.kp + at * D + 16 * (tid % per_row));
+            vraw[i] = *reinterpret_cast<const u4*>(a.vp + at * D + 16 * (tid % per_row));
+        }
+        if (wave == 0) {
+            const int64_t at = group_row(a, table, h, kKeyTile * tile + (lane & ~15), sq.kv);
+            sc_bad = at < 0 || kKeyTile * tile + lane >= sq.kv;
+            ksc = sc_bad ? 0.0f : a.ks[at + (lane & 15)];
+            vsc = sc_bad ? 0.0f : a.vs[at + (lane & 15)];
+        }
+    };
+    if (t < t1) load(t);
+
+    for (; t < t1; ++t) {
+        const int key0 = kKeyTile * t;
+        __syncthreads();  // the last tile's reads are over
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int kr = (tid + 256 * i) / per_row, col = 16 * (tid % per_row);
+            u4 kw = kraw[i], vw = vraw[i];
+            if (KIND == kFp8 && (grow[i] < 0 || key0 + kr >= sq.kv)) kw = vw = (u4){0, 0, 0, 0};
+            h8* kd = reinterpret_cast<h8*>(sk + kr * KS + col);
+            h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
+            kd[0] = unpack8<KIND>(kw.x, kw.y);
+            kd[1] = unpack8<KIND>(kw.z, kw.w);
+            vd[0] = unpack8<KIND>(vw.x, vw.y);
+            vd[1] = unpack8<KIND>(vw.z, vw.w);
+        }
+        if (wave == 0) {
+            // A value scale of NaN goes with the key's, whose score a row that does
+            // not see the key leaves out; times a probability of zero it would not.
+            const bool nan = vsc != vsc;
+            sks[lane] = nan ? vsc : ksc;
+            sbad[lane] = sc_bad ? 1.0f : 0.0f;
+            float vmax = nan ? 0.0f : vsc;
+#pragma unroll
+            for (int st = 1; st < 64; st *= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, st));
+            const float now = next_nu(nu, vmax);
+            svs[lane] = now > 0.0f && !nan ? vsc * (kPScale / now) : 0.0f;
+            if (lane == 0) snu = now;
+        }
+        __syncthreads();
+        if (t + 1 < t1) load(t + 1);
+        const float now = snu, was = nu;
+        nu = now;
+        const float nr = nu_ratio(was, now);
+        if (key0 >= wave_end) {
+            if (nr != 1.0f) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[i] *= nr;
+            }
+            continue;
+        }
+
+        f16 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
+            const _Float16* p = sk + (32 * u + r32) * KS + 8 * hf;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const h8 k = *reinterpret_cast<const h8*>(p + 16 * i);
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s[u], 0, 0, 0);
+                if constexpr (SPLIT) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i], s[u], 0, 0, 0);
+            }
+        }
+        // Scores times the key scales; result register j holds key 8 (j / 4) + 4 hf + j % 4.
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const f4 sc = *reinterpret_cast<const f4*>(sks + 32 * u + 2 * j + 4 * hf);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[u][j + e] *= sc[e];
+            }
+        // Past the wave's first row, past the sequence's end or in a page that is not there.
+        if (key0 + kKeyTile > wave_all || key0 + kKeyTile > sq.kv || __any(sbad[lane] != 0.0f)) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int k = 32 * u + 8 * (j / 4) + 4 * hf + j % 4;
+                    if (key0 + k > last || sbad[k] != 0.0f) s[u][j] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, s[u][j]);
+        top = max_halves(top);
+        const float mn = fmaxf(m, top), safe = mn == -INFINITY ? 0.0f : mn;
+        const float lalpha = fast_exp2((m - safe) * rowf), alpha = lalpha * nr;
+        m = mn;
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+        }
+        l *= lalpha;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {  // 16 keys
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = fast_exp2((s[u][8 * g + j] - safe) * rowf);
+                    l += w[j];
+                }
+                const f4 s0 = *reinterpret_cast<const f4*>(svs + 32 * u + 16 * g + 4 * hf);
+                const f4 s1 = *reinterpret_cast<const f4*>(svs + 32 * u + 16 * g + 8 + 4 * hf);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] *= s0[j];
+                    w[4 + j] *= s1[j];
+                }
+                h8 ph, pl;
+                if constexpr (SPLIT) split8(w, ph, pl);
+                else ph = round8(w);
+                const int i16 = lane & 15;
+                const _Float16* p = sv + (32 * u + 16 * g + 4 * hf + (i16 >> 2)) * VS + 16 * (r32 >> 4) + 4 * (i16 & 3);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const h8 v = join(read_tr(p + 32 * i), read_tr(p + 32 * i + 8 * VS));
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[i], 0, 0, 0);
+                    if constexpr (SPLIT) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[i], 0, 0, 0);
+                }
+            }
+    }
+
+    if (!has_row) return;
+    l = sum_halves(l);
+    const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
+    float f = nu * (1.0f / kPScale);
+    if (a.nsplit > 1) {
+        if (hf == 0) a.ml[prow] = (f2){m * rowf, l};
+    } else {
+        f *= l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const int d = 32 * i + 2 * j + 4 * hf;
+            const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
+            if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+            else store4(a.out, a.dt, tok * a.o_token + head * a.o_head + d, v);
+        }
+}
+
+// The splits of a row joined, in their order.
+template <int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    constexpr int L = D / 4;
+    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int d = 4 * (threadIdx.x % L);
+    const int64_t n = (int64_t)a.T * a.Hq;
+    if (row >= n) return;
+    const int tok = (int)(row / a.Hq), head = (int)(row % a.Hq);
+    if (a.cu && (tok < a.cu[0] || tok >= a.cu[a.B])) return;
+    float top = -INFINITY, sum = 0.0f;
+    for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.ml[s * n + row].x);
+    const float safe = top == -INFINITY ? 0.0f : top;
+    f4 v = {0, 0, 0, 0};
+    for (int s = 0; s < a.nsplit; ++s) {
+        const f2 ml = a.ml[s * n + row];
+        const float f = fast_exp2(ml.x - safe);
+        sum += f * ml.y;
+        v += *reinterpret_cast<const f4*>(a.part + (s * n + row) * D + d) * f;
+    }
+    v *= sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    store4(a.out, a.dt, tok * a.o_token + head * a.o_head + d, v);
+}
+
+// ------------------------------------------------------------------ host
+
+struct AttnPlan {
+    int keys, rows, nsplit, nslots;  // which kernels run, splits of the keys, slots of the rows kernel
+    size_t bytes;                    // workspace
+};
+
+// Splits: enough workgroups for every compute unit twice, each with at least
+// 256 keys of the longest sequence that the table can hold.
+AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int n_cu) {
+    const int G = Hq / H;
+    AttnPlan p{};
+    p.keys = G <= 16;
+    p.rows = cu ? (int64_t)T * G > 16 : G > 16;
+    p.nslots = cu ? (int)((int64_t)T * G / kRowTile) + B : B * ((G + kRowTile - 1) / kRowTile);
+    const int64_t wgs = (int64_t)H * (p.rows && T > 2 * B ? p.nslots : B);
+    int64_t s = std::max<int64_t>(1, (2 * n_cu + wgs - 1) / wgs);
+    s = std::min<int64_t>(s, std::max<int64_t>(1, capacity / 256));
+    s = std::min<int64_t>(s, 64);
+    if (wgs >= n_cu) s = 1;
+    p.nsplit = (int)s;
+    p.bytes = s > 1 ? (size_t)s * T * Hq * (D * 4 + 8) : 0;
+    return p;
+}
+
+int cu_count() {
+    static int n[64] = {};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (n[dev] == 0) {
+        int v = 0;
+        n[dev] = hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0 ? v : 256;
+    }
+    return n[dev];
+}
+
+template <int D, int KIND, bool SPLIT>
+void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+    if (p.keys) attn_keys_kernel<D, KIND, SPLIT><<<(unsigned)a.B * a.H * a.nsplit, 256, 0, st>>>(a);
+    if (p.rows) attn_rows_kernel<D, KIND, SPLIT><<<(unsigned)a.nslots * a.H * a.nsplit, 256, 0, st>>>(a);
+    if (a.nsplit > 1) {
+        constexpr int rows = 256 / (D / 4);
+        attn_join_kernel<D><<<(unsigned)(((int64_t)a.T * a.Hq + rows - 1) / rows), 256, 0, st>>>(a);
+    }
+}
+
+template <int D>
+void launch1(const AttnArgs& a, const AttnPlan& p, int kind, hipStream_t st) {
+    const bool split = a.dt == kF32;
+    if (kind == kInt8) split ? launch3<D, kInt8, true>(a, p, st) : launch3<D, kInt8, false>(a, p, st);
+    else split ? launch3<D, kFp8, true>(a, p, st) : launch3<D, kFp8, false>(a, p, st);
+}
+
+bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, bool has_cu, int* pshift) {
+    if (!c || (c->kind != kInt8 && c->kind != kFp8)) {
+        bq_set_error("paged_attention: needs a cache of kind 0 (INT8) or 1 (e4m3)");
+        return false;
+    }
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) {
+        bq_set_error("paged_attention: head_dim must be 64, 128 or 256, got %d", c->head_dim);
+        return false;
+    }
+    int s = 4;
+    while (s < 10 && (1 << s) != c->page_size) ++s;
+    if ((1 << s) != c->page_size || c->num_pages < 1 || c->kv_heads < 1 || c->kv_heads > 4096 ||
+        c->num_pages > (INT32_MAX >> s)) {
+        bq_set_error("paged_attention: needs a page size of 16 to 1024 that is a power of two, at least one page, 1 to "
+                     "4096 heads and fewer than 2^31 slots (got page size %d, %d pages, %d heads)",
+                     c->page_size, c->num_pages, c->kv_heads);
+        return false;
+    }
+    if (T < 0 || B < 0 || heads < 1 || heads > 65536 || heads % c->kv_heads || table_w < 0 ||
+        table_w > (INT32_MAX >> s) || (!has_cu && T != B)) {
+        bq_set_error("paged_attention: needs query heads in multiples of the %d key-value heads, and one token a "
+                     "sequence where no offsets are given (got %d tokens, %d sequences, %d heads, %d table columns)",
+                     c->kv_heads, T, B, heads, table_w);
+        return false;
+    }
+    // Workgroups and rows are counted in 32 bits.
+    if ((int64_t)T * heads > INT32_MAX / 64 || (int64_t)B * c->kv_heads > INT32_MAX / 64) {
+        bq_set_error("paged_attention: %d tokens of %d heads in %d sequences are too many for one call", T, heads, B);
+        return false;
+    }
+    *pshift = s;
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t i4_paged_attention_workspace(const i4_kv_cache* cache, int T, int B, int heads, int table_w, int has_cu) {
+    int ps = 0;
+    if (!check_shape(cache, T, B, heads, table_w, has_cu != 0, &ps)) return -2;
+    if (T == 0 || B == 0) return 0;
+    return (int64_t)plan_attn(T, B, heads, cache->kv_heads, cache->head_dim, has_cu != 0, (int64_t)table_w << ps,
+                              cu_count())
+        .bytes;
+}
+
+int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
+                           int dtype, const int32_t* dTable, int64_t table_row, int table_w, const int32_t* dKvLens,
+                           const int32_t* dCu, int B, float scale, void* dOut, int64_t o_token, int64_t o_head,
+                           void* dWork, int64_t work_bytes, void* stream) {
+    int ps = 0;
+    if (!check_shape(cache, T, B, heads, table_w, dCu != nullptr, &ps)) return -2;
+    if (dtype < kF32 || dtype > kF16 || !(scale > 0.0f) || scale > 1e30f) {
+        bq_set_error("paged_attention: needs a type of 0 to 2 and a positive finite scale (got %d, %g)", dtype, scale);
+        return -2;
+    }
+    if (T == 0 || B == 0) return 0;
+    if (!cache->k || !cache->v || !cache->k_scale || !cache->v_scale || !dQ || !dOut || !dKvLens ||
+        (table_w > 0 && !dTable)) {
+        bq_set_error("paged_attention: null device pointer");
+        return -2;
+    }
+    AttnArgs a{};
+    a.q = dQ;
+    a.out = dOut;
+    a.q_token = q_token;
+    a.q_head = q_head;
+    a.o_token = o_token;
+    a.o_head = o_head;
+    a.kp = static_cast<const uint8_t*>(cache->k);
+    a.vp = static_cast<const uint8_t*>(cache->v);
+    a.ks = cache->k_scale;
+    a.vs = cache->v_scale;
+    a.table = dTable;
+    a.table_row = table_row;
+    a.table_w = table_w;
+    a.kv_lens = dKvLens;
+    a.cu = dCu;
+    a.T = T;
+    a.B = B;
+    a.Hq = heads;
+    a.H = cache->kv_heads;
+    a.G = heads / cache->kv_heads;
+    a.P = cache->num_pages;
+    a.pshift = ps;
+    a.dt = dtype;
+    a.scale = scale * kLog2e;
+    const AttnPlan p =
+        plan_attn(T, B, heads, a.H, cache->head_dim, dCu != nullptr, (int64_t)table_w << ps, cu_count());
+    if (p.bytes > 0 && (!dWork || work_bytes < (int64_t)p.bytes)) {
+        bq_set_error("paged_attention: needs a workspace of %zu bytes, got %lld", p.bytes, (long long)work_bytes);
+        return -4;
+    }
+    a.nsplit = p.nsplit;
+    a.nslots = p.nslots;
+    a.part = static_cast<float*>(dWork);
+    a.ml = reinterpret_cast<f2*>(a.part + (size_t)p.nsplit * T * heads * cache->head_dim);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    (void)hipGetLastError();
+    if (cache->head_dim == 64) launch1<64>(a, p, cache->kind, st);
+    else if (cache->head_dim == 128) launch1<128>(a, p, cache->kind, st);
+    else launch1<256>(a, p, cache->kind, st);
+    return launched("paged_attention") ? 0 : -5;
+}
+
+}  // extern "C"

@@ -41,6 +41,7 @@
 #include <vector>
 
 #include "../../include/breeze_qmm.h"
+#include "mix_common.h"
 #include "qmm_common.h"
 
 using namespace bq;
@@ -2229,6 +2230,16 @@ bool check_dims(int N, int K, int bits) {
 }
 
 }  // namespace
+
+// For the library's other translation units (mix_common.h).
+void bq_set_error(const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    set_err("%s", buf);
+}
 
 // ====================================================================== C ABI
 

@@ -199,6 +199,62 @@ int i4_block_dots_dev(void* handle, const float* dA, int M, int32_t* dCs, void* 
  * `stream`.  Returns 0, or a negative code with i4_last_error() set. */
 int i4_rmsnorm_dev(const float* dX, const float* dW, int M, int H, float eps, float* dOut, void* stream);
 
+/* ---- the decoder's token mixers ---------------------------------------
+ *
+ * What runs between a layer's projections (the reference computes it inside
+ * its decoder, kernel/qwen35_decoder.cpp:218-428, over an unquantized cache).
+ * Device pointers, asynchronous on `stream`, on the current device; element
+ * types are 0 fp32, 1 bf16, 2 fp16.  Each call owns no memory: a workspace,
+ * where one is needed, is the caller's, so calls on different streams and
+ * captured graphs share nothing.  Every entry point returns 0, or a negative
+ * code with i4_last_error() set. */
+
+/* One layer's keys and values in pages.  k, v: [num_pages, kv_heads,
+ * page_size, head_dim] bytes, INT8 (kind 0) or e4m3 (kind 1); k_scale,
+ * v_scale: fp32 [num_pages, kv_heads, page_size], one for each token and head.
+ * head_dim is 64, 128 or 256, page_size a power of two from 16 to 1024.  k and
+ * v are 16-byte aligned.  A token's slot is page * page_size + its place in
+ * the page. */
+typedef struct {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int num_pages, kv_heads, page_size, head_dim, kind;
+} i4_kv_cache;
+
+/* Quantizes T tokens' keys and values [T, kv_heads, head_dim] (element
+ * strides per token and head, multiples of four; the last dimension
+ * contiguous; 16-byte aligned) into the cache's slots dSlots[T]; a slot that
+ * is negative or past the cache skips its token.  INT8: scale = max|x| / 127,
+ * value = the whole number nearest to x / scale, ties to even.  e4m3: scale =
+ * the smallest power of two that brings the row within 448.  A row with an
+ * infinity or NaN gets the scale NaN.  A slot is given at most once a call. */
+int i4_kv_write_dev(const i4_kv_cache* cache, const void* dK, const void* dV, int64_t k_token, int64_t k_head,
+                    int64_t v_token, int64_t v_head, int T, int dtype, const int32_t* dSlots, void* stream);
+
+/* Reads T slots back: dK, dV [T, kv_heads, head_dim] contiguous, value times
+ * scale, rounded once to the type.  Zeros where a slot is not the cache's. */
+int i4_kv_read_dev(const i4_kv_cache* cache, void* dK, void* dV, int T, int dtype, const int32_t* dSlots,
+                   void* stream);
+
+/* Causal attention of new tokens over the cache, which holds their keys and
+ * values already.  dQ [T, heads, head_dim] packs the B sequences' new tokens:
+ * sequence b has dCu[b] .. dCu[b + 1] - 1 (dCu NULL: token b), and query head
+ * i reads key-value head i / (heads / kv_heads).  dTable [B, table_w] (int32,
+ * row stride table_row) holds its pages in order, dKvLens[b] its keys, the new
+ * ones included: new token i of q_len sees the keys up to dKvLens[b] - q_len +
+ * i.  A row that sees no key gets zeros; keys in pages outside the cache and
+ * past the table are not seen; rows outside every sequence are left as they
+ * were.  scale > 0.  dOut [T, heads, head_dim] of dQ's type, strides as dQ's.
+ * dWork: as many bytes as i4_paged_attention_workspace says for the same
+ * shapes (0: may be NULL), 16-byte aligned. */
+int64_t i4_paged_attention_workspace(const i4_kv_cache* cache, int T, int B, int heads, int table_w, int has_cu);
+int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
+                           int dtype, const int32_t* dTable, int64_t table_row, int table_w, const int32_t* dKvLens,
+                           const int32_t* dCu, int B, float scale, void* dOut, int64_t o_token, int64_t o_head,
+                           void* dWork, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
