@@ -10,8 +10,8 @@ Modules mirror the reference's public surface for this path:
 - ``loader`` for the external-data mapping of breeze/loader.py (weights go
   from the mapped file to the GPU without a host copy);
 - ``attention`` for the token mixers of the decoder
-  (kernel/qwen35_decoder.cpp:218-428): the quantized paged cache and attention
-  over it.
+  (kernel/qwen35_decoder.cpp:218-428): the quantized paged cache, attention
+  over it and gated linear attention.
 
 The compute lives in ``libbreeze_qmm.so``, hand-written HIP behind a C ABI
 (include/breeze_qmm.h).

@@ -13,8 +13,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(PKG), "csrc")
 # Host code and small kernels; the decode and prefill kernels, one unit per
 # (bits, activation mode) so the device passes run side by side.
-# Then the token mixers (the paged cache, attention over it).
-MIXERS = ["kv_cache.hip", "paged_attn.hip"]
+# Then the token mixers (the paged cache, attention over it, gated linear attention).
+MIXERS = ["kv_cache.hip", "paged_attn.hip", "gla.hip"]
 SOURCES = ["qmm.hip", "pf16_w4.hip", "pf16_w8.hip", "pf_w4_i8.hip", *MIXERS] + [f"{k}_w{b}_{m}.hip" for k in ("dec", "pf") for b in (4, 8) for m in ("hp", "lp")]
 LIB_NAME = "libbreeze_qmm.so"
 

@@ -7,6 +7,9 @@ quantized projections (``hip_backend``).
 - ``paged_attention``: causal attention of new tokens (one a sequence, or a
   chunk) over that cache, in place of the decoder's full attention
   (kernel/qwen35_decoder.cpp:334-395, which keeps fp32 keys and values).
+- ``gated_linear_attention``: the linear-attention layers' recurrence
+  (kernel/qwen35_decoder.cpp:46-121), one token at a time from a kept state or
+  whole prompts in chunks.
 
 Tensors are fp32, bf16 or fp16 on one gfx950 GPU.  Calls are asynchronous on
 the current stream, own no memory between calls (a workspace comes from
@@ -213,6 +216,13 @@ def _no_overlap(out, t, what):
         raise ValueError(f"out overlaps {what}: it may be {what} itself, or apart from it")
 
 
+def _apart(out, t):
+    """`out` shares no memory with an input of a call that reads it late."""
+    a, b = _span(out), _span(t)
+    if a[0] < b[1] and b[0] < a[1]:
+        raise ValueError("out overlaps an input")
+
+
 def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=None):
     """Causal attention of new tokens over the cache; ``[T, heads, head_dim]``
     of q's type.
@@ -270,3 +280,104 @@ def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=N
             kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, scale, out.data_ptr(), *out.stride()[:2],
             None if work is None else work.data_ptr(), n, hb._torch_stream(q)), "i4_paged_attention_dev")
     return out
+
+
+def _gates(t, shape, what):
+    torch = hb._torch
+    if tuple(t.shape) != shape or t.dtype not in _dtypes:
+        raise ValueError(f"{what} must be {shape} of float32, bfloat16 or float16, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype is not torch.float32 or (shape[1] > 1 and t.stride(1) != 1):
+        t = t.to(torch.float32).contiguous()
+    return t
+
+
+def _state(t, shape, device, what):
+    torch = hb._torch
+    if t.dtype is not torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() & 15:
+        raise ValueError(f"{what} must be contiguous, 16-byte aligned float32 {shape}, got {t.dtype} {tuple(t.shape)} "
+                         f"(strides {t.stride()})")
+
+
+def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, scale=None, out=None, state_out=None):
+    """Linear attention with a decay for each head and token, by the delta rule
+    where ``beta`` is given; ``(o, state)``.
+
+    For each value head, with the q and k of key head i // (v_heads //
+    k_heads)::
+
+        S_t = exp(g_t) S_{t-1} + k_t u_t^T          o_t = scale S_t^T q_t
+        u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t)      (v_t without beta)
+
+    ``q``, ``k``: ``[T, k_heads, k_dim]``; ``v``: ``[T, v_heads, v_dim]``, of one
+    type (views of a wider projection are read in place).  ``g``, ``beta``:
+    ``[T, v_heads]``; g is the decay's logarithm, at most 0 (-inf drops the
+    state).  ``state``: fp32 ``[B, v_heads, k_dim, v_dim]``, what each sequence
+    starts from (None: zeros).  ``cu_seqlens``: int32 ``[B + 1]``, where each
+    sequence's tokens begin and the last one's end; None: one token a sequence,
+    B = T.  A sequence without tokens keeps its state; rows outside every
+    sequence are not written.  k_dim is 64 or 128, v_dim a multiple of 16 up to
+    1024; ``scale`` is k_dim ** -0.5.
+
+    The new state goes to ``state_out`` (``state`` itself, or apart from it) or
+    to a new tensor.  State and sums are fp32; the products of prompts keep 22
+    bits of every operand.  Sequences of more than 16 tokens, and one that is
+    alone in its call, go in chunks of 64: a NaN or infinity there reaches all
+    rows of its chunk and those after it."""
+    torch = _torch()
+    if q.dim() != 3 or v.dim() != 3 or k.shape != q.shape or v.shape[0] != q.shape[0]:
+        raise ValueError(f"q and k must be [T, k_heads, k_dim] and v [T, v_heads, v_dim], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    T, Hk, Dk = q.shape
+    _, Hv, Dv = v.shape
+    dt = _type(q, "q")
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise ValueError(f"q, k and v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if not Hk or not Hv or Hv % Hk or Dk not in (64, 128) or Dv % 16 or not 16 <= Dv <= 1024:
+        raise ValueError(f"needs v_heads in multiples of k_heads, k_dim 64 or 128 and v_dim a multiple of 16 up to 1024, "
+                         f"got {Hv} of {Dv} and {Hk} of {Dk}")
+    g = _gates(g, (T, Hv), "g")
+    if beta is not None:
+        beta = _gates(beta, (T, Hv), "beta")
+    if cu_seqlens is None:
+        B = T
+    else:
+        B = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
+        if B < 0:
+            raise ValueError(f"cu_seqlens must be [B + 1], got {tuple(cu_seqlens.shape)}")
+        _ints(cu_seqlens, (B + 1,), "cu_seqlens")
+    shape = (B, Hv, Dk, Dv)
+    if state is not None:
+        _state(state, shape, q.device, "state")
+    if state_out is not None:
+        _state(state_out, shape, q.device, "state_out")
+    if scale is None:
+        scale = Dk ** -0.5
+    elif not -1e30 < scale < 1e30:
+        raise ValueError(f"scale must be finite, got {scale}")
+    _same_device(q.device, k, v, g, beta, state, cu_seqlens, state_out, out)
+    given = out is not None
+    out = _output(out, q, (T, Hv, Dv), "out")
+    if state_out is None:
+        state_out = torch.empty(shape, dtype=torch.float32, device=q.device)
+    elif state is not None:
+        _no_overlap(state_out, state, "state")
+    if B == 0:
+        return out, state_out
+    with _Current(q.device):
+        q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+        if given:
+            for t in (q, k, v, g, beta, state, state_out):
+                if t is not None:
+                    _apart(out, t)
+        n = hb._lib.i4_gated_linear_attention_workspace(T, B, Hk, Hv, Dk, Dv, dt, cu_seqlens is not None,
+                                                        beta is not None)
+        if n < 0:
+            raise ValueError(hb.last_error())
+        work = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None
+        hb._check_rc(hb._lib.i4_gated_linear_attention_dev(
+            q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], g.data_ptr(),
+            g.stride(0), None if beta is None else beta.data_ptr(), 0 if beta is None else beta.stride(0), T, Hk, Hv, Dk,
+            Dv, dt, None if cu_seqlens is None else cu_seqlens.data_ptr(), B, scale,
+            None if state is None else state.data_ptr(), state_out.data_ptr(), out.data_ptr(), *out.stride()[:2],
+            None if work is None else work.data_ptr(), n, hb._torch_stream(q)), "i4_gated_linear_attention_dev")
+    return out, state_out

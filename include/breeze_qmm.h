@@ -255,6 +255,30 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
                            const int32_t* dCu, int B, float scale, void* dOut, int64_t o_token, int64_t o_head,
                            void* dWork, int64_t work_bytes, void* stream);
 
+/* Gated linear attention (the decoder's linear-attention layers,
+ * kernel/qwen35_decoder.cpp:46-121), for each of v_heads heads, with the q and
+ * k of key head i / (v_heads / k_heads):
+ *   S_t = exp(g_t) S_{t-1} + k_t u_t^T,   o_t = scale S_t^T q_t,
+ *   u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t), or v_t where dBeta is NULL.
+ * dQ, dK [T, k_heads, k_dim], dV, dOut [T, v_heads, v_dim] of one type (element
+ * strides per token and head, multiples of four; last dimension contiguous;
+ * 16-byte aligned); dG (logarithms of the decays, at most 0; -infinity drops
+ * the state), dBeta: fp32 [T, v_heads], strides per token.  Sequence b's tokens
+ * are dCu[b] .. dCu[b + 1] - 1 (dCu NULL: token b).  dStateIn (NULL: zeros),
+ * dStateOut (may be dStateIn): fp32 [B, v_heads, k_dim, v_dim]; a sequence
+ * without tokens keeps its state.  k_dim 64 or 128, v_dim a multiple of 16 up
+ * to 1024.  Rows outside every sequence are left as they were.  dWork: as many
+ * bytes as i4_gated_linear_attention_workspace says for the same shapes (0: may
+ * be NULL), 256-byte aligned. */
+int64_t i4_gated_linear_attention_workspace(int T, int B, int k_heads, int v_heads, int k_dim, int v_dim, int dtype,
+                                            int has_cu, int has_beta);
+int i4_gated_linear_attention_dev(const void* dQ, int64_t q_token, int64_t q_head, const void* dK, int64_t k_token,
+                                  int64_t k_head, const void* dV, int64_t v_token, int64_t v_head, const float* dG,
+                                  int64_t g_token, const float* dBeta, int64_t beta_token, int T, int k_heads,
+                                  int v_heads, int k_dim, int v_dim, int dtype, const int32_t* dCu, int B, float scale,
+                                  const float* dStateIn, float* dStateOut, void* dOut, int64_t o_token, int64_t o_head,
+                                  void* dWork, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,3 +94,29 @@ def attend(q, cache, table, kv_lens, q_lens, scale, split):
                 out[start:start + n, h], bound[start:start + n, h] = o, worst + small
         start += n
     return out, bound
+
+
+def recur(q, k, v, g, beta, state, q_lens, scale):
+    """(o, state, size) of the gated recurrence in fp64; size [B, Hv, Dv] is the
+    largest norm of a state's column, or of a token's v there, on the way."""
+    rep = v.shape[1] // k.shape[1]
+    q, k = (x.cpu().double().repeat_interleave(rep, 1) for x in (q, k))
+    v, g = v.cpu().double(), g.cpu().double()
+    Hv, Dk, Dv = v.shape[1], q.shape[2], v.shape[2]
+    o = torch.zeros_like(v)
+    states, sizes, start = [], [], 0
+    for b, n in enumerate(q_lens):
+        S = torch.zeros((Hv, Dk, Dv), dtype=F64) if state is None else state[b].cpu().double()
+        size = S.norm(dim=1)
+        for t in range(start, start + n):
+            S = S * g[t].exp()[:, None, None]
+            u = v[t]
+            if beta is not None:
+                u = beta[t].cpu().double()[:, None] * (u - (k[t][:, None] @ S)[:, 0])
+            S = S + k[t][:, :, None] * u[:, None]
+            o[t] = scale * (q[t][:, None] @ S)[:, 0]
+            size = torch.maximum(size, torch.maximum(S.norm(dim=1), v[t].abs() * k[t].norm(dim=1)[:, None]))
+        states.append(S)
+        sizes.append(size)
+        start += n
+    return o, torch.stack(states), torch.stack(sizes)
