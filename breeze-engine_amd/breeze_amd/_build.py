@@ -14,8 +14,7 @@ CSRC = os.path.join(os.path.dirname(PKG), "csrc")
 # Host code and small kernels; the decode and prefill kernels, one unit per
 # (bits, activation mode) so the device passes run side by side.
 # Then the token mixers (the paged cache, attention over it, gated linear attention).
-MIXERS = ["kv_cache.hip", "paged_attn.hip", "gla.hip"]
-SOURCES = ["qmm.hip", "pf16_w4.hip", "pf16_w8.hip", "pf_w4_i8.hip", *MIXERS] + [f"{k}_w{b}_{m}.hip" for k in ("dec", "pf") for b in (4, 8) for m in ("hp", "lp")]
+SOURCES = ["qmm.hip", "pf16_w4.hip", "pf16_w8.hip", "pf_w4_i8.hip", "kv_cache.hip", "paged_attn.hip", "gla.hip"] + [f"{k}_w{b}_{m}.hip" for k in ("dec", "pf") for b in (4, 8) for m in ("hp", "lp")]
 LIB_NAME = "libbreeze_qmm.so"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -48,9 +47,9 @@ DEVICE_FLAGS = [
     # kernel's first loads do not wait for a kernarg fetch.
     "-mllvm", "-amdgpu-kernarg-preload-count=14",
 ]
-# The token mixers': their accumulators may take the accumulation registers, and
-# their arguments are one structure.
-MIXER_FLAGS = DEVICE_FLAGS[:4]
+# Attention's 128-row workgroups hold more than 256 registers a lane: their
+# accumulators take the accumulation registers.
+ATTN_FLAGS = DEVICE_FLAGS[:4]
 
 
 def lib_path():
@@ -84,7 +83,7 @@ def build(verbose=False):
         objs = [os.path.join(work, f"{i}.o") for i in range(len(srcs))]
         try:
             running = [(_run([HIPCC, "-x", "hip", *FLAGS,
-                              *(MIXER_FLAGS if os.path.basename(s) in MIXERS else DEVICE_FLAGS),
+                              *(ATTN_FLAGS if os.path.basename(s) == "paged_attn.hip" else DEVICE_FLAGS),
                               "--offload-device-only", "-c", s, "-o", fb], verbose), s) for s, fb in zip(srcs, fatbins)]
             finish(running, "device pass")
             running = [(_run([HIPCC, "-x", "hip", *FLAGS, "--offload-host-only", "-Xclang",

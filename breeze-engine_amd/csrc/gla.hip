@@ -10,12 +10,12 @@
 // of C = 64 tokens.  With G_i the sum of a chunk's g up to token i and S_0 the
 // state before it,
 //
-//   (I + A) U = diag(beta) (V - diag(e^G) K S_0),
+//   (I + A) U = diag(beta) (V - diag(e^G) K S_0) = diag(beta) X,
 //   A_ij = beta_i e^{G_i - G_j} (k_i . k_j)  for j < i,
 //   O = scale (diag(e^G) Q S_0 + M U),  M_ij = e^{G_i - G_j} (q_i . k_j)  for j <= i,
 //   S_C = e^{G_C} S_0 + sum_j e^{G_C - G_j} k_j u_j^T.
 //
-// gla_intra_kernel computes T = (I + A)^{-1} and M for all chunks at once;
+// gla_intra_kernel computes T = (I + A)^{-1} diag(beta) and M for all chunks at once;
 // gla_inter_kernel walks a sequence's chunks with S in registers, 16 of its
 // columns a wave.
 //
@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kShort = 16;
+constexpr int kFac = 256;  // 2 * 64 + 3, and what one load to LDS brings
 
 struct GlaArgs {
     const void* q;
@@ -48,12 +49,9 @@ struct GlaArgs {
     const float* s_in;  // [B, Hv, Dk, Dv]; null: zeros
     float* s_out;
     const int32_t* cu;  // null: one token a sequence
-    _Float16* kf;       // [slots][Hk][hi, lo][64][Dk]
-    _Float16* qf;
-    _Float16* tf;  // [slots][Hv][hi, lo][64][64]
-    _Float16* mf;
-    float* unit;  // [slots][Hk][2]: what one unit of kf and of qf is worth
-    float* fac;   // [slots][Hv][4][64]: e^G, beta, e^{G_C - G}, worth of a unit of T's row
+    uint8_t* kq;        // [slots][Hk]: operands of k (hi, lo), then of q
+    uint8_t* tm;        // [slots][Hv]: operands of M (hi, lo), then of T
+    float* fac;   // [slots][Hv][kFac]: e^G, e^{G_C - G}, what a unit of T's, k's and q's operands is worth
     int T, B, Hk, Hv, rep, Dv, dt, nslots;
     int nshort;  // sequences of up to this many tokens are gla_step_kernel's
     float scale;
@@ -68,14 +66,22 @@ __device__ inline Span span_of(const GlaArgs& a, int b) {
     return {q0, q1 - q0};
 }
 
-__device__ inline float load1(const void* p, int dt, int64_t i) {
-    if (dt == kF32) return static_cast<const float*>(p)[i];
-    const uint16_t w = static_cast<const uint16_t*>(p)[i];
-    return dt == kBF16 ? bits_f((uint32_t)w << 16) : (float)__builtin_bit_cast(_Float16, w);
+// One element as it is stored, and its value.
+template <int DT>
+__device__ inline uint32_t raw1(const void* p, int64_t i) {
+    if constexpr (DT == kF32) return static_cast<const uint32_t*>(p)[i];
+    else return static_cast<const uint16_t*>(p)[i];
 }
-__device__ inline void store1(void* p, int dt, int64_t i, float x) {
-    if (dt == kF32) static_cast<float*>(p)[i] = x;
-    else if (dt == kBF16) static_cast<uint16_t*>(p)[i] = (uint16_t)to_bf16(x);
+template <int DT>
+__device__ inline float value1(uint32_t w) {
+    if constexpr (DT == kF32) return bits_f(w);
+    else if constexpr (DT == kBF16) return bits_f(w << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+}
+template <int DT>
+__device__ inline void store1(void* p, int64_t i, float x) {
+    if constexpr (DT == kF32) static_cast<float*>(p)[i] = x;
+    else if constexpr (DT == kBF16) static_cast<uint16_t*>(p)[i] = (uint16_t)to_bf16(x);
     else static_cast<uint16_t*>(p)[i] = __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
@@ -88,7 +94,7 @@ __device__ inline float clean_g(float g) { return g < -1e4f ? -1e4f : g; }
 // A wave for 16 columns of one sequence's and head's state: lane (row r mod 16,
 // four columns).  Before the update both S^T k and S^T q are summed over the
 // rows, since S_t^T q = e^g S_{t-1}^T q + (k . q) u: one exchange a token.
-template <int DK>
+template <int DK, int DT>
 __global__ __launch_bounds__(256) void gla_step_kernel(GlaArgs a) {
     constexpr int R = DK / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -109,10 +115,10 @@ __global__ __launch_bounds__(256) void gla_step_kernel(GlaArgs a) {
         f4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            kv[i] = load1(a.k, a.dt, t * a.k_token + hk * a.k_head + r0 + 16 * i);
-            qv[i] = load1(a.q, a.dt, t * a.q_token + hk * a.q_head + r0 + 16 * i);
+            kv[i] = value1<DT>(raw1<DT>(a.k, t * a.k_token + hk * a.k_head + r0 + 16 * i));
+            qv[i] = value1<DT>(raw1<DT>(a.q, t * a.q_token + hk * a.q_head + r0 + 16 * i));
         }
-        const f4 v = load4(a.v, a.dt, t * a.v_token + hv * a.v_head + col);
+        const f4 v = load4(a.v, DT, t * a.v_token + hv * a.v_head + col);
         const float decay = expf(clean_g(a.g[t * a.g_token + hv]));
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -147,7 +153,7 @@ __global__ __launch_bounds__(256) void gla_step_kernel(GlaArgs a) {
         for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) S[i][j] = __builtin_fmaf(kv[i], u[j], S[i][j]);
-        if (r0 == 0) store4(a.o, a.dt, t * a.o_token + hv * a.o_head + col, o);
+        if (r0 == 0) store4(a.o, DT, t * a.o_token + hv * a.o_head + col, o);
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) *reinterpret_cast<f4*>(a.s_out + at + (int64_t)(r0 + 16 * i) * a.Dv + col) = S[i];
@@ -183,17 +189,51 @@ __device__ inline bool chunk_of(const GlaArgs& a, int slot, int& tok, int& n) {
     return sp.n > a.nshort && c >= 0 && n > 0;
 }
 
+typedef __attribute__((address_space(3))) s4* lds_s4;
+__device__ inline h4 read_tr(const void* p) {
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p)));
+}
+__device__ inline h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+// Columns 4 c + 0..3 and 16 + 4 c + 0..3 of a row, from its column 4 c.
+__device__ inline h8 read_rows(const _Float16* p) {
+    return join(*reinterpret_cast<const h4*>(p), *reinterpret_cast<const h4*>(p + 16));
+}
+
+// Operands between the kernels.  A 16 x 32 operand of the matrix instruction is
+// 1 KB, 16 bytes a lane (row r, quarter c): columns 4 c + 0..3 and 16 + 4 c +
+// 0..3, the order in which a result's rows come as the other operand.  Lane
+// (r, c)'s 16 bytes lie at place 16 c + (r ^ 4 (c & 1)), which also lets the
+// transposed reads of k for the state's update touch twice the banks.
+__device__ inline int place(int r, int c) { return 16 * c + (r ^ ((c & 1) << 2)); }
+
+// T and M are lower triangular: row tile t has column slabs 0 .. t / 2, six
+// operands in all.
+constexpr int kTri = 6;
+constexpr int kTriBytes = kTri * 1024;
+__host__ __device__ constexpr int tri(int t, int s) { return t + (t == 3) + s; }
+
+constexpr int kq_bytes(int dk, bool lo) { return 2 * (lo ? 2 : 1) * 4 * (dk / 32) * 1024; }
+constexpr int tm_bytes(bool delta) { return (delta ? 4 : 2) * kTriBytes; }
+
 // One workgroup for a chunk and a key head: the products k_i . k_j and
 // q_i . k_j once, then T and M for each of its value heads.
-template <int DK, bool LO, bool DELTA>
-__global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
-    constexpr int KS = DK + 8, AS = kChunk + 4, L = DK / 4, NP = kChunk * L / 256;
+template <int DK, int DT, bool DELTA>
+__global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
+    constexpr bool LO = DT == kF32;  // two terms of q and k
+    constexpr int KS = DK + 8, AS = kChunk + 4, L = DK / 4, NP = kChunk * L / 256, SS = DK / 32;
     constexpr int NT = LO ? 2 : 1;
-    __shared__ __align__(16) _Float16 sk[NT][kChunk * KS], sq[NT][kChunk * KS];
-    __shared__ __align__(16) float sa[kChunk * AS], st[kChunk * AS], sm[kChunk * AS];
+    constexpr int kIn = 2 * NT * kChunk * KS * 2, kOut = (DELTA ? 3 : 1) * kChunk * AS * 4;
+    __shared__ __align__(16) uint8_t lds[kIn > kOut ? kIn : kOut];
     __shared__ double sg[kChunk];
-    __shared__ float sbeta[kChunk];
+    __shared__ __align__(16) float sbeta[kChunk];
     __shared__ uint32_t stop[2][4];
+    _Float16* const in = reinterpret_cast<_Float16*>(lds);  // k hi, k lo, q hi, q lo
+    _Float16* const sk = in;
+    _Float16* const sq = in + NT * kChunk * KS;
+    constexpr int kLow = (NT - 1) * kChunk * KS;
+    float* const sm = reinterpret_cast<float*>(lds);  // once the products are done
+    float* const sa = sm + kChunk * AS;
+    float* const st = sa + kChunk * AS;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % a.Hk, slot = blockIdx.x / a.Hk;
@@ -206,11 +246,13 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int row = (tid + 256 * i) / L, d = 4 * (tid % L);
-        kx[i] = qx[i] = (f4){0, 0, 0, 0};
-        if (row < n) {
-            kx[i] = load4(a.k, a.dt, (int64_t)(tok + row) * a.k_token + hk * a.k_head + d);
-            qx[i] = load4(a.q, a.dt, (int64_t)(tok + row) * a.q_token + hk * a.q_head + d);
-        }
+        const int64_t at = tok + min(row, n - 1);
+        kx[i] = load4(a.k, DT, at * a.k_token + hk * a.k_head + d);
+        qx[i] = load4(a.q, DT, at * a.q_token + hk * a.q_head + d);
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        if ((tid + 256 * i) / L >= n) kx[i] = qx[i] = (f4){0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t x = abs_bits(kx[i][j]), y = abs_bits(qx[i][j]);
@@ -235,10 +277,6 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
     }
     const float kup = to_top<3>(kt), qup = to_top<3>(qt), kunit = inverse_pow2(kup), qunit = inverse_pow2(qup);
     const int64_t ck = (int64_t)slot * a.Hk + hk;
-    if (tid == 0) {
-        a.unit[2 * ck] = kunit;
-        a.unit[2 * ck + 1] = qunit;
-    }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int row = (tid + 256 * i) / L, d = 4 * (tid % L);
@@ -248,20 +286,27 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = w ? qx[i][j] * qup : kx[i][j] * kup;
             const h4 hi = __builtin_convertvector(x, h4);
-            _Float16* s = w ? sq[0] : sk[0];
-            _Float16* out = (w ? a.qf : a.kf) + ck * (NT * kChunk * DK) + row * DK + d;
-            *reinterpret_cast<h4*>(s + row * KS + d) = hi;
-            *reinterpret_cast<h4*>(out) = hi;
+            _Float16* s = (w ? sq : sk) + row * KS + d;
+            *reinterpret_cast<h4*>(s) = hi;
             if constexpr (LO) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] -= (float)hi[j];
-                const h4 lo = __builtin_convertvector(x, h4);
-                *reinterpret_cast<h4*>((w ? sq[NT - 1] : sk[NT - 1]) + row * KS + d) = lo;
-                *reinterpret_cast<h4*>(out + kChunk * DK) = lo;
+                *reinterpret_cast<h4*>(s + kLow) = __builtin_convertvector(x, h4);
             }
         }
     }
     __syncthreads();
+
+    // The other kernel's operands of k and q.
+    {
+        h8* out = reinterpret_cast<h8*>(a.kq + ck * kq_bytes(DK, LO));
+#pragma unroll
+        for (int i = 0; i < 2 * NT * 4 * SS / 4; ++i) {
+            const int f = 4 * i + wave, part = f / (4 * SS), t = f % (4 * SS) / SS, s = f % SS;
+            const int c = lane >> 4, r = (lane & 15) ^ ((c & 1) << 2);
+            out[f * 64 + lane] = read_rows(in + part * kChunk * KS + (16 * t + r) * KS + 32 * s + 4 * c);
+        }
+    }
 
     // Wave w: rows 16 w ..; columns up to them.
     const int r16 = lane & 15, c = lane >> 4;
@@ -269,19 +314,19 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) kk[t] = qk[t] = (f4){0, 0, 0, 0};
 #pragma unroll
-    for (int s = 0; s < DK / 32; ++s) {
+    for (int s = 0; s < SS; ++s) {
         const int ar = (16 * wave + r16) * KS + 32 * s + 8 * c;
-        const h8 ak = *reinterpret_cast<const h8*>(sk[0] + ar), aq = *reinterpret_cast<const h8*>(sq[0] + ar);
-        const h8 akl = *reinterpret_cast<const h8*>(sk[NT - 1] + ar), aql = *reinterpret_cast<const h8*>(sq[NT - 1] + ar);
+        const h8 ak = *reinterpret_cast<const h8*>(sk + ar), aq = *reinterpret_cast<const h8*>(sq + ar);
+        const h8 akl = *reinterpret_cast<const h8*>(sk + kLow + ar), aql = *reinterpret_cast<const h8*>(sq + kLow + ar);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             if (t > wave) continue;
             const int br = (16 * t + r16) * KS + 32 * s + 8 * c;
-            const h8 b = *reinterpret_cast<const h8*>(sk[0] + br);
+            const h8 b = *reinterpret_cast<const h8*>(sk + br);
             if constexpr (DELTA) kk[t] = mfma16(ak, b, kk[t]);
             qk[t] = mfma16(aq, b, qk[t]);
             if constexpr (LO) {
-                const h8 bl = *reinterpret_cast<const h8*>(sk[NT - 1] + br);
+                const h8 bl = *reinterpret_cast<const h8*>(sk + kLow + br);
                 if constexpr (DELTA) kk[t] = mfma16(akl, b, mfma16(ak, bl, kk[t]));
                 qk[t] = mfma16(aql, b, mfma16(aq, bl, qk[t]));
             }
@@ -291,7 +336,7 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
     for (int r = 0; r < a.rep; ++r) {
         const int hv = hk * a.rep + r;
         const int64_t cv = (int64_t)slot * a.Hv + hv;
-        float* fac = a.fac + cv * (4 * kChunk);
+        float* fac = a.fac + cv * kFac;
         if (wave == 0) {
             const bool is = lane < n;
             double G = is ? (double)clean_g(a.g[(int64_t)(tok + lane) * a.g_token + hv]) : 0.0;
@@ -305,11 +350,10 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
             sg[lane] = G;
             sbeta[lane] = be;
             fac[lane] = expf((float)G);
-            fac[kChunk + lane] = be;
-            fac[2 * kChunk + lane] = expf((float)(__shfl(G, 63) - G));
+            fac[kChunk + lane] = expf((float)(__shfl(G, 63) - G));
         }
-        __syncthreads();
-        // A and M, the blocks past the diagonal as zeros.
+        __syncthreads();  // the first time, the products' operands are read too
+        // A and M; the blocks past the diagonal that an operand reaches into are zeros.
         {
             double gi[4];
             float bi[4];
@@ -320,16 +364,19 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
+                if (t > (wave | 1)) continue;
                 const int j = 16 * t + r16;
                 const double gj = sg[j];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 16 * wave + 4 * c + e;
                     float av = 0.0f, mv = 0.0f;
-                    if (j <= i) {
+                    if (t <= wave) {
                         const float x = expf((float)(gi[e] - gj));
-                        mv = x * qk[t][e];
+                        mv = j <= i ? x * qk[t][e] : 0.0f;
                         av = j < i ? bi[e] * x * kk[t][e] : 0.0f;
+                    } else if (DELTA) {
+                        st[i * AS + j] = 0.0f;
                     }
                     sm[i * AS + j] = mv;
                     if constexpr (DELTA) sa[i * AS + j] = av;
@@ -337,6 +384,7 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
             }
         }
         __syncthreads();
+        float tup = 1.0f;
         if constexpr (DELTA) {
             // The four blocks on the diagonal: a lane solves one column of one.
             if (wave == 0) {
@@ -379,269 +427,461 @@ __global__ __launch_bounds__(256) void gla_intra_kernel(GlaArgs a) {
                 }
             }
             __syncthreads();
-        }
-        // Out as two fp16 terms: four lanes a row, sixteen values each.
-        const int row = tid >> 2, q4 = 16 * (tid & 3);
-        const bool past = q4 > (row & ~15);
-#pragma unroll
-        for (int w = 0; w < (DELTA ? 2 : 1); ++w) {
-            const float* src = (w ? st : sm) + row * AS + q4;
-            float x[16];
+            // T diag(beta), its largest value to [2^12, 2^13).
+            const int row = tid >> 2, q4 = 16 * (tid & 3);
             uint32_t top = 0;
+            if (q4 <= row)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[j] = past ? 0.0f : src[j];
-                top = max(top, abs_bits(x[j]));
-            }
-            if (w) {
-                top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-                top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-                const float up = to_top<12>(top);
-                if (q4 == 0) fac[3 * kChunk + row] = inverse_pow2(up);
+                for (int j = 0; j < 16; j += 4) {
+                    const f4 x = *reinterpret_cast<const f4*>(st + row * AS + q4 + j);
+                    const f4 be = *reinterpret_cast<const f4*>(sbeta + q4 + j);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] *= up;
-            }
-            _Float16* out = (w ? a.tf : a.mf) + cv * (2 * kChunk * kChunk) + row * kChunk + q4;
-#pragma unroll
-            for (int j = 0; j < 16; j += 8) {
-                h8 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    hi[e] = (_Float16)x[j + e];
-                    lo[e] = (_Float16)(x[j + e] - (float)hi[e]);
+                    for (int e = 0; e < 4; ++e) top = max(top, abs_bits(x[e] * be[e]));
                 }
-                *reinterpret_cast<h8*>(out + j) = hi;
-                *reinterpret_cast<h8*>(out + kChunk * kChunk + j) = lo;
-            }
+#pragma unroll
+            for (int s = 1; s < 64; s *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+            if (lane == 0) stop[0][wave] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = max(top, stop[0][w]);
+            tup = to_top<12>(top);
+            if (tid == 0) fac[2 * kChunk] = inverse_pow2(tup);
         }
+        if (tid == 0) {
+            fac[2 * kChunk + 1] = kunit;
+            fac[2 * kChunk + 2] = qunit;
+        }
+        // Out as operands of two terms.
+        h8* out = reinterpret_cast<h8*>(a.tm + cv * tm_bytes(DELTA));
+#pragma unroll
+        for (int w = 0; w < (DELTA ? 2 : 1); ++w)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int f = 4 * i + wave;
+                if (f >= kTri) continue;
+                const int t = f < 2 ? f : f < 4 ? 2 : 3, s = f - tri(t, 0);
+                const int cc = lane >> 4, rr = (lane & 15) ^ ((cc & 1) << 2);
+                const float* p = (w ? st : sm) + (16 * t + rr) * AS + 32 * s + 4 * cc;
+                f4 x = *reinterpret_cast<const f4*>(p), y = *reinterpret_cast<const f4*>(p + 16);
+                if (w) {
+                    x *= *reinterpret_cast<const f4*>(sbeta + 32 * s + 4 * cc) * tup;
+                    y *= *reinterpret_cast<const f4*>(sbeta + 32 * s + 16 + 4 * cc) * tup;
+                }
+                const h4 xh = __builtin_convertvector(x, h4), yh = __builtin_convertvector(y, h4);
+                const f4 xl = x - __builtin_convertvector(xh, f4), yl = y - __builtin_convertvector(yh, f4);
+                out[(2 * kTri * w + f) * 64 + lane] = join(xh, yh);
+                out[(2 * kTri * w + kTri + f) * 64 + lane] =
+                    join(__builtin_convertvector(xl, h4), __builtin_convertvector(yl, h4));
+            }
         __syncthreads();
     }
 }
 
 // ------------------------------------------------------------------ from chunk to chunk
 
-// Values in a result's layout (rows 16 t + 4 c + e, one column a lane) as the
-// operand of a contraction over those rows, two fp16 terms scaled for the
-// column; returns what a unit is worth.  Slab s holds tiles 2 s and 2 s + 1.
-template <int NT>
-__device__ inline float to_operand(const f4* x, h8* hi, h8* lo) {
-    uint32_t top = 0;
+// The largest magnitude of a column that four lanes hold (rows 16 t + 4 c + e).
+template <int N>
+__device__ inline float column_top(const f4* x) {
+    float top = 0.0f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < N; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, abs_bits(x[t][e]));
-    top = f_bits(max_halves(max_rows16(bits_f(top))));  // magnitudes order as their bits do
-    const float up = to_top<12>(top);
+        for (int e = 0; e < 4; e += 2) top = fmaxf(fmaxf(top, __builtin_fabsf(x[t][e])), __builtin_fabsf(x[t][e + 1]));
+    return max_halves(max_rows16(top));
+}
+
+// x p and y q as two fp16 terms: each is one instruction, which multiplies,
+// subtracts the first term in fp32 and rounds.
+__device__ inline void two_terms(float x, float y, float p, float q, uint32_t& hi, uint32_t& lo) {
+    uint32_t h, l;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(x), "v"(p));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(y), "v"(q));
+    asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x), "v"(p), "v"(h));
+    asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(y), "v"(q), "v"(h));
+    hi = h;
+    lo = l;
+}
+
+// Values in a result's layout times `up` (times `rows`' factor for their row)
+// as the operand of a contraction over those rows.  Slab s holds tiles 2 s and
+// 2 s + 1.
+template <int N>
+__device__ inline void to_operand(const f4* x, float up, const float* rows, int c, h8* hi, h8* lo) {
 #pragma unroll
-    for (int s = 0; s < NT / 2; ++s)
+    for (int s = 0; s < N / 2; ++s) {
+        u4 h, l;
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const f4 v = x[2 * s + (j >> 2)];
-            const float p = v[j & 3] * up, q = v[(j & 3) + 1] * up;
-            const h2 a = to_h2(p, q);
-            const h2 b = to_h2(p - (float)a[0], q - (float)a[1]);
-            hi[s][j] = a[0];
-            hi[s][j + 1] = a[1];
-            lo[s][j] = b[0];
-            lo[s][j + 1] = b[1];
+        for (int j = 0; j < 2; ++j) {
+            const f4 v = x[2 * s + j];
+            f4 f = {up, up, up, up};
+            if (rows) f *= *reinterpret_cast<const f4*>(rows + 16 * (2 * s + j) + 4 * c);
+            uint32_t a, b;
+            two_terms(v[0], v[1], f[0], f[1], a, b);
+            h[2 * j] = a;
+            l[2 * j] = b;
+            two_terms(v[2], v[3], f[2], f[3], a, b);
+            h[2 * j + 1] = a;
+            l[2 * j + 1] = b;
         }
-    return inverse_pow2(up);
+        hi[s] = __builtin_bit_cast(h8, h);
+        lo[s] = __builtin_bit_cast(h8, l);
+    }
 }
 
-typedef __attribute__((address_space(3))) s4* lds_s4;
-__device__ inline h4 read_tr(const _Float16* p) {
-    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p)));
+// 16 bytes a lane from `src` to LDS at `lds` + 16 * lane.  The compiler does not
+// see the load: its reader waits for it by hand.
+__device__ inline void load_lds(const uint8_t* src, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds) : "memory");
 }
-__device__ inline h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
-// The operand whose contraction index runs in a result's order: 4 c + 0..3, 16 + 4 c + 0..3.
-__device__ inline h8 read_rows(const _Float16* p) {
-    return join(*reinterpret_cast<const h4*>(p), *reinterpret_cast<const h4*>(p + 16));
+__device__ inline uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(p);
+}
+template <int N>
+__device__ inline void wait_loads() {  // vmcnt(N)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <int DK, bool LO, bool DELTA>
+// A lower triangular factor (T or M) times 16 columns, both of two terms.
+__device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, const h8* xl, f4* acc) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 0)], xh[0], (f4){0, 0, 0, 0});
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 0)], xl[0], acc[t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = mfma16(lo[tri(t, 0)], xh[0], acc[t]);
+#pragma unroll
+    for (int t = 2; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 1)], xh[1], acc[t]);
+#pragma unroll
+    for (int t = 2; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 1)], xl[1], acc[t]);
+#pragma unroll
+    for (int t = 2; t < 4; ++t) acc[t] = mfma16(lo[tri(t, 1)], xh[1], acc[t]);
+}
+
+// Four waves for 32 columns of a head's state: two carry 16 columns each from
+// chunk to chunk (K S, T X, the state's update), and each hands its operands to
+// one of the other two, which computes the rows of O and brings the next
+// chunk's operands of k and q to LDS.  A wave of each kind a SIMD: what one
+// waits for, its own next product, the other does not.
+//
+// Bound by the chain through the state: per chunk 114 matrix instructions
+// (1,824 cycles of fp32 calls) and about as much in conversions, exchanges of
+// column maxima and LDS reads between them.  All eight products in one wave
+// and 64 columns a workgroup took 5.0 us a chunk (the LDS reads of four waves,
+// 480 KB, alone 1.6).
+template <int DK, int DT, bool DELTA>
 __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
-    constexpr int KS = DK + 8, TS = kChunk + 8, NT = LO ? 2 : 1;
-    constexpr int NK = NT * kChunk * DK / 8 / 256, NM = 2 * kChunk * kChunk / 8 / 256;
-    constexpr int ST = DK / 16, SS = DK / 32;  // tiles and slabs of the state's rows
-    __shared__ __align__(16) _Float16 sk[NT][kChunk * KS], sq[NT][kChunk * KS];
-    __shared__ __align__(16) _Float16 sm[2][kChunk * TS], stt[2][DELTA ? kChunk * TS : 8];
-    __shared__ __align__(16) float sf[4][kChunk];
+    constexpr bool LO = DT == kF32;
+    constexpr int NT = LO ? 2 : 1, ST = DK / 16, SS = DK / 32;  // tiles and slabs of the state's rows
+    constexpr int kPart = 4 * SS * 1024, kBuf = kq_bytes(DK, LO);
+    __shared__ __align__(1024) uint8_t skq[2][kBuf];       // operands of k, then of q
+    __shared__ __align__(1024) uint8_t ss[2][2 * SS * 1024];  // the state's operands, hi and lo
+    __shared__ __align__(1024) uint8_t su[2][4 * 1024];       // U's
+    __shared__ __align__(1024) float sf[2][kFac];
+    __shared__ float sunits[2][2][16];  // what a unit of those is worth, for each column
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r16 = lane & 15, c = lane >> 4;
-    const int blocks = (a.Dv + 63) / 64;
-    const int cb = blockIdx.x % blocks, hv = blockIdx.x / blocks % a.Hv, b = blockIdx.x / blocks / a.Hv;
+    const int pair = wave & 1, r16 = lane & 15, c = lane >> 4;
+    // A head's workgroups are B * Hv apart: on one XCD, whose L2 then holds what they share, wherever 8 divides that.
+    const int heads = a.B * a.Hv, cb = blockIdx.x / heads, hv = blockIdx.x % heads % a.Hv, b = blockIdx.x % heads / a.Hv;
     const Span sp = span_of(a, b);
     if (sp.n <= a.nshort) return;
-    const int hk = hv / a.rep, col0 = 64 * cb + 16 * wave, col = col0 + r16;
+    const int hk = hv / a.rep, col0 = 32 * cb + 16 * pair;
     const bool mine = col0 < a.Dv;  // 16 columns are there or not, for the whole wave
+    const int col = (mine ? col0 : 0) + r16;
     const int nchunk = (sp.n + kChunk - 1) / kChunk, slot0 = sp.q0 / kChunk + b;
     const int64_t at = ((int64_t)b * a.Hv + hv) * DK * a.Dv + col;
+    const int rd = 16 * place(r16, c);  // where the lane's 16 bytes of an operand lie
+    const auto op = [&](const uint8_t* base, int f) { return *reinterpret_cast<const h8*>(base + 1024 * f + rd); };
+    const auto tm_of = [&](int ch) { return a.tm + ((int64_t)(slot0 + ch) * a.Hv + hv) * tm_bytes(DELTA); };
 
-    f4 S[ST];
+    if (wave >= 2) {  // ---------------------------------------------------- the rows of O
+        // k's and q's operands and the factors of chunk ch, on their way.
+        const auto fetch = [&](int ch, int part) {  // a quarter of them
+            const uint8_t* src = a.kq + ((int64_t)(slot0 + ch) * a.Hk + hk) * kBuf + 1024 * pair + 16 * lane;
+            const uint32_t dst = lds_address(skq[ch & 1]) + 1024 * pair;
+#pragma unroll
+            for (int i = 0; i < kBuf / 8192; ++i)
+                load_lds(src + 2048 * (4 * i + part), dst + 2048 * (4 * i + part));
+            if (pair == 0 && part == 0)
+                load_lds(reinterpret_cast<const uint8_t*>(a.fac + ((int64_t)(slot0 + ch) * a.Hv + hv) * kFac) + 16 * lane,
+                         lds_address(sf[ch & 1]));
+        };
+        f4 y[4];
+        const auto store = [&](int ch, bool full) {
+            const int first = kChunk * ch + 4 * c;
+            const int64_t p = (int64_t)(sp.q0 + first) * a.o_token + hv * a.o_head + col;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (full || first + 16 * t + e < sp.n) store1<DT>(a.o, p + (16 * t + e) * a.o_token, y[t][e]);
+        };
+        if (nchunk > 0)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fetch(0, i);
+        wait_loads<0>();
+        __syncthreads();
+        for (int ch = 0; ch < nchunk; ++ch) {
+            h8 mh[kTri], ml[kTri];
+            const h8* mp = reinterpret_cast<const h8*>(tm_of(ch));
+#pragma unroll
+            for (int f = 0; f < kTri; ++f) {
+                mh[f] = mp[64 * f + rd / 16];
+                ml[f] = mp[64 * (kTri + f) + rd / 16];
+            }
+            // Q S: the operands of one slab are read while those of the one before it are multiplied.
+            const uint8_t* const qb = skq[ch & 1] + NT * kPart;
+            f4 qs[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) qs[t] = (f4){0, 0, 0, 0};
+            h8 oh[2][4], ol[2][4], sh[2], sl[2];
+            const auto get = [&](int s) {
+                sh[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * s + 16 * lane);
+                sl[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    oh[s & 1][t] = op(qb, t * SS + s);
+                    if constexpr (LO) ol[s & 1][t] = op(qb + kPart, t * SS + s);
+                }
+            };
+            get(0);
+#pragma unroll
+            for (int s = 0; s < SS; ++s) {
+                if (s + 1 < SS) get(s + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) qs[t] = mfma16(oh[s & 1][t], sh[s & 1], qs[t]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) qs[t] = mfma16(oh[s & 1][t], sl[s & 1], qs[t]);
+                if constexpr (LO)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) qs[t] = mfma16(ol[s & 1][t], sh[s & 1], qs[t]);
+                if (ch + 1 < nchunk)
+#pragma unroll
+                    for (int i = 4 * s / SS; i < 4 * (s + 1) / SS; ++i) fetch(ch + 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const float* const fac = sf[ch & 1];
+            const float w1 = fac[2 * kChunk + 2] * sunits[0][pair][r16] * a.scale;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const f4 eg = *reinterpret_cast<const f4*>(fac + 16 * t + 4 * c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qs[t][e] *= eg[e] * w1;
+            }
+            const float w2 = fac[2 * kChunk + 1] * fac[2 * kChunk + 2] * a.scale;
+            __syncthreads();  // U is there
+            h8 uh[2], ul[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                uh[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * s + 16 * lane);
+                ul[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * (2 + s) + 16 * lane);
+            }
+            const float w3 = w2 * sunits[1][pair][r16];
+            f4 acc[4];
+            tri_product(mh, ml, uh, ul, acc);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[t][e] = __builtin_fmaf(acc[t][e], w3, qs[t][e]);
+            // The stores come last and stay on their way; the loads before them are waited for.
+            if (ch + 1 < nchunk) {
+                if (mine) {
+                    store(ch, true);
+                    wait_loads<16>();
+                } else {
+                    wait_loads<0>();
+                }
+            } else if (mine) {
+                store(ch, sp.n == kChunk * nchunk);
+            }
+            __syncthreads();  // the next state is there, and the next chunk's operands
+        }
+        return;
+    }
+
+    // ------------------------------------------------------------------ the state
+    f4 S[ST];  // the state is S times sworth
+    float sworth = 1.0f;
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            S[t][e] = mine && a.s_in ? a.s_in[at + (int64_t)(16 * t + 4 * c + e) * a.Dv] : 0.0f;
+        for (int e = 0; e < 4; ++e) S[t][e] = 0.0f;
+    if (a.s_in)
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[t][e] = a.s_in[at + (int64_t)(16 * t + 4 * c + e) * a.Dv];
 
-    u4 kr[NK], qr[NK], mr[NM], tr[DELTA ? NM : 1];
-    float fr, ku, qu;
-    f4 v[4];
-    const auto load = [&](int ch) {
-        const int64_t ck = (int64_t)(slot0 + ch) * a.Hk + hk, cv = (int64_t)(slot0 + ch) * a.Hv + hv;
-        const u4* kp = reinterpret_cast<const u4*>(a.kf + ck * (NT * kChunk * DK));
-        const u4* qp = reinterpret_cast<const u4*>(a.qf + ck * (NT * kChunk * DK));
-        const u4* mp = reinterpret_cast<const u4*>(a.mf + cv * (2 * kChunk * kChunk));
-        const u4* tp = reinterpret_cast<const u4*>(a.tf + cv * (2 * kChunk * kChunk));
+    uint32_t v[4][4];
+    const auto load_v = [&](int ch) {
+        const int first = kChunk * ch + 4 * c;
+        if (kChunk * (ch + 1) <= sp.n) {
+            const int64_t p = (int64_t)(sp.q0 + first) * a.v_token + hv * a.v_head + col;
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            kr[i] = kp[tid + 256 * i];
-            qr[i] = qp[tid + 256 * i];
-        }
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < NM; ++i) {
-            mr[i] = mp[tid + 256 * i];
-            if constexpr (DELTA) tr[i] = tp[tid + 256 * i];
+                for (int e = 0; e < 4; ++e) v[t][e] = raw1<DT>(a.v, p + (16 * t + e) * a.v_token);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[t][e] = raw1<DT>(a.v, (int64_t)(sp.q0 + min(first + 16 * t + e, sp.n - 1)) * a.v_token +
+                                                hv * a.v_head + col);
         }
-        fr = a.fac[cv * (4 * kChunk) + tid];
-        ku = a.unit[2 * ck];
-        qu = a.unit[2 * ck + 1];
+    };
+    h8 th[kTri], tl[kTri];
+    const auto load_t = [&](int ch) {
+        const h8* tp = reinterpret_cast<const h8*>(tm_of(ch) + 2 * kTriBytes);
+#pragma unroll
+        for (int f = 0; f < kTri; ++f) {
+            th[f] = tp[64 * f + rd / 16];
+            tl[f] = tp[64 * (kTri + f) + rd / 16];
+        }
+    };
+    h8 sh[SS], sl[SS];
+    float sunit;
+    const auto hand_over = [&]() {
+        const float up = to_top<12>(f_bits(column_top<ST>(S)));
+        sunit = inverse_pow2(up) * sworth;
+        to_operand<ST>(S, up, nullptr, c, sh, sl);
+#pragma unroll
+        for (int s = 0; s < SS; ++s) {
+            *reinterpret_cast<h8*>(ss[pair] + 1024 * s + 16 * lane) = sh[s];
+            *reinterpret_cast<h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane) = sl[s];
+        }
+        if (c == 0) sunits[0][pair][r16] = sunit;
+    };
+    if (nchunk > 0) {
+        load_v(0);
+        if constexpr (DELTA) load_t(0);
+    }
+    hand_over();
+    __syncthreads();
+
+    // The transposed reads: key 4 c + r16 / 4 of a tile, values 4 (r16 & 3) + 0..3 of 16.
+    const int rt = 16 * place(4 * c + (r16 >> 2), r16 & 3);
+    for (int ch = 0; ch < nchunk; ++ch) {
+        const uint8_t* const kb = skq[ch & 1];
+        const float* const fac = sf[ch & 1];
+        const float kunit = fac[2 * kChunk + 1];
+        f4 u[4];  // U is u times uworth
+        float uworth = 1.0f;
+        f4 x[4];
+        const int left = sp.n - kChunk * ch - 4 * c;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = kChunk * ch + 16 * t + 4 * c + e;
-                v[t][e] = mine && i < sp.n ? load1(a.v, a.dt, (int64_t)(sp.q0 + i) * a.v_token + hv * a.v_head + col) : 0.0f;
+            for (int e = 0; e < 4; ++e) x[t][e] = 16 * t + e < left ? value1<DT>(v[t][e]) : 0.0f;
+        if constexpr (DELTA) {
+            f4 ks[4], eg[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                ks[t] = (f4){0, 0, 0, 0};
+                eg[t] = *reinterpret_cast<const f4*>(fac + 16 * t + 4 * c);
             }
-    };
-    load(0);
-
-    for (int ch = 0; ch < nchunk; ++ch) {
-        __syncthreads();
+            h8 oh[2][4], ol[2][4];
+            const auto get = [&](int s) {
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            constexpr int per = DK / 8;
-            const int x = tid + 256 * i, row = x / per, half = row / kChunk;
-            *reinterpret_cast<u4*>(sk[half] + (row % kChunk) * KS + 8 * (x % per)) = kr[i];
-            *reinterpret_cast<u4*>(sq[half] + (row % kChunk) * KS + 8 * (x % per)) = qr[i];
-        }
-#pragma unroll
-        for (int i = 0; i < NM; ++i) {
-            const int x = tid + 256 * i, row = x / 8, half = row / kChunk;
-            *reinterpret_cast<u4*>(sm[half] + (row % kChunk) * TS + 8 * (x % 8)) = mr[i];
-            if constexpr (DELTA) *reinterpret_cast<u4*>(stt[half] + (row % kChunk) * TS + 8 * (x % 8)) = tr[i];
-        }
-        sf[tid >> 6][tid & 63] = fr;
-        const float kunit = ku, qunit = qu;
-        f4 x[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = v[t];
-        __syncthreads();
-        if (ch + 1 < nchunk) load(ch + 1);
-
-        // K S and Q S.
-        h8 sh[SS], sl[SS];
-        const float sunit = to_operand<ST>(S, sh, sl);
-        f4 ks[4], qs[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            ks[t] = qs[t] = (f4){0, 0, 0, 0};
+                for (int t = 0; t < 4; ++t) {
+                    oh[s & 1][t] = op(kb, t * SS + s);
+                    if constexpr (LO) ol[s & 1][t] = op(kb + kPart, t * SS + s);
+                }
+            };
+            get(0);
 #pragma unroll
             for (int s = 0; s < SS; ++s) {
-                const int p = (16 * t + r16) * KS + 32 * s + 4 * c;
-                const h8 qh = read_rows(sq[0] + p);
-                qs[t] = mfma16(qh, sl[s], mfma16(qh, sh[s], qs[t]));
-                if constexpr (LO) qs[t] = mfma16(read_rows(sq[NT - 1] + p), sh[s], qs[t]);
-                if constexpr (DELTA) {
-                    const h8 kh = read_rows(sk[0] + p);
-                    ks[t] = mfma16(kh, sl[s], mfma16(kh, sh[s], ks[t]));
-                    if constexpr (LO) ks[t] = mfma16(read_rows(sk[NT - 1] + p), sh[s], ks[t]);
-                }
-            }
-        }
-        h8 uh[2], ul[2];
-        f4 u[4];
-        if constexpr (DELTA) {
-            const float w = kunit * sunit;
+                if (s + 1 < SS) get(s + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const f4 eg = *reinterpret_cast<const f4*>(&sf[0][16 * t + 4 * c]);
-                const f4 be = *reinterpret_cast<const f4*>(&sf[1][16 * t + 4 * c]);
+                for (int t = 0; t < 4; ++t) ks[t] = mfma16(oh[s & 1][t], sh[s], ks[t]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[t][e] = be[e] * __builtin_fmaf(-eg[e] * w, ks[t][e], x[t][e]);
+                for (int t = 0; t < 4; ++t) ks[t] = mfma16(oh[s & 1][t], sl[s], ks[t]);
+                if constexpr (LO)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) ks[t] = mfma16(ol[s & 1][t], sh[s], ks[t]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            const float w = -kunit * sunit;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[t][e] = __builtin_fmaf(eg[t][e] * w, ks[t][e], x[t][e]);
             h8 xh[2], xl[2];
-            const float xunit = to_operand<4>(x, xh, xl);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                f4 acc = {0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s <= t / 2; ++s) {
-                    const int p = (16 * t + r16) * TS + 32 * s + 4 * c;
-                    const h8 th = read_rows(stt[0] + p), tl = read_rows(stt[1] + p);
-                    acc = mfma16(tl, xh[s], mfma16(th, xl[s], mfma16(th, xh[s], acc)));
-                }
-                const f4 tw = *reinterpret_cast<const f4*>(&sf[3][16 * t + 4 * c]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[t][e] = acc[e] * (tw[e] * xunit);
-            }
+            const float xup = to_top<12>(f_bits(column_top<4>(x)));
+            to_operand<4>(x, xup, nullptr, c, xh, xl);
+            tri_product(th, tl, xh, xl, u);
+            uworth = fac[2 * kChunk] * inverse_pow2(xup);
         } else {
 #pragma unroll
             for (int t = 0; t < 4; ++t) u[t] = x[t];
         }
-        const float uunit = to_operand<4>(u, uh, ul);
-        // O = scale (e^G Q S + M U).
+        const float uup = to_top<12>(f_bits(column_top<4>(u))), uunit = inverse_pow2(uup) * uworth;
+        h8 uh[2], ul[2];
+        to_operand<4>(u, uup, nullptr, c, uh, ul);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            *reinterpret_cast<h8*>(su[pair] + 1024 * s + 16 * lane) = uh[s];
+            *reinterpret_cast<h8*>(su[pair] + 1024 * (2 + s) + 16 * lane) = ul[s];
+        }
+        if (c == 0) sunits[1][pair][r16] = uunit;
+        __syncthreads();
+        if (ch + 1 < nchunk) {
+            load_v(ch + 1);
+            if constexpr (DELTA) load_t(ch + 1);
+        }
+        // S = e^{G_C} S + K^T (e^{G_C - G} U), summed in the units of this product; a
+        // product too small to show beside the state does not set them.
         {
-            const float w1 = qunit * sunit * a.scale, w2 = kunit * qunit * uunit * a.scale;
+            constexpr int GT = 2;  // tiles of the state's rows a group
+            h8 oh[2][GT][2], ol[2][GT][2];
+            const auto get = [&](int g) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                f4 acc = {0, 0, 0, 0};
+                for (int i = 0; i < GT; ++i)
 #pragma unroll
-                for (int s = 0; s <= t / 2; ++s) {
-                    const int p = (16 * t + r16) * TS + 32 * s + 4 * c;
-                    const h8 mh = read_rows(sm[0] + p), ml = read_rows(sm[1] + p);
-                    acc = mfma16(ml, uh[s], mfma16(mh, ul[s], mfma16(mh, uh[s], acc)));
-                }
-                const f4 eg = *reinterpret_cast<const f4*>(&sf[0][16 * t + 4 * c]);
+                    for (int s = 0; s < 2; ++s) {
+                        const int t = GT * g + i;
+                        const uint8_t* p = kb + ((2 * s) * SS + (t >> 1)) * 1024 + rt + 8 * (t & 1);
+                        oh[g & 1][i][s] = join(read_tr(p), read_tr(p + SS * 1024));
+                        if constexpr (LO) ol[g & 1][i][s] = join(read_tr(p + kPart), read_tr(p + kPart + SS * 1024));
+                    }
+            };
+            get(0);
+            const float worth = fmaxf(fmaxf(uunit * kunit, sworth * 0x1p-60f), 0x1p-100f);
+            to_operand<4>(u, uworth * kunit * inverse_pow2(worth), fac + kChunk, c, uh, ul);
+            const float keep = fac[kChunk - 1] * (sworth * inverse_pow2(worth));
+            sworth = worth;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = kChunk * ch + 16 * t + 4 * c + e;
-                    const float y = __builtin_fmaf(eg[e] * w1, qs[t][e], acc[e] * w2);
-                    if (mine && i < sp.n) store1(a.o, a.dt, (int64_t)(sp.q0 + i) * a.o_token + hv * a.o_head + col, y);
-                }
+            for (int t = 0; t < ST; ++t) S[t] *= keep;
+#pragma unroll
+            for (int g = 0; g < ST / GT; ++g) {
+                if (g + 1 < ST / GT) get(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int i = 0; i < GT; ++i) S[GT * g + i] = mfma16(oh[g & 1][i][s], uh[s], S[GT * g + i]);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int i = 0; i < GT; ++i) S[GT * g + i] = mfma16(oh[g & 1][i][s], ul[s], S[GT * g + i]);
+                if constexpr (LO)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int i = 0; i < GT; ++i) S[GT * g + i] = mfma16(ol[g & 1][i][s], uh[s], S[GT * g + i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        // S = e^{G_C} S + K^T (e^{G_C - G} U).
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const f4 de = *reinterpret_cast<const f4*>(&sf[2][16 * t + 4 * c]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) u[t][e] *= de[e];
-        }
-        const float dunit = to_operand<4>(u, uh, ul) * kunit, all = sf[0][kChunk - 1];
-#pragma unroll
-        for (int t = 0; t < ST; ++t) {
-            f4 acc = {0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int p = (32 * s + 4 * c + (r16 >> 2)) * KS + 16 * t + 4 * (r16 & 3);
-                const h8 kh = join(read_tr(sk[0] + p), read_tr(sk[0] + p + 16 * KS));
-                acc = mfma16(kh, ul[s], mfma16(kh, uh[s], acc));
-                if constexpr (LO) {
-                    const h8 kl = join(read_tr(sk[NT - 1] + p), read_tr(sk[NT - 1] + p + 16 * KS));
-                    acc = mfma16(kl, uh[s], acc);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) S[t][e] = __builtin_fmaf(all, S[t][e], acc[e] * dunit);
-        }
+        if (ch + 1 < nchunk) hand_over();
+        __syncthreads();
     }
     if (!mine) return;
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a.s_out[at + (int64_t)(16 * t + 4 * c + e) * a.Dv] = S[t][e];
+        for (int e = 0; e < 4; ++e) a.s_out[at + (int64_t)(16 * t + 4 * c + e) * a.Dv] = S[t][e] * sworth;
 }
 
 // ------------------------------------------------------------------ host
@@ -649,7 +889,7 @@ __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
 struct GlaPlan {
     bool chunks;
     int nslots;
-    size_t kf, mf, unit, fac, bytes;
+    size_t kq, tm, fac, bytes;
 };
 
 GlaPlan plan_gla(int T, int B, int Hk, int Hv, int Dk, int dtype, bool cu, bool delta) {
@@ -658,29 +898,34 @@ GlaPlan plan_gla(int T, int B, int Hk, int Hv, int Dk, int dtype, bool cu, bool 
     if (!p.chunks) return p;
     p.nslots = T / kChunk + B;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    p.kf = up((size_t)p.nslots * Hk * (dtype == kF32 ? 2 : 1) * kChunk * Dk * 2);
-    p.mf = up((size_t)p.nslots * Hv * 2 * kChunk * kChunk * 2);
-    p.unit = up((size_t)p.nslots * Hk * 8);
-    p.fac = up((size_t)p.nslots * Hv * 4 * kChunk * 4);
-    p.bytes = 2 * p.kf + (delta ? 2 : 1) * p.mf + p.unit + p.fac;
+    p.kq = up((size_t)p.nslots * Hk * kq_bytes(Dk, dtype == kF32));
+    p.tm = up((size_t)p.nslots * Hv * tm_bytes(delta));
+    p.fac = up((size_t)p.nslots * Hv * kFac * 4);
+    p.bytes = p.kq + p.tm + p.fac;
     return p;
 }
 
-template <int DK, bool LO, bool DELTA>
+template <int DK, int DT, bool DELTA>
 void launch3(const GlaArgs& a, const GlaPlan& p, hipStream_t st) {
     if (p.chunks) {
-        gla_intra_kernel<DK, LO, DELTA><<<(unsigned)p.nslots * a.Hk, 256, 0, st>>>(a);
-        gla_inter_kernel<DK, LO, DELTA><<<(unsigned)a.B * a.Hv * ((a.Dv + 63) / 64), 256, 0, st>>>(a);
+        gla_intra_kernel<DK, DT, DELTA><<<(unsigned)p.nslots * a.Hk, 256, 0, st>>>(a);
+        gla_inter_kernel<DK, DT, DELTA><<<(unsigned)a.B * a.Hv * ((a.Dv + 31) / 32), 256, 0, st>>>(a);
     }
     const int64_t waves = (int64_t)a.B * a.Hv * (a.Dv / 16);
-    if (a.nshort >= 0) gla_step_kernel<DK><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
+    if (a.nshort >= 0) gla_step_kernel<DK, DT><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
+}
+
+template <int DK, int DT>
+void launch2(const GlaArgs& a, const GlaPlan& p, hipStream_t st) {
+    if (a.beta) launch3<DK, DT, true>(a, p, st);
+    else launch3<DK, DT, false>(a, p, st);
 }
 
 template <int DK>
 void launch1(const GlaArgs& a, const GlaPlan& p, hipStream_t st) {
-    const bool lo = a.dt == kF32;
-    if (a.beta) lo ? launch3<DK, true, true>(a, p, st) : launch3<DK, false, true>(a, p, st);
-    else lo ? launch3<DK, true, false>(a, p, st) : launch3<DK, false, false>(a, p, st);
+    if (a.dt == kF32) launch2<DK, kF32>(a, p, st);
+    else if (a.dt == kBF16) launch2<DK, kBF16>(a, p, st);
+    else launch2<DK, kF16>(a, p, st);
 }
 
 bool check(int T, int B, int Hk, int Hv, int Dk, int Dv, int dtype, bool cu) {
@@ -759,13 +1004,9 @@ int i4_gated_linear_attention_dev(const void* dQ, int64_t q_token, int64_t q_hea
     // One sequence alone is never worth a third launch that may find nothing to do.
     a.nshort = !p.chunks ? 1 << 30 : B == 1 ? -1 : kShort;
     uint8_t* w = static_cast<uint8_t*>(dWork);
-    a.kf = reinterpret_cast<_Float16*>(w);
-    a.qf = reinterpret_cast<_Float16*>(w + p.kf);
-    a.mf = reinterpret_cast<_Float16*>(w + 2 * p.kf);
-    a.tf = reinterpret_cast<_Float16*>(w + 2 * p.kf + p.mf);
-    w += 2 * p.kf + (dBeta ? 2 : 1) * p.mf;
-    a.unit = reinterpret_cast<float*>(w);
-    a.fac = reinterpret_cast<float*>(w + p.unit);
+    a.kq = w;
+    a.tm = w + p.kq;
+    a.fac = reinterpret_cast<float*>(w + p.kq + p.tm);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     if (k_dim == 64) launch1<64>(a, p, st);
