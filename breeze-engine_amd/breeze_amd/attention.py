@@ -97,7 +97,9 @@ class KVCache:
     float8_e4m3fn; ``k_scale``, ``v_scale``: fp32 ``[pages, kv_heads,
     page_size]``.  A value is the stored number times its token's and head's
     scale.  ``head_dim`` is 64, 128 or 256; ``page_size`` a power of two from 16
-    to 1024.  The tensors are kept as given and written in place."""
+    to 1024.  The tensors are kept as given and written in place.  A token's row
+    that attention may see has been written by ``kv_write``; what unwritten rows
+    hold does not matter."""
 
     def __init__(self, k, v, k_scale, v_scale):
         torch = _torch()

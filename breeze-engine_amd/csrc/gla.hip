@@ -528,19 +528,6 @@ __device__ inline void to_operand(const f4* x, float up, const float* rows, int 
     }
 }
 
-// 16 bytes a lane from `src` to LDS at `lds` + 16 * lane.  The compiler does not
-// see the load: its reader waits for it by hand.
-__device__ inline void load_lds(const uint8_t* src, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds) : "memory");
-}
-__device__ inline uint32_t lds_address(const void* p) {
-    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(p);
-}
-template <int N>
-__device__ inline void wait_loads() {  // vmcnt(N)
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
 // A lower triangular factor (T or M) times 16 columns, both of two terms.
 __device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, const h8* xl, f4* acc) {
 #pragma unroll

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 // Sets the calling thread's i4_last_error() text (qmm.hip).
 void bq_set_error(const char* fmt, ...) __attribute__((format(printf, 1, 2), visibility("hidden")));
@@ -113,6 +114,31 @@ __device__ inline float sum_rows16(float x) {
     return bits_f(r[0]) + bits_f(r[1]);
 }
 
+// The max over a wave, in all lanes.
+__device__ inline float max_wave(float x) {
+    const auto turned = [](float v, auto n) {
+        return bits_f((uint32_t)__builtin_amdgcn_mov_dpp((int)f_bits(v), 0x120 + decltype(n)::value, 0xF, 0xF, true));
+    };
+    x = fmaxf(x, turned(x, std::integral_constant<int, 1>()));  // row_ror:1, 2, 4, 8 within 16 lanes
+    x = fmaxf(x, turned(x, std::integral_constant<int, 2>()));
+    x = fmaxf(x, turned(x, std::integral_constant<int, 4>()));
+    x = fmaxf(x, turned(x, std::integral_constant<int, 8>()));
+    return max_halves(max_rows16(x));
+}
+
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 16 bytes a lane from `src` to LDS at `lds` + 16 * lane.  The compiler does not
+// see the load: its reader waits for it by hand.
+__device__ inline void load_lds(const uint8_t* src, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds) : "memory");
+}
+__device__ inline uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(p);
+}
+template <int N>
+__device__ inline void wait_loads() {  // vmcnt(N)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 }  // namespace mx

@@ -42,6 +42,8 @@ struct AttnArgs {
     const int32_t* table;
     const int32_t* kv_lens;
     const int32_t* cu;  // null: one token a sequence
+    uint8_t* unpacked;  // [B][H][tiles]: the copy that long chunks read
+    int tiles;          // of 64 keys, in the whole table
     float* part;        // [nsplit][T * Hq][D] when nsplit > 1
     f2* ml;             // [nsplit][T * Hq] (maximum, sum)
     int64_t table_row;
@@ -49,22 +51,24 @@ struct AttnArgs {
     float scale;  // softmax scale * log2(e)
 };
 
-// The weights of the second product are p * vs * 2^12 / nu: at most 2^15 while
-// the tile's value scales are at most 8 nu.
-constexpr float kPScale = 4096.0f;
+// The weights of the second product are p * vs * 2^9 / nu: at most 2^15 while
+// the tile's value scales are at most 8 nu and p at most 8 (a row's scores are
+// taken relative to a reference that they may pass by kSlack in log2).
+constexpr float kPScale = 512.0f, kSlack = 3.0f;
 
 typedef __attribute__((address_space(3))) s4* lds_s4;
 
 __device__ inline h4 read_tr(const _Float16* p) {
     return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p)));
 }
+__device__ inline f16 mfma32(h8 a, h8 b, f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ inline h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // The power of two that a tile's value scales are taken relative to: kept
-// while the largest is within (nu / 256, 8 nu].
+// while the largest is within (nu / 16, 8 nu].
 __device__ inline float next_nu(float nu, float vmax) {
     if (!(vmax > 0.0f) || vmax > 3e38f) return nu;
-    if (vmax <= nu * 8.0f && vmax > nu * 0x1p-8f) return nu;
+    if (vmax <= nu * 8.0f && vmax > nu * 0x1p-4f) return nu;
     const float want = bits_f(max(f_bits(vmax) & 0x7F800000u, 1u << 23));
     return nu > 0.0f ? fmaxf(want, nu * 0x1p-100f) : want;
 }
@@ -88,12 +92,12 @@ __device__ inline Seq sequence(const AttnArgs& a, int b) {
 }
 
 // Cache row (in rows of D) of the 16 keys from `key` on for head h; -1 where
-// the sequence or its table has none.
+// the sequence or its table has none.  kv > 0.
 __device__ inline int64_t group_row(const AttnArgs& a, const int32_t* table, int h, int key, int kv) {
-    if (key >= kv) return -1;
-    const int page = table[key >> a.pshift];
-    if (page < 0 || page >= a.P) return -1;
-    return (((int64_t)page * a.H + h) << a.pshift) + (key & ((1 << a.pshift) - 1));
+    const int page = table[min(key, kv - 1) >> a.pshift];
+    const bool is = key < kv && page >= 0 && page < a.P;
+    const int64_t row = (((int64_t)page * a.H + h) << a.pshift) + (key & ((1 << a.pshift) - 1));
+    return is ? row : -1;
 }
 
 __device__ inline uint32_t lane_max_u32(uint32_t x, int step) { return max(x, (uint32_t)__shfl_xor((int)x, step)); }
@@ -136,8 +140,9 @@ __device__ inline h8 round8(const float* w) {
 // keys and values are on their way while this one is computed, 16 KB a wave
 // (D = 256), and no wave waits for another before the end.
 
-template <int D, int KIND, bool SPLIT>
+template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
+    constexpr bool SPLIT = DT == kF32;
     constexpr int KC = D / 64;        // 16-byte chunks of a key a lane takes (a quarter of each 64 values)
     constexpr int VC = D / 32;        // 16-byte chunks of a tile's values a lane takes
     constexpr int VS = D + 16;        // LDS row of a key's values: the transposed reads' four rows fall on unlike banks
@@ -168,7 +173,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
                 f4 v = {0, 0, 0, 0};
-                if (has_row) v = load4(a.q, a.dt, tok * a.q_token + head * a.q_head + 64 * i + 16 * c + j);
+                if (has_row) v = load4(a.q, DT, tok * a.q_token + head * a.q_head + 64 * i + 16 * c + j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[16 * i + j + e] = v[e];
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     int64_t row[2];
     const auto rows_of = [&](int tile, int64_t* r) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) r[u] = tile < t1 ? group_row(a, table, h, 32 * tile + 16 * u, sq.kv) : -1;
+        for (int u = 0; u < 2; ++u) r[u] = group_row(a, table, h, 32 * tile + 16 * u, sq.kv);
     };
     const auto load = [&](const int64_t* r) {
 #pragma unroll
@@ -224,10 +229,12 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
             vraw[i] = *reinterpret_cast<const u4*>(a.vp + (at + (kr & 15)) * D + 16 * (chunk % per_row));
         }
     };
-    rows_of(t, row);
-    if (t < t1) load(row);
-    int64_t next[2];
-    rows_of(t + 4, next);
+    int64_t next[2] = {-1, -1};
+    if (t < t1) {
+        rows_of(t, row);
+        load(row);
+        rows_of(t + 4, next);
+    }
 
     for (; t < t1; t += 4) {
         const int key0 = 32 * t;
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
         for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(so + (w * 16 + r) * OS + d) * f[w];
         v *= inv;
         if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
-        else store4(a.out, a.dt, ot * a.o_token + oh * a.o_head + d, v);
+        else store4(a.out, DT, ot * a.o_token + oh * a.o_head + d, v);
     }
 }
 
@@ -361,8 +368,62 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
 
 constexpr int kRowTile = 128, kKeyTile = 64;
 
-template <int D, int KIND, bool SPLIT>
+// The 128 rows of a slot: their sequence (-1: none, or one of the other
+// kernel's) and the first of them.  Sequence b's tiles take the slots from
+// cu[b] * G / 128 + b on, which leaves room for all without a pass over the lengths.
+__device__ inline int rows_of_slot(const AttnArgs& a, int slot, Seq& sq, int64_t& first) {
+    const int per = (a.G + kRowTile - 1) / kRowTile;
+    int b = 0;
+    if (a.cu) {
+        int hi = a.B;
+        while (hi - b > 1) {
+            const int mid = (b + hi) >> 1;
+            const int64_t start = (int64_t)min(max(a.cu[mid], 0), a.T) * a.G / kRowTile + mid;
+            if (start <= slot) b = mid;
+            else hi = mid;
+        }
+    } else {
+        b = slot / per;
+    }
+    sq = sequence(a, b);
+    const int64_t rows = (int64_t)sq.n * a.G;
+    first = (slot - (a.cu ? (int64_t)sq.q0 * a.G / kRowTile + b : (int64_t)b * per)) * kRowTile;
+    return rows <= 16 || first < 0 || first >= rows ? -1 : b;
+}
+
+// A row's queries as operands (values 16 s + 8 (lane / 32) + 0..7 for slab s,
+// from element `at` on), scaled; returns what a score is worth in log2.
+template <int D, int DT>
+__device__ inline float load_queries(const AttnArgs& a, int64_t at, h8* hi, h8* lo) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            const f4 v = load4(a.q, DT, at + 16 * s + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, f_bits(v[e]) & 0x7FFFFFFFu);
+        }
+    top = lane_max_u32(top, 32);
+    const float up = row_scale(top);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            const f4 v = load4(a.q, DT, at + 16 * s + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[j + e] = v[e] * up;
+        }
+        if constexpr (DT == kF32) split8(w, hi[s], lo[s]);
+        else hi[s] = round8(w);
+    }
+    return a.scale / up;
+}
+
+template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnArgs a) {
+    constexpr bool SPLIT = DT == kF32;
     constexpr int KS = D + 8, VS = D + 16;  // LDS rows of a key: reads of one instruction fall on unlike banks
     constexpr int NC = D / 64;              // 16-byte chunks a thread loads of a tile's keys (and of its values)
     constexpr int per_row = D / 16;
@@ -374,25 +435,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     const int r32 = lane & 31, hf = lane >> 5;
     const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.nsplit;
     const int slot = a.nslots - 1 - ss / a.nsplit;  // a prompt's last rows see the most keys: first
-    // Sequence b's tiles take the slots from cu[b] * G / 128 + b on, which leaves
-    // room for all of them without a pass over the lengths.
-    int b = 0;
-    if (a.cu) {
-        int hi = a.B;
-        while (hi - b > 1) {
-            const int mid = (b + hi) >> 1;
-            const int64_t start = (int64_t)min(max(a.cu[mid], 0), a.T) * a.G / kRowTile + mid;
-            if (start <= slot) b = mid;
-            else hi = mid;
-        }
-    } else {
-        b = slot / ((a.G + kRowTile - 1) / kRowTile);
-    }
-    const Seq sq = sequence(a, b);
+    Seq sq;
+    int64_t first;
+    const int b = rows_of_slot(a, slot, sq, first);
     const int64_t rows = (int64_t)sq.n * a.G;
-    const int64_t before = a.cu ? (int64_t)sq.q0 * a.G / kRowTile + b : (int64_t)b * ((a.G + kRowTile - 1) / kRowTile);
-    const int64_t first = (slot - before) * kRowTile;
-    if (rows <= 16 || first < 0 || first >= rows) return;
+    if (b < 0) return;
     const int64_t row = first + 32 * wave + r32;
     const bool has_row = row < rows;
     const int tok_in = has_row ? (int)(row / a.G) : 0;
@@ -406,34 +453,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     const int wave_all = seen_by(first + 32 * wave);
 
     h8 qh[D / 16], ql[SPLIT ? D / 16 : 1];
-    float rowf;
-    {
-        uint32_t top = 0;
-        const int64_t at = tok * a.q_token + head * a.q_head + 8 * hf;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                const f4 v = load4(a.q, a.dt, at + 16 * s + j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = max(top, f_bits(v[e]) & 0x7FFFFFFFu);
-            }
-        top = lane_max_u32(top, 32);
-        const float up = row_scale(top);
-        rowf = a.scale / up;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            float w[8];
-#pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                const f4 v = load4(a.q, a.dt, at + 16 * s + j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[j + e] = v[e] * up;
-            }
-            if constexpr (SPLIT) split8(w, qh[s], ql[s]);
-            else qh[s] = round8(w);
-        }
-    }
+    const float rowf = load_queries<D, DT>(a, tok * a.q_token + head * a.q_head + 8 * hf, qh, ql);
 
     const int ntile = (min(wg_end, sq.kv) + kKeyTile - 1) / kKeyTile, per = (ntile + a.nsplit - 1) / a.nsplit;
     const int t1 = min((split + 1) * per, ntile);
@@ -603,7 +623,261 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
             const int d = 32 * i + 2 * j + 4 * hf;
             const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
             if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
-            else store4(a.out, a.dt, tok * a.o_token + head * a.o_head + d, v);
+            else store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
+        }
+}
+
+// ------------------------------------------------------------------ many rows over one unpacked copy
+//
+// A long chunk reads every key once for each 128 of its rows, and unpacking a
+// tile costs the kernel above about half as much vector work as its softmax.
+// So where a sequence has kUnpackRows rows or more, its keys and values are
+// first unpacked once, to fp16 (exactly), in the order of the matrix
+// instructions' operands (1 KB each, 16 bytes a lane), V transposed, with the
+// scales beside them.  Tiles then come straight to LDS.
+
+constexpr int kHead = 1024;  // a tile's scales: ks[64], vs[64], 1 where a key is not there [64], largest vs, any not there
+template <int D>
+constexpr int tile_bytes() { return kKeyTile * D * 4 + kHead; }
+
+template <int D, int KIND>
+__global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
+    constexpr int VS = D + 16, NC = D / 64, per_row = D / 16, KF = D / 8;  // KF operands of K, as many of V
+    __shared__ __align__(16) _Float16 sv[kKeyTile * VS], sk[kKeyTile * VS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t items = (int64_t)a.B * a.H * a.tiles;
+    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+        const int tile = (int)(it % a.tiles), h = (int)(it / a.tiles % a.H), b = (int)(it / a.tiles / a.H);
+        const Seq sq = sequence(a, b);
+        if (tile * kKeyTile >= sq.kv || (int64_t)sq.n * a.G <= 16) continue;
+        const int32_t* table = a.table + b * a.table_row;
+        uint8_t* out = a.unpacked + it * tile_bytes<D>();
+        if (wave == 0) {
+            const int64_t at = group_row(a, table, h, kKeyTile * tile + (lane & ~15), sq.kv);
+            const bool bad = at < 0 || kKeyTile * tile + lane >= sq.kv;
+            const int64_t from = (at < 0 ? 0 : at) + (lane & 15);
+            const float ks = a.ks[from], vs = a.vs[from];
+            // A value scale of NaN goes with the key's, whose score a row that does
+            // not see the key leaves out; times a probability of zero it would not.
+            const bool nan = vs != vs;
+            const float vv = bad || nan ? 0.0f : vs, vmax = max_wave(vv);
+            float* head = reinterpret_cast<float*>(out + kKeyTile * D * 4);
+            head[lane] = bad ? 0.0f : nan ? vs : ks;
+            head[64 + lane] = vv;
+            head[128 + lane] = bad ? 1.0f : 0.0f;
+            head[192 + lane] = lane == 0 ? vmax : __any(bad) ? 1.0f : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int kr = (tid + 256 * i) / per_row, col = 16 * (tid % per_row);
+            const int64_t row = group_row(a, table, h, kKeyTile * tile + (kr & ~15), sq.kv);
+            const bool is = row >= 0 && kKeyTile * tile + kr < sq.kv;
+            const int64_t at = ((row < 0 ? 0 : row) + (kr & 15)) * D + col;
+            u4 kw = *reinterpret_cast<const u4*>(a.kp + at), vw = *reinterpret_cast<const u4*>(a.vp + at);
+            if (!is) kw = vw = (u4){0, 0, 0, 0};
+            h8* kd = reinterpret_cast<h8*>(sk + kr * VS + col);
+            h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
+            kd[0] = unpack8<KIND>(kw.x, kw.y);
+            kd[1] = unpack8<KIND>(kw.z, kw.w);
+            vd[0] = unpack8<KIND>(vw.x, vw.y);
+            vd[1] = unpack8<KIND>(vw.z, vw.w);
+        }
+        __syncthreads();
+        h8* ko = reinterpret_cast<h8*>(out);
+#pragma unroll
+        for (int i = 0; i < KF / 4; ++i) {
+            const int f = 4 * i + wave;
+            // K: keys 32 u + lane % 32, values 16 s + 8 (lane / 32) + 0..7.
+            const int u = f / (D / 16), sl = f % (D / 16), r32 = lane & 31, hf = lane >> 5, i16 = lane & 15;
+            ko[64 * f + lane] = *reinterpret_cast<const h8*>(sk + (32 * u + r32) * VS + 16 * sl + 8 * hf);
+            // V: value 32 t + lane % 32, keys 16 g + 4 (lane / 32) + 0..3 and 8 more.
+            const int g = f / (D / 32), t = f % (D / 32);
+            const _Float16* p = sv + (16 * g + 4 * hf + (i16 >> 2)) * VS + 32 * t + 16 * (r32 >> 4) + 4 * (i16 & 3);
+            ko[64 * (KF + f) + lane] = join(read_tr(p), read_tr(p + 8 * VS));
+        }
+        __syncthreads();
+    }
+}
+
+// As attn_rows_kernel, over the copy.  The scores of tile t + 1 are computed
+// beside the softmax of tile t, which they do not wait for, then the weighted
+// values of tile t; K of tile t + 2 and V of tile t + 1 are on their way.
+template <int D, int DT>
+__global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) void attn_tiles_kernel(AttnArgs a) {
+    constexpr bool SPLIT = DT == kF32;
+    constexpr int KB = kKeyTile * D * 2;
+    __shared__ __align__(1024) uint8_t sk[2][KB], sv[2][KB];
+    __shared__ __align__(1024) float sh[2][kHead / 4];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r32 = lane & 31, hf = lane >> 5;
+    const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.nsplit;
+    const int slot = a.nslots - 1 - ss / a.nsplit;  // a prompt's last rows see the most keys: first
+    Seq sq;
+    int64_t first;
+    const int b = rows_of_slot(a, slot, sq, first);
+    if (b < 0) return;
+    const int64_t rows = (int64_t)sq.n * a.G, row = first + 32 * wave + r32;
+    const bool has_row = row < rows;
+    const int tok_in = has_row ? (int)(row / a.G) : 0;
+    const int tok = sq.q0 + tok_in, head = h * a.G + (has_row ? (int)(row % a.G) : 0);
+    const int last = has_row ? sq.kv - sq.n + tok_in : -1;
+    // Keys that the workgroup's last row sees, and keys that all of the wave's rows see.
+    const auto seen_by = [&](int64_t r) { return max(sq.kv - sq.n + (int)(min(r, rows - 1) / a.G) + 1, 0); };
+    const int wg_end = min(seen_by(first + kRowTile - 1), sq.kv);
+    const int wave_all = first + 32 * wave + 31 < rows ? min(seen_by(first + 32 * wave), sq.kv) : 0;
+
+    h8 qh[D / 16], ql[SPLIT ? D / 16 : 1];
+    const float rowf = load_queries<D, DT>(a, tok * a.q_token + head * a.q_head + 8 * hf, qh, ql);
+
+    const int ntile = (wg_end + kKeyTile - 1) / kKeyTile, per = (ntile + a.nsplit - 1) / a.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const uint8_t* const tiles = a.unpacked + ((int64_t)b * a.H + h) * a.tiles * tile_bytes<D>();
+
+    f16 o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    // The sums o and l are in units in which a probability of 1 is 2^9 / nu.
+    float m = -INFINITY, l = 0.0f, nu = 0.0f;
+
+    // Past the last tile the loads repeat it.
+    const auto fetch = [&](int t, int from, uint8_t* to) {
+        const uint8_t* src = tiles + (int64_t)min(t, t1 - 1) * tile_bytes<D>() + from + 1024 * wave + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < KB / 4096; ++i) load_lds(src + 4096 * i, lds_address(to) + 1024 * wave + 4096 * i);
+    };
+    const auto fetch_head = [&](int t) {
+        if (wave == 0)
+            load_lds(tiles + (int64_t)min(t, t1 - 1) * tile_bytes<D>() + 2 * KB + 16 * lane, lds_address(sh[t & 1]));
+    };
+    f16 s[2];
+    const auto scores = [&](const uint8_t* kb) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
+        const h8* p = reinterpret_cast<const h8*>(kb) + lane;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const h8 k0 = p[64 * i], k1 = p[64 * (D / 16 + i)];
+            s[0] = mfma32(k0, qh[i], s[0]);
+            s[1] = mfma32(k1, qh[i], s[1]);
+            if constexpr (SPLIT) {
+                s[0] = mfma32(k0, ql[i], s[0]);
+                s[1] = mfma32(k1, ql[i], s[1]);
+            }
+        }
+    };
+    if (t0 < t1) {
+        fetch(t0, 0, sk[t0 & 1]);
+        fetch_head(t0);
+        fetch(t0 + 1, 0, sk[(t0 + 1) & 1]);
+        fetch(t0, KB, sv[t0 & 1]);
+        wait_loads<0>();
+        __syncthreads();
+        scores(sk[t0 & 1]);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int key0 = kKeyTile * t, par = t & 1;
+        wait_loads<0>();
+        __syncthreads();  // K of t + 1 and V of t are there; K of t and V of t - 1 are read
+        fetch(t + 2, 0, sk[par]);
+        fetch(t + 1, KB, sv[par ^ 1]);
+        fetch_head(t + 1);
+        const float* const hd = sh[par];
+        const float now = fmaxf(next_nu(nu, hd[192]), 0x1p-100f), nr = nu_ratio(nu, now), unit = __builtin_log2f(kPScale / now);
+        nu = now;
+        f16 x[2];
+        // Scores times the key scales; result register j holds key 8 (j / 4) + 4 hf + j % 4.
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const f4 sc = *reinterpret_cast<const f4*>(hd + 32 * u + 2 * j + 4 * hf);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][j + e] = s[u][j + e] * sc[e];
+            }
+        // Past the wave's first row, past the sequence's end or in a page that is not there.
+        if (key0 + kKeyTile > wave_all || hd[193] != 0.0f) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const f4 bad = *reinterpret_cast<const f4*>(hd + 128 + 32 * u + 2 * j + 4 * hf);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int k = key0 + 32 * u + 2 * j + 4 * hf + e;
+                        x[u][j + e] = k > last || bad[e] != 0.0f ? -INFINITY : x[u][j + e];
+                    }
+                }
+        }
+        scores(sk[par ^ 1]);
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, x[u][j]), x[u][j + 1]);
+        top = max_halves(top);
+        // The reference moves only once a row's scores pass it by kSlack.
+        const bool moves = (top - m) * rowf > kSlack;
+        const float f = moves ? fast_exp2((m - top) * rowf) : 1.0f;
+        m = moves ? top : m;
+        const float alpha = f * nr, base = __builtin_fmaf(m == -INFINITY ? 0.0f : -m, rowf, unit);
+        l *= alpha;
+        h8 ph[4], pl[SPLIT ? 4 : 1];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {  // 16 keys
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = fast_exp2(__builtin_fmaf(x[g >> 1][8 * (g & 1) + j], rowf, base));
+                l += w[j];
+            }
+            const f4 s0 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 4 * hf);
+            const f4 s1 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 8 + 4 * hf);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] *= s0[j];
+                w[4 + j] *= s1[j];
+            }
+            if constexpr (SPLIT) split8(w, ph[g], pl[g]);
+            else ph[g] = round8(w);
+        }
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+        }
+        const h8* p = reinterpret_cast<const h8*>(sv[par]) + lane;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                const h8 v = p[64 * (g * (D / 32) + i)];
+                o[i] = mfma32(v, ph[g], o[i]);
+                if constexpr (SPLIT) o[i] = mfma32(v, pl[g], o[i]);
+            }
+    }
+    wait_loads<0>();  // none may land in LDS that is another workgroup's
+
+    if (!has_row) return;
+    l = sum_halves(l);
+    const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
+    float f = nu * (1.0f / kPScale);
+    if (a.nsplit > 1) {
+        if (hf == 0) a.ml[prow] = (f2){m * rowf, l * f};
+    } else {
+        f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const int d = 32 * i + 2 * j + 4 * hf;
+            const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
+            if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+            else store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
         }
 }
 
@@ -634,9 +908,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // ------------------------------------------------------------------ host
 
 struct AttnPlan {
-    int keys, rows, nsplit, nslots;  // which kernels run, splits of the keys, slots of the rows kernel
-    size_t bytes;                    // workspace
+    int keys, rows, nsplit, nslots;  // which kernels run, splits of the keys, slots of the rows kernels
+    int tiles;                       // of the unpacked copy of each sequence; 0: none
+    size_t copy, bytes;              // of the copies, of the workspace
 };
+
+// Rows a sequence from which on its keys are unpacked once for all of them, and
+// the most that the copies may take.
+constexpr int kUnpackRows = 512;
+constexpr size_t kUnpackMost = (size_t)4 << 30;
 
 // Splits: enough workgroups for every compute unit twice, each with at least
 // 256 keys of the longest sequence that the table can hold.
@@ -652,7 +932,13 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
     s = std::min<int64_t>(s, 64);
     if (wgs >= n_cu) s = 1;
     p.nsplit = (int)s;
-    p.bytes = s > 1 ? (size_t)s * T * Hq * (D * 4 + 8) : 0;
+    if (p.rows && (int64_t)T * G >= (int64_t)kUnpackRows * B) {
+        const int64_t tiles = (capacity + kKeyTile - 1) / kKeyTile;
+        p.copy = (size_t)B * H * tiles * (kKeyTile * D * 4 + kHead);
+        if (p.copy <= kUnpackMost) p.tiles = (int)tiles;
+        else p.copy = 0;
+    }
+    p.bytes = p.copy + (s > 1 ? (size_t)s * T * Hq * (D * 4 + 8) : 0);
     return p;
 }
 
@@ -667,21 +953,33 @@ int cu_count() {
     return n[dev];
 }
 
-template <int D, int KIND, bool SPLIT>
+template <int D, int KIND, int DT>
 void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-    if (p.keys) attn_keys_kernel<D, KIND, SPLIT><<<(unsigned)a.B * a.H * a.nsplit, 256, 0, st>>>(a);
-    if (p.rows) attn_rows_kernel<D, KIND, SPLIT><<<(unsigned)a.nslots * a.H * a.nsplit, 256, 0, st>>>(a);
-    if (a.nsplit > 1) {
-        constexpr int rows = 256 / (D / 4);
-        attn_join_kernel<D><<<(unsigned)(((int64_t)a.T * a.Hq + rows - 1) / rows), 256, 0, st>>>(a);
+    if (p.keys) attn_keys_kernel<D, KIND, DT><<<(unsigned)a.B * a.H * a.nsplit, 256, 0, st>>>(a);
+    if (p.rows && p.tiles) {
+        const int64_t items = (int64_t)a.B * a.H * a.tiles;
+        attn_unpack_kernel<D, KIND><<<(unsigned)std::min<int64_t>(items, 2048), 256, 0, st>>>(a);
+        attn_tiles_kernel<D, DT><<<(unsigned)a.nslots * a.H * a.nsplit, 256, 0, st>>>(a);
+    } else if (p.rows) {
+        attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nsplit, 256, 0, st>>>(a);
     }
+}
+
+template <int D, int KIND>
+void launch2(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+    if (a.dt == kF32) launch3<D, KIND, kF32>(a, p, st);
+    else if (a.dt == kBF16) launch3<D, KIND, kBF16>(a, p, st);
+    else launch3<D, KIND, kF16>(a, p, st);
 }
 
 template <int D>
 void launch1(const AttnArgs& a, const AttnPlan& p, int kind, hipStream_t st) {
-    const bool split = a.dt == kF32;
-    if (kind == kInt8) split ? launch3<D, kInt8, true>(a, p, st) : launch3<D, kInt8, false>(a, p, st);
-    else split ? launch3<D, kFp8, true>(a, p, st) : launch3<D, kFp8, false>(a, p, st);
+    if (kind == kInt8) launch2<D, kInt8>(a, p, st);
+    else launch2<D, kFp8>(a, p, st);
+    if (a.nsplit > 1) {
+        constexpr int rows = 256 / (D / 4);
+        attn_join_kernel<D><<<(unsigned)(((int64_t)a.T * a.Hq + rows - 1) / rows), 256, 0, st>>>(a);
+    }
 }
 
 bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, bool has_cu, int* pshift) {
@@ -780,7 +1078,9 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
     }
     a.nsplit = p.nsplit;
     a.nslots = p.nslots;
-    a.part = static_cast<float*>(dWork);
+    a.tiles = p.tiles;
+    a.unpacked = static_cast<uint8_t*>(dWork);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(dWork) + p.copy);
     a.ml = reinterpret_cast<f2*>(a.part + (size_t)p.nsplit * T * heads * cache->head_dim);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();

@@ -213,7 +213,8 @@ int i4_rmsnorm_dev(const float* dX, const float* dW, int M, int H, float eps, fl
  * page_size, head_dim] bytes, INT8 (kind 0) or e4m3 (kind 1); k_scale,
  * v_scale: fp32 [num_pages, kv_heads, page_size], one for each token and head.
  * head_dim is 64, 128 or 256, page_size a power of two from 16 to 1024.  k and
- * v are 16-byte aligned.  A token's slot is page * page_size + its place in
+ * v are 16-byte aligned.  e4m3 pages hold no NaN in rows that attention may see
+ * (i4_kv_write_dev stores none).  A token's slot is page * page_size + its place in
  * the page. */
 typedef struct {
     void* k;

@@ -89,8 +89,10 @@ def attend(q, cache, table, kv_lens, q_lens, scale, split):
                 err = err + 2.0 ** -22 + (2.0 ** -21 if split else half_step(torch.float16)) + kv * 2.0 ** -24
                 pv = p * err
                 worst = pv @ vv.abs() + pv.sum(-1, keepdim=True) * (p @ vv.abs())
-                # Weights below fp16's normal range keep an absolute step instead.
-                small = 2.0 ** -36 * (seen.double() @ vv.abs())
+                # A weight errs by no less than half of fp16's smallest step, 2^-25, in units
+                # in which a probability of 1 times the tile's largest value scale is 2^9 / 16
+                # or more: 2^-30 of the largest value for each key.
+                small = 2.0 ** -30 * seen.sum(-1, keepdim=True) * vv.abs().max()
                 out[start:start + n, h], bound[start:start + n, h] = o, worst + small
         start += n
     return out, bound

@@ -110,6 +110,18 @@ def test_a_chunk_of_a_long_context(att, dtype, heads, H, D):
     _run(att, 4, "int8", dtype, heads, H, D, 64, [70], [3000], extra=20)
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("heads,H,D,page", [(6, 1, 256, 16), (8, 2, 128, 64), (12, 3, 64, 32)])
+@pytest.mark.parametrize("q_lens,ctx,extra", [([300], [0], 0), ([1, 260, 2, 400], [300, 77, 0, 63], 3),
+                                              ([129], [1500], 9)])
+def test_long_chunks(att, kind, dtype, heads, H, D, page, q_lens, ctx, extra):
+    """Enough rows a sequence that its keys are unpacked once for all of them."""
+    if D == 256 and len(q_lens) == 1 and q_lens[0] == 300 and dtype == "bf16":
+        _run(att, 40, kind, dtype, heads, H, D, page, [1300], [5], spread=4.0)
+    _run(att, 41, kind, dtype, heads, H, D, page, q_lens, ctx, extra)
+
+
 @pytest.mark.parametrize("heads", [17, 128, 129, 300])
 def test_many_heads_of_one_key_head(att, heads):
     _run(att, 5, "int8", "bf16", heads, 1, 64, 16, [1, 1], [40, 3], single=True)
@@ -140,7 +152,7 @@ def test_queries_of_any_size(att, dtype):
 
 
 @pytest.mark.parametrize("kind", ["int8", "fp8"])
-@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("n", [1, 20, 150])
 def test_rows_that_see_nothing(att, kind, n):
     """No keys, fewer keys than new tokens, and pages that are not the cache's."""
     gen = torch.Generator().manual_seed(9)
@@ -158,6 +170,13 @@ def test_rows_that_see_nothing(att, kind, n):
     # Lengths past the table and negative ones.
     lens = torch.tensor([-3, 1 << 30, -(1 << 31), 2147483647, 33], dtype=torch.int32)
     got = att.paged_attention(q.cuda(), cache, table.cuda(), lens.cuda(), _cu(q_lens).cuda())
+    if kind == "fp8":
+        # Keys that were never written count as there now, and e4m3 pages may not hold
+        # NaN there (kv_write stores none): only the other sequences have values.
+        for b in (0, 2, 4):
+            part = slice(b * n, b * n + n)
+            _check(got[part], q[part], cache, table[b:b + 1], lens[b:b + 1].tolist(), [n], 128 ** -0.5, torch.float32)
+        return
     _check(got, q, cache, table, lens.tolist(), q_lens, 128 ** -0.5, torch.float32)
 
 
@@ -180,14 +199,16 @@ def test_rows_outside_the_sequences_stay(att, heads, H):
     torch.cuda.synchronize()
 
 
-def test_nan_rows_stay_apart(att):
+@pytest.mark.parametrize("n", [40, 200])
+def test_nan_rows_stay_apart(att, n):
     """A query with NaN or infinity spoils its own row; a key that a row does
     not see spoils nothing."""
     gen = torch.Generator().manual_seed(11)
-    n, heads = 40, 4
-    cache, table = _cache(att, gen, [100], 1, 64, 16, "int8")
+    heads = 4
+    cache, table = _cache(att, gen, [100 if n < 100 else n], 1, 64, 16, "int8")
     q = torch.randn((n, heads, 64), generator=gen)
-    lens, cu = torch.tensor([100], dtype=torch.int32).cuda(), _cu([n]).cuda()
+    kv = 100 if n < 100 else n
+    lens, cu = torch.tensor([kv], dtype=torch.int32).cuda(), _cu([n]).cuda()
     clean = att.paged_attention(q.cuda(), cache, table.cuda(), lens, cu)
     x = q.clone()
     x[5, 1, 3], x[30, 2, 0] = float("nan"), float("inf")
@@ -197,7 +218,7 @@ def test_nan_rows_stay_apart(att):
     assert torch.equal(got[keep.cuda()], clean[keep.cuda()])
     assert torch.isnan(got[5, 1]).all() and torch.isnan(got[30, 2]).all()
     # The last key's row turns to NaN: only the last token sees it.
-    slot = int(table[0, 99 // 16]) * 16 + 99 % 16
+    slot = int(table[0, (kv - 1) // 16]) * 16 + (kv - 1) % 16
     bad = torch.full((1, 1, 64), float("nan")).cuda()
     att.kv_write(cache, bad, bad, torch.tensor([slot], dtype=torch.int32).cuda())
     got = att.paged_attention(q.cuda(), cache, table.cuda(), lens, cu)
@@ -238,7 +259,7 @@ def test_repeats_bit_for_bit_on_streams_and_in_graphs(att):
     kv = [1500, 40, 700]
     cache, table = _cache(att, gen, kv, 2, 128, 16, "int8")
     table, lens = table.cuda(), torch.tensor(kv, dtype=torch.int32).cuda()
-    for q_lens in ([1, 1, 1], [30, 1, 5]):
+    for q_lens in ([1, 1, 1], [30, 1, 5], [300, 30, 200]):
         cu = None if max(q_lens) == 1 else _cu(q_lens).cuda()
         qs = [torch.randn((sum(q_lens), 8, 128), generator=gen).cuda() for _ in range(4)]
         want = [att.paged_attention(q, cache, table, lens, cu) for q in qs]
@@ -281,7 +302,7 @@ def test_far_pages(att):
     for c, pages in ((cache, [P - 1, 17]), (small, [0, 1])):
         slots = (torch.tensor(pages)[j // page] * page + j % page).to(torch.int32).cuda()
         att.kv_write(c, k, v, slots)
-    for n in (1, 50):
+    for n in (1, 50, 600):
         q = torch.randn((n, 8, D), generator=gen).cuda()
         lens, cu = torch.tensor([1100], dtype=torch.int32).cuda(), _cu([n]).cuda()
         a = att.paged_attention(q, cache, torch.tensor([[P - 1, 17]], dtype=torch.int32).cuda(), lens, cu)
