@@ -273,7 +273,7 @@ def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=N
         q = _rows(q, "q")
         if given:
             _no_overlap(out, q, "q")
-        n = hb._lib.i4_paged_attention_workspace(cache._p, T, B, heads, cols, cu_q is not None)
+        n = hb._lib.i4_paged_attention_workspace(cache._p, T, B, heads, dt, cols, cu_q is not None)
         if n < 0:
             raise ValueError(hb.last_error())
         work = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None

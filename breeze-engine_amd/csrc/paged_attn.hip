@@ -45,9 +45,10 @@ struct AttnArgs {
     uint8_t* unpacked;  // [B][H][tiles]: the copy that long chunks read
     int tiles;          // of 64 keys, in the whole table
     float* part;        // [nsplit][T * Hq][D] when nsplit > 1
-    f2* ml;             // [nsplit][T * Hq] (maximum, sum)
+    f2* ml;             // [nsplit][T * Hq]: maximum and sum; a first one of (infinity, 0): the row is done
     int64_t table_row;
-    int T, B, Hq, H, G, P, pshift, table_w, nsplit, nslots, dt;
+    int T, B, Hq, H, G, P, pshift, table_w, nslots, dt;
+    int nsplit, nkeys, nrows;  // splits that the workspace has room for, and those of the two kinds of kernels
     float scale;  // softmax scale * log2(e)
 };
 
@@ -100,6 +101,16 @@ __device__ inline int64_t group_row(const AttnArgs& a, const int32_t* table, int
     return is ? row : -1;
 }
 
+// Where a row's sums go: the output, or (a kernel of more than one split) the
+// workspace; there, the splits that the kernel does not have are marked empty.
+__device__ inline void mark_row(const AttnArgs& a, int own, int split, int64_t row, float top, float sum) {
+    if (a.nsplit == 1) return;
+    const int64_t n = (int64_t)a.T * a.Hq;
+    a.ml[split * n + row] = own > 1 ? (f2){top, sum} : (f2){INFINITY, 0.0f};
+    if (split == 0)
+        for (int s = own; s < a.nsplit; ++s) a.ml[s * n + row] = (f2){-INFINITY, 0.0f};
+}
+
 __device__ inline uint32_t lane_max_u32(uint32_t x, int step) { return max(x, (uint32_t)__shfl_xor((int)x, step)); }
 
 // The power of two that brings a row whose largest magnitude has these bits to [2^13, 2^14).
@@ -150,9 +161,10 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     constexpr int kLds = 4 * 32 * VS * 2 > 4 * 16 * OS * 4 ? 4 * 32 * VS * 2 : 4 * 16 * OS * 4;
     __shared__ __align__(16) uint8_t lds[kLds];
     __shared__ float sm[4][16], sl[4][16], snu[4];
+    __shared__ __align__(16) h8 sql[SPLIT ? D / 32 * 64 : 1];  // the queries' second terms, the same for all waves
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.H, bs = blockIdx.x / a.H, split = bs % a.nsplit, b = bs / a.nsplit;
+    const int h = blockIdx.x % a.H, bs = blockIdx.x / a.H, split = bs % a.nkeys, b = bs / a.nkeys;
     const Seq sq = sequence(a, b);
     const int rows = sq.n * a.G;
     if (rows <= 0 || rows > 16) return;
@@ -163,37 +175,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     const bool has_row = r16 < rows;
     const int tok = sq.q0 + (has_row ? r16 / a.G : 0), head = h * a.G + (has_row ? r16 % a.G : 0);
     const int last = has_row ? sq.kv - sq.n + r16 / a.G : -1;  // the last key that the row sees
-    h8 qh[D / 32], ql[SPLIT ? D / 32 : 1];
-    float rowf;
-    {
-        float x[D / 4];
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < KC; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                f4 v = {0, 0, 0, 0};
-                if (has_row) v = load4(a.q, DT, tok * a.q_token + head * a.q_head + 64 * i + 16 * c + j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[16 * i + j + e] = v[e];
-                    top = max(top, f_bits(v[e]) & 0x7FFFFFFFu);
-                }
-            }
-        top = lane_max_u32(lane_max_u32(top, 16), 32);
-        const float up = row_scale(top);
-        rowf = a.scale / up;
-#pragma unroll
-        for (int s = 0; s < D / 32; ++s) {
-            float w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = x[8 * s + j] * up;
-            if constexpr (SPLIT) split8(w, qh[s], ql[s]);
-            else qh[s] = round8(w);
-        }
-    }
-
-    const int ntile = (sq.kv + 31) >> 5, per = (ntile + a.nsplit - 1) / a.nsplit;
+    const int ntile = (sq.kv + 31) >> 5, per = (ntile + a.nkeys - 1) / a.nkeys;
     const int t1 = min((split + 1) * per, ntile);
     int t = split * per + wave;
 
@@ -235,6 +217,42 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
         load(row);
         rows_of(t + 4, next);
     }
+    h8 qh[D / 32];
+    float rowf;
+    {
+        float x[D / 4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                f4 v = {0, 0, 0, 0};
+                if (has_row) v = load4(a.q, DT, tok * a.q_token + head * a.q_head + 64 * i + 16 * c + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[16 * i + j + e] = v[e];
+                    top = max(top, f_bits(v[e]) & 0x7FFFFFFFu);
+                }
+            }
+        top = lane_max_u32(lane_max_u32(top, 16), 32);
+        const float up = row_scale(top);
+        rowf = a.scale / up;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = x[8 * s + j] * up;
+            if constexpr (SPLIT) {
+                h8 lo;
+                split8(w, qh[s], lo);
+                if (wave == 0) sql[64 * s + lane] = lo;
+            } else {
+                qh[s] = round8(w);
+            }
+        }
+    }
+
+    if constexpr (SPLIT) __syncthreads();
 
     for (; t < t1; t += 4) {
         const int key0 = 32 * t;
@@ -260,8 +278,8 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
                 s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * i], s[u], 0, 0, 0);
                 s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * i + 1], s[u], 0, 0, 0);
                 if constexpr (SPLIT) {
-                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[2 * i], s[u], 0, 0, 0);
-                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[2 * i + 1], s[u], 0, 0, 0);
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, sql[64 * (2 * i) + lane], s[u], 0, 0, 0);
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, sql[64 * (2 * i + 1) + lane], s[u], 0, 0, 0);
                 }
             }
         }
@@ -344,8 +362,8 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     }
     const int ot = sq.q0 + r / a.G, oh = h * a.G + r % a.G;
     const int64_t orow = (int64_t)ot * a.Hq + oh, prow = (int64_t)split * a.T * a.Hq + orow;
-    const float inv = a.nsplit > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-    if (a.nsplit > 1 && part == 0) a.ml[prow] = (f2){top, sum};
+    const float inv = a.nkeys > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    if (part == 0) mark_row(a, a.nkeys, split, orow, top, sum);
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
         const int d = 64 * i + 4 * part;
@@ -353,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(so + (w * 16 + r) * OS + d) * f[w];
         v *= inv;
-        if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+        if (a.nkeys > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
         else store4(a.out, DT, ot * a.o_token + oh * a.o_head + d, v);
     }
 }
@@ -433,8 +451,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r32 = lane & 31, hf = lane >> 5;
-    const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.nsplit;
-    const int slot = a.nslots - 1 - ss / a.nsplit;  // a prompt's last rows see the most keys: first
+    const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.nrows;
+    const int slot = a.nslots - 1 - ss / a.nrows;  // a prompt's last rows see the most keys: first
     Seq sq;
     int64_t first;
     const int b = rows_of_slot(a, slot, sq, first);
@@ -455,7 +473,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     h8 qh[D / 16], ql[SPLIT ? D / 16 : 1];
     const float rowf = load_queries<D, DT>(a, tok * a.q_token + head * a.q_head + 8 * hf, qh, ql);
 
-    const int ntile = (min(wg_end, sq.kv) + kKeyTile - 1) / kKeyTile, per = (ntile + a.nsplit - 1) / a.nsplit;
+    const int ntile = (min(wg_end, sq.kv) + kKeyTile - 1) / kKeyTile, per = (ntile + a.nrows - 1) / a.nrows;
     const int t1 = min((split + 1) * per, ntile);
     int t = split * per;
     const int32_t* table = a.table + b * a.table_row;
@@ -611,18 +629,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     l = sum_halves(l);
     const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
     float f = nu * (1.0f / kPScale);
-    if (a.nsplit > 1) {
-        if (hf == 0) a.ml[prow] = (f2){m * rowf, l};
-    } else {
-        f *= l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    }
+    if (hf == 0) mark_row(a, a.nrows, split, orow, m * rowf, l);
+    if (a.nrows == 1) f *= l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
             const int d = 32 * i + 2 * j + 4 * hf;
             const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
-            if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+            if (a.nrows > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
             else store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
         }
 }
@@ -711,8 +726,8 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r32 = lane & 31, hf = lane >> 5;
-    const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.nsplit;
-    const int slot = a.nslots - 1 - ss / a.nsplit;  // a prompt's last rows see the most keys: first
+    const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.nrows;
+    const int slot = a.nslots - 1 - ss / a.nrows;  // a prompt's last rows see the most keys: first
     Seq sq;
     int64_t first;
     const int b = rows_of_slot(a, slot, sq, first);
@@ -730,7 +745,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
     h8 qh[D / 16], ql[SPLIT ? D / 16 : 1];
     const float rowf = load_queries<D, DT>(a, tok * a.q_token + head * a.q_head + 8 * hf, qh, ql);
 
-    const int ntile = (wg_end + kKeyTile - 1) / kKeyTile, per = (ntile + a.nsplit - 1) / a.nsplit;
+    const int ntile = (wg_end + kKeyTile - 1) / kKeyTile, per = (ntile + a.nrows - 1) / a.nrows;
     const int t0 = split * per, t1 = min(t0 + per, ntile);
     const uint8_t* const tiles = a.unpacked + ((int64_t)b * a.H + h) * a.tiles * tile_bytes<D>();
 
@@ -865,42 +880,83 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
     l = sum_halves(l);
     const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
     float f = nu * (1.0f / kPScale);
-    if (a.nsplit > 1) {
-        if (hf == 0) a.ml[prow] = (f2){m * rowf, l * f};
-    } else {
-        f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    }
+    if (hf == 0) mark_row(a, a.nrows, split, orow, m * rowf, l * f);
+    if (a.nrows == 1) f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
             const int d = 32 * i + 2 * j + 4 * hf;
             const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
-            if (a.nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+            if (a.nrows > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
             else store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
         }
 }
 
-// The splits of a row joined, in their order.
-template <int D>
+// Splits.  Single tokens: a split's keys cost a workgroup no more than its
+// start does while they are few, and one long sequence among short ones must
+// not be one workgroup's; so as many as bring a workgroup's keys down to
+// kSplitMin while compute units are idle, and to kSplitKeys at least.  Chunks:
+// the number that wastes the least of the last round of workgroups, each split
+// of at least kSplitRows keys.
+constexpr int kSplitMin = 128, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
+
+// The splits of a row joined: D/4 lanes a split and NG splits of a row at a
+// time, their sums then in the order of the splits.
+template <int D, int NG>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    constexpr int L = D / 4;
-    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    const int d = 4 * (threadIdx.x % L);
+    constexpr int L = D / 4, RW = 256 / L / NG;  // rows a workgroup
+    __shared__ __align__(16) float sv[NG > 1 ? 256 / L : 1][D];
+    __shared__ float sw[256 / L][kSplitMost];
     const int64_t n = (int64_t)a.T * a.Hq;
-    if (row >= n) return;
+    const int part = threadIdx.x / L, g = part % NG, d = 4 * (threadIdx.x % L);
+    const int64_t row = (int64_t)blockIdx.x * RW + part / NG;
     const int tok = (int)(row / a.Hq), head = (int)(row % a.Hq);
-    if (a.cu && (tok < a.cu[0] || tok >= a.cu[a.B])) return;
-    float top = -INFINITY, sum = 0.0f;
-    for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.ml[s * n + row].x);
-    const float safe = top == -INFINITY ? 0.0f : top;
+    bool mine = row < n && !(a.cu && (tok < a.cu[0] || tok >= a.cu[a.B]));
     f4 v = {0, 0, 0, 0};
-    for (int s = 0; s < a.nsplit; ++s) {
-        const f2 ml = a.ml[s * n + row];
-        const float f = fast_exp2(ml.x - safe);
-        sum += f * ml.y;
-        v += *reinterpret_cast<const f4*>(a.part + (s * n + row) * D + d) * f;
+    float sum = 0.0f;
+    // The splits' maxima and sums first, one or more a lane; sw: a split's weight.
+    {
+        constexpr int PER = kSplitMost / L;
+        const int lane = threadIdx.x % L;
+        f2 ml[PER];
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int s = lane + L * i;
+            ml[i] = mine && s < a.nsplit ? a.ml[s * n + row] : (f2){-INFINITY, 0.0f};
+            top = fmaxf(top, ml[i].x);
+        }
+#pragma unroll
+        for (int st = 1; st < L; st *= 2) top = fmaxf(top, __shfl_xor(top, st));
+        mine = mine && top != INFINITY;  // else the row is done
+        const float safe = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float f = fast_exp2(ml[i].x - safe);
+            sum += ml[i].y == 0.0f && ml[i].x == -INFINITY ? 0.0f : f * ml[i].y;
+            // An empty split's sums are not there: marked by a weight below zero.
+            sw[part][lane + L * i] = ml[i].y == 0.0f && ml[i].x == -INFINITY ? -1.0f : f;
+        }
+#pragma unroll
+        for (int st = 1; st < L; st *= 2) sum += __shfl_xor(sum, st);
     }
+    if (mine) {
+#pragma unroll 8
+        for (int s = g; s < a.nsplit; s += NG) {
+            const float f = sw[part][s];
+            if (f < 0.0f) continue;
+            v += *reinterpret_cast<const f4*>(a.part + (s * n + row) * D + d) * f;
+        }
+    }
+    if constexpr (NG > 1) {
+        *reinterpret_cast<f4*>(&sv[part][d]) = v;
+        __syncthreads();
+        if (g > 0) return;
+#pragma unroll
+        for (int i = 1; i < NG; ++i) v += *reinterpret_cast<const f4*>(&sv[part + i][d]);
+    }
+    if (!mine) return;
     v *= sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
     store4(a.out, a.dt, tok * a.o_token + head * a.o_head + d, v);
 }
@@ -908,7 +964,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // ------------------------------------------------------------------ host
 
 struct AttnPlan {
-    int keys, rows, nsplit, nslots;  // which kernels run, splits of the keys, slots of the rows kernels
+    int keys, rows, nslots;          // which kernels run, slots of the rows kernels
+    int nkeys, nrows, nsplit;        // splits of the keys: of the two kinds of kernels, room for
     int tiles;                       // of the unpacked copy of each sequence; 0: none
     size_t copy, bytes;              // of the copies, of the workspace
 };
@@ -918,27 +975,40 @@ struct AttnPlan {
 constexpr int kUnpackRows = 512;
 constexpr size_t kUnpackMost = (size_t)4 << 30;
 
-// Splits: enough workgroups for every compute unit twice, each with at least
-// 256 keys of the longest sequence that the table can hold.
-AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int n_cu) {
+AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int dtype, int n_cu) {
     const int G = Hq / H;
     AttnPlan p{};
     p.keys = G <= 16;
     p.rows = cu ? (int64_t)T * G > 16 : G > 16;
     p.nslots = cu ? (int)((int64_t)T * G / kRowTile) + B : B * ((G + kRowTile - 1) / kRowTile);
-    const int64_t wgs = (int64_t)H * (p.rows && T > 2 * B ? p.nslots : B);
-    int64_t s = std::max<int64_t>(1, (2 * n_cu + wgs - 1) / wgs);
-    s = std::min<int64_t>(s, std::max<int64_t>(1, capacity / 256));
-    s = std::min<int64_t>(s, 64);
-    if (wgs >= n_cu) s = 1;
-    p.nsplit = (int)s;
+    p.nkeys = p.nrows = 1;
+    if (p.keys) {
+        // With chunks among the sequences the single tokens are not what fills the units.
+        const int64_t wgs = (int64_t)B * H;
+        const int64_t idle = (int64_t)T * G > 16 * (int64_t)B ? 1 : std::min<int64_t>((2 * n_cu + wgs - 1) / wgs, capacity / kSplitMin);
+        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, B > 1 || !cu ? capacity / kSplitKeys : 1), kSplitMost));
+    }
+    if (p.rows) {
+        const int64_t wgs = (int64_t)p.nslots * H, room = (int64_t)n_cu * (D == 256 || (D == 128 && dtype == kF32) ? 1 : 2);
+        // A prompt's workgroups, the longest first, fill the last round by themselves.
+        const bool causal = wgs >= room && 2 * (int64_t)T >= capacity * B;
+        double best = 1e30;
+        for (int64_t s = 1; s <= 16 && (s == 1 || (s * kSplitRows <= capacity && wgs < 4 * room && !causal)); ++s) {
+            const double cost = (double)((wgs * s + room - 1) / room) / s * (1.0 + 0.02 * (s - 1));
+            if (cost < best) {
+                best = cost;
+                p.nrows = (int)s;
+            }
+        }
+    }
     if (p.rows && (int64_t)T * G >= (int64_t)kUnpackRows * B) {
         const int64_t tiles = (capacity + kKeyTile - 1) / kKeyTile;
         p.copy = (size_t)B * H * tiles * (kKeyTile * D * 4 + kHead);
         if (p.copy <= kUnpackMost) p.tiles = (int)tiles;
         else p.copy = 0;
     }
-    p.bytes = p.copy + (s > 1 ? (size_t)s * T * Hq * (D * 4 + 8) : 0);
+    p.nsplit = std::max(p.nkeys, p.nrows);
+    p.bytes = p.copy + (p.nsplit > 1 ? (size_t)p.nsplit * T * Hq * (D * 4 + 8) : 0);
     return p;
 }
 
@@ -955,13 +1025,13 @@ int cu_count() {
 
 template <int D, int KIND, int DT>
 void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-    if (p.keys) attn_keys_kernel<D, KIND, DT><<<(unsigned)a.B * a.H * a.nsplit, 256, 0, st>>>(a);
+    if (p.keys) attn_keys_kernel<D, KIND, DT><<<(unsigned)a.B * a.H * a.nkeys, 256, 0, st>>>(a);
     if (p.rows && p.tiles) {
         const int64_t items = (int64_t)a.B * a.H * a.tiles;
         attn_unpack_kernel<D, KIND><<<(unsigned)std::min<int64_t>(items, 2048), 256, 0, st>>>(a);
-        attn_tiles_kernel<D, DT><<<(unsigned)a.nslots * a.H * a.nsplit, 256, 0, st>>>(a);
+        attn_tiles_kernel<D, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
     } else if (p.rows) {
-        attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nsplit, 256, 0, st>>>(a);
+        attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
     }
 }
 
@@ -977,8 +1047,11 @@ void launch1(const AttnArgs& a, const AttnPlan& p, int kind, hipStream_t st) {
     if (kind == kInt8) launch2<D, kInt8>(a, p, st);
     else launch2<D, kFp8>(a, p, st);
     if (a.nsplit > 1) {
-        constexpr int rows = 256 / (D / 4);
-        attn_join_kernel<D><<<(unsigned)(((int64_t)a.T * a.Hq + rows - 1) / rows), 256, 0, st>>>(a);
+        // Few rows: all of a workgroup's lanes for one, so that many splits are read at once.
+        constexpr int NG = 256 / (D / 4);
+        const int64_t n = (int64_t)a.T * a.Hq;
+        if (n <= 2048) attn_join_kernel<D, NG><<<(unsigned)n, 256, 0, st>>>(a);
+        else attn_join_kernel<D, 1><<<(unsigned)((n + NG - 1) / NG), 256, 0, st>>>(a);
     }
 }
 
@@ -1020,11 +1093,12 @@ bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, boo
 
 extern "C" {
 
-int64_t i4_paged_attention_workspace(const i4_kv_cache* cache, int T, int B, int heads, int table_w, int has_cu) {
+int64_t i4_paged_attention_workspace(const i4_kv_cache* cache, int T, int B, int heads, int dtype, int table_w,
+                                     int has_cu) {
     int ps = 0;
     if (!check_shape(cache, T, B, heads, table_w, has_cu != 0, &ps)) return -2;
     if (T == 0 || B == 0) return 0;
-    return (int64_t)plan_attn(T, B, heads, cache->kv_heads, cache->head_dim, has_cu != 0, (int64_t)table_w << ps,
+    return (int64_t)plan_attn(T, B, heads, cache->kv_heads, cache->head_dim, has_cu != 0, (int64_t)table_w << ps, dtype,
                               cu_count())
         .bytes;
 }
@@ -1071,12 +1145,14 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
     a.dt = dtype;
     a.scale = scale * kLog2e;
     const AttnPlan p =
-        plan_attn(T, B, heads, a.H, cache->head_dim, dCu != nullptr, (int64_t)table_w << ps, cu_count());
+        plan_attn(T, B, heads, a.H, cache->head_dim, dCu != nullptr, (int64_t)table_w << ps, dtype, cu_count());
     if (p.bytes > 0 && (!dWork || work_bytes < (int64_t)p.bytes)) {
         bq_set_error("paged_attention: needs a workspace of %zu bytes, got %lld", p.bytes, (long long)work_bytes);
         return -4;
     }
     a.nsplit = p.nsplit;
+    a.nkeys = p.nkeys;
+    a.nrows = p.nrows;
     a.nslots = p.nslots;
     a.tiles = p.tiles;
     a.unpacked = static_cast<uint8_t*>(dWork);
