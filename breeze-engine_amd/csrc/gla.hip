@@ -21,7 +21,9 @@
 //
 // Numerics.  Products run on the fp16 matrix instructions with each operand
 // as two fp16 terms (hi, and what hi leaves; 22 bits and more) and three
-// products, fp32 sums; q, k and v given as bf16 or fp16 are one term.  A power
+// products, fp32 sums; q and k given as bf16 or fp16 are one term, and so are
+// the state and U where they only make rows of O of such a type (11 bits; the
+// state itself and U go on with two).  A power
 // of two for each tile, row or column puts the largest value where fp16 has
 // room; it changes no digit.  T is computed in fp32.  Sums of g are taken in
 // 64 bits: e^{G_i - G_j} would lose what G_i and G_j have in common.
@@ -528,18 +530,22 @@ __device__ inline void to_operand(const f4* x, float up, const float* rows, int 
     }
 }
 
-// A lower triangular factor (T or M) times 16 columns, both of two terms.
+// A lower triangular factor (T or M) of two terms times 16 columns of two, or
+// (rows of O that are rounded to a half type) of one.
+template <bool TWO>
 __device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, const h8* xl, f4* acc) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 0)], xh[0], (f4){0, 0, 0, 0});
+    if constexpr (TWO)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 0)], xl[0], acc[t]);
+        for (int t = 0; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 0)], xl[0], acc[t]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[t] = mfma16(lo[tri(t, 0)], xh[0], acc[t]);
 #pragma unroll
     for (int t = 2; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 1)], xh[1], acc[t]);
+    if constexpr (TWO)
 #pragma unroll
-    for (int t = 2; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 1)], xl[1], acc[t]);
+        for (int t = 2; t < 4; ++t) acc[t] = mfma16(hi[tri(t, 1)], xl[1], acc[t]);
 #pragma unroll
     for (int t = 2; t < 4; ++t) acc[t] = mfma16(lo[tri(t, 1)], xh[1], acc[t]);
 }
@@ -556,13 +562,15 @@ __device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, con
 // and 64 columns a workgroup took 5.0 us a chunk (the LDS reads of four waves,
 // 480 KB, alone 1.6).
 template <int DK, int DT, bool DELTA>
-__global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
+__global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaArgs a) {
     constexpr bool LO = DT == kF32;
     constexpr int NT = LO ? 2 : 1, ST = DK / 16, SS = DK / 32;  // tiles and slabs of the state's rows
     constexpr int kPart = 4 * SS * 1024, kBuf = kq_bytes(DK, LO);
     __shared__ __align__(1024) uint8_t skq[2][kBuf];       // operands of k, then of q
-    __shared__ __align__(1024) uint8_t ss[2][2 * SS * 1024];  // the state's operands, hi and lo
-    __shared__ __align__(1024) uint8_t su[2][4 * 1024];       // U's
+    // What the state's waves hand over: the state's operands and U's, one term of each
+    // for rows of O that are rounded to bf16 or fp16 (80 KB of LDS in all: two workgroups a unit).
+    __shared__ __align__(1024) uint8_t ss[2][NT * SS * 1024];
+    __shared__ __align__(1024) uint8_t su[2][NT * 2 * 1024];
     __shared__ __align__(1024) float sf[2][kFac];
     __shared__ float sunits[2][2][16];  // what a unit of those is worth, for each column
 
@@ -624,7 +632,7 @@ __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
             h8 oh[2][4], ol[2][4], sh[2], sl[2];
             const auto get = [&](int s) {
                 sh[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * s + 16 * lane);
-                sl[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane);
+                if constexpr (LO) sl[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     oh[s & 1][t] = op(qb, t * SS + s);
@@ -638,11 +646,12 @@ __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) qs[t] = mfma16(oh[s & 1][t], sh[s & 1], qs[t]);
+                if constexpr (LO) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) qs[t] = mfma16(oh[s & 1][t], sl[s & 1], qs[t]);
-                if constexpr (LO)
+                    for (int t = 0; t < 4; ++t) qs[t] = mfma16(oh[s & 1][t], sl[s & 1], qs[t]);
 #pragma unroll
                     for (int t = 0; t < 4; ++t) qs[t] = mfma16(ol[s & 1][t], sh[s & 1], qs[t]);
+                }
                 if (ch + 1 < nchunk)
 #pragma unroll
                     for (int i = 4 * s / SS; i < 4 * (s + 1) / SS; ++i) fetch(ch + 1, i);
@@ -662,11 +671,11 @@ __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 uh[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * s + 16 * lane);
-                ul[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * (2 + s) + 16 * lane);
+                if constexpr (LO) ul[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * (2 + s) + 16 * lane);
             }
             const float w3 = w2 * sunits[1][pair][r16];
             f4 acc[4];
-            tri_product(mh, ml, uh, ul, acc);
+            tri_product<LO>(mh, ml, uh, ul, acc);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -736,7 +745,7 @@ __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
 #pragma unroll
         for (int s = 0; s < SS; ++s) {
             *reinterpret_cast<h8*>(ss[pair] + 1024 * s + 16 * lane) = sh[s];
-            *reinterpret_cast<h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane) = sl[s];
+            if constexpr (LO) *reinterpret_cast<h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane) = sl[s];
         }
         if (c == 0) sunits[0][pair][r16] = sunit;
     };
@@ -798,7 +807,7 @@ __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
             h8 xh[2], xl[2];
             const float xup = to_top<12>(f_bits(column_top<4>(x)));
             to_operand<4>(x, xup, nullptr, c, xh, xl);
-            tri_product(th, tl, xh, xl, u);
+            tri_product<true>(th, tl, xh, xl, u);
             uworth = fac[2 * kChunk] * inverse_pow2(xup);
         } else {
 #pragma unroll
@@ -810,7 +819,7 @@ __global__ __launch_bounds__(256, 1) void gla_inter_kernel(GlaArgs a) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             *reinterpret_cast<h8*>(su[pair] + 1024 * s + 16 * lane) = uh[s];
-            *reinterpret_cast<h8*>(su[pair] + 1024 * (2 + s) + 16 * lane) = ul[s];
+            if constexpr (LO) *reinterpret_cast<h8*>(su[pair] + 1024 * (2 + s) + 16 * lane) = ul[s];
         }
         if (c == 0) sunits[1][pair][r16] = uunit;
         __syncthreads();

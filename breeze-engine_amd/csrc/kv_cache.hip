@@ -59,11 +59,19 @@ __device__ inline uint32_t quantize4(f4 x, uint32_t top, float& scale) {
         return 0;
     }
     if constexpr (KIND == kInt8) {
-        scale = bits_f(top) / 127.0f;
-        if (scale == 0.0f) return 0;
-        // Far below 1 the reciprocal would overflow and s / 2 lose a bit: both sides times 2^64.
-        const float up = top < 0x21800000u ? 0x1p64f : 1.0f;  // below 2^-60
-        const float s = scale * up, inv = 1.0f / s;
+        // max|x| / 127: the product with the rounded reciprocal, corrected once, is the
+        // quotient correctly rounded (the correction's remainder is exact) while nothing
+        // is subnormal.
+        constexpr float r127 = 1.0f / 127.0f;
+        const float q = bits_f(top) * r127;
+        scale = __builtin_fmaf(__builtin_fmaf(-q, 127.0f, bits_f(top)), r127, q);
+        float up = 1.0f;
+        if (top < 0x21800000u) {  // below 2^-60: s / 2 would lose a bit, the reciprocal overflow
+            scale = bits_f(top) / 127.0f;
+            if (scale == 0.0f) return 0;
+            up = 0x1p64f;
+        }
+        const float s = scale * up, inv = __builtin_amdgcn_rcpf(s);  // nearest() puts right what it is off
         uint32_t w = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
