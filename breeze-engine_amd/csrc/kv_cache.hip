@@ -95,27 +95,26 @@ __device__ inline uint32_t quantize4(f4 x, uint32_t top, float& scale) {
     }
 }
 
-template <int D, int KIND>
+template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a) {
     constexpr int L = D / 4, R = 256 / L;  // lanes a row, rows a pass
-    const int h = blockIdx.y >> 1, lane = threadIdx.x % L;
-    const bool val = blockIdx.y & 1;
+    const int lane = threadIdx.x % L;
+    const bool val = blockIdx.y;
     const void* src = val ? a.v : a.k;
     const int64_t ts = val ? a.v_token : a.k_token, hs = val ? a.v_head : a.k_head;
     uint8_t* pages = val ? a.vp : a.kp;
     float* scales = val ? a.vs : a.ks;
-    const int t0 = blockIdx.x * (R * kUnroll) + threadIdx.x / L;
+    const int64_t r0 = (int64_t)blockIdx.x * (R * kUnroll) + threadIdx.x / L, rows = (int64_t)a.T * a.H;
     f4 x[kUnroll];
     int64_t slot[kUnroll];
+    int head[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-        const int t = t0 + u * R;
-        slot[u] = -1;
-        x[u] = (f4){0, 0, 0, 0};
-        if (t < a.T) {
-            slot[u] = a.slots[t];
-            x[u] = load4(src, a.dt, t * ts + h * hs + lane * 4);
-        }
+        const int64_t r = min(r0 + u * R, rows - 1);
+        const int t = (int)((uint32_t)r / (uint32_t)a.H);
+        head[u] = (int)r - t * a.H;
+        slot[u] = a.slots[t];
+        x[u] = load4(src, DT, t * ts + head[u] * hs + lane * 4);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -123,59 +122,67 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = max(top, f_bits(x[u][i]) & 0x7FFFFFFFu);
         top = max_lanes<L>(top);
-        if (slot[u] < 0 || slot[u] >= a.n_slots) continue;
+        if (r0 + u * R >= rows || slot[u] < 0 || slot[u] >= a.n_slots) continue;
         float scale;
         const uint32_t w = quantize4<KIND>(x[u], top, scale);
-        const int64_t row = (((slot[u] >> a.pshift) * a.H + h) << a.pshift) + (slot[u] & ((1 << a.pshift) - 1));
+        const int64_t row = (((slot[u] >> a.pshift) * a.H + head[u]) << a.pshift) + (slot[u] & ((1 << a.pshift) - 1));
         *reinterpret_cast<uint32_t*>(pages + row * D + lane * 4) = w;
         if (lane == 0) scales[row] = scale;
     }
 }
 
-template <int D, int KIND>
+template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a) {
     constexpr int L = D / 4, R = 256 / L;
-    const int h = blockIdx.y >> 1, lane = threadIdx.x % L;
-    const bool val = blockIdx.y & 1;
+    const int lane = threadIdx.x % L;
+    const bool val = blockIdx.y;
     void* dst = val ? a.vo : a.ko;
     const uint8_t* pages = val ? a.vp : a.kp;
     const float* scales = val ? a.vs : a.ks;
-    const int t0 = blockIdx.x * (R * kUnroll) + threadIdx.x / L;
+    const int64_t r0 = (int64_t)blockIdx.x * (R * kUnroll) + threadIdx.x / L, rows = (int64_t)a.T * a.H;
     uint32_t w[kUnroll];
     float s[kUnroll];
+    bool is[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-        const int t = t0 + u * R;
-        w[u] = 0;
-        s[u] = 0.0f;
-        const int64_t slot = t < a.T ? a.slots[t] : -1;
-        if (slot >= 0 && slot < a.n_slots) {
-            const int64_t row = (((slot >> a.pshift) * a.H + h) << a.pshift) + (slot & ((1 << a.pshift) - 1));
-            w[u] = *reinterpret_cast<const uint32_t*>(pages + row * D + lane * 4);
-            s[u] = scales[row];
-        }
+        const int64_t r = min(r0 + u * R, rows - 1);
+        const int t = (int)((uint32_t)r / (uint32_t)a.H), h = (int)r - t * a.H;
+        int64_t slot = a.slots[t];
+        is[u] = slot >= 0 && slot < a.n_slots;
+        slot = is[u] ? slot : 0;  // read, not used
+        const int64_t row = (((slot >> a.pshift) * a.H + h) << a.pshift) + (slot & ((1 << a.pshift) - 1));
+        w[u] = *reinterpret_cast<const uint32_t*>(pages + row * D + lane * 4);
+        s[u] = scales[row];
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-        const int t = t0 + u * R;
-        if (t >= a.T) continue;
+        if (r0 + u * R >= rows) continue;
         const h2 lo = unpack2<KIND, false>(w[u]), hi = unpack2<KIND, true>(w[u]);
-        const f4 y = {(float)lo[0] * s[u], (float)lo[1] * s[u], (float)hi[0] * s[u], (float)hi[1] * s[u]};
-        store4(dst, a.dt, ((int64_t)t * a.H + h) * D + lane * 4, y);
+        f4 y = {(float)lo[0] * s[u], (float)lo[1] * s[u], (float)hi[0] * s[u], (float)hi[1] * s[u]};
+        if (!is[u]) y = (f4){0, 0, 0, 0};
+        store4(dst, DT, (r0 + u * R) * D + lane * 4, y);
     }
+}
+
+template <int D, int KIND, int DT>
+void launch3(const KvArgs& a, bool write, hipStream_t st) {
+    constexpr int per = 256 / (D / 4) * kUnroll;
+    const dim3 grid((unsigned)(((int64_t)a.T * a.H + per - 1) / per), 2);
+    if (write) kv_write_kernel<D, KIND, DT><<<grid, 256, 0, st>>>(a);
+    else kv_read_kernel<D, KIND, DT><<<grid, 256, 0, st>>>(a);
+}
+
+template <int D, int KIND>
+void launch2(const KvArgs& a, bool write, hipStream_t st) {
+    if (a.dt == kF32) launch3<D, KIND, kF32>(a, write, st);
+    else if (a.dt == kBF16) launch3<D, KIND, kBF16>(a, write, st);
+    else launch3<D, KIND, kF16>(a, write, st);
 }
 
 template <int D>
 void launch(const KvArgs& a, int kind, bool write, hipStream_t st) {
-    constexpr int per = 256 / (D / 4) * kUnroll;
-    const dim3 grid((a.T + per - 1) / per, 2 * a.H);
-    if (write) {
-        if (kind == kInt8) kv_write_kernel<D, kInt8><<<grid, 256, 0, st>>>(a);
-        else kv_write_kernel<D, kFp8><<<grid, 256, 0, st>>>(a);
-    } else {
-        if (kind == kInt8) kv_read_kernel<D, kInt8><<<grid, 256, 0, st>>>(a);
-        else kv_read_kernel<D, kFp8><<<grid, 256, 0, st>>>(a);
-    }
+    if (kind == kInt8) launch2<D, kInt8>(a, write, st);
+    else launch2<D, kFp8>(a, write, st);
 }
 
 int kv_call(const i4_kv_cache* c, KvArgs a, int T, int dtype, bool write, void* stream, const char* what) {
@@ -202,6 +209,10 @@ int kv_call(const i4_kv_cache* c, KvArgs a, int T, int dtype, bool write, void* 
     }
     if (dtype < kF32 || dtype > kF16 || T < 0) {
         bq_set_error("%s: needs a type of 0 to 2 and T >= 0 (got %d, %d)", what, dtype, T);
+        return -2;
+    }
+    if ((int64_t)T * c->kv_heads > INT32_MAX) {
+        bq_set_error("%s: %d tokens of %d heads are too many for one call", what, T, c->kv_heads);
         return -2;
     }
     if (T == 0) return 0;
