@@ -23,6 +23,7 @@ import ctypes
 from . import hip_backend as hb
 
 _dtypes = None  # torch dtype -> the library's number for it
+_current = None  # the current device's index
 
 
 class _CCache(ctypes.Structure):
@@ -32,9 +33,11 @@ class _CCache(ctypes.Structure):
 
 
 def _torch():
-    global _dtypes
-    torch = hb._import_torch()
-    if _dtypes is None:
+    global _dtypes, _current
+    torch = hb._torch
+    if torch is None or _dtypes is None:
+        torch = hb._import_torch()
+        _current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         _dtypes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
     return torch
 
@@ -56,38 +59,40 @@ def _rows(t, what):
 
 
 def _ints(t, shape, what):
-    torch = hb._torch
-    if t.dtype is not torch.int32 or tuple(t.shape) != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dtype is not hb._torch.int32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{what} must be int32 of shape {shape} with a contiguous last dimension, "
                          f"got {t.dtype} {tuple(t.shape)} (strides {t.stride()})")
     return t
 
 
-def _same_device(device, *tensors):
+def _same_device(index, *tensors):
+    """All tensors lie on GPU `index` (-1: a tensor that is not on one)."""
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors lie on {t.device} and {device}: all must be on one GPU")
-    if device.type != "cuda":
-        raise ValueError(f"tensors lie on {device}: they must be on a GPU")
-    hb._require_lib()
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"a tensor lies on {t.device}: all must be on one GPU")
+    if index < 0:
+        raise ValueError("tensors must be on a GPU")
+    if hb._lib is None:
+        hb._require_lib()
 
 
-class _Current:
-    """Makes a tensor's device the current one for a call, where it is another."""
+def _workspace(shape, kind, device):
+    """(tensor or None, bytes) of a call's workspace; what a shape needs is asked once."""
+    key = (kind, device.index, shape)
+    n = _needs.get(key)
+    if n is None:
+        query = (hb._lib.i4_paged_attention_workspace if kind == "paged"
+                 else hb._lib.i4_gated_linear_attention_workspace)
+        n = query(*shape)
+        if n < 0:
+            raise ValueError(hb.last_error())
+        if len(_needs) >= 4096:
+            _needs.clear()
+        _needs[key] = n
+    return (hb._torch.empty((n,), dtype=hb._torch.uint8, device=device) if n else None), n
 
-    def __init__(self, device):
-        torch = hb._torch
-        self._other = None
-        if device.index != torch.cuda.current_device():
-            self._other = torch.cuda.device(device)
 
-    def __enter__(self):
-        if self._other is not None:
-            self._other.__enter__()
-
-    def __exit__(self, *e):
-        if self._other is not None:
-            self._other.__exit__(*e)
+_needs = {}
 
 
 class KVCache:
@@ -126,7 +131,7 @@ class KVCache:
                 raise ValueError(f"cache tensors lie on {t.device} and {k.device}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = P, H, page, D
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self._c = _CCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, H, page, D,
                           kinds[k.dtype])
         self._p = ctypes.addressof(self._c)
@@ -156,22 +161,27 @@ def kv_write(cache, k, v, slots):
     to x / scale, ties to even.  e4m3: the scale is the smallest power of two
     that brings the row within 448.  A row that holds an infinity or NaN reads
     back as NaN."""
-    _torch()
+    torch = _torch()
     shape = (k.shape[0] if k.dim() else 0, cache.kv_heads, cache.head_dim)
-    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+    if k.shape != shape or v.shape != shape:
         raise ValueError(f"k and v must be [T, {cache.kv_heads}, {cache.head_dim}], got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
     dt = _type(k, "k")
     if v.dtype is not k.dtype:
         raise ValueError(f"k and v must have one type, got {k.dtype} and {v.dtype}")
     _ints(slots, (shape[0],), "slots")
-    _same_device(cache.device, k, v, slots)
+    _same_device(cache._index, k, v, slots)
     if shape[0] == 0:
         return
-    with _Current(cache.device):
-        k, v = _rows(k, "k"), _rows(v, "v")
-        hb._check_rc(hb._lib.i4_kv_write_dev(cache._p, k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2],
-                                             shape[0], dt, slots.data_ptr(), hb._torch_stream(k)), "i4_kv_write_dev")
+    if cache._index != _current():
+        with torch.cuda.device(cache.device):
+            return kv_write(cache, k, v, slots)
+    k, v = _rows(k, "k"), _rows(v, "v")
+    ks, vs = k.stride(), v.stride()
+    rc = hb._lib.i4_kv_write_dev(cache._p, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], shape[0], dt,
+                                 slots.data_ptr(), hb._torch_stream(k))
+    if rc:
+        hb._check_rc(rc, "i4_kv_write_dev")
 
 
 def kv_read(cache, slots, dtype):
@@ -183,12 +193,18 @@ def kv_read(cache, slots, dtype):
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     T = slots.shape[0] if slots.dim() else 0
     _ints(slots, (T,), "slots")
-    _same_device(cache.device, slots)
-    k, v = (torch.empty((T, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device) for _ in range(2))
+    _same_device(cache._index, slots)
+    if cache._index != _current():
+        with torch.cuda.device(cache.device):
+            return kv_read(cache, slots, dtype)
+    shape = (T, cache.kv_heads, cache.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=cache.device)
+    v = torch.empty(shape, dtype=dtype, device=cache.device)
     if T:
-        with _Current(cache.device):
-            hb._check_rc(hb._lib.i4_kv_read_dev(cache._p, k.data_ptr(), v.data_ptr(), T, _dtypes[dtype],
-                                                slots.data_ptr(), hb._torch_stream(k)), "i4_kv_read_dev")
+        rc = hb._lib.i4_kv_read_dev(cache._p, k.data_ptr(), v.data_ptr(), T, _dtypes[dtype], slots.data_ptr(),
+                                    hb._torch_stream(k))
+        if rc:
+            hb._check_rc(rc, "i4_kv_read_dev")
     return k, v
 
 
@@ -197,7 +213,7 @@ def _output(out, like, shape, what):
     if out is None:
         return torch.empty(shape, dtype=like.dtype, device=like.device)
     st = out.stride()
-    if out.dtype is not like.dtype or tuple(out.shape) != shape or out.device != like.device:
+    if out.dtype is not like.dtype or out.shape != shape or out.device != like.device:
         raise ValueError(f"{what} must be {like.dtype} {shape} on {like.device}, got {out.dtype} {tuple(out.shape)} on "
                          f"{out.device}")
     if st[2] != 1 or (st[0] | st[1]) & 3 or out.data_ptr() & 15 or st[1] < shape[2] or st[0] < shape[1] * st[1]:
@@ -247,9 +263,9 @@ def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=N
     products exactly.  fp32 queries and their probabilities keep 22 bits; with
     bf16 and fp16 the probabilities are rounded to fp16's 11."""
     torch = _torch()
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.kv_heads or not q.shape[1]:
+    T, heads, D = q.shape if q.dim() == 3 else (0, 0, 0)
+    if D != cache.head_dim or heads % cache.kv_heads or not heads:
         raise ValueError(f"q must be [T, a multiple of {cache.kv_heads} heads, {cache.head_dim}], got {tuple(q.shape)}")
-    T, heads, D = q.shape
     dt = _type(q, "q")
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [B, columns], got {tuple(block_table.shape)}")
@@ -264,29 +280,32 @@ def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=N
         scale = D ** -0.5
     elif not 0 < scale < 1e30:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    _same_device(cache.device, q, block_table, kv_lens, cu_q, out)
+    _same_device(cache._index, q, block_table, kv_lens, cu_q, out)
     given = out is not None
     out = _output(out, q, (T, heads, D), "out")
     if T == 0 or B == 0:
         return out
-    with _Current(cache.device):
-        q = _rows(q, "q")
-        if given:
-            _no_overlap(out, q, "q")
-        n = hb._lib.i4_paged_attention_workspace(cache._p, T, B, heads, dt, cols, cu_q is not None)
-        if n < 0:
-            raise ValueError(hb.last_error())
-        work = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None
-        hb._check_rc(hb._lib.i4_paged_attention_dev(
-            cache._p, q.data_ptr(), *q.stride()[:2], T, heads, dt, block_table.data_ptr(), block_table.stride(0), cols,
-            kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, scale, out.data_ptr(), *out.stride()[:2],
-            None if work is None else work.data_ptr(), n, hb._torch_stream(q)), "i4_paged_attention_dev")
+    if cache._index != _current():
+        with torch.cuda.device(cache.device):
+            return paged_attention(q, cache, block_table, kv_lens, cu_q, scale, out)
+    q = _rows(q, "q")
+    if given:
+        _no_overlap(out, q, "q")
+    lib = hb._lib
+    work, n = _workspace((cache.kv_heads, cache.page_size, D, T, B, heads, dt, cols, cu_q is not None), "paged", q.device)
+    qs, os = q.stride(), out.stride()
+    rc = lib.i4_paged_attention_dev(
+        cache._p, q.data_ptr(), qs[0], qs[1], T, heads, dt, block_table.data_ptr(), block_table.stride(0), cols,
+        kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, scale, out.data_ptr(), os[0], os[1],
+        None if work is None else work.data_ptr(), n, hb._torch_stream(q))
+    if rc:
+        hb._check_rc(rc, "i4_paged_attention_dev")
     return out
 
 
 def _gates(t, shape, what):
     torch = hb._torch
-    if tuple(t.shape) != shape or t.dtype not in _dtypes:
+    if t.shape != shape or t.dtype not in _dtypes:
         raise ValueError(f"{what} must be {shape} of float32, bfloat16 or float16, got {t.dtype} {tuple(t.shape)}")
     if t.dtype is not torch.float32 or (shape[1] > 1 and t.stride(1) != 1):
         t = t.to(torch.float32).contiguous()
@@ -295,7 +314,7 @@ def _gates(t, shape, what):
 
 def _state(t, shape, device, what):
     torch = hb._torch
-    if t.dtype is not torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() & 15:
+    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous() or t.data_ptr() & 15:
         raise ValueError(f"{what} must be contiguous, 16-byte aligned float32 {shape}, got {t.dtype} {tuple(t.shape)} "
                          f"(strides {t.stride()})")
 
@@ -356,7 +375,8 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
         scale = Dk ** -0.5
     elif not -1e30 < scale < 1e30:
         raise ValueError(f"scale must be finite, got {scale}")
-    _same_device(q.device, k, v, g, beta, state, cu_seqlens, state_out, out)
+    index = q.get_device()
+    _same_device(index, k, v, g, beta, state, cu_seqlens, state_out, out)
     given = out is not None
     out = _output(out, q, (T, Hv, Dv), "out")
     if state_out is None:
@@ -365,21 +385,27 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
         _no_overlap(state_out, state, "state")
     if B == 0:
         return out, state_out
-    with _Current(q.device):
-        q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
-        if given:
-            for t in (q, k, v, g, beta, state, state_out):
-                if t is not None:
-                    _apart(out, t)
-        n = hb._lib.i4_gated_linear_attention_workspace(T, B, Hk, Hv, Dk, Dv, dt, cu_seqlens is not None,
-                                                        beta is not None)
-        if n < 0:
-            raise ValueError(hb.last_error())
-        work = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None
-        hb._check_rc(hb._lib.i4_gated_linear_attention_dev(
-            q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], g.data_ptr(),
-            g.stride(0), None if beta is None else beta.data_ptr(), 0 if beta is None else beta.stride(0), T, Hk, Hv, Dk,
-            Dv, dt, None if cu_seqlens is None else cu_seqlens.data_ptr(), B, scale,
-            None if state is None else state.data_ptr(), state_out.data_ptr(), out.data_ptr(), *out.stride()[:2],
-            None if work is None else work.data_ptr(), n, hb._torch_stream(q)), "i4_gated_linear_attention_dev")
+    if index != _current():
+        with torch.cuda.device(q.device):
+            return gated_linear_attention(q, k, v, g, beta, state, cu_seqlens, scale, out, state_out)
+    q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    if given:
+        for t in (q, k, v, g, beta, state, state_out):
+            if t is not None:
+                _apart(out, t)
+    lib = hb._lib
+    if cu_seqlens is None:
+        work, n = None, 0
+    else:
+        work, n = _workspace((T, B, Hk, Hv, Dk, Dv, dt, True, beta is not None),
+                             "gla", q.device)
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    rc = lib.i4_gated_linear_attention_dev(
+        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], g.data_ptr(), g.stride(0),
+        None if beta is None else beta.data_ptr(), 0 if beta is None else beta.stride(0), T, Hk, Hv, Dk, Dv, dt,
+        None if cu_seqlens is None else cu_seqlens.data_ptr(), B, scale, None if state is None else state.data_ptr(),
+        state_out.data_ptr(), out.data_ptr(), os[0], os[1], None if work is None else work.data_ptr(), n,
+        hb._torch_stream(q))
+    if rc:
+        hb._check_rc(rc, "i4_gated_linear_attention_dev")
     return out, state_out

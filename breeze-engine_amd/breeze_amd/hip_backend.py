@@ -102,7 +102,7 @@ try:
     _lib.i4_kv_read_dev.restype = _i
     _lib.i4_kv_read_dev.argtypes = [_vp, _vp, _vp, _i, _i, _vp, _vp]
     _lib.i4_paged_attention_workspace.restype = _i64
-    _lib.i4_paged_attention_workspace.argtypes = [_vp, _i, _i, _i, _i, _i, _i]
+    _lib.i4_paged_attention_workspace.argtypes = [_i] * 9
     _lib.i4_paged_attention_dev.restype = _i
     _lib.i4_paged_attention_dev.argtypes = [_vp, _vp, _i64, _i64, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i,
                                             ctypes.c_float, _vp, _i64, _i64, _vp, _i64, _vp]

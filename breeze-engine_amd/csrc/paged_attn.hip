@@ -1093,8 +1093,14 @@ bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, boo
 
 extern "C" {
 
-int64_t i4_paged_attention_workspace(const i4_kv_cache* cache, int T, int B, int heads, int dtype, int table_w,
-                                     int has_cu) {
+int64_t i4_paged_attention_workspace(int kv_heads, int page_size, int head_dim, int T, int B, int heads, int dtype,
+                                     int table_w, int has_cu) {
+    i4_kv_cache c{};
+    c.num_pages = 1;
+    c.kv_heads = kv_heads;
+    c.page_size = page_size;
+    c.head_dim = head_dim;
+    const i4_kv_cache* cache = &c;
     int ps = 0;
     if (!check_shape(cache, T, B, heads, table_w, has_cu != 0, &ps)) return -2;
     if (T == 0 || B == 0) return 0;

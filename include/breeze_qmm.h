@@ -250,8 +250,8 @@ int i4_kv_read_dev(const i4_kv_cache* cache, void* dK, void* dV, int T, int dtyp
  * were.  scale > 0.  dOut [T, heads, head_dim] of dQ's type, strides as dQ's.
  * dWork: as many bytes as i4_paged_attention_workspace says for the same
  * shapes (0: may be NULL), 16-byte aligned. */
-int64_t i4_paged_attention_workspace(const i4_kv_cache* cache, int T, int B, int heads, int dtype, int table_w,
-                                     int has_cu);
+int64_t i4_paged_attention_workspace(int kv_heads, int page_size, int head_dim, int T, int B, int heads, int dtype,
+                                     int table_w, int has_cu);
 int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
                            int dtype, const int32_t* dTable, int64_t table_row, int table_w, const int32_t* dKvLens,
                            const int32_t* dCu, int B, float scale, void* dOut, int64_t o_token, int64_t o_head,
