@@ -48,6 +48,7 @@ struct AttnArgs {
     f2* ml;             // [nsplit][T * Hq]: maximum and sum; a first one of (infinity, 0): the row is done
     int64_t table_row;
     int T, B, Hq, H, G, P, pshift, table_w, nslots, dt;
+    int few;                   // rows up to which a sequence is attn_keys_kernel's
     int nsplit, nkeys, nrows;  // splits that the workspace has room for, and those of the two kinds of kernels
     float scale;  // softmax scale * log2(e)
 };
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     const int h = blockIdx.x % a.H, bs = blockIdx.x / a.H, split = bs % a.nkeys, b = bs / a.nkeys;
     const Seq sq = sequence(a, b);
     const int rows = sq.n * a.G;
-    if (rows <= 0 || rows > 16) return;
+    if (rows <= 0 || rows > a.few) return;
     const int r16 = lane & 15, c = lane >> 4;
     const int32_t* table = a.table + b * a.table_row;
 
@@ -271,17 +272,19 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
         f4 s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            s[u] = (f4){0, 0, 0, 0};
+            f4 s1 = {0, 0, 0, 0};  // a chain of its own: one tile is all that a wave may have
+            s[u] = s1;
 #pragma unroll
             for (int i = 0; i < KC; ++i) {
                 const h8 k0 = unpack8<KIND>(kraw[u][i].x, kraw[u][i].y), k1 = unpack8<KIND>(kraw[u][i].z, kraw[u][i].w);
                 s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * i], s[u], 0, 0, 0);
-                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * i + 1], s[u], 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * i + 1], s1, 0, 0, 0);
                 if constexpr (SPLIT) {
                     s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, sql[64 * (2 * i) + lane], s[u], 0, 0, 0);
-                    s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, sql[64 * (2 * i + 1) + lane], s[u], 0, 0, 0);
+                    s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, sql[64 * (2 * i + 1) + lane], s1, 0, 0, 0);
                 }
             }
+            s[u] += s1;
         }
         float x[8], vw[8];
         bool see[8];
@@ -406,7 +409,7 @@ __device__ inline int rows_of_slot(const AttnArgs& a, int slot, Seq& sq, int64_t
     sq = sequence(a, b);
     const int64_t rows = (int64_t)sq.n * a.G;
     first = (slot - (a.cu ? (int64_t)sq.q0 * a.G / kRowTile + b : (int64_t)b * per)) * kRowTile;
-    return rows <= 16 || first < 0 || first >= rows ? -1 : b;
+    return rows <= a.few || first < 0 || first >= rows ? -1 : b;
 }
 
 // A row's queries as operands (values 16 s + 8 (lane / 32) + 0..7 for slab s,
@@ -664,7 +667,7 @@ __global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
         const int tile = (int)(it % a.tiles), h = (int)(it / a.tiles % a.H), b = (int)(it / a.tiles / a.H);
         const Seq sq = sequence(a, b);
-        if (tile * kKeyTile >= sq.kv || (int64_t)sq.n * a.G <= 16) continue;
+        if (tile * kKeyTile >= sq.kv || (int64_t)sq.n * a.G <= a.few) continue;
         const int32_t* table = a.table + b * a.table_row;
         uint8_t* out = a.unpacked + it * tile_bytes<D>();
         if (wave == 0) {
@@ -899,7 +902,8 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 // kSplitMin while compute units are idle, and to kSplitKeys at least.  Chunks:
 // the number that wastes the least of the last round of workgroups, each split
 // of at least kSplitRows keys.
-constexpr int kSplitMin = 128, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
+constexpr int kFewRows = 16;
+constexpr int kSplitMin = 64, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
 
 // The splits of a row joined: D/4 lanes a split and NG splits of a row at a
 // time, their sums then in the order of the splits.
@@ -978,15 +982,17 @@ constexpr size_t kUnpackMost = (size_t)4 << 30;
 AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int dtype, int n_cu) {
     const int G = Hq / H;
     AttnPlan p{};
-    p.keys = G <= 16;
-    p.rows = cu ? (int64_t)T * G > 16 : G > 16;
+    p.rows = cu ? (int64_t)T * G > kFewRows : G > kFewRows;
+    // One sequence alone is never worth a second launch that may find nothing to do.
+    p.keys = G <= kFewRows && !(p.rows && B == 1);
     p.nslots = cu ? (int)((int64_t)T * G / kRowTile) + B : B * ((G + kRowTile - 1) / kRowTile);
     p.nkeys = p.nrows = 1;
     if (p.keys) {
         // With chunks among the sequences the single tokens are not what fills the units.
         const int64_t wgs = (int64_t)B * H;
-        const int64_t idle = (int64_t)T * G > 16 * (int64_t)B ? 1 : std::min<int64_t>((2 * n_cu + wgs - 1) / wgs, capacity / kSplitMin);
-        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, B > 1 || !cu ? capacity / kSplitKeys : 1), kSplitMost));
+        const int64_t fill = (2 * n_cu + wgs - 1) / wgs;
+        const int64_t idle = (int64_t)T * G > kFewRows * (int64_t)B ? 1 : std::min<int64_t>(fill, capacity / kSplitMin);
+        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), kSplitMost));
     }
     if (p.rows) {
         const int64_t wgs = (int64_t)p.nslots * H, room = (int64_t)n_cu * (D == 256 || (D == 128 && dtype == kF32) ? 1 : 2);
@@ -1158,6 +1164,7 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
     }
     a.nsplit = p.nsplit;
     a.nkeys = p.nkeys;
+    a.few = p.keys ? kFewRows : 0;
     a.nrows = p.nrows;
     a.nslots = p.nslots;
     a.tiles = p.tiles;
