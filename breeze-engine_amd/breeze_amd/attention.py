@@ -234,11 +234,11 @@ def _no_overlap(out, t, what):
         raise ValueError(f"out overlaps {what}: it may be {what} itself, or apart from it")
 
 
-def _apart(out, t):
-    """`out` shares no memory with an input of a call that reads it late."""
+def _apart(out, t, what):
+    """An output shares no memory with an input of a call that reads it late."""
     a, b = _span(out), _span(t)
     if a[0] < b[1] and b[0] < a[1]:
-        raise ValueError("out overlaps an input")
+        raise ValueError(f"{what} overlaps an input")
 
 
 def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=None):
@@ -379,7 +379,8 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
     _same_device(index, k, v, g, beta, state, cu_seqlens, state_out, out)
     given = out is not None
     out = _output(out, q, (T, Hv, Dv), "out")
-    if state_out is None:
+    state_given = state_out is not None
+    if not state_given:
         state_out = torch.empty(shape, dtype=torch.float32, device=q.device)
     elif state is not None:
         _no_overlap(state_out, state, "state")
@@ -392,7 +393,11 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
     if given:
         for t in (q, k, v, g, beta, state, state_out):
             if t is not None:
-                _apart(out, t)
+                _apart(out, t, "out")
+    if state_given:
+        for t in (q, k, v, g, beta):
+            if t is not None:
+                _apart(state_out, t, "state_out")
     lib = hb._lib
     if cu_seqlens is None:
         work, n = None, 0

@@ -933,8 +933,8 @@ bool check(int T, int B, int Hk, int Hv, int Dk, int Dv, int dtype, bool cu) {
                      T, B, Hk, Hv, Dk, Dv, dtype);
         return false;
     }
-    // Workgroups are counted in 32 bits.
-    if (((int64_t)T / kChunk + B) * Hk > INT32_MAX / 2 || (int64_t)B * Hv * (Dv / 16) > INT32_MAX / 2) {
+    // A launch has fewer than 2^24 workgroups.
+    if (((int64_t)T / kChunk + B) * Hk > (1 << 23) || (int64_t)B * Hv * (Dv / 16) > (1 << 23)) {
         bq_set_error("gated_linear_attention: %d tokens in %d sequences are too many for one call", T, B);
         return false;
     }

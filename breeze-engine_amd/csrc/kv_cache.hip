@@ -211,7 +211,7 @@ int kv_call(const i4_kv_cache* c, KvArgs a, int T, int dtype, bool write, void* 
         bq_set_error("%s: needs a type of 0 to 2 and T >= 0 (got %d, %d)", what, dtype, T);
         return -2;
     }
-    if ((int64_t)T * c->kv_heads > INT32_MAX) {
+    if ((int64_t)T * c->kv_heads > (1 << 27)) {  // a launch has fewer than 2^24 workgroups
         bq_set_error("%s: %d tokens of %d heads are too many for one call", what, T, c->kv_heads);
         return -2;
     }

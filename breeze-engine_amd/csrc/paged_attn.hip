@@ -42,13 +42,14 @@ struct AttnArgs {
     const int32_t* table;
     const int32_t* kv_lens;
     const int32_t* cu;  // null: one token a sequence
-    uint8_t* unpacked;  // [B][H][tiles]: the copy that long chunks read
+    uint8_t* unpacked;  // [copies][H][tiles]: the copies that long chunks read
     int tiles;          // of 64 keys, in the whole table
+    int by_seq;         // a copy for each sequence; else for those of kBigRows rows or more
     float* part;        // [nsplit][T * Hq][D] when nsplit > 1
     f2* ml;             // [nsplit][T * Hq]: maximum and sum; a first one of (infinity, 0): the row is done
     int64_t table_row;
     int T, B, Hq, H, G, P, pshift, table_w, nslots, dt;
-    int few;                   // rows up to which a sequence is attn_keys_kernel's
+    int few, big;              // attn_rows_kernel's sequences have more than `few` and fewer than `big` rows
     int nsplit, nkeys, nrows;  // splits that the workspace has room for, and those of the two kinds of kernels
     float scale;  // softmax scale * log2(e)
 };
@@ -389,8 +390,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
 
 constexpr int kRowTile = 128, kKeyTile = 64;
 
-// The 128 rows of a slot: their sequence (-1: none, or one of the other
-// kernel's) and the first of them.  Sequence b's tiles take the slots from
+// The 128 rows of a slot: their sequence (-1: none) and the first of them.  Sequence b's tiles take the slots from
 // cu[b] * G / 128 + b on, which leaves room for all without a pass over the lengths.
 __device__ inline int rows_of_slot(const AttnArgs& a, int slot, Seq& sq, int64_t& first) {
     const int per = (a.G + kRowTile - 1) / kRowTile;
@@ -409,7 +409,7 @@ __device__ inline int rows_of_slot(const AttnArgs& a, int slot, Seq& sq, int64_t
     sq = sequence(a, b);
     const int64_t rows = (int64_t)sq.n * a.G;
     first = (slot - (a.cu ? (int64_t)sq.q0 * a.G / kRowTile + b : (int64_t)b * per)) * kRowTile;
-    return rows <= a.few || first < 0 || first >= rows ? -1 : b;
+    return first < 0 || first >= rows ? -1 : b;
 }
 
 // A row's queries as operands (values 16 s + 8 (lane / 32) + 0..7 for slab s,
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     int64_t first;
     const int b = rows_of_slot(a, slot, sq, first);
     const int64_t rows = (int64_t)sq.n * a.G;
-    if (b < 0) return;
+    if (b < 0 || rows <= a.few || rows >= a.big) return;
     const int64_t row = first + 32 * wave + r32;
     const bool has_row = row < rows;
     const int tok_in = has_row ? (int)(row / a.G) : 0;
@@ -654,6 +654,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
 // instructions' operands (1 KB each, 16 bytes a lane), V transposed, with the
 // scales beside them.  Tiles then come straight to LDS.
 
+// Rows from which on a sequence has a copy where not all have one.  Two such
+// sequences' first rows are that far apart, so first row / kBigRows tells them apart.
+constexpr int kBigRows = 256;
+__device__ inline int copy_of(const AttnArgs& a, const Seq& sq, int b) {
+    return a.by_seq ? b : (int)((int64_t)sq.q0 * a.G / kBigRows);
+}
+
 constexpr int kHead = 1024;  // a tile's scales: ks[64], vs[64], 1 where a key is not there [64], largest vs, any not there
 template <int D>
 constexpr int tile_bytes() { return kKeyTile * D * 4 + kHead; }
@@ -667,9 +674,15 @@ __global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
         const int tile = (int)(it % a.tiles), h = (int)(it / a.tiles % a.H), b = (int)(it / a.tiles / a.H);
         const Seq sq = sequence(a, b);
-        if (tile * kKeyTile >= sq.kv || (int64_t)sq.n * a.G <= a.few) continue;
+        if ((int64_t)sq.n * a.G < a.big) {
+            // None of this sequence's: on to the next one's first.
+            const int64_t next = (int64_t)(b + 1) * a.H * a.tiles;
+            it += (next - 1 - it) / gridDim.x * gridDim.x;
+            continue;
+        }
+        if (tile * kKeyTile >= sq.kv) continue;
         const int32_t* table = a.table + b * a.table_row;
-        uint8_t* out = a.unpacked + it * tile_bytes<D>();
+        uint8_t* out = a.unpacked + (((int64_t)copy_of(a, sq, b) * a.H + h) * a.tiles + tile) * tile_bytes<D>();
         if (wave == 0) {
             const int64_t at = group_row(a, table, h, kKeyTile * tile + (lane & ~15), sq.kv);
             const bool bad = at < 0 || kKeyTile * tile + lane >= sq.kv;
@@ -734,8 +747,8 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
     Seq sq;
     int64_t first;
     const int b = rows_of_slot(a, slot, sq, first);
-    if (b < 0) return;
     const int64_t rows = (int64_t)sq.n * a.G, row = first + 32 * wave + r32;
+    if (b < 0 || rows < a.big) return;
     const bool has_row = row < rows;
     const int tok_in = has_row ? (int)(row / a.G) : 0;
     const int tok = sq.q0 + tok_in, head = h * a.G + (has_row ? (int)(row % a.G) : 0);
@@ -750,7 +763,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 
     const int ntile = (wg_end + kKeyTile - 1) / kKeyTile, per = (ntile + a.nrows - 1) / a.nrows;
     const int t0 = split * per, t1 = min(t0 + per, ntile);
-    const uint8_t* const tiles = a.unpacked + ((int64_t)b * a.H + h) * a.tiles * tile_bytes<D>();
+    const uint8_t* const tiles = a.unpacked + ((int64_t)copy_of(a, sq, b) * a.H + h) * a.tiles * tile_bytes<D>();
 
     f16 o[D / 32];
 #pragma unroll
@@ -903,6 +916,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 // the number that wastes the least of the last round of workgroups, each split
 // of at least kSplitRows keys.
 constexpr int kFewRows = 16;
+constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer than 2^32
 constexpr int kSplitMin = 64, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
 
 // The splits of a row joined: D/4 lanes a split and NG splits of a row at a
@@ -970,13 +984,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 struct AttnPlan {
     int keys, rows, nslots;          // which kernels run, slots of the rows kernels
     int nkeys, nrows, nsplit;        // splits of the keys: of the two kinds of kernels, room for
-    int tiles;                       // of the unpacked copy of each sequence; 0: none
+    int tiles, by_seq, direct;       // of an unpacked copy, 0: none; one for each sequence; attn_rows_kernel runs
     size_t copy, bytes;              // of the copies, of the workspace
 };
 
-// Rows a sequence from which on its keys are unpacked once for all of them, and
-// the most that the copies may take.
-constexpr int kUnpackRows = 512;
+// Copies are made for calls of kUnpackRows rows or more: of every sequence where
+// they have kUnpackMean rows on average, else of those of kBigRows or more; at
+// most kUnpackMost bytes.
+constexpr int kUnpackRows = 512, kUnpackMean = 64;
 constexpr size_t kUnpackMost = (size_t)4 << 30;
 
 AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int dtype, int n_cu) {
@@ -992,14 +1007,14 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
         const int64_t wgs = (int64_t)B * H;
         const int64_t fill = (2 * n_cu + wgs - 1) / wgs;
         const int64_t idle = (int64_t)T * G > kFewRows * (int64_t)B ? 1 : std::min<int64_t>(fill, capacity / kSplitMin);
-        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), kSplitMost));
+        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), std::min<int64_t>(kSplitMost, kMostBlocks / wgs)));
     }
     if (p.rows) {
         const int64_t wgs = (int64_t)p.nslots * H, room = (int64_t)n_cu * (D == 256 || (D == 128 && dtype == kF32) ? 1 : 2);
         // A prompt's workgroups, the longest first, fill the last round by themselves.
         const bool causal = wgs >= room && 2 * (int64_t)T >= capacity * B;
         double best = 1e30;
-        for (int64_t s = 1; s <= 16 && (s == 1 || (s * kSplitRows <= capacity && wgs < 4 * room && !causal)); ++s) {
+        for (int64_t s = 1; s <= 16 && (s == 1 || (s * kSplitRows <= capacity && wgs < 4 * room && !causal && s * wgs <= kMostBlocks)); ++s) {
             const double cost = (double)((wgs * s + room - 1) / room) / s * (1.0 + 0.02 * (s - 1));
             if (cost < best) {
                 best = cost;
@@ -1007,11 +1022,17 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
             }
         }
     }
-    if (p.rows && (int64_t)T * G >= (int64_t)kUnpackRows * B) {
-        const int64_t tiles = (capacity + kKeyTile - 1) / kKeyTile;
-        p.copy = (size_t)B * H * tiles * (kKeyTile * D * 4 + kHead);
-        if (p.copy <= kUnpackMost) p.tiles = (int)tiles;
-        else p.copy = 0;
+    p.direct = p.rows;
+    if (p.rows && (int64_t)T * G >= kUnpackRows) {
+        const int64_t tiles = (capacity + kKeyTile - 1) / kKeyTile, some = (int64_t)T * G / kBigRows + 1;
+        const size_t one = (size_t)H * tiles * (kKeyTile * D * 4 + kHead);
+        p.by_seq = (int64_t)T * G >= (int64_t)kUnpackMean * B && (one == 0 || (size_t)B <= kUnpackMost / one);
+        const int64_t copies = p.by_seq ? B : some;
+        if (one > 0 && (size_t)copies <= kUnpackMost / one) {
+            p.tiles = (int)tiles;
+            p.copy = copies * one;
+            p.direct = !p.by_seq;
+        }
     }
     p.nsplit = std::max(p.nkeys, p.nrows);
     p.bytes = p.copy + (p.nsplit > 1 ? (size_t)p.nsplit * T * Hq * (D * 4 + 8) : 0);
@@ -1032,12 +1053,11 @@ int cu_count() {
 template <int D, int KIND, int DT>
 void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     if (p.keys) attn_keys_kernel<D, KIND, DT><<<(unsigned)a.B * a.H * a.nkeys, 256, 0, st>>>(a);
-    if (p.rows && p.tiles) {
+    if (p.direct) attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
+    if (p.tiles) {
         const int64_t items = (int64_t)a.B * a.H * a.tiles;
         attn_unpack_kernel<D, KIND><<<(unsigned)std::min<int64_t>(items, 2048), 256, 0, st>>>(a);
         attn_tiles_kernel<D, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
-    } else if (p.rows) {
-        attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
     }
 }
 
@@ -1086,9 +1106,10 @@ bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, boo
                      c->kv_heads, T, B, heads, table_w);
         return false;
     }
-    // Workgroups and rows are counted in 32 bits.
-    if ((int64_t)T * heads > INT32_MAX / 64 || (int64_t)B * c->kv_heads > INT32_MAX / 64) {
-        bq_set_error("paged_attention: %d tokens of %d heads in %d sequences are too many for one call", T, heads, B);
+    // A launch has fewer than 2^24 workgroups, and keys are counted in 32 bits with some room.
+    if ((int64_t)T * heads > (1 << 28) || (int64_t)B * c->kv_heads > kMostBlocks || table_w > ((1 << 30) >> s)) {
+        bq_set_error("paged_attention: %d tokens of %d heads in %d sequences of up to %d pages are too much for one call", T,
+                     heads, B, table_w);
         return false;
     }
     *pshift = s;
@@ -1165,6 +1186,8 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
     a.nsplit = p.nsplit;
     a.nkeys = p.nkeys;
     a.few = p.keys ? kFewRows : 0;
+    a.by_seq = p.by_seq;
+    a.big = !p.tiles ? INT32_MAX : p.by_seq ? a.few + 1 : kBigRows;
     a.nrows = p.nrows;
     a.nslots = p.nslots;
     a.tiles = p.tiles;

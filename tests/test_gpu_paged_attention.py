@@ -122,6 +122,16 @@ def test_long_chunks(att, kind, dtype, heads, H, D, page, q_lens, ctx, extra):
     _run(att, 41, kind, dtype, heads, H, D, page, q_lens, ctx, extra)
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("heads,H,D", [(6, 1, 256), (8, 2, 128), (12, 3, 64)])
+def test_long_chunks_among_many_sequences(att, kind, dtype, heads, H, D):
+    """Copies for the long chunks only, beside single tokens and short chunks."""
+    q_lens = [1, 3, 1, 130, 1, 1, 20, 0, 1, 1, 75, 64, 1, 1, 1, 1, 1, 90] + [1] * 12
+    ctx = [7 * i % 131 for i in range(len(q_lens))]
+    _run(att, 42, kind, dtype, heads, H, D, 16, q_lens, ctx)
+
+
 @pytest.mark.parametrize("heads", [17, 128, 129, 300])
 def test_many_heads_of_one_key_head(att, heads):
     _run(att, 5, "int8", "bf16", heads, 1, 64, 16, [1, 1], [40, 3], single=True)

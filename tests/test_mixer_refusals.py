@@ -109,9 +109,9 @@ def test_outputs_and_overlaps():
     att._no_overlap(buf[:2], buf[3:], "q")
     with pytest.raises(ValueError):
         att._no_overlap(buf[1:], buf[:4], "q")
-    att._apart(buf[:2], buf[2:])
+    att._apart(buf[:2], buf[2:], "out")
     with pytest.raises(ValueError):
-        att._apart(buf[:2], buf[1:])
+        att._apart(buf[:2], buf[1:], "out")
 
 
 def _c_cache(**kw):
