@@ -49,6 +49,7 @@ struct AttnArgs {
     f2* ml;             // [nsplit][T * Hq]: maximum and sum; a first one of (infinity, 0): the row is done
     int64_t table_row;
     int T, B, Hq, H, G, P, pshift, table_w, nslots, dt;
+    int ntile16;               // workgroups for a sequence's rows in attn_keys_kernel
     int few, big;              // attn_rows_kernel's sequences have more than `few` and fewer than `big` rows
     int nsplit, nkeys, nrows;  // splits that the workspace has room for, and those of the two kinds of kernels
     float scale;  // softmax scale * log2(e)
@@ -147,9 +148,9 @@ __device__ inline h8 round8(const float* w) {
 
 // ------------------------------------------------------------------ few rows: the keys shared out
 //
-// One workgroup for a sequence's up to 16 rows (new tokens times the query
-// heads of one key-value head), one key-value head and one split of the keys;
-// its four waves take tiles of 32 keys in turn.  Bound by HBM: the next tile's
+// One workgroup for 16 of a sequence's up to few_rows() rows (new tokens times the
+// query heads of one key-value head), one key-value head and one split of the
+// keys; its four waves take tiles of 32 keys in turn.  Bound by HBM: the next tile's
 // keys and values are on their way while this one is computed, 16 KB a wave
 // (D = 256), and no wave waits for another before the end.
 
@@ -166,17 +167,19 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     __shared__ __align__(16) h8 sql[SPLIT ? D / 32 * 64 : 1];  // the queries' second terms, the same for all waves
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.H, bs = blockIdx.x / a.H, split = bs % a.nkeys, b = bs / a.nkeys;
+    const int h = blockIdx.x % a.H, tile16 = blockIdx.x / a.H % a.ntile16, bs = blockIdx.x / a.H / a.ntile16;
+    const int split = bs % a.nkeys, b = bs / a.nkeys;
     const Seq sq = sequence(a, b);
-    const int rows = sq.n * a.G;
-    if (rows <= 0 || rows > a.few) return;
+    if ((int64_t)sq.n * a.G > a.few) return;
+    const int row0 = 16 * tile16, rows = min(sq.n * a.G - row0, 16);  // this workgroup's
+    if (rows <= 0) return;
     const int r16 = lane & 15, c = lane >> 4;
     const int32_t* table = a.table + b * a.table_row;
 
     // The query operand: row r16, values 64 i + 16 c + 8 half + 0..7 for slab 2 i + half.
     const bool has_row = r16 < rows;
-    const int tok = sq.q0 + (has_row ? r16 / a.G : 0), head = h * a.G + (has_row ? r16 % a.G : 0);
-    const int last = has_row ? sq.kv - sq.n + r16 / a.G : -1;  // the last key that the row sees
+    const int row = row0 + (has_row ? r16 : 0), tok = sq.q0 + row / a.G, head = h * a.G + row % a.G;
+    const int last = has_row ? sq.kv - sq.n + row / a.G : -1;  // the last key that the row sees
     const int ntile = (sq.kv + 31) >> 5, per = (ntile + a.nkeys - 1) / a.nkeys;
     const int t1 = min((split + 1) * per, ntile);
     int t = split * per + wave;
@@ -190,7 +193,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     f4 ksc[2], vsc[2];
     _Float16* vt = reinterpret_cast<_Float16*>(lds) + wave * (32 * VS);
 
-    int64_t row[2];
+    int64_t at2[2];
     const auto rows_of = [&](int tile, int64_t* r) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) r[u] = group_row(a, table, h, 32 * tile + 16 * u, sq.kv);
@@ -215,8 +218,8 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
     };
     int64_t next[2] = {-1, -1};
     if (t < t1) {
-        rows_of(t, row);
-        load(row);
+        rows_of(t, at2);
+        load(at2);
         rows_of(t + 4, next);
     }
     h8 qh[D / 32];
@@ -258,14 +261,14 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
 
     for (; t < t1; t += 4) {
         const int key0 = 32 * t;
-        const bool tail = key0 + 32 > sq.kv || row[0] < 0 || row[1] < 0;
+        const bool tail = key0 + 32 > sq.kv || at2[0] < 0 || at2[1] < 0;
         // Values to LDS, [key][d] in fp16.
 #pragma unroll
         for (int i = 0; i < VC; ++i) {
             constexpr int per_row = D / 16;
             const int chunk = lane + 64 * i, kr = chunk / per_row;
             u4 w = vraw[i];
-            if (KIND == kFp8 && tail && (key0 + kr >= sq.kv || row[kr >> 4] < 0)) w = (u4){0, 0, 0, 0};
+            if (KIND == kFp8 && tail && (key0 + kr >= sq.kv || at2[kr >> 4] < 0)) w = (u4){0, 0, 0, 0};
             h8* dst = reinterpret_cast<h8*>(vt + kr * VS + 16 * (chunk % per_row));
             dst[0] = unpack8<KIND>(w.x, w.y);
             dst[1] = unpack8<KIND>(w.z, w.w);
@@ -293,15 +296,15 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int u = j >> 2, key = key0 + 16 * u + 4 * c + (j & 3);
-            see[j] = key <= last && row[u] >= 0;
+            see[j] = key <= last && at2[u] >= 0;
             x[j] = see[j] ? s[u][j & 3] * ksc[u][j & 3] : -INFINITY;
             vw[j] = see[j] ? vsc[u][j & 3] : 0.0f;
             top = fmaxf(top, x[j]);
             vmax = fmaxf(vmax, vw[j]);
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) row[u] = next[u];
-        if (t + 4 < t1) load(row);
+        for (int u = 0; u < 2; ++u) at2[u] = next[u];
+        if (t + 4 < t1) load(at2);
         rows_of(t + 8, next);
 
         top = max_halves(max_rows16(top));
@@ -364,7 +367,7 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
         sum += f[w] * sl[w][r];
         f[w] *= snu[w];
     }
-    const int ot = sq.q0 + r / a.G, oh = h * a.G + r % a.G;
+    const int ot = sq.q0 + (row0 + r) / a.G, oh = h * a.G + (row0 + r) % a.G;
     const int64_t orow = (int64_t)ot * a.Hq + oh, prow = (int64_t)split * a.T * a.Hq + orow;
     const float inv = a.nkeys > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
     if (part == 0) mark_row(a, a.nkeys, split, orow, top, sum);
@@ -385,8 +388,8 @@ __global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
 // One workgroup for 128 rows of a sequence, one key-value head and one split
 // of the keys; each of its four waves holds 32 rows' queries and sums, and
 // tiles of 64 keys pass through LDS, unpacked to fp16 on the way in.  The next
-// tile's bytes are loaded while this one is computed.  Sequences of up to 16
-// rows are the other kernel's.
+// tile's bytes are loaded while this one is computed.  Sequences of few rows
+// are attn_keys_kernel's.
 
 constexpr int kRowTile = 128, kKeyTile = 64;
 
@@ -915,7 +918,10 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 // kSplitMin while compute units are idle, and to kSplitKeys at least.  Chunks:
 // the number that wastes the least of the last round of workgroups, each split
 // of at least kSplitRows keys.
-constexpr int kFewRows = 16;
+// Rows up to which 16 a workgroup over the same keys are faster than 128 (us over
+// 16000 keys, INT8, bf16: 8 / 16 / 32 tokens of 4 heads of 128 to a key head
+// 30 / 47 / - against 50 / 52 / 55; 8 / 16 tokens of 6 heads of 256 39 / 59 against 105 / 93).
+constexpr int few_rows(int D) { return D == 256 ? 128 : 64; }
 constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer than 2^32
 constexpr int kSplitMin = 64, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
 
@@ -982,32 +988,36 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // ------------------------------------------------------------------ host
 
 struct AttnPlan {
-    int keys, rows, nslots;          // which kernels run, slots of the rows kernels
+    int keys, ntile16, rows, nslots;  // which kernels run, workgroups a sequence, slots of the rows kernels
     int nkeys, nrows, nsplit;        // splits of the keys: of the two kinds of kernels, room for
     int tiles, by_seq, direct;       // of an unpacked copy, 0: none; one for each sequence; attn_rows_kernel runs
     size_t copy, bytes;              // of the copies, of the workspace
 };
 
-// Copies are made for calls of kUnpackRows rows or more: of every sequence where
+// Copies are made for calls of kUnpackRows rows or more (heads of 256, whose sums
+// leave attn_rows_kernel no registers for the unpacking: 120 -> 73 us at 768 rows,
+// 95 -> 63 at 96; heads of 128 are even there): of every sequence where
 // they have kUnpackMean rows on average, else of those of kBigRows or more; at
 // most kUnpackMost bytes.
-constexpr int kUnpackRows = 512, kUnpackMean = 64;
+constexpr int kUnpackRows = 512, kUnpackRows256 = 64, kUnpackMean = 64;
 constexpr size_t kUnpackMost = (size_t)4 << 30;
 
 AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int dtype, int n_cu) {
     const int G = Hq / H;
     AttnPlan p{};
-    p.rows = cu ? (int64_t)T * G > kFewRows : G > kFewRows;
+    const int few = few_rows(D);
+    p.rows = cu ? (int64_t)T * G > few : G > few;
     // One sequence alone is never worth a second launch that may find nothing to do.
-    p.keys = G <= kFewRows && !(p.rows && B == 1);
+    p.keys = G <= few && !(p.rows && B == 1);
     p.nslots = cu ? (int)((int64_t)T * G / kRowTile) + B : B * ((G + kRowTile - 1) / kRowTile);
     p.nkeys = p.nrows = 1;
     if (p.keys) {
         // With chunks among the sequences the single tokens are not what fills the units.
-        const int64_t wgs = (int64_t)B * H;
+        p.ntile16 = (int)((std::min<int64_t>(few, (cu ? (int64_t)T : 1) * G) + 15) / 16);
+        const int64_t wgs = (int64_t)B * H * (cu ? 1 : p.ntile16);
         const int64_t fill = (2 * n_cu + wgs - 1) / wgs;
-        const int64_t idle = (int64_t)T * G > kFewRows * (int64_t)B ? 1 : std::min<int64_t>(fill, capacity / kSplitMin);
-        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), std::min<int64_t>(kSplitMost, kMostBlocks / wgs)));
+        const int64_t idle = (int64_t)T * G > few * (int64_t)B ? 1 : std::min<int64_t>(fill, capacity / kSplitMin);
+        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), std::min<int64_t>(kSplitMost, std::max<int64_t>(1, kMostBlocks / ((int64_t)B * H * p.ntile16)))));
     }
     if (p.rows) {
         const int64_t wgs = (int64_t)p.nslots * H, room = (int64_t)n_cu * (D == 256 || (D == 128 && dtype == kF32) ? 1 : 2);
@@ -1023,7 +1033,7 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
         }
     }
     p.direct = p.rows;
-    if (p.rows && (int64_t)T * G >= kUnpackRows) {
+    if (p.rows && (int64_t)T * G >= (D == 256 ? kUnpackRows256 : kUnpackRows)) {
         const int64_t tiles = (capacity + kKeyTile - 1) / kKeyTile, some = (int64_t)T * G / kBigRows + 1;
         const size_t one = (size_t)H * tiles * (kKeyTile * D * 4 + kHead);
         p.by_seq = (int64_t)T * G >= (int64_t)kUnpackMean * B && (one == 0 || (size_t)B <= kUnpackMost / one);
@@ -1052,7 +1062,7 @@ int cu_count() {
 
 template <int D, int KIND, int DT>
 void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-    if (p.keys) attn_keys_kernel<D, KIND, DT><<<(unsigned)a.B * a.H * a.nkeys, 256, 0, st>>>(a);
+    if (p.keys) attn_keys_kernel<D, KIND, DT><<<(unsigned)a.B * a.H * a.ntile16 * a.nkeys, 256, 0, st>>>(a);
     if (p.direct) attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
     if (p.tiles) {
         const int64_t items = (int64_t)a.B * a.H * a.tiles;
@@ -1106,8 +1116,8 @@ bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, boo
                      c->kv_heads, T, B, heads, table_w);
         return false;
     }
-    // A launch has fewer than 2^24 workgroups, and keys are counted in 32 bits with some room.
-    if ((int64_t)T * heads > (1 << 28) || (int64_t)B * c->kv_heads > kMostBlocks || table_w > ((1 << 30) >> s)) {
+    // A launch has fewer than 2^24 workgroups (eight a sequence and head at most here), and keys are counted in 32 bits with some room.
+    if ((int64_t)T * heads > (1 << 28) || (int64_t)B * c->kv_heads > kMostBlocks / 8 || table_w > ((1 << 30) >> s)) {
         bq_set_error("paged_attention: %d tokens of %d heads in %d sequences of up to %d pages are too much for one call", T,
                      heads, B, table_w);
         return false;
@@ -1185,10 +1195,11 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
     }
     a.nsplit = p.nsplit;
     a.nkeys = p.nkeys;
-    a.few = p.keys ? kFewRows : 0;
+    a.few = p.keys ? few_rows(cache->head_dim) : 0;
     a.by_seq = p.by_seq;
     a.big = !p.tiles ? INT32_MAX : p.by_seq ? a.few + 1 : kBigRows;
     a.nrows = p.nrows;
+    a.ntile16 = p.ntile16;
     a.nslots = p.nslots;
     a.tiles = p.tiles;
     a.unpacked = static_cast<uint8_t*>(dWork);
