@@ -155,7 +155,7 @@ __device__ inline h8 round8(const float* w) {
 // (D = 256), and no wave waits for another before the end.
 
 template <int D, int KIND, int DT>
-__global__ __launch_bounds__(256, 2) void attn_keys_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_kernel(AttnArgs a) {
     constexpr bool SPLIT = DT == kF32;
     constexpr int KC = D / 64;        // 16-byte chunks of a key a lane takes (a quarter of each 64 values)
     constexpr int VC = D / 32;        // 16-byte chunks of a tile's values a lane takes
@@ -923,7 +923,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 // 30 / 47 / - against 50 / 52 / 55; 8 / 16 tokens of 6 heads of 256 39 / 59 against 105 / 93).
 constexpr int few_rows(int D) { return D == 256 ? 128 : 64; }
 constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer than 2^32
-constexpr int kSplitMin = 64, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
+constexpr int kSplitMin = 64, kSplitMixed = 1024, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
 
 // The splits of a row joined: D/4 lanes a split and NG splits of a row at a
 // time, their sums then in the order of the splits.
@@ -1012,11 +1012,13 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
     p.nslots = cu ? (int)((int64_t)T * G / kRowTile) + B : B * ((G + kRowTile - 1) / kRowTile);
     p.nkeys = p.nrows = 1;
     if (p.keys) {
-        // With chunks among the sequences the single tokens are not what fills the units.
         p.ntile16 = (int)((std::min<int64_t>(few, (cu ? (int64_t)T : 1) * G) + 15) / 16);
         const int64_t wgs = (int64_t)B * H * (cu ? 1 : p.ntile16);
+        // With chunks among the sequences the single tokens are not what fills the units,
+        // but one of a long context must not outlast the chunks.
         const int64_t fill = (2 * n_cu + wgs - 1) / wgs;
-        const int64_t idle = (int64_t)T * G > few * (int64_t)B ? 1 : std::min<int64_t>(fill, capacity / kSplitMin);
+        const int64_t idle = (int64_t)T * G > few * (int64_t)B ? std::min<int64_t>(16, capacity / kSplitMixed)
+                                                                  : std::min<int64_t>(fill, capacity / kSplitMin);
         p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), std::min<int64_t>(kSplitMost, std::max<int64_t>(1, kMostBlocks / ((int64_t)B * H * p.ntile16)))));
     }
     if (p.rows) {
