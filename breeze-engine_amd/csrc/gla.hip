@@ -93,6 +93,9 @@ __device__ inline float clean_g(float g) { return g < -1e4f ? -1e4f : g; }
 
 // ------------------------------------------------------------------ short sequences
 
+// Bound by HBM: 64 tokens of 48 heads, 128 x 128 states (403 MB): 84 to 88 us,
+// 4.6 to 4.8 TB/s, the rate of a large copy.  One token: 4.8 us.
+//
 // A wave for 16 columns of one sequence's and head's state: lane (row r mod 16,
 // four columns).  Before the update both S^T k and S^T q are summed over the
 // rows, since S_t^T q = e^g S_{t-1}^T q + (k . q) u: one exchange a token.
@@ -218,7 +221,10 @@ constexpr int kq_bytes(int dk, bool lo) { return 2 * (lo ? 2 : 1) * 4 * (dk / 32
 constexpr int tm_bytes(bool delta) { return (delta ? 4 : 2) * kTriBytes; }
 
 // One workgroup for a chunk and a key head: the products k_i . k_j and
-// q_i . k_j once, then T and M for each of its value heads.
+// q_i . k_j once, then T and M for each of its value heads.  64 chunks of 16 key
+// and 48 value heads, fp32: 59 us, of which 28 for the operands of k and q (134
+// MB in and out) and 10 for each value head's T and M (25 KB a chunk and head
+// out, and a chain of small triangular products).
 template <int DK, int DT, bool DELTA>
 __global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
     constexpr bool LO = DT == kF32;  // two terms of q and k
@@ -558,9 +564,10 @@ __device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, con
 //
 // Bound by the chain through the state: per chunk 114 matrix instructions
 // (1,824 cycles of fp32 calls) and about as much in conversions, exchanges of
-// column maxima and LDS reads between them.  All eight products in one wave
-// and 64 columns a workgroup took 5.0 us a chunk (the LDS reads of four waves,
-// 480 KB, alone 1.6).
+// column maxima and LDS reads between them; 3.0 us a chunk, of which the
+// update's products take 0.6 and the hand-over 0.4 (64 chunks of 48 heads of
+// 128 x 128, 192 workgroups: 195 us).  All products in one wave and 64 columns
+// a workgroup took 5.0 (the LDS reads of four waves, 480 KB, alone 1.6).
 template <int DK, int DT, bool DELTA>
 __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaArgs a) {
     constexpr bool LO = DT == kF32;
