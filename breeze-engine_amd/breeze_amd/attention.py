@@ -261,7 +261,8 @@ def paged_attention(q, cache, block_table, kv_lens, cu_q=None, scale=None, out=N
 
     Sums and softmax statistics are fp32 and the cache's values enter the
     products exactly.  fp32 queries and their probabilities keep 22 bits; with
-    bf16 and fp16 the probabilities are rounded to fp16's 11."""
+    bf16, and with fp16 in chunks of 512 keys and more, the probabilities are
+    rounded to fp16's 11."""
     torch = _torch()
     T, heads, D = q.shape if q.dim() == 3 else (0, 0, 0)
     if D != cache.head_dim or heads % cache.kv_heads or not heads:
@@ -331,8 +332,8 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
 
     ``q``, ``k``: ``[T, k_heads, k_dim]``; ``v``: ``[T, v_heads, v_dim]``, of one
     type (views of a wider projection are read in place).  ``g``, ``beta``:
-    ``[T, v_heads]``; g is the decay's logarithm, at most 0 (-inf drops the
-    state).  ``state``: fp32 ``[B, v_heads, k_dim, v_dim]``, what each sequence
+    ``[T, v_heads]``; g is the decay's logarithm, at most 0 (-inf drops a
+    finite state).  ``state``: fp32 ``[B, v_heads, k_dim, v_dim]``, what each sequence
     starts from (None: zeros).  ``cu_seqlens``: int32 ``[B + 1]``, where each
     sequence's tokens begin and the last one's end; None: one token a sequence,
     B = T.  A sequence without tokens keeps its state; rows outside every

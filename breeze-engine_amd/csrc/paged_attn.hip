@@ -9,12 +9,14 @@
 // run on the fp16 matrix instructions with exact cache operands and fp32 sums.
 // q is scaled by a power of two for each row (its largest magnitude lands in
 // [2^13, 2^14)), which bf16 and fp16 queries survive exactly; fp32 queries are
-// split into two fp16 terms (22 bits), as are their probabilities.  bf16 and
-// fp16 calls round the probabilities once to fp16's 11 bits, three more than
-// a bf16 output keeps and as many as an fp16 one.  The key scales multiply the
-// scores and the value scales the probabilities; the latter are held relative
-// to a power of two `nu` near the tile's largest value scale, so that the fp16
-// range covers them whatever the values' size.  Running maxima and sums are fp32.
+// split into two fp16 terms (22 bits), as are their probabilities.  bf16 calls
+// round the probabilities once to fp16's 11 bits, three more than their output
+// keeps.  For fp16 that is as many, and a second term costs half as many matrix
+// instructions again: few rows, and rows of few keys, take it, the others not.
+// The key scales multiply the scores and the value scales the probabilities; the
+// latter are held relative to a power of two `nu` near the tile's largest value
+// scale, so that the fp16 range covers them whatever the values' size.  Running
+// maxima and sums are fp32.
 //
 // Both kernels compute S^T = K Q^T and O^T = V^T P^T: a lane then holds one
 // query row's scores, and the first product's result is the second one's
@@ -24,6 +26,7 @@
 #include "mix_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/breeze_qmm.h"
 
@@ -160,7 +163,8 @@ __device__ inline h8 round8(const float* w) {
 
 template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_kernel(AttnArgs a) {
-    constexpr bool SPLIT = DT == kF32;
+    constexpr bool SPLIT = DT == kF32;    // two terms of the queries
+    constexpr bool PSPLIT = DT != kBF16;  // and of the probabilities: the matrix rate is not what binds here
     constexpr int KC = D / 64;        // 16-byte chunks of a key a lane takes (a quarter of each 64 values)
     constexpr int VC = D / 32;        // 16-byte chunks of a tile's values a lane takes
     constexpr int VS = D + 16;        // LDS row of a key's values: the transposed reads' four rows fall on unlike banks
@@ -335,14 +339,14 @@ __global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys
             w[j] = vw[j] == 0.0f ? 0.0f : p * (vw[j] * up);
         }
         h8 ph, pl;
-        if constexpr (SPLIT) split8(w, ph, pl);
+        if constexpr (PSPLIT) split8(w, ph, pl);
         else ph = round8(w);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             const _Float16* p = vt + (4 * c + (r16 >> 2)) * VS + 16 * i + 4 * (r16 & 3);
             const h8 v = join(read_tr(p), read_tr(p + 16 * VS));
             o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[i], 0, 0, 0);
-            if constexpr (SPLIT) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[i], 0, 0, 0);
+            if constexpr (PSPLIT) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[i], 0, 0, 0);
         }
     }
 
@@ -451,7 +455,7 @@ __device__ inline float load_queries(const AttnArgs& a, int64_t at, h8* hi, h8* 
 
 template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnArgs a) {
-    constexpr bool SPLIT = DT == kF32;
+    constexpr bool SPLIT = DT == kF32, PSPLIT = DT != kBF16;  // two terms of the queries, and of the probabilities
     constexpr int KS = D + 8, VS = D + 16;  // LDS rows of a key: reads of one instruction fall on unlike banks
     constexpr int NC = D / 64;              // 16-byte chunks a thread loads of a tile's keys (and of its values)
     constexpr int per_row = D / 16;
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
                     w[4 + j] *= s1[j];
                 }
                 h8 ph, pl;
-                if constexpr (SPLIT) split8(w, ph, pl);
+                if constexpr (PSPLIT) split8(w, ph, pl);
                 else ph = round8(w);
                 const int i16 = lane & 15;
                 const _Float16* p = sv + (32 * u + 16 * g + 4 * hf + (i16 >> 2)) * VS + 16 * (r32 >> 4) + 4 * (i16 & 3);
@@ -630,7 +634,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
                 for (int i = 0; i < D / 32; ++i) {
                     const h8 v = join(read_tr(p + 32 * i), read_tr(p + 32 * i + 8 * VS));
                     o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[i], 0, 0, 0);
-                    if constexpr (SPLIT) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[i], 0, 0, 0);
+                    if constexpr (PSPLIT) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[i], 0, 0, 0);
                 }
             }
     }
@@ -664,6 +668,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
 // Rows from which on a sequence has a copy where not all have one.  Two such
 // sequences' first rows are that far apart, so first row / kBigRows tells them apart.
 constexpr int kBigRows = 256;
+// fp16 rows of fewer keys than this take two terms of the probabilities: one term's rounding is as large as
+// the output's own, and where a few keys hold most of a row it does not average out
+// (a 4096-token prompt of 32/8 heads of 128: 190 us with one term throughout, 195 so).
+constexpr int kTwoTerms = 512;
 __device__ inline int copy_of(const AttnArgs& a, const Seq& sq, int b) {
     return a.by_seq ? b : (int)((int64_t)sq.q0 * a.G / kBigRows);
 }
@@ -824,85 +832,94 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
         __syncthreads();
         scores(sk[t0 & 1]);
     }
-    for (int t = t0; t < t1; ++t) {
-        const int key0 = kKeyTile * t, par = t & 1;
-        wait_loads<0>();
-        __syncthreads();  // K of t + 1 and V of t are there; K of t and V of t - 1 are read
-        fetch(t + 2, 0, sk[par]);
-        fetch(t + 1, KB, sv[par ^ 1]);
-        fetch_head(t + 1);
-        const float* const hd = sh[par];
-        const float now = fmaxf(next_nu(nu, hd[192]), 0x1p-100f), nr = nu_ratio(nu, now), unit = __builtin_log2f(kPScale / now);
-        nu = now;
-        f16 x[2];
-        // Scores times the key scales; result register j holds key 8 (j / 4) + 4 hf + j % 4.
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const f4 sc = *reinterpret_cast<const f4*>(hd + 32 * u + 2 * j + 4 * hf);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[u][j + e] = s[u][j + e] * sc[e];
-            }
-        // Past the wave's first row, past the sequence's end or in a page that is not there.
-        if (key0 + kKeyTile > wave_all || hd[193] != 0.0f) {
+    const auto run = [&](auto terms) {
+        constexpr bool two = decltype(terms)::value;
+        for (int t = t0; t < t1; ++t) {
+            const int key0 = kKeyTile * t, par = t & 1;
+            wait_loads<0>();
+            __syncthreads();  // K of t + 1 and V of t are there; K of t and V of t - 1 are read
+            fetch(t + 2, 0, sk[par]);
+            fetch(t + 1, KB, sv[par ^ 1]);
+            fetch_head(t + 1);
+            const float* const hd = sh[par];
+            const float now = fmaxf(next_nu(nu, hd[192]), 0x1p-100f), nr = nu_ratio(nu, now), unit = __builtin_log2f(kPScale / now);
+            nu = now;
+            f16 x[2];
+            // Scores times the key scales; result register j holds key 8 (j / 4) + 4 hf + j % 4.
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    const f4 bad = *reinterpret_cast<const f4*>(hd + 128 + 32 * u + 2 * j + 4 * hf);
+                    const f4 sc = *reinterpret_cast<const f4*>(hd + 32 * u + 2 * j + 4 * hf);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int k = key0 + 32 * u + 2 * j + 4 * hf + e;
-                        x[u][j + e] = k > last || bad[e] != 0.0f ? -INFINITY : x[u][j + e];
+                    for (int e = 0; e < 4; ++e) x[u][j + e] = s[u][j + e] * sc[e];
+                }
+            // Past the wave's first row, past the sequence's end or in a page that is not there.
+            if (key0 + kKeyTile > wave_all || hd[193] != 0.0f) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const f4 bad = *reinterpret_cast<const f4*>(hd + 128 + 32 * u + 2 * j + 4 * hf);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int k = key0 + 32 * u + 2 * j + 4 * hf + e;
+                            x[u][j + e] = k > last || bad[e] != 0.0f ? -INFINITY : x[u][j + e];
+                        }
                     }
+            }
+            scores(sk[par ^ 1]);
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, x[u][j]), x[u][j + 1]);
+            top = max_halves(top);
+            // The reference moves only once a row's scores pass it by kSlack.
+            const bool moves = (top - m) * rowf > kSlack;
+            const float f = moves ? fast_exp2((m - top) * rowf) : 1.0f;
+            m = moves ? top : m;
+            const float alpha = f * nr, base = __builtin_fmaf(m == -INFINITY ? 0.0f : -m, rowf, unit);
+            l *= alpha;
+            h8 ph[4], pl[two ? 4 : 1];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {  // 16 keys
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = fast_exp2(__builtin_fmaf(x[g >> 1][8 * (g & 1) + j], rowf, base));
+                    l += w[j];
+                }
+                const f4 s0 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 4 * hf);
+                const f4 s1 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 8 + 4 * hf);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] *= s0[j];
+                    w[4 + j] *= s1[j];
+                }
+                if constexpr (two) split8(w, ph[g], pl[g]);
+                else ph[g] = round8(w);
+            }
+            if (__any(alpha != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+            }
+            const h8* p = reinterpret_cast<const h8*>(sv[par]) + lane;
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const h8 v = p[64 * (g * (D / 32) + i)];
+                    o[i] = mfma32(v, ph[g], o[i]);
+                    if constexpr (two) o[i] = mfma32(v, pl[g], o[i]);
                 }
         }
-        scores(sk[par ^ 1]);
-        float top = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, x[u][j]), x[u][j + 1]);
-        top = max_halves(top);
-        // The reference moves only once a row's scores pass it by kSlack.
-        const bool moves = (top - m) * rowf > kSlack;
-        const float f = moves ? fast_exp2((m - top) * rowf) : 1.0f;
-        m = moves ? top : m;
-        const float alpha = f * nr, base = __builtin_fmaf(m == -INFINITY ? 0.0f : -m, rowf, unit);
-        l *= alpha;
-        h8 ph[4], pl[SPLIT ? 4 : 1];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {  // 16 keys
-            float w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] = fast_exp2(__builtin_fmaf(x[g >> 1][8 * (g & 1) + j], rowf, base));
-                l += w[j];
-            }
-            const f4 s0 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 4 * hf);
-            const f4 s1 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 8 + 4 * hf);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[j] *= s0[j];
-                w[4 + j] *= s1[j];
-            }
-            if constexpr (SPLIT) split8(w, ph[g], pl[g]);
-            else ph[g] = round8(w);
-        }
-        if (__any(alpha != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
-        }
-        const h8* p = reinterpret_cast<const h8*>(sv[par]) + lane;
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const h8 v = p[64 * (g * (D / 32) + i)];
-                o[i] = mfma32(v, ph[g], o[i]);
-                if constexpr (SPLIT) o[i] = mfma32(v, pl[g], o[i]);
-            }
+    };
+    if constexpr (DT == kF16) {
+        if (seen_by(first) < kTwoTerms) run(std::true_type());
+        else run(std::false_type());
+    } else {
+        run(std::bool_constant<SPLIT>());
     }
     wait_loads<0>();  // none may land in LDS that is another workgroup's
 

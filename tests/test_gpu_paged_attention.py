@@ -49,23 +49,24 @@ def _cu(q_lens):
     return torch.tensor(cu, dtype=torch.int32)
 
 
-def _check(got, q, cache, table, kv_lens, q_lens, scale, dtype):
+def _check(got, q, cache, table, kv_lens, q_lens, scale, dtype, fine=False):
     T = sum(q_lens)
-    want, bound = attend(q[:T], cache, table, kv_lens, q_lens, scale, dtype is torch.float32)
+    want, bound = attend(q[:T], cache, table, kv_lens, q_lens, scale, fine or dtype is torch.float32)
     # One rounding to the type: half a step of the value, or of the smallest normal
     # number, below which the steps stay as wide (fp16: 2^-24, so half is 2^-25).
     bound = bound + half_step(dtype) * (want.abs() + bound).clamp_min(torch.finfo(dtype).smallest_normal)
     got = got[:T].cpu().double()
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and not torch.isinf(got).any()
-    fine = ~torch.isnan(want)
-    off, bound = (got - want).abs()[fine], bound[fine]
+    is_number = ~torch.isnan(want)
+    off, bound = (got - want).abs()[is_number], bound[is_number]
     assert torch.isfinite(bound).all()
     worst = (off / bound).max().item() if off.numel() else 0.0
     print(f"error / bound {worst:.3f}", flush=True)
     assert worst <= 1.0
 
 
-def _run(att, seed, kind, dtype, heads, H, D, page, q_lens, ctx, extra=0, single=False, scale=None, spread=1.0):
+def _run(att, seed, kind, dtype, heads, H, D, page, q_lens, ctx, extra=0, single=False, scale=None, spread=1.0,
+         fine=False):
     gen = torch.Generator().manual_seed(seed)
     kv_lens = [c + n for c, n in zip(ctx, q_lens)]
     cache, table = _cache(att, gen, kv_lens, H, D, page, kind, extra, spread)
@@ -73,7 +74,7 @@ def _run(att, seed, kind, dtype, heads, H, D, page, q_lens, ctx, extra=0, single
     lens = torch.tensor(kv_lens, dtype=torch.int32)
     got = att.paged_attention(q.cuda(), cache, table.cuda(), lens.cuda(), None if single else _cu(q_lens).cuda(),
                               scale)
-    _check(got, q, cache, table, kv_lens, q_lens, scale or D ** -0.5, DT[dtype])
+    _check(got, q, cache, table, kv_lens, q_lens, scale or D ** -0.5, DT[dtype], fine)
 
 
 ONE = [0, 1, 15, 16, 31, 32, 99, 127, 128, 500]
@@ -130,6 +131,15 @@ def test_long_chunks_among_many_sequences(att, kind, dtype, heads, H, D):
     q_lens = [1, 3, 1, 130, 1, 1, 20, 0, 1, 1, 75, 64, 1, 1, 1, 1, 1, 90] + [1] * 12
     ctx = [7 * i % 131 for i in range(len(q_lens))]
     _run(att, 42, kind, dtype, heads, H, D, 16, q_lens, ctx)
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("heads,H,D", [(6, 1, 256), (8, 2, 128), (12, 3, 64)])
+@pytest.mark.parametrize("q_lens,ctx,extra", [([1, 1, 1], [0, 3, 2000], 0), ([2, 9, 4], [700, 0, 33], 0),
+                                              ([20, 33, 1], [7, 0, 60], 0), ([300], [0], 0), ([130, 380], [300, 0], 3)])
+def test_fp16_rows_that_take_two_terms(att, kind, heads, H, D, q_lens, ctx, extra):
+    """Few rows, or fewer than 512 keys: the output's rounding is the only one to 11 bits."""
+    _run(att, 44, kind, "fp16", heads, H, D, 16, q_lens, ctx, extra, single=max(q_lens) == 1, fine=True)
 
 
 @pytest.mark.parametrize("heads", [17, 128, 129, 300])
