@@ -161,21 +161,22 @@ __device__ inline h8 round8(const float* w) {
 // of 64 keys, 14.6 in 32 of 128, and the join 7.2; latency, of the table, the
 // keys and one tile's chain of products.
 
+// LDS row of a key's values: the transposed reads' four rows fall on unlike banks.
+constexpr int keys_row(int D) { return D + 16; }
+constexpr int keys_lds(int D) { return std::max(4 * 32 * keys_row(D) * 2, 4 * 16 * (D + 4) * 4); }
+
+// lds: keys_lds(D) bytes; sql: the queries' second terms, the same for all waves.
 template <int D, int KIND, int DT>
-__global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_kernel(AttnArgs a) {
+__device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_t* lds, float (*sm)[16], float (*sl)[16],
+                                            float* snu, h8* sql) {
     constexpr bool SPLIT = DT == kF32;    // two terms of the queries
     constexpr bool PSPLIT = DT != kBF16;  // and of the probabilities: the matrix rate is not what binds here
     constexpr int KC = D / 64;        // 16-byte chunks of a key a lane takes (a quarter of each 64 values)
     constexpr int VC = D / 32;        // 16-byte chunks of a tile's values a lane takes
-    constexpr int VS = D + 16;        // LDS row of a key's values: the transposed reads' four rows fall on unlike banks
-    constexpr int OS = D + 4;
-    constexpr int kLds = 4 * 32 * VS * 2 > 4 * 16 * OS * 4 ? 4 * 32 * VS * 2 : 4 * 16 * OS * 4;
-    __shared__ __align__(16) uint8_t lds[kLds];
-    __shared__ float sm[4][16], sl[4][16], snu[4];
-    __shared__ __align__(16) h8 sql[SPLIT ? D / 32 * 64 : 1];  // the queries' second terms, the same for all waves
+    constexpr int VS = keys_row(D), OS = D + 4;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.H, tile16 = blockIdx.x / a.H % a.ntile16, bs = blockIdx.x / a.H / a.ntile16;
+    const int h = block % a.H, tile16 = block / a.H % a.ntile16, bs = block / a.H / a.ntile16;
     const int split = bs % a.nkeys, b = bs / a.nkeys;
     const Seq sq = sequence(a, b);
     if ((int64_t)sq.n * a.G > a.few) return;
@@ -389,6 +390,14 @@ __global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys
         if (a.nkeys > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
         else store4(a.out, DT, ot * a.o_token + oh * a.o_head + d, v);
     }
+}
+
+template <int D, int KIND, int DT>
+__global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_kernel(AttnArgs a) {
+    __shared__ __align__(16) uint8_t lds[keys_lds(D)];
+    __shared__ float sm[4][16], sl[4][16], snu[4];
+    __shared__ __align__(16) h8 sql[DT == kF32 ? D / 32 * 64 : 1];
+    attend_keys<D, KIND, DT>(a, blockIdx.x, lds, sm, sl, snu, sql);
 }
 
 // ------------------------------------------------------------------ many rows: the rows shared out
@@ -680,19 +689,22 @@ constexpr int kHead = 1024;  // a tile's scales: ks[64], vs[64], 1 where a key i
 template <int D>
 constexpr int tile_bytes() { return kKeyTile * D * 4 + kHead; }
 
+constexpr int unpack_lds(int D) { return 2 * kKeyTile * (D + 16) * 2; }
+
+// lds: unpack_lds(D) bytes.
 template <int D, int KIND>
-__global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
+__device__ __forceinline__ void unpack_tiles(const AttnArgs& a, unsigned block, unsigned blocks, uint8_t* lds) {
     constexpr int VS = D + 16, NC = D / 64, per_row = D / 16, KF = D / 8;  // KF operands of K, as many of V
-    __shared__ __align__(16) _Float16 sv[kKeyTile * VS], sk[kKeyTile * VS];
+    _Float16 *const sv = reinterpret_cast<_Float16*>(lds), *const sk = sv + kKeyTile * VS;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t items = (int64_t)a.B * a.H * a.tiles;
-    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    for (int64_t it = block; it < items; it += blocks) {
         const int tile = (int)(it % a.tiles), h = (int)(it / a.tiles % a.H), b = (int)(it / a.tiles / a.H);
         const Seq sq = sequence(a, b);
         if ((int64_t)sq.n * a.G < a.big) {
             // None of this sequence's: on to the next one's first.
             const int64_t next = (int64_t)(b + 1) * a.H * a.tiles;
-            it += (next - 1 - it) / gridDim.x * gridDim.x;
+            it += (next - 1 - it) / blocks * blocks;
             continue;
         }
         if (tile * kKeyTile >= sq.kv) continue;
@@ -743,6 +755,23 @@ __global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
         }
         __syncthreads();
     }
+}
+
+template <int D, int KIND>
+__global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
+    __shared__ __align__(16) uint8_t lds[unpack_lds(D)];
+    unpack_tiles<D, KIND>(a, blockIdx.x, gridDim.x, lds);
+}
+
+// Both, where a call has few rows of some sequences and many of others: the first
+// `keys` workgroups are attn_keys_kernel's.  Each waits on memory most of its time.
+template <int D, int KIND, int DT>
+__global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_unpack_kernel(AttnArgs a, unsigned keys) {
+    __shared__ __align__(16) uint8_t lds[std::max(keys_lds(D), unpack_lds(D))];
+    __shared__ float sm[4][16], sl[4][16], snu[4];
+    __shared__ __align__(16) h8 sql[DT == kF32 ? D / 32 * 64 : 1];
+    if (blockIdx.x < keys) attend_keys<D, KIND, DT>(a, blockIdx.x, lds, sm, sl, snu, sql);
+    else unpack_tiles<D, KIND>(a, blockIdx.x - keys, gridDim.x - keys, lds);
 }
 
 // As attn_rows_kernel, over the copy.  The scores of tile t + 1 are computed
@@ -1092,13 +1121,13 @@ int cu_count() {
 
 template <int D, int KIND, int DT>
 void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-    if (p.keys) attn_keys_kernel<D, KIND, DT><<<(unsigned)a.B * a.H * a.ntile16 * a.nkeys, 256, 0, st>>>(a);
+    const unsigned keys = p.keys ? (unsigned)a.B * a.H * a.ntile16 * a.nkeys : 0;
+    const unsigned unpack = (unsigned)std::min<int64_t>((int64_t)a.B * a.H * a.tiles, 2048);
+    if (keys && unpack) attn_keys_unpack_kernel<D, KIND, DT><<<keys + unpack, 256, 0, st>>>(a, keys);
+    else if (keys) attn_keys_kernel<D, KIND, DT><<<keys, 256, 0, st>>>(a);
+    else if (unpack) attn_unpack_kernel<D, KIND><<<unpack, 256, 0, st>>>(a);
     if (p.direct) attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
-    if (p.tiles) {
-        const int64_t items = (int64_t)a.B * a.H * a.tiles;
-        attn_unpack_kernel<D, KIND><<<(unsigned)std::min<int64_t>(items, 2048), 256, 0, st>>>(a);
-        attn_tiles_kernel<D, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
-    }
+    if (p.tiles) attn_tiles_kernel<D, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
 }
 
 template <int D, int KIND>
