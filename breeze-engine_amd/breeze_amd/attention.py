@@ -16,7 +16,7 @@ the current stream, own no memory between calls (a workspace comes from
 torch's allocator) and can be captured into graphs.  Shapes, types and strides
 are checked here and raise ``ValueError``; what lies on the GPU (lengths,
 offsets, page and slot numbers) is checked by the kernels, which skip what is
-out of range.  There is no CPU fallback.
+out of range.  Outputs carry no gradient.  There is no CPU fallback.
 """
 import ctypes
 

@@ -764,7 +764,9 @@ __global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
 }
 
 // Both, where a call has few rows of some sequences and many of others: the first
-// `keys` workgroups are attn_keys_kernel's.  Each waits on memory most of its time.
+// `keys` workgroups are attn_keys_kernel's.  Each waits on memory most of its time:
+// 31 us together, 26 and 13 one after the other (8 sequences of 1 to 700 tokens behind
+// up to 5000, 32/8 heads of 128, bf16, INT8).
 template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_unpack_kernel(AttnArgs a, unsigned keys) {
     __shared__ __align__(16) uint8_t lds[std::max(keys_lds(D), unpack_lds(D))];
