@@ -24,8 +24,9 @@
 // products, fp32 sums; q and k given as bf16 or fp16 are one term, and so are
 // the state and U where they only make rows of O of such a type (11 bits; the
 // state itself and U go on with two).  A power
-// of two for each tile, row or column puts the largest value where fp16 has
-// room; it changes no digit.  T is computed in fp32.  Sums of g are taken in
+// of two for each tile (of q and k: each chunk and head) or column puts the
+// largest value where fp16 has room; what a second term cannot hold then is
+// 2^-28 of a chunk's largest q or k, 2^-37 of a column's largest.  T is computed in fp32.  Sums of g are taken in
 // 64 bits: e^{G_i - G_j} would lose what G_i and G_j have in common.
 #include "mix_common.h"
 

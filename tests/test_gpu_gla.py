@@ -146,6 +146,19 @@ def test_alike_keys_and_whole_betas(att, dtype):
     _check(o, S, *x, lens)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+def test_queries_and_keys_of_unlike_size(att, dtype):
+    """Rows down to 2^-12 of their chunk's largest: an element's error, 2^-28 of that at most
+    beside its 22 bits, is 2^-16 of such a row's, of the bound's 2^-12."""
+    lens = [130, 70]
+    x = list(_inputs(33, lens, 2, 4, 128, 32, dtype))
+    gen = torch.Generator().manual_seed(34)
+    for i in (0, 1):
+        x[i] = (x[i].float() * torch.exp2(-12 * torch.rand((200, 2, 1), generator=gen))).to(x[i].dtype)
+    o, S = att.gated_linear_attention(*_cuda(*x), _cu(lens).cuda())
+    _check(o, S, *x, lens)
+
+
 def test_values_of_any_size(att):
     """Large and tiny values, in one column, one token, a whole head."""
     lens = [100, 3]
