@@ -157,8 +157,8 @@ __device__ inline h8 round8(const float* w) {
 // keys and values are on their way while this one is computed, 16 KB a wave
 // (D = 256), and no wave waits for another before the end.  64 single tokens
 // over 100 to 16000 keys of 8 heads of 128 (537 MB): 126 us, 4.3 TB/s, and the
-// join 5.2.  One token over 4101 keys of 4 heads of 256: 11.4 us in 64 splits
-// of 64 keys, 14.6 in 32 of 128, and the join 7.2; latency, of the table, the
+// join 5.3.  One token over 4101 keys of 4 heads of 256: 11 us in 64 splits
+// of 64 keys, 14.6 in 32 of 128, and the join 7.4; latency, of the table, the
 // keys and one tile's chain of products.
 
 // LDS row of a key's values: the transposed reads' four rows fall on unlike banks.
@@ -392,8 +392,14 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
     }
 }
 
-template <int D, int KIND, int DT>
-__global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_kernel(AttnArgs a) {
+// Workgroups a compute unit.  fp32 with heads of 256 spills 54 registers a lane at
+// two, whose traffic weighs where a workgroup has few rows and waits for HBM: 32
+// single tokens over up to 8000 keys of 4 heads 100 us at two, 54 at one; 12 tokens
+// over 6000 keys, 72 rows, 50 and 56.
+constexpr int keys_per_unit(int D, int DT, bool lone) { return D == 256 && DT == kF32 && lone ? 1 : D == 256 || DT == kF32 ? 2 : 3; }
+
+template <int D, int KIND, int DT, bool LONE>
+__global__ __launch_bounds__(256, keys_per_unit(D, DT, LONE)) void attn_keys_kernel(AttnArgs a) {
     __shared__ __align__(16) uint8_t lds[keys_lds(D)];
     __shared__ float sm[4][16], sl[4][16], snu[4];
     __shared__ __align__(16) h8 sql[DT == kF32 ? D / 32 * 64 : 1];
@@ -768,7 +774,7 @@ __global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
 // 31 us together, 26 and 13 one after the other (8 sequences of 1 to 700 tokens behind
 // up to 5000, 32/8 heads of 128, bf16, INT8).
 template <int D, int KIND, int DT>
-__global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys_unpack_kernel(AttnArgs a, unsigned keys) {
+__global__ __launch_bounds__(256, keys_per_unit(D, DT, false)) void attn_keys_unpack_kernel(AttnArgs a, unsigned keys) {
     __shared__ __align__(16) uint8_t lds[std::max(keys_lds(D), unpack_lds(D))];
     __shared__ float sm[4][16], sl[4][16], snu[4];
     __shared__ __align__(16) h8 sql[DT == kF32 ? D / 32 * 64 : 1];
@@ -781,7 +787,7 @@ __global__ __launch_bounds__(256, D == 256 || DT == kF32 ? 2 : 3) void attn_keys
 // values of tile t; K of tile t + 2 and V of tile t + 1 are on their way.
 //
 // Bound by the issue of matrix and vector instructions together: on a 4096-token
-// prompt of 32/8 heads of 128 (fp16, 137 GFLOP, 165 to 195 us) they were busy 41%
+// prompt of 32/8 heads of 128 (fp16, 137 GFLOP, 175 to 220 us) they were busy 41%
 // and 54% of the cycles, one beside the other hardly ever, whatever the waves'
 // priorities and the order of the code.  1024 tokens behind 31744, 24/4 heads
 // of 256, fp32 (812 GFLOP, twice that in two-term products): 1.63 ms, 995
@@ -1048,6 +1054,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 struct AttnPlan {
     int keys, ntile16, rows, nslots;  // which kernels run, workgroups a sequence, slots of the rows kernels
+    int lone;                        // the keys kernel's sequences are mostly of one token
     int nkeys, nrows, nsplit;        // splits of the keys: of the two kinds of kernels, room for
     int tiles, by_seq, direct;       // of an unpacked copy, 0: none; one for each sequence; attn_rows_kernel runs
     size_t copy, bytes;              // of the copies, of the workspace
@@ -1076,7 +1083,9 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
         // With chunks among the sequences the single tokens are not what fills the units,
         // but one of a long context must not outlast the chunks.
         const int64_t fill = (2 * n_cu + wgs - 1) / wgs;
-        const int64_t idle = (int64_t)T * G > few * (int64_t)B ? std::min<int64_t>(16, capacity / kSplitMixed)
+        const bool mixed = (int64_t)T * G > few * (int64_t)B;
+        p.lone = p.ntile16 == 1 || mixed;
+        const int64_t idle = mixed ? std::min<int64_t>(16, capacity / kSplitMixed)
                                                                   : std::min<int64_t>(fill, capacity / kSplitMin);
         p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), std::min<int64_t>(kSplitMost, std::max<int64_t>(1, kMostBlocks / ((int64_t)B * H * p.ntile16)))));
     }
@@ -1125,9 +1134,15 @@ template <int D, int KIND, int DT>
 void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     const unsigned keys = p.keys ? (unsigned)a.B * a.H * a.ntile16 * a.nkeys : 0;
     const unsigned unpack = (unsigned)std::min<int64_t>((int64_t)a.B * a.H * a.tiles, 2048);
-    if (keys && unpack) attn_keys_unpack_kernel<D, KIND, DT><<<keys + unpack, 256, 0, st>>>(a, keys);
-    else if (keys) attn_keys_kernel<D, KIND, DT><<<keys, 256, 0, st>>>(a);
-    else if (unpack) attn_unpack_kernel<D, KIND><<<unpack, 256, 0, st>>>(a);
+    // At one workgroup a unit the copy would go at half its rate.
+    const bool alone = p.lone && keys_per_unit(D, DT, true) == 1;
+    if (keys && unpack && !alone) {
+        attn_keys_unpack_kernel<D, KIND, DT><<<keys + unpack, 256, 0, st>>>(a, keys);
+    } else {
+        if (keys && alone) attn_keys_kernel<D, KIND, DT, keys_per_unit(D, DT, true) == 1><<<keys, 256, 0, st>>>(a);
+        else if (keys) attn_keys_kernel<D, KIND, DT, false><<<keys, 256, 0, st>>>(a);
+        if (unpack) attn_unpack_kernel<D, KIND><<<unpack, 256, 0, st>>>(a);
+    }
     if (p.direct) attn_rows_kernel<D, KIND, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
     if (p.tiles) attn_tiles_kernel<D, DT><<<(unsigned)a.nslots * a.H * a.nrows, 256, 0, st>>>(a);
 }
