@@ -395,8 +395,13 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
 // Workgroups a compute unit.  fp32 with heads of 256 spills 54 registers a lane at
 // two, whose traffic weighs where a workgroup has few rows and waits for HBM: 32
 // single tokens over up to 8000 keys of 4 heads 100 us at two, 54 at one; 12 tokens
-// over 6000 keys, 72 rows, 50 and 56.
-constexpr int keys_per_unit(int D, int DT, bool lone) { return D == 256 && DT == kF32 && lone ? 1 : D == 256 || DT == kF32 ? 2 : 3; }
+// over 6000 keys, 72 rows, 50 and 56.  Half types with heads of 128 spill 3 at three
+// (INT8: 64 tokens over 100 to 16000 keys 148 us, at two 140), which many rows beside
+// chunks are faster at.
+constexpr int keys_per_unit(int D, int DT, bool lone) {
+    if (D == 256 && DT == kF32) return lone ? 1 : 2;
+    return D == 256 || DT == kF32 || (D == 128 && lone) ? 2 : 3;
+}
 
 template <int D, int KIND, int DT, bool LONE>
 __global__ __launch_bounds__(256, keys_per_unit(D, DT, LONE)) void attn_keys_kernel(AttnArgs a) {
@@ -1139,7 +1144,8 @@ void launch3(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     if (keys && unpack && !alone) {
         attn_keys_unpack_kernel<D, KIND, DT><<<keys + unpack, 256, 0, st>>>(a, keys);
     } else {
-        if (keys && alone) attn_keys_kernel<D, KIND, DT, keys_per_unit(D, DT, true) == 1><<<keys, 256, 0, st>>>(a);
+        constexpr bool kLone = keys_per_unit(D, DT, true) != keys_per_unit(D, DT, false);
+        if (keys && p.lone) attn_keys_kernel<D, KIND, DT, kLone><<<keys, 256, 0, st>>>(a);
         else if (keys) attn_keys_kernel<D, KIND, DT, false><<<keys, 256, 0, st>>>(a);
         if (unpack) attn_unpack_kernel<D, KIND><<<unpack, 256, 0, st>>>(a);
     }
