@@ -55,7 +55,8 @@ def _rows(t, what):
     st = t.stride()
     if st[2] == 1 and not (st[0] | st[1]) & 3 and not t.data_ptr() & 15:
         return t
-    return t.contiguous() if st[2] != 1 or (st[0] | st[1]) & 3 else t.clone()
+    # A new tensor in any case: contiguous() gives one token back as it is, whose stride does not count.
+    return t.clone(memory_format=_torch().contiguous_format)
 
 
 def _ints(t, shape, what):
