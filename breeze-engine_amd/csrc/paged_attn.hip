@@ -49,7 +49,7 @@ struct AttnArgs {
     int tiles;          // of 64 keys, in the whole table
     int by_seq;         // a copy for each sequence; else for those of kBigRows rows or more
     float* part;        // [nsplit][T * Hq][D] when nsplit > 1
-    f2* ml;             // [nsplit][T * Hq]: maximum and sum; a first one of (infinity, 0): the row is done
+    f2* ml;             // [nsplit][T * Hq]: maximum and sum; a first sum below zero: the row is done
     int64_t table_row;
     int T, B, Hq, H, G, P, pshift, table_w, nslots, dt;
     int ntile16;               // workgroups for a sequence's rows in attn_keys_kernel
@@ -112,7 +112,7 @@ __device__ inline int64_t group_row(const AttnArgs& a, const int32_t* table, int
 __device__ inline void mark_row(const AttnArgs& a, int own, int split, int64_t row, float top, float sum) {
     if (a.nsplit == 1) return;
     const int64_t n = (int64_t)a.T * a.Hq;
-    a.ml[split * n + row] = own > 1 ? (f2){top, sum} : (f2){INFINITY, 0.0f};
+    a.ml[split * n + row] = own > 1 ? (f2){top, sum} : (f2){0.0f, -1.0f};  // no sum of exponentials is below zero
     if (split == 0)
         for (int s = own; s < a.nsplit; ++s) a.ml[s * n + row] = (f2){-INFINITY, 0.0f};
 }
@@ -1007,6 +1007,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int64_t row = (int64_t)blockIdx.x * RW + part / NG;
     const int tok = (int)(row / a.Hq), head = (int)(row % a.Hq);
     bool mine = row < n && !(a.cu && (tok < a.cu[0] || tok >= a.cu[a.B]));
+    mine = mine && !(a.ml[row].y < 0.0f);  // else the row is done
     f4 v = {0, 0, 0, 0};
     float sum = 0.0f;
     // The splits' maxima and sums first, one or more a lane; sw: a split's weight.
@@ -1023,7 +1024,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         }
 #pragma unroll
         for (int st = 1; st < L; st *= 2) top = fmaxf(top, __shfl_xor(top, st));
-        mine = mine && top != INFINITY;  // else the row is done
         const float safe = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
