@@ -14,9 +14,10 @@
 // keeps.  For fp16 that is as many, and a second term costs half as many matrix
 // instructions again: few rows, and rows of few keys, take it, the others not.
 // The key scales multiply the scores and the value scales the probabilities; the
-// latter are held relative to a power of two `nu` near the tile's largest value
-// scale, so that the fp16 range covers them whatever the values' size.  Running
-// maxima and sums are fp32.
+// latter are held relative to a power of two `nu` near the largest value scale
+// that the row sees in the tile (a later token's values, however large, take no
+// bits from an earlier one's row), so that the fp16 range covers them whatever the
+// values' size.  Running maxima and sums are fp32.
 //
 // Both kernels compute S^T = K Q^T and O^T = V^T P^T: a lane then holds one
 // query row's scores, and the first product's result is the second one's
@@ -71,7 +72,7 @@ __device__ inline h4 read_tr(const _Float16* p) {
 __device__ inline f16 mfma32(h8 a, h8 b, f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ inline h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// The power of two that a tile's value scales are taken relative to: kept
+// The power of two that a row's value scales in a tile are taken relative to: kept
 // while the largest is within (nu / 16, 8 nu].
 __device__ inline float next_nu(float nu, float vmax) {
     if (!(vmax > 0.0f) || vmax > 3e38f) return nu;
@@ -168,7 +169,7 @@ constexpr int keys_lds(int D) { return std::max(4 * 32 * keys_row(D) * 2, 4 * 16
 // lds: keys_lds(D) bytes; sql: the queries' second terms, the same for all waves.
 template <int D, int KIND, int DT>
 __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_t* lds, float (*sm)[16], float (*sl)[16],
-                                            float* snu, h8* sql) {
+                                            float (*snu)[16], h8* sql) {
     constexpr bool SPLIT = DT == kF32;    // two terms of the queries
     constexpr bool PSPLIT = DT != kBF16;  // and of the probabilities: the matrix rate is not what binds here
     constexpr int KC = D / 64;        // 16-byte chunks of a key a lane takes (a quarter of each 64 values)
@@ -317,9 +318,7 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
         rows_of(t + 8, next);
 
         top = max_halves(max_rows16(top));
-        vmax = max_halves(max_rows16(vmax));
-#pragma unroll
-        for (int st = 1; st < 16; st *= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, st));  // rows see unlike keys
+        vmax = max_halves(max_rows16(vmax));  // of the keys that the row sees: what others hold is not its concern
         const float now = next_nu(nu, vmax), was = nu;
         nu = now;
         const float mn = fmaxf(m, top), safe = mn == -INFINITY ? 0.0f : mn;
@@ -358,8 +357,8 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
     if (c == 0) {
         sm[wave][r16] = m * rowf;  // in units of log2
         sl[wave][r16] = l;
+        snu[wave][r16] = nu * (1.0f / kPScale);
     }
-    if (lane == 0) snu[wave] = nu * (1.0f / kPScale);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
         *reinterpret_cast<f4*>(so + (wave * 16 + r16) * OS + 16 * i + 4 * c) = o[i];
@@ -374,7 +373,7 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
     for (int w = 0; w < 4; ++w) {
         f[w] = fast_exp2(sm[w][r] - safe);
         sum += f[w] * sl[w][r];
-        f[w] *= snu[w];
+        f[w] *= snu[w][r];
     }
     const int ot = sq.q0 + (row0 + r) / a.G, oh = h * a.G + (row0 + r) % a.G;
     const int64_t orow = (int64_t)ot * a.Hq + oh, prow = (int64_t)split * a.T * a.Hq + orow;
@@ -406,7 +405,7 @@ constexpr int keys_per_unit(int D, int DT, bool lone) {
 template <int D, int KIND, int DT, bool LONE>
 __global__ __launch_bounds__(256, keys_per_unit(D, DT, LONE)) void attn_keys_kernel(AttnArgs a) {
     __shared__ __align__(16) uint8_t lds[keys_lds(D)];
-    __shared__ float sm[4][16], sl[4][16], snu[4];
+    __shared__ float sm[4][16], sl[4][16], snu[4][16];
     __shared__ __align__(16) h8 sql[DT == kF32 ? D / 32 * 64 : 1];
     attend_keys<D, KIND, DT>(a, blockIdx.x, lds, sm, sl, snu, sql);
 }
@@ -481,7 +480,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     constexpr int per_row = D / 16;
     __shared__ __align__(16) _Float16 sk[kKeyTile * KS], sv[kKeyTile * VS];
     __shared__ __align__(16) float sks[kKeyTile], svs[kKeyTile];
-    __shared__ float sbad[kKeyTile], snu;
+    __shared__ float sbad[kKeyTile], smax;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r32 = lane & 31, hf = lane >> 5;
@@ -565,22 +564,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
             float vmax = nan ? 0.0f : vsc;
 #pragma unroll
             for (int st = 1; st < 64; st *= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, st));
-            const float now = next_nu(nu, vmax);
-            svs[lane] = now > 0.0f && !nan ? vsc * (kPScale / now) : 0.0f;
-            if (lane == 0) snu = now;
+            svs[lane] = nan ? 0.0f : vsc;
+            if (lane == 0) smax = vmax;
         }
         __syncthreads();
         if (t + 1 < t1) load(t + 1);
-        const float now = snu, was = nu;
-        nu = now;
-        const float nr = nu_ratio(was, now);
-        if (key0 >= wave_end) {
-            if (nr != 1.0f) {
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) o[i] *= nr;
-            }
-            continue;
-        }
+        if (key0 >= wave_end) continue;
 
         f16 s[2];
 #pragma unroll
@@ -596,7 +585,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
             }
         }
         // Scores times the key scales; result register j holds key 8 (j / 4) + 4 hf + j % 4.
-        float top = -INFINITY;
+        float top = -INFINITY, vmax = smax;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -605,16 +594,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[u][j + e] *= sc[e];
             }
-        // Past the wave's first row, past the sequence's end or in a page that is not there.
+        // Past the wave's first row, past the sequence's end or in a page that is not
+        // there: neither a score, nor among the values that set the row's units.
         if (key0 + kKeyTile > wave_all || key0 + kKeyTile > sq.kv || __any(sbad[lane] != 0.0f)) {
+            vmax = 0.0f;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int k = 32 * u + 8 * (j / 4) + 4 * hf + j % 4;
-                    if (key0 + k > last || sbad[k] != 0.0f) s[u][j] = -INFINITY;
+                    const bool out = key0 + k > last || sbad[k] != 0.0f;
+                    s[u][j] = out ? -INFINITY : s[u][j];
+                    vmax = fmaxf(vmax, out ? 0.0f : svs[k]);
                 }
+            vmax = max_halves(vmax);
         }
+        const float now = next_nu(nu, vmax), nr = nu_ratio(nu, now), up = now > 0.0f ? kPScale / now : 0.0f;
+        nu = now;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -642,8 +638,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
                 const f4 s1 = *reinterpret_cast<const f4*>(svs + 32 * u + 16 * g + 8 + 4 * hf);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    w[j] *= s0[j];
-                    w[4 + j] *= s1[j];
+                    w[j] *= s0[j] * up;
+                    w[4 + j] *= s1[j] * up;
                 }
                 h8 ph, pl;
                 if constexpr (PSPLIT) split8(w, ph, pl);
@@ -781,7 +777,7 @@ __global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
 template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256, keys_per_unit(D, DT, false)) void attn_keys_unpack_kernel(AttnArgs a, unsigned keys) {
     __shared__ __align__(16) uint8_t lds[std::max(keys_lds(D), unpack_lds(D))];
-    __shared__ float sm[4][16], sl[4][16], snu[4];
+    __shared__ float sm[4][16], sl[4][16], snu[4][16];
     __shared__ __align__(16) h8 sql[DT == kF32 ? D / 32 * 64 : 1];
     if (blockIdx.x < keys) attend_keys<D, KIND, DT>(a, blockIdx.x, lds, sm, sl, snu, sql);
     else unpack_tiles<D, KIND>(a, blockIdx.x - keys, gridDim.x - keys, lds);
@@ -884,8 +880,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
             fetch(t + 1, KB, sv[par ^ 1]);
             fetch_head(t + 1);
             const float* const hd = sh[par];
-            const float now = fmaxf(next_nu(nu, hd[192]), 0x1p-100f), nr = nu_ratio(nu, now), unit = __builtin_log2f(kPScale / now);
-            nu = now;
+            float vmax = hd[192];
             f16 x[2];
             // Scores times the key scales; result register j holds key 8 (j / 4) + 4 hf + j % 4.
 #pragma unroll
@@ -896,20 +891,28 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[u][j + e] = s[u][j + e] * sc[e];
                 }
-            // Past the wave's first row, past the sequence's end or in a page that is not there.
+            // Past the wave's first row, past the sequence's end or in a page that is not
+            // there: neither a score, nor among the values that set the row's units.
             if (key0 + kKeyTile > wave_all || hd[193] != 0.0f) {
+                vmax = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
                         const f4 bad = *reinterpret_cast<const f4*>(hd + 128 + 32 * u + 2 * j + 4 * hf);
+                        const f4 vs = *reinterpret_cast<const f4*>(hd + 64 + 32 * u + 2 * j + 4 * hf);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int k = key0 + 32 * u + 2 * j + 4 * hf + e;
-                            x[u][j + e] = k > last || bad[e] != 0.0f ? -INFINITY : x[u][j + e];
+                            const bool out = k > last || bad[e] != 0.0f;
+                            x[u][j + e] = out ? -INFINITY : x[u][j + e];
+                            vmax = fmaxf(vmax, out ? 0.0f : vs[e]);
                         }
                     }
+                vmax = max_halves(vmax);
             }
+            const float now = fmaxf(next_nu(nu, vmax), 0x1p-100f), nr = nu_ratio(nu, now), unit = __builtin_log2f(kPScale / now);
+            nu = now;
             scores(sk[par ^ 1]);
             float top = -INFINITY;
 #pragma unroll
