@@ -73,14 +73,19 @@ __device__ inline f16 mfma32(h8 a, h8 b, f16 c) { return __builtin_amdgcn_mfma_f
 __device__ inline h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // The power of two that a row's value scales in a tile are taken relative to: kept
-// while the largest is within (nu / 16, 8 nu].
-__device__ inline float next_nu(float nu, float vmax) {
-    if (!(vmax > 0.0f) || vmax > 3e38f) return nu;
-    if (vmax <= nu * 8.0f && vmax > nu * 0x1p-4f) return nu;
-    const float want = bits_f(max(f_bits(vmax) & 0x7F800000u, 1u << 23));
-    return nu > 0.0f ? fmaxf(want, nu * 0x1p-100f) : want;
+// while the largest is within (nu / 16, 8 nu], `least` at least.  `peak` is the
+// largest one yet, times what is left of its keys' weights.  The sums in units of
+// nu / 2^9 are at most keys * 8 * 8 * 448 * 2^9 * peak / nu, below 2^54 peak / nu for
+// 2^30 keys, so with nu at 2^-60 peak or more they stay within fp32; what a smaller
+// one would keep of the present tile is below 2^-80 of the sums.  No step divides
+// by more than 2^100, which fp32 holds.
+__device__ inline float next_nu(float nu, float vmax, float peak, float least) {
+    if (!(vmax > 0.0f) || vmax > 3e38f || (vmax <= nu * 8.0f && vmax > nu * 0x1p-4f)) return nu;
+    const float want = fmaxf(fmaxf(vmax, peak * 0x1p-60f), fmaxf(nu * 0x1p-100f, least));
+    return bits_f(f_bits(want) & 0x7F800000u);
 }
-__device__ inline float nu_ratio(float was, float now) { return was > 0.0f ? was / now : 1.0f; }
+// 2^9 / nu is finite: with value scales of fp32's smallest normal number a weight is 2 then.
+constexpr float kLeastNu = 0x1p-118f;
 
 struct Seq {
     int q0, n, kv;  // first token, new tokens, keys
@@ -197,7 +202,7 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
     f4 o[D / 16];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[i] = (f4){0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f, nu = 0.0f;
+    float m = -INFINITY, l = 0.0f, nu = kLeastNu, peak = 0.0f;
 
     u4 kraw[2][KC], vraw[VC];
     f4 ksc[2], vsc[2];
@@ -319,18 +324,19 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
 
         top = max_halves(max_rows16(top));
         vmax = max_halves(max_rows16(vmax));  // of the keys that the row sees: what others hold is not its concern
-        const float now = next_nu(nu, vmax), was = nu;
-        nu = now;
         const float mn = fmaxf(m, top), safe = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = fast_exp2((m - safe) * rowf) * nu_ratio(was, now);
         const float lalpha = fast_exp2((m - safe) * rowf);
         m = mn;
+        peak *= lalpha;
+        const float now = next_nu(nu, vmax, peak, kLeastNu), alpha = lalpha * (nu / now);
+        nu = now;
+        peak = fmaxf(peak, now);
         if (__any(alpha != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
         }
         l *= lalpha;
-        const float up = nu > 0.0f ? kPScale / nu : 0.0f;
+        const float up = kPScale / nu;
         float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -516,7 +522,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-    float m = -INFINITY, l = 0.0f, nu = 0.0f;
+    float m = -INFINITY, l = 0.0f, nu = kLeastNu, peak = 0.0f;
 
     u4 kraw[NC], vraw[NC];
     int64_t grow[NC];    // cache rows of the groups of 16 keys that this wave's chunks belong to
@@ -609,16 +615,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
                 }
             vmax = max_halves(vmax);
         }
-        const float now = next_nu(nu, vmax), nr = nu_ratio(nu, now), up = now > 0.0f ? kPScale / now : 0.0f;
-        nu = now;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, s[u][j]);
         top = max_halves(top);
         const float mn = fmaxf(m, top), safe = mn == -INFINITY ? 0.0f : mn;
-        const float lalpha = fast_exp2((m - safe) * rowf), alpha = lalpha * nr;
+        const float lalpha = fast_exp2((m - safe) * rowf);
         m = mn;
+        peak *= lalpha;
+        const float now = next_nu(nu, vmax, peak, kLeastNu), alpha = lalpha * (nu / now), up = kPScale / now;
+        nu = now;
+        peak = fmaxf(peak, now);
         if (__any(alpha != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
@@ -830,8 +838,11 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-    // The sums o and l are in units in which a probability of 1 is 2^9 / nu.
-    float m = -INFINITY, l = 0.0f, nu = 0.0f;
+    // A tile's weights are computed in units in which a probability of 1 is 2^9 / nu, at
+    // most 2^119 of those eight, so that a lane's 32 add up to less than fp32 holds.
+    // Past nu = 2^96 (values of 1e31) the smallest of them fall out of its range.
+    constexpr float least = 0x1p-110f;
+    float m = -INFINITY, l = 0.0f, nu = least, peak = 0.0f, unit = __builtin_log2f(kPScale / least);
 
     // Past the last tile the loads repeat it.
     const auto fetch = [&](int t, int from, uint8_t* to) {
@@ -911,21 +922,39 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
                     }
                 vmax = max_halves(vmax);
             }
-            const float now = fmaxf(next_nu(nu, vmax), 0x1p-100f), nr = nu_ratio(nu, now), unit = __builtin_log2f(kPScale / now);
-            nu = now;
-            scores(sk[par ^ 1]);
-            float top = -INFINITY;
+            const auto largest = [&] {
+                float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, x[u][j]), x[u][j + 1]);
-            top = max_halves(top);
+                    for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, x[u][j]), x[u][j + 1]);
+                return max_halves(top);
+            };
             // The reference moves only once a row's scores pass it by kSlack.
-            const bool moves = (top - m) * rowf > kSlack;
-            const float f = moves ? fast_exp2((m - top) * rowf) : 1.0f;
-            m = moves ? top : m;
-            const float alpha = f * nr, base = __builtin_fmaf(m == -INFINITY ? 0.0f : -m, rowf, unit);
-            l *= alpha;
+            const auto move = [&] {
+                const float top = largest();
+                const bool moves = (top - m) * rowf > kSlack;
+                const float f = moves ? fast_exp2((m - top) * rowf) : 1.0f;
+                m = moves ? top : m;
+                return f;
+            };
+            // Rarely a row's units change, its reference with them; here, since a branch behind
+            // the next scores' matrix instructions would keep the softmax from running beside them.
+            if (__any(!(vmax <= nu * 8.0f && vmax > nu * 0x1p-4f))) {
+                const float f = move();
+                l *= f;
+                peak *= f;
+                const float now = next_nu(nu, vmax, peak, least), alpha = f * (nu / now);
+                unit = __builtin_log2f(kPScale / now);
+                nu = now;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+            }
+            scores(sk[par ^ 1]);
+            const float f = move();
+            peak = fmaxf(peak * f, nu);
+            const float base = __builtin_fmaf(m == -INFINITY ? 0.0f : -m, rowf, unit);
+            float sum = 0.0f;
             h8 ph[4], pl[two ? 4 : 1];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {  // 16 keys
@@ -933,7 +962,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     w[j] = fast_exp2(__builtin_fmaf(x[g >> 1][8 * (g & 1) + j], rowf, base));
-                    l += w[j];
+                    sum += w[j];
                 }
                 const f4 s0 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 4 * hf);
                 const f4 s1 = *reinterpret_cast<const f4*>(hd + 64 + 16 * g + 8 + 4 * hf);
@@ -945,9 +974,10 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
                 if constexpr (two) split8(w, ph[g], pl[g]);
                 else ph[g] = round8(w);
             }
-            if (__any(alpha != 1.0f)) {
+            l = __builtin_fmaf(sum, nu * (1.0f / kPScale), l * f);
+            if (__any(f != 1.0f)) {
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+                for (int i = 0; i < D / 32; ++i) o[i] *= f;
             }
             const h8* p = reinterpret_cast<const h8*>(sv[par]) + lane;
 #pragma unroll
@@ -972,8 +1002,8 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
     l = sum_halves(l);
     const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
     float f = nu * (1.0f / kPScale);
-    if (hf == 0) mark_row(a, a.nrows, split, orow, m * rowf, l * f);
-    if (a.nrows == 1) f = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+    if (hf == 0) mark_row(a, a.nrows, split, orow, m * rowf, l);
+    if (a.nrows == 1) f *= l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
