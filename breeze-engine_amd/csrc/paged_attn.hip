@@ -132,6 +132,12 @@ __device__ inline float row_scale(uint32_t top) {
     return top == 0 ? 1.0f : bits_f((uint32_t)(min(max(e, -126), 100) + 127) << 23);
 }
 
+// What a score is worth in log2, for a row scaled by `up`: positive and finite, since
+// times infinity (a key that is not seen) or 0 (the largest score's own difference) it
+// must not be NaN.  A row with a NaN or infinity has one too: its scores are NaN, where
+// it sees a key at all.
+__device__ inline float score_worth(float scale, float up) { return fminf(fmaxf(scale / up, 0x1p-149f), 0x1p127f); }
+
 // Splits w into fp16 terms: hi, and what hi leaves.
 __device__ inline void split8(const float* w, h8& hi, h8& lo) {
 #pragma unroll
@@ -256,7 +262,7 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
             }
         top = lane_max_u32(lane_max_u32(top, 16), 32);
         const float up = row_scale(top);
-        rowf = a.scale / up;
+        rowf = score_worth(a.scale, up);
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
             float w[8];
@@ -475,7 +481,7 @@ __device__ inline float load_queries(const AttnArgs& a, int64_t at, h8* hi, h8* 
         if constexpr (DT == kF32) split8(w, hi[s], lo[s]);
         else hi[s] = round8(w);
     }
-    return a.scale / up;
+    return score_worth(a.scale, up);
 }
 
 template <int D, int KIND, int DT>
