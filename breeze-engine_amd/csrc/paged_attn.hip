@@ -959,7 +959,17 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
             scores(sk[par ^ 1]);
             const float f = move();
             peak = fmaxf(peak * f, nu);
-            const float base = __builtin_fmaf(m == -INFINITY ? 0.0f : -m, rowf, unit);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float base = __builtin_fmaf(-ref, rowf, unit);
+            // m rowf is rounded once here, by less than half while it is below 2^22; past that
+            // the difference is taken first, else the largest weight would be 2 to that error.
+            if (__any(__builtin_fabsf(ref) * rowf > 0x1p22f)) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[u][j] -= ref;
+                base = unit;
+            }
             float sum = 0.0f;
             h8 ph[4], pl[two ? 4 : 1];
 #pragma unroll

@@ -89,3 +89,26 @@ def test_softmax_scales_that_leave_no_difference(att, n, kv, D, scale, size):
     mean = (v.abs().cumsum(0) / torch.arange(1, kv + 1).double()[:, None])[kv - n:]
     bound = mean * (kv * 2.0 ** -24 + 2.0 ** -20) + 2.0 ** -30 * kv * v.abs().max()
     assert ((got.cpu().double() - want[:, None]).abs() <= bound[:, None]).all()
+
+
+@pytest.mark.parametrize("n,kv", FORMS)
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("scale,size", [(1.0, 1e6), (1.0, 1e8), (1.0, 1e15), (1e20, 1e15)])
+def test_scores_so_large_that_one_key_is_left(att, n, kv, D, scale, size):
+    """Scores whose differences are all past what the softmax can tell from 0: the
+    value of the largest one's key, whatever the scores' own last bits amount to."""
+    gen = torch.Generator().manual_seed(4)
+    cache, table, _ = _setup(att, gen, kv, D)
+    at = torch.arange(kv, dtype=torch.int32).cuda()
+    k, v = (t.cpu().double()[:, 0] for t in att.kv_read(cache, at, torch.float32))
+    q = size * torch.randn((n, 4, D), generator=gen)
+    got = att.paged_attention(q.cuda(), cache, table, torch.tensor([kv], dtype=torch.int32).cuda(), _cu([n]), scale=scale)
+    s = torch.einsum("nhd,kd->nhk", q.double(), k)
+    s.masked_fill_((torch.arange(kv)[None] > torch.arange(kv - n, kv)[:, None])[:, None], -float("inf"))
+    want = v[s.argmax(-1)]
+    # The value itself, its weight held in 22 bits and relative to the tile's largest value.
+    bound = want.abs() * 2.0 ** -20 + 2.0 ** -30 * kv * v.abs().max()
+    two = s.topk(2, dim=-1).values
+    clear = (two[..., 0] - two[..., -1]) > 1e-4 * two[..., 0].abs()  # no two keys near enough to swap places
+    assert clear.double().mean() > 0.9
+    assert ((got.cpu().double() - want).abs() <= bound)[clear].all()
