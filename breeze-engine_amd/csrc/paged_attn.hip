@@ -49,13 +49,20 @@ struct AttnArgs {
     uint8_t* unpacked;  // [copies][H][tiles]: the copies that long chunks read
     int tiles;          // of 64 keys, in the whole table
     int by_seq;         // a copy for each sequence; else for those of kBigRows rows or more
-    float* part;        // [nsplit][T * Hq][D] when nsplit > 1
-    f2* ml;             // [nsplit][T * Hq]: maximum and sum; a first sum below zero: the row is done
+    // Sums of rows whose keys are split, one set for each kind of kernel, where that kind
+    // has more than one split: [nkeys][krows][D] and [nrows][T * Hq][D], with maximum and
+    // sum of each.  A first sum below zero: the row is not this kind's.
+    float* kpart;
+    float* rpart;
+    f2* kml;
+    f2* rml;
+    int64_t krows;
+    int kper;           // attn_keys_kernel's rows are [B][H][kper] (0: [T][Hq])
     int64_t table_row;
     int T, B, Hq, H, G, P, pshift, table_w, nslots, dt;
     int ntile16;               // workgroups for a sequence's rows in attn_keys_kernel
     int few, big;              // attn_rows_kernel's sequences have more than `few` and fewer than `big` rows
-    int nsplit, nkeys, nrows;  // splits that the workspace has room for, and those of the two kinds of kernels
+    int nkeys, nrows;          // splits of the keys: of the two kinds of kernels
     float scale;  // softmax scale * log2(e)
 };
 
@@ -113,14 +120,12 @@ __device__ inline int64_t group_row(const AttnArgs& a, const int32_t* table, int
     return is ? row : -1;
 }
 
-// Where a row's sums go: the output, or (a kernel of more than one split) the
-// workspace; there, the splits that the kernel does not have are marked empty.
-__device__ inline void mark_row(const AttnArgs& a, int own, int split, int64_t row, float top, float sum) {
-    if (a.nsplit == 1) return;
-    const int64_t n = (int64_t)a.T * a.Hq;
-    a.ml[split * n + row] = own > 1 ? (f2){top, sum} : (f2){0.0f, -1.0f};  // no sum of exponentials is below zero
-    if (split == 0)
-        for (int s = own; s < a.nsplit; ++s) a.ml[s * n + row] = (f2){-INFINITY, 0.0f};
+constexpr f2 kNotMine = {0.0f, -1.0f};  // no sum of exponentials is below zero
+
+// attn_keys_kernel's row among its sums: token `tok`, query head `head`, which is row
+// `row` of sequence b and key head h.
+__device__ inline int64_t keys_row_of(const AttnArgs& a, int b, int h, int row, int tok, int head) {
+    return a.kper ? ((int64_t)b * a.H + h) * a.kper + row : (int64_t)tok * a.Hq + head;
 }
 
 __device__ inline uint32_t lane_max_u32(uint32_t x, int step) { return max(x, (uint32_t)__shfl_xor((int)x, step)); }
@@ -388,9 +393,12 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
         f[w] *= snu[w][r];
     }
     const int ot = sq.q0 + (row0 + r) / a.G, oh = h * a.G + (row0 + r) % a.G;
-    const int64_t orow = (int64_t)ot * a.Hq + oh, prow = (int64_t)split * a.T * a.Hq + orow;
+    const int64_t prow = split * a.krows + keys_row_of(a, b, h, row0 + r, ot, oh);
     const float inv = a.nkeys > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-    if (part == 0) mark_row(a, a.nkeys, split, orow, top, sum);
+    if (part == 0) {
+        if (a.nkeys > 1) a.kml[prow] = (f2){top, sum};
+        if (a.nrows > 1 && split == 0) a.rml[(int64_t)ot * a.Hq + oh] = kNotMine;
+    }
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
         const int d = 64 * i + 4 * part;
@@ -398,7 +406,7 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
 #pragma unroll
         for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(so + (w * 16 + r) * OS + d) * f[w];
         v *= inv;
-        if (a.nkeys > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+        if (a.nkeys > 1) *reinterpret_cast<f4*>(a.kpart + prow * D + d) = v;
         else store4(a.out, DT, ot * a.o_token + oh * a.o_head + d, v);
     }
 }
@@ -452,6 +460,12 @@ __device__ inline int rows_of_slot(const AttnArgs& a, int slot, Seq& sq, int64_t
     const int64_t rows = (int64_t)sq.n * a.G;
     first = (slot - (a.cu ? (int64_t)sq.q0 * a.G / kRowTile + b : (int64_t)b * per)) * kRowTile;
     return first < 0 || first >= rows ? -1 : b;
+}
+
+// A row's maximum and sum, and where attn_keys_kernel's sums are by tokens too, that it is not among them.
+__device__ inline void mark_row(const AttnArgs& a, int split, int64_t row, float top, float sum) {
+    if (a.nrows > 1) a.rml[(int64_t)split * a.T * a.Hq + row] = (f2){top, sum};
+    if (a.nkeys > 1 && !a.kper && split == 0) a.kml[row] = kNotMine;
 }
 
 // A row's queries as operands (values 16 s + 8 (lane / 32) + 0..7 for slab s,
@@ -673,7 +687,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
     l = sum_halves(l);
     const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
     float f = nu * (1.0f / kPScale);
-    if (hf == 0) mark_row(a, a.nrows, split, orow, m * rowf, l);
+    if (hf == 0) mark_row(a, split, orow, m * rowf, l);
     if (a.nrows == 1) f *= l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -681,7 +695,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_rows_kernel(AttnAr
         for (int j = 0; j < 16; j += 4) {
             const int d = 32 * i + 2 * j + 4 * hf;
             const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
-            if (a.nrows > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+            if (a.nrows > 1) *reinterpret_cast<f4*>(a.rpart + prow * D + d) = v;
             else store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
         }
 }
@@ -1018,7 +1032,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
     l = sum_halves(l);
     const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
     float f = nu * (1.0f / kPScale);
-    if (hf == 0) mark_row(a, a.nrows, split, orow, m * rowf, l);
+    if (hf == 0) mark_row(a, split, orow, m * rowf, l);
     if (a.nrows == 1) f *= l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -1026,7 +1040,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
         for (int j = 0; j < 16; j += 4) {
             const int d = 32 * i + 2 * j + 4 * hf;
             const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
-            if (a.nrows > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
+            if (a.nrows > 1) *reinterpret_cast<f4*>(a.rpart + prow * D + d) = v;
             else store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
         }
 }
@@ -1045,51 +1059,68 @@ constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer th
 constexpr int kSplitMin = 64, kSplitMixed = 1024, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
 
 // The splits of a row joined: D/4 lanes a split and NG splits of a row at a
-// time, their sums then in the order of the splits.
+// time, their sums then in the order of the splits.  First the rows that
+// attn_keys_kernel split, then the other kernels'.
 template <int D, int NG>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     constexpr int L = D / 4, RW = 256 / L / NG;  // rows a workgroup
     __shared__ __align__(16) float sv[NG > 1 ? 256 / L : 1][D];
     __shared__ float sw[256 / L][kSplitMost];
-    const int64_t n = (int64_t)a.T * a.Hq;
     const int part = threadIdx.x / L, g = part % NG, d = 4 * (threadIdx.x % L);
-    const int64_t row = (int64_t)blockIdx.x * RW + part / NG;
-    const int tok = (int)(row / a.Hq), head = (int)(row % a.Hq);
-    bool mine = row < n && !(a.cu && (tok < a.cu[0] || tok >= a.cu[a.B]));
-    mine = mine && !(a.ml[row].y < 0.0f);  // else the row is done
+    int64_t row = (int64_t)blockIdx.x * RW + part / NG;
+    const int64_t nk = a.nkeys > 1 ? a.krows : 0;
+    const bool keys = row < nk;
+    const int64_t n = keys ? nk : (int64_t)a.T * a.Hq;  // rows of this kind
+    if (!keys) row -= nk;
+    const int nsplit = keys ? a.nkeys : a.nrows;
+    const f2* const ml = keys ? a.kml : a.rml;
+    const float* const sums = keys ? a.kpart : a.rpart;
+    int tok = 0, head = 0;
+    bool mine = row < n && nsplit > 1;
+    if (keys && a.kper) {
+        const int r = (int)(row % a.kper), h = (int)(row / a.kper % a.H), b = (int)(row / a.kper / a.H);
+        const Seq sq = sequence(a, b);
+        mine = (int64_t)sq.n * a.G <= a.few && r < sq.n * a.G;
+        tok = sq.q0 + r / a.G;
+        head = h * a.G + r % a.G;
+    } else if (mine) {
+        tok = (int)(row / a.Hq);
+        head = (int)(row % a.Hq);
+        mine = !(a.cu && (tok < a.cu[0] || tok >= a.cu[a.B])) && !(ml[row].y < 0.0f);
+    }
     f4 v = {0, 0, 0, 0};
     float sum = 0.0f;
     // The splits' maxima and sums first, one or more a lane; sw: a split's weight.
     {
         constexpr int PER = kSplitMost / L;
         const int lane = threadIdx.x % L;
-        f2 ml[PER];
+        f2 x[PER];
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int s = lane + L * i;
-            ml[i] = mine && s < a.nsplit ? a.ml[s * n + row] : (f2){-INFINITY, 0.0f};
-            top = fmaxf(top, ml[i].x);
+            x[i] = mine && s < nsplit ? ml[s * n + row] : (f2){-INFINITY, 0.0f};
+            top = fmaxf(top, x[i].x);
         }
 #pragma unroll
         for (int st = 1; st < L; st *= 2) top = fmaxf(top, __shfl_xor(top, st));
         const float safe = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const float f = fast_exp2(ml[i].x - safe);
-            sum += ml[i].y == 0.0f && ml[i].x == -INFINITY ? 0.0f : f * ml[i].y;
-            // An empty split's sums are not there: marked by a weight below zero.
-            sw[part][lane + L * i] = ml[i].y == 0.0f && ml[i].x == -INFINITY ? -1.0f : f;
+            const float f = fast_exp2(x[i].x - safe);
+            sum += x[i].y == 0.0f && x[i].x == -INFINITY ? 0.0f : f * x[i].y;
+            // An empty split's sums add nothing and are not read: marked by a weight below zero.
+            sw[part][lane + L * i] = x[i].y == 0.0f && x[i].x == -INFINITY ? -1.0f : f;
         }
 #pragma unroll
         for (int st = 1; st < L; st *= 2) sum += __shfl_xor(sum, st);
     }
     if (mine) {
 #pragma unroll 8
-        for (int s = g; s < a.nsplit; s += NG) {
+        for (int s = g; s < nsplit; s += NG) {
             const float f = sw[part][s];
             if (f < 0.0f) continue;
-            v += *reinterpret_cast<const f4*>(a.part + (s * n + row) * D + d) * f;
+            v += *reinterpret_cast<const f4*>(sums + (s * n + row) * D + d) * f;
         }
     }
     if constexpr (NG > 1) {
@@ -1109,9 +1140,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 struct AttnPlan {
     int keys, ntile16, rows, nslots;  // which kernels run, workgroups a sequence, slots of the rows kernels
     int lone;                        // the keys kernel's sequences are mostly of one token
-    int nkeys, nrows, nsplit;        // splits of the keys: of the two kinds of kernels, room for
+    int nkeys, nrows;                // splits of the keys: of the two kinds of kernels
+    int64_t krows;                   // rows that attn_keys_kernel has sums for where it splits
+    int kper;                        // of each sequence and key head; 0: of each token and head
     int tiles, by_seq, direct;       // of an unpacked copy, 0: none; one for each sequence; attn_rows_kernel runs
-    size_t copy, bytes;              // of the copies, of the workspace
+    size_t copy, kpart, rpart, bytes;  // of the copies, of the two kinds' sums (without maxima), of the workspace
 };
 
 // Copies are made for calls of kUnpackRows rows or more (heads of 256, whose sums
@@ -1121,11 +1154,15 @@ struct AttnPlan {
 // most kUnpackMost bytes.
 constexpr int kUnpackRows = 512, kUnpackRows256 = 64, kUnpackMean = 64;
 constexpr size_t kUnpackMost = (size_t)4 << 30;
+// Bytes that the split rows' sums of either kind of kernel may take: a table of many
+// columns asks for many splits, and a call may have many rows.
+constexpr size_t kPartMost = (size_t)512 << 20;
 
 AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int dtype, int n_cu) {
     const int G = Hq / H;
     AttnPlan p{};
     const int few = few_rows(D);
+    const size_t row_bytes = (size_t)D * 4 + 8;  // a row's sums, maximum and sum of one split
     p.rows = cu ? (int64_t)T * G > few : G > few;
     // One sequence alone is never worth a second launch that may find nothing to do.
     p.keys = G <= few && !(p.rows && B == 1);
@@ -1139,16 +1176,29 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
         const int64_t fill = (2 * n_cu + wgs - 1) / wgs;
         const bool mixed = (int64_t)T * G > few * (int64_t)B;
         p.lone = p.ntile16 == 1 || mixed;
-        const int64_t idle = mixed ? std::min<int64_t>(16, capacity / kSplitMixed)
-                                                                  : std::min<int64_t>(fill, capacity / kSplitMin);
-        p.nkeys = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(idle, capacity / kSplitKeys), std::min<int64_t>(kSplitMost, std::max<int64_t>(1, kMostBlocks / ((int64_t)B * H * p.ntile16)))));
+        const int64_t idle = mixed ? std::min<int64_t>(16, capacity / kSplitMixed) : std::min(fill, capacity / kSplitMin);
+        // The sequences' rows by themselves where that is fewer than all of the call's: one
+        // long chunk beside single tokens has no sums here.
+        const int64_t kper = std::min<int64_t>(few, (int64_t)T * G), by_seq = (int64_t)B * H * kper;
+        p.krows = (int64_t)T * Hq;
+        if (cu && by_seq < p.krows) {
+            p.krows = by_seq;
+            p.kper = (int)kper;
+        }
+        const int64_t blocks = kMostBlocks / ((int64_t)B * H * p.ntile16), room = (int64_t)(kPartMost / (p.krows * row_bytes));
+        const int64_t most = std::max<int64_t>(1, std::min({(int64_t)kSplitMost, blocks, room}));
+        p.nkeys = (int)std::max<int64_t>(1, std::min(std::max(idle, capacity / kSplitKeys), most));
     }
     if (p.rows) {
         const int64_t wgs = (int64_t)p.nslots * H, room = (int64_t)n_cu * (D == 256 || (D == 128 && dtype == kF32) ? 1 : 2);
         // A prompt's workgroups, the longest first, fill the last round by themselves.
         const bool causal = wgs >= room && 2 * (int64_t)T >= capacity * B;
         double best = 1e30;
-        for (int64_t s = 1; s <= 16 && (s == 1 || (s * kSplitRows <= capacity && wgs < 4 * room && !causal && s * wgs <= kMostBlocks)); ++s) {
+        const auto may = [&](int64_t s) {
+            return s * kSplitRows <= capacity && wgs < 4 * room && !causal && s * wgs <= kMostBlocks &&
+                   (size_t)s * T * Hq * row_bytes <= kPartMost;
+        };
+        for (int64_t s = 1; s <= 16 && (s == 1 || may(s)); ++s) {
             const double cost = (double)((wgs * s + room - 1) / room) / s * (1.0 + 0.02 * (s - 1));
             if (cost < best) {
                 best = cost;
@@ -1168,8 +1218,10 @@ AttnPlan plan_attn(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity
             p.direct = !p.by_seq;
         }
     }
-    p.nsplit = std::max(p.nkeys, p.nrows);
-    p.bytes = p.copy + (p.nsplit > 1 ? (size_t)p.nsplit * T * Hq * (D * 4 + 8) : 0);
+    const size_t nk = p.nkeys > 1 ? (size_t)p.nkeys * p.krows : 0, nr = p.nrows > 1 ? (size_t)p.nrows * T * Hq : 0;
+    p.kpart = nk * D * 4;
+    p.rpart = nr * D * 4;
+    p.bytes = p.copy + (nk + nr) * row_bytes;
     return p;
 }
 
@@ -1213,10 +1265,10 @@ template <int D>
 void launch1(const AttnArgs& a, const AttnPlan& p, int kind, hipStream_t st) {
     if (kind == kInt8) launch2<D, kInt8>(a, p, st);
     else launch2<D, kFp8>(a, p, st);
-    if (a.nsplit > 1) {
+    if (a.nkeys > 1 || a.nrows > 1) {
         // Few rows: all of a workgroup's lanes for one, so that many splits are read at once.
         constexpr int NG = 256 / (D / 4);
-        const int64_t n = (int64_t)a.T * a.Hq;
+        const int64_t n = (a.nkeys > 1 ? a.krows : 0) + (a.nrows > 1 ? (int64_t)a.T * a.Hq : 0);
         if (n <= 2048) attn_join_kernel<D, NG><<<(unsigned)n, 256, 0, st>>>(a);
         else attn_join_kernel<D, 1><<<(unsigned)((n + NG - 1) / NG), 256, 0, st>>>(a);
     }
@@ -1324,7 +1376,6 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
         bq_set_error("paged_attention: needs a workspace of %zu bytes, got %lld", p.bytes, (long long)work_bytes);
         return -4;
     }
-    a.nsplit = p.nsplit;
     a.nkeys = p.nkeys;
     a.few = p.keys ? few_rows(cache->head_dim) : 0;
     a.by_seq = p.by_seq;
@@ -1334,8 +1385,13 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
     a.nslots = p.nslots;
     a.tiles = p.tiles;
     a.unpacked = static_cast<uint8_t*>(dWork);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(dWork) + p.copy);
-    a.ml = reinterpret_cast<f2*>(a.part + (size_t)p.nsplit * T * heads * cache->head_dim);
+    uint8_t* const sums = static_cast<uint8_t*>(dWork) + p.copy;
+    a.kpart = reinterpret_cast<float*>(sums);
+    a.rpart = reinterpret_cast<float*>(sums + p.kpart);
+    a.kml = reinterpret_cast<f2*>(sums + p.kpart + p.rpart);
+    a.rml = a.kml + (p.nkeys > 1 ? p.nkeys * p.krows : 0);
+    a.krows = p.krows;
+    a.kper = p.kper;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     if (cache->head_dim == 64) launch1<64>(a, p, cache->kind, st);
