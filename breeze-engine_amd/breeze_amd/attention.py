@@ -344,7 +344,9 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
     The new state goes to ``state_out`` (``state`` itself, or apart from it) or
     to a new tensor.  State and sums are fp32; the products of prompts keep 22
     bits of every operand, of q and k down to 2^-28 of the largest in their chunk
-    of 64 tokens and head.  Sequences of more than 16 tokens, and one that is
+    of 64 tokens and head, of v and the state down to 2^-37 of the largest in their
+    column there.  With bf16 the state and u have 11 bits in the products that make
+    rows of o, three more than those keep.  Sequences of more than 16 tokens, and one that is
     alone in its call, go in chunks of 64: a NaN or infinity there reaches all
     rows of its chunk and those after it."""
     torch = _torch()

@@ -22,8 +22,8 @@
 // Numerics.  Products run on the fp16 matrix instructions with each operand
 // as two fp16 terms (hi, and what hi leaves; 22 bits and more) and three
 // products, fp32 sums; q and k given as bf16 or fp16 are one term, and so are
-// the state and U where they only make rows of O of such a type (11 bits; the
-// state itself and U go on with two).  A power
+// the state and U where they only make rows of O of bf16 (11 bits, three more than
+// those keep; the state itself and U go on with two).  A power
 // of two for each tile (of q and k: each chunk and head) or column puts the
 // largest value where fp16 has room; what a second term cannot hold then is
 // 2^-28 of a chunk's largest q or k, 2^-37 of a column's largest.  T is computed in fp32.  Sums of g are taken in
@@ -538,7 +538,7 @@ __device__ inline void to_operand(const f4* x, float up, const float* rows, int 
 }
 
 // A lower triangular factor (T or M) of two terms times 16 columns of two, or
-// (rows of O that are rounded to a half type) of one.
+// (rows of O that are rounded to bf16) of one.
 template <bool TWO>
 __device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, const h8* xl, f4* acc) {
 #pragma unroll
@@ -570,15 +570,16 @@ __device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, con
 // 128 x 128, 192 workgroups: 195 us).  All products in one wave and 64 columns
 // a workgroup took 5.0 (the LDS reads of four waves, 480 KB, alone 1.6).
 template <int DK, int DT, bool DELTA>
-__global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaArgs a) {
-    constexpr bool LO = DT == kF32;
-    constexpr int NT = LO ? 2 : 1, ST = DK / 16, SS = DK / 32;  // tiles and slabs of the state's rows
+__global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 2) void gla_inter_kernel(GlaArgs a) {
+    constexpr bool LO = DT == kF32;      // two terms of q and k
+    constexpr bool TWO = DT != kBF16;    // two of the state and U for the rows of O
+    constexpr int NT = LO ? 2 : 1, NO = TWO ? 2 : 1, ST = DK / 16, SS = DK / 32;  // tiles and slabs of the state's rows
     constexpr int kPart = 4 * SS * 1024, kBuf = kq_bytes(DK, LO);
     __shared__ __align__(1024) uint8_t skq[2][kBuf];       // operands of k, then of q
     // What the state's waves hand over: the state's operands and U's, one term of each
-    // for rows of O that are rounded to bf16 or fp16 (80 KB of LDS in all: two workgroups a unit).
-    __shared__ __align__(1024) uint8_t ss[2][NT * SS * 1024];
-    __shared__ __align__(1024) uint8_t su[2][NT * 2 * 1024];
+    // for rows of O that are rounded to bf16 (80 KB of LDS in all: two workgroups a unit).
+    __shared__ __align__(1024) uint8_t ss[2][NO * SS * 1024];
+    __shared__ __align__(1024) uint8_t su[2][NO * 2 * 1024];
     __shared__ __align__(1024) float sf[2][kFac];
     __shared__ float sunits[2][2][16];  // what a unit of those is worth, for each column
 
@@ -640,7 +641,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaA
             h8 oh[2][4], ol[2][4], sh[2], sl[2];
             const auto get = [&](int s) {
                 sh[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * s + 16 * lane);
-                if constexpr (LO) sl[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane);
+                if constexpr (TWO) sl[s & 1] = *reinterpret_cast<const h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     oh[s & 1][t] = op(qb, t * SS + s);
@@ -654,12 +655,12 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaA
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) qs[t] = mfma16(oh[s & 1][t], sh[s & 1], qs[t]);
-                if constexpr (LO) {
+                if constexpr (TWO)
 #pragma unroll
                     for (int t = 0; t < 4; ++t) qs[t] = mfma16(oh[s & 1][t], sl[s & 1], qs[t]);
+                if constexpr (LO)
 #pragma unroll
                     for (int t = 0; t < 4; ++t) qs[t] = mfma16(ol[s & 1][t], sh[s & 1], qs[t]);
-                }
                 if (ch + 1 < nchunk)
 #pragma unroll
                     for (int i = 4 * s / SS; i < 4 * (s + 1) / SS; ++i) fetch(ch + 1, i);
@@ -679,11 +680,11 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaA
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 uh[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * s + 16 * lane);
-                if constexpr (LO) ul[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * (2 + s) + 16 * lane);
+                if constexpr (TWO) ul[s] = *reinterpret_cast<const h8*>(su[pair] + 1024 * (2 + s) + 16 * lane);
             }
             const float w3 = w2 * sunits[1][pair][r16];
             f4 acc[4];
-            tri_product<LO>(mh, ml, uh, ul, acc);
+            tri_product<TWO>(mh, ml, uh, ul, acc);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -753,7 +754,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaA
 #pragma unroll
         for (int s = 0; s < SS; ++s) {
             *reinterpret_cast<h8*>(ss[pair] + 1024 * s + 16 * lane) = sh[s];
-            if constexpr (LO) *reinterpret_cast<h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane) = sl[s];
+            if constexpr (TWO) *reinterpret_cast<h8*>(ss[pair] + 1024 * (SS + s) + 16 * lane) = sl[s];
         }
         if (c == 0) sunits[0][pair][r16] = sunit;
     };
@@ -827,7 +828,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void gla_inter_kernel(GlaA
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             *reinterpret_cast<h8*>(su[pair] + 1024 * s + 16 * lane) = uh[s];
-            if constexpr (LO) *reinterpret_cast<h8*>(su[pair] + 1024 * (2 + s) + 16 * lane) = ul[s];
+            if constexpr (TWO) *reinterpret_cast<h8*>(su[pair] + 1024 * (2 + s) + 16 * lane) = ul[s];
         }
         if (c == 0) sunits[1][pair][r16] = uunit;
         __syncthreads();

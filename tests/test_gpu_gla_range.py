@@ -1,0 +1,53 @@
+"""Gated linear attention of prompts: what their products keep."""
+import pytest
+import torch
+
+from mixers_plain import recur
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def att(gpu):
+    from breeze_amd import attention
+    return attention
+
+
+def _cu(lens):
+    return torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32)
+
+
+def _excess_norm(got, want):
+    """The norm of what is left of |got - want| after one rounding to got's type."""
+    f = torch.finfo(got.dtype)
+    got, off = got.double(), (got.double() - want).abs()
+    step = torch.exp2(torch.floor(torch.log2(torch.maximum(got.abs(), want.abs()).clamp_min(f.smallest_normal)))) * f.eps
+    return (off - step / 2).clamp_min(0).norm()
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("Hk,Hv,Dk,Dv", [(2, 6, 128, 128), (1, 2, 64, 80)])
+@pytest.mark.parametrize("lens", [[64], [130, 17, 300], [700]])
+def test_fp16_rows_are_rounded_once(att, delta, Hk, Hv, Dk, Dv, lens):
+    """Rows of fp16 prompts: products of 22 bits, then one rounding.  |o - want| is at
+    most half a step plus the error before it; the latter's norm is at most 5 sqrt(c)
+    2^-20 of the rows' and state's (five products in a row, c chunks), so what is left
+    over half a step has no larger one.  Operands of 11 bits would leave 2^-13."""
+    gen = torch.Generator().manual_seed(len(lens))
+    rand = lambda *s: torch.randn(s, generator=gen)  # noqa: E731
+    unit = lambda x: x / x.norm(dim=-1, keepdim=True)  # noqa: E731
+    T = sum(lens)
+    q, k, v = unit(rand(T, Hk, Dk)).half(), (0.999 * unit(rand(T, Hk, Dk))).half(), rand(T, Hv, Dv).half()
+    g, state = -torch.exp(3 * torch.rand((T, Hv), generator=gen) - 4), rand(len(lens), Hv, Dk, Dv)
+    beta = torch.sigmoid(rand(T, Hv)) if delta else None
+    o, _ = att.gated_linear_attention(*(None if t is None else t.cuda() for t in (q, k, v, g, beta, state)), _cu(lens).cuda())
+    want, _, size = recur(q, k, v, g, beta, state, lens, Dk ** -0.5)
+    start = 0
+    for b, n in enumerate(lens):
+        part = slice(start, start + n)
+        rel = 5 * (-(-n // 64)) ** 0.5 * 2.0 ** -20
+        whole = want[part].norm() + Dk ** -0.5 * size[b].norm() * q[part].double().norm(dim=-1).max()
+        left = _excess_norm(o[part].cpu(), want[part])
+        print(f"{n} tokens: {(left / (rel * whole)).item():.3f} of the bound", flush=True)
+        assert left <= rel * whole
+        start += n
