@@ -837,7 +837,8 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
             if constexpr (DELTA) load_t(ch + 1);
         }
         // S = e^{G_C} S + K^T (e^{G_C - G} U), summed in the units of this product; a
-        // product too small to show beside the state does not set them.
+        // product too small to show beside the state does not set them (S is at most 2^13
+        // sunit, so 2^93 in units of 2^-80 of that).
         {
             constexpr int GT = 2;  // tiles of the state's rows a group
             h8 oh[2][GT][2], ol[2][GT][2];
@@ -853,7 +854,7 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
                     }
             };
             get(0);
-            const float worth = fmaxf(fmaxf(uunit * kunit, sworth * 0x1p-60f), 0x1p-100f);
+            const float worth = fmaxf(fmaxf(uunit * kunit, sworth * 0x1p-60f), fmaxf(sunit * 0x1p-80f, 0x1p-100f));
             to_operand<4>(u, uworth * kunit * inverse_pow2(worth), fac + kChunk, c, uh, ul);
             const float keep = fac[kChunk - 1] * (sworth * inverse_pow2(worth));
             sworth = worth;

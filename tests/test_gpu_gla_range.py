@@ -1,4 +1,5 @@
-"""Gated linear attention of prompts: what their products keep."""
+"""Gated linear attention of prompts: what their products keep, and states far
+larger than what is added to them."""
 import pytest
 import torch
 
@@ -15,6 +16,29 @@ def att(gpu):
 
 def _cu(lens):
     return torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("n", [100, 300, 700])
+def test_a_large_state_and_tiny_additions(att, delta, n):
+    """A state of 1e10 to which products of 1e-38 are added, chunk after chunk: it
+    stays, within its fp32 products' errors, and does not leave fp32 in the units
+    of what is added."""
+    gen = torch.Generator().manual_seed(n)
+    rand = lambda *s: torch.randn(s, generator=gen)  # noqa: E731
+    Hv, Dk, Dv = 2, 64, 48
+    q, k, v = rand(n, 1, Dk), 1e-19 * rand(n, 1, Dk), 1e-19 * rand(n, Hv, Dv)
+    g, state = torch.full((n, Hv), -1e-3), 1e10 * rand(1, Hv, Dk, Dv)
+    beta = torch.sigmoid(rand(n, Hv)) if delta else None
+    o, S = att.gated_linear_attention(*(None if t is None else t.cuda() for t in (q, k, v, g, beta, state)), _cu([n]).cuda())
+    want_o, want_S, _ = recur(q, k, v, g, beta, state, [n], Dk ** -0.5)
+    # A chunk multiplies the state by one decay (an exponential's last bits and one
+    # rounding, 2^-22) and rounds it; rows of O have 64 terms of 22 bits and the like.
+    chunks = -(-n // 64)
+    assert torch.isfinite(S).all() and torch.isfinite(o).all()
+    assert ((S.cpu().double() - want_S).abs() <= (chunks + 1) * 2.0 ** -22 * state.double().abs()).all()
+    size = (q.double().abs().repeat(1, Hv, 1).unsqueeze(-1) * state[0].double().abs()).sum(2) * Dk ** -0.5
+    assert ((o.cpu().double() - want_o).abs() <= (chunks + 66) * 2.0 ** -21 * size).all()
 
 
 def _excess_norm(got, want):
