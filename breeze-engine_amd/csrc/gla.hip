@@ -30,6 +30,8 @@
 // 64 bits: e^{G_i - G_j} would lose what G_i and G_j have in common.
 #include "mix_common.h"
 
+#include <algorithm>
+
 #include "../../include/breeze_qmm.h"
 
 using namespace mx;
@@ -55,7 +57,8 @@ struct GlaArgs {
     uint8_t* kq;        // [slots][Hk]: operands of k (hi, lo), then of q
     uint8_t* tm;        // [slots][Hv]: operands of M (hi, lo), then of T
     float* fac;   // [slots][Hv][kFac]: e^G, e^{G_C - G}, what a unit of T's, k's and q's operands is worth
-    int T, B, Hk, Hv, rep, Dv, dt, nslots;
+    int slot0, slot1;   // the chunks' slots that the workspace holds now
+    int T, B, Hk, Hv, rep, Dv, dt;
     int nshort;  // sequences of up to this many tokens are gla_step_kernel's
     float scale;
 };
@@ -245,9 +248,9 @@ __global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
     float* const st = sa + kChunk * AS;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x % a.Hk, slot = blockIdx.x / a.Hk;
+    const int hk = blockIdx.x % a.Hk, slot = blockIdx.x / a.Hk;  // counted from slot0 on
     int tok, n;
-    if (!chunk_of(a, slot, tok, n)) return;
+    if (!chunk_of(a, a.slot0 + slot, tok, n)) return;
 
     // q and k, scaled to [2^3, 2^4) so that their products fit fp16 too.
     f4 kx[NP], qx[NP];
@@ -592,7 +595,10 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
     const int hk = hv / a.rep, col0 = 32 * cb + 16 * pair;
     const bool mine = col0 < a.Dv;  // 16 columns are there or not, for the whole wave
     const int col = (mine ? col0 : 0) + r16;
-    const int nchunk = (sp.n + kChunk - 1) / kChunk, slot0 = sp.q0 / kChunk + b;
+    // Its chunks whose slots are here; one without any writes its state in the first segment.
+    const int chunks = (sp.n + kChunk - 1) / kChunk, slot0 = sp.q0 / kChunk + b - a.slot0;
+    const int begin = max(-slot0, 0), nchunk = min(chunks, a.slot1 - a.slot0 - slot0);
+    if (begin >= nchunk && (chunks > 0 || a.slot0 > 0)) return;
     const int64_t at = ((int64_t)b * a.Hv + hv) * DK * a.Dv + col;
     const int rd = 16 * place(r16, c);  // where the lane's 16 bytes of an operand lie
     const auto op = [&](const uint8_t* base, int f) { return *reinterpret_cast<const h8*>(base + 1024 * f + rd); };
@@ -620,12 +626,12 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
                 for (int e = 0; e < 4; ++e)
                     if (full || first + 16 * t + e < sp.n) store1<DT>(a.o, p + (16 * t + e) * a.o_token, y[t][e]);
         };
-        if (nchunk > 0)
+        if (begin < nchunk)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fetch(0, i);
+            for (int i = 0; i < 4; ++i) fetch(begin, i);
         wait_loads<0>();
         __syncthreads();
-        for (int ch = 0; ch < nchunk; ++ch) {
+        for (int ch = begin; ch < nchunk; ++ch) {
             h8 mh[kTri], ml[kTri];
             const h8* mp = reinterpret_cast<const h8*>(tm_of(ch));
 #pragma unroll
@@ -698,7 +704,7 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
                     wait_loads<0>();
                 }
             } else if (mine) {
-                store(ch, sp.n == kChunk * nchunk);
+                store(ch, sp.n >= kChunk * nchunk);
             }
             __syncthreads();  // the next state is there, and the next chunk's operands
         }
@@ -712,11 +718,12 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
     for (int t = 0; t < ST; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[t][e] = 0.0f;
-    if (a.s_in)
+    const float* const from = begin > 0 ? a.s_out : a.s_in;  // the segment before left it there
+    if (from)
 #pragma unroll
         for (int t = 0; t < ST; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[t][e] = a.s_in[at + (int64_t)(16 * t + 4 * c + e) * a.Dv];
+            for (int e = 0; e < 4; ++e) S[t][e] = from[at + (int64_t)(16 * t + 4 * c + e) * a.Dv];
 
     uint32_t v[4][4];
     const auto load_v = [&](int ch) {
@@ -758,16 +765,16 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
         }
         if (c == 0) sunits[0][pair][r16] = sunit;
     };
-    if (nchunk > 0) {
-        load_v(0);
-        if constexpr (DELTA) load_t(0);
+    if (begin < nchunk) {
+        load_v(begin);
+        if constexpr (DELTA) load_t(begin);
     }
     hand_over();
     __syncthreads();
 
     // The transposed reads: key 4 c + r16 / 4 of a tile, values 4 (r16 & 3) + 0..3 of 16.
     const int rt = 16 * place(4 * c + (r16 >> 2), r16 & 3);
-    for (int ch = 0; ch < nchunk; ++ch) {
+    for (int ch = begin; ch < nchunk; ++ch) {
         const uint8_t* const kb = skq[ch & 1];
         const float* const fac = sf[ch & 1];
         const float kunit = fac[2 * kChunk + 1];
@@ -894,27 +901,35 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
 
 struct GlaPlan {
     bool chunks;
-    int nslots;
+    int nslots, segment;  // slots of chunks, and how many of them the workspace holds at a time
     size_t kq, tm, fac, bytes;
 };
+
+// The chunks' operands take about as much as the call's own tensors, 36 KB a token of 16/48
+// heads of 128 in fp32; past these bytes they go in segments, one after the other,
+// with the states in between where the call leaves them at its end.
+constexpr size_t kMostOperands = (size_t)1 << 30;
 
 GlaPlan plan_gla(int T, int B, int Hk, int Hv, int Dk, int dtype, bool cu, bool delta) {
     GlaPlan p{};
     p.chunks = cu && T > kShort;
     if (!p.chunks) return p;
     p.nslots = T / kChunk + B;
-    const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    p.kq = up((size_t)p.nslots * Hk * kq_bytes(Dk, dtype == kF32));
-    p.tm = up((size_t)p.nslots * Hv * tm_bytes(delta));
-    p.fac = up((size_t)p.nslots * Hv * kFac * 4);
+    const size_t kq = (size_t)Hk * kq_bytes(Dk, dtype == kF32), tm = (size_t)Hv * tm_bytes(delta), fac = (size_t)Hv * kFac * 4;
+    p.segment = (int)std::max<size_t>(1, std::min<size_t>(p.nslots, kMostOperands / (kq + tm + fac)));
+    p.kq = p.segment * kq;  // multiples of 1024 bytes
+    p.tm = p.segment * tm;
+    p.fac = p.segment * fac;
     p.bytes = p.kq + p.tm + p.fac;
     return p;
 }
 
 template <int DK, int DT, bool DELTA>
-void launch3(const GlaArgs& a, const GlaPlan& p, hipStream_t st) {
-    if (p.chunks) {
-        gla_intra_kernel<DK, DT, DELTA><<<(unsigned)p.nslots * a.Hk, 256, 0, st>>>(a);
+void launch3(GlaArgs a, const GlaPlan& p, hipStream_t st) {
+    for (int at = 0; at < p.nslots; at += p.segment) {
+        a.slot0 = at;
+        a.slot1 = std::min(at + p.segment, p.nslots);
+        gla_intra_kernel<DK, DT, DELTA><<<(unsigned)(a.slot1 - at) * a.Hk, 256, 0, st>>>(a);
         gla_inter_kernel<DK, DT, DELTA><<<(unsigned)a.B * a.Hv * ((a.Dv + 31) / 32), 256, 0, st>>>(a);
     }
     const int64_t waves = (int64_t)a.B * a.Hv * (a.Dv / 16);
@@ -1006,7 +1021,6 @@ int i4_gated_linear_attention_dev(const void* dQ, int64_t q_token, int64_t q_hea
         bq_set_error("gated_linear_attention: needs a workspace of %zu bytes, got %lld", p.bytes, (long long)work_bytes);
         return -4;
     }
-    a.nslots = p.nslots;
     // One sequence alone is never worth a third launch that may find nothing to do.
     a.nshort = !p.chunks ? 1 << 30 : B == 1 ? -1 : kShort;
     uint8_t* w = static_cast<uint8_t*>(dWork);

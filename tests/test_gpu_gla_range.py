@@ -1,8 +1,9 @@
-"""Gated linear attention of prompts: what their products keep, and states far
-larger than what is added to them."""
+"""Gated linear attention of prompts: what their products keep, states far larger
+than what is added to them, and long prompts, which go in segments."""
 import pytest
 import torch
 
+from breeze_amd import hip_backend as hb
 from mixers_plain import recur
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +76,42 @@ def test_fp16_rows_are_rounded_once(att, delta, Hk, Hv, Dk, Dv, lens):
         print(f"{n} tokens: {(left / (rel * whole)).item():.3f} of the bound", flush=True)
         assert left <= rel * whole
         start += n
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[9000, 5, 0, 31500, 70, 12345], [31000, 31000], [45000]])
+def test_long_prompts_in_segments(att, dtype, lens):
+    """More chunks than the workspace holds at once (about 30000 tokens of these heads in
+    fp32, 38000 in bf16), in one call and sequence by sequence, long ones in parts:
+    the same bits, since a state's units are powers of two."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    Hk, Hv, D, T = 16, 48, 128, sum(lens)
+    assert hb._lib.i4_gated_linear_attention_workspace(T, len(lens), Hk, Hv, D, D, 0 if dtype == torch.float32 else 1, 1, 1) > 0.99 * 2 ** 30
+    unit = lambda x: x / x.norm(dim=-1, keepdim=True)  # noqa: E731
+    q, k, v = unit(rand(T, Hk, D)).to(dtype), unit(rand(T, Hk, D)).to(dtype), rand(T, Hv, D).to(dtype)
+    g, beta = -torch.exp(-7 + 5 * torch.rand((T, Hv), generator=gen, device="cuda")), torch.sigmoid(rand(T, Hv))
+    state = rand(len(lens), Hv, D, D)
+    want = state.clone()
+    o, S = att.gated_linear_attention(q, k, v, g, beta, state, _cu(lens).cuda())
+    o2, S2 = att.gated_linear_attention(q, k, v, g, beta, want.clone(), _cu(lens).cuda())  # the workspace holds the last call's
+    assert torch.equal(o, o2) and torch.equal(S, S2) and torch.equal(state, want)
+    start = 0
+    for b, n in enumerate(lens):
+        s, at = want[b:b + 1].clone(), start
+        while at < start + n or n == 0:
+            part = min(230 * 64, start + n - at)  # whole chunks, but for the last
+            cut = slice(at, at + part)
+            x, _ = att.gated_linear_attention(q[cut], k[cut], v[cut], g[cut], beta[cut], s, _cu([part]).cuda(), state_out=s)
+            assert torch.equal(x, o[cut]), (b, at)
+            at += part
+            if n == 0:
+                break
+        assert torch.equal(s[0], S[b]), b
+        start += n
+    # In place, and from zeros.
+    att.gated_linear_attention(q, k, v, g, beta, state, _cu(lens).cuda(), state_out=state)
+    assert torch.equal(state, S)
+    a = att.gated_linear_attention(q, k, v, g, beta, None, _cu(lens).cuda())
+    b = att.gated_linear_attention(q, k, v, g, beta, torch.zeros_like(state), _cu(lens).cuda())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

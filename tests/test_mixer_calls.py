@@ -54,3 +54,16 @@ def test_workspaces_have_a_bound():
                                 assert n <= 5 << 30, (D, kv_heads, heads, T, B, keys)
         for B in (1, 64, 4096, 32768):
             assert _attention_bytes(8, 16, D, B, B, 64, 1, 1 << 16, 0) <= 512 << 20
+
+
+def test_workspaces_of_long_prompts():
+    """Gated linear attention holds 1 GiB of chunks' operands at a time."""
+    query = hb._lib.i4_gated_linear_attention_workspace
+    for k_heads, v_heads, k_dim, v_dim in ((16, 48, 128, 128), (1, 1, 64, 16), (32, 32, 128, 256), (64, 256, 128, 128)):
+        for T in (17, 1000, 4096, 40000, 131072, 1 << 20):
+            for B in (1, 7, 1000):
+                for dtype in (0, 1, 2):
+                    for beta in (0, 1):
+                        assert 0 < query(T, B, k_heads, v_heads, k_dim, v_dim, dtype, 1, beta) <= 1 << 30
+    # A call of fewer operands holds them all: 25 chunks' slots of 2 times 64 KB and 6 times 25 KB.
+    assert query(1536, 1, 2, 6, 128, 128, 0, 1, 1) == 25 * (2 * 65536 + 6 * 25600)
