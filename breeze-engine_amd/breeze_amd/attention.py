@@ -346,9 +346,12 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
     bits of every operand, of q and k down to 2^-28 of the largest in their chunk
     of 64 tokens and head, of v and the state down to 2^-37 of the largest in their
     column there.  With bf16 the state and u have 11 bits in the products that make
-    rows of o, three more than those keep.  Sequences of more than 16 tokens, and one that is
-    alone in its call, go in chunks of 64: a NaN or infinity there reaches all
-    rows of its chunk and those after it."""
+    rows of o, three more than those keep.
+
+    A NaN in k, v, g or beta reaches its token's row and those after it (from v: in its
+    column), one in q its own row; no earlier ones.  Sequences of more than 16
+    tokens, in a call of several or alone, go in chunks of 64, where an infinity
+    does as NaN does."""
     torch = _torch()
     if q.dim() != 3 or v.dim() != 3 or k.shape != q.shape or v.shape[0] != q.shape[0]:
         raise ValueError(f"q and k must be [T, k_heads, k_dim] and v [T, v_heads, v_dim], got {tuple(q.shape)}, "

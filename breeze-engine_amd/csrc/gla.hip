@@ -40,7 +40,7 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kShort = 16;
-constexpr int kFac = 256;  // 2 * 64 + 3, and what one load to LDS brings
+constexpr int kFac = 256;  // 2 * 64 + 4, and what one load to LDS brings
 
 struct GlaArgs {
     const void* q;
@@ -56,7 +56,9 @@ struct GlaArgs {
     const int32_t* cu;  // null: one token a sequence
     uint8_t* kq;        // [slots][Hk]: operands of k (hi, lo), then of q
     uint8_t* tm;        // [slots][Hv]: operands of M (hi, lo), then of T
-    float* fac;   // [slots][Hv][kFac]: e^G, e^{G_C - G}, what a unit of T's, k's and q's operands is worth
+    // [slots][Hv][kFac]: e^G, e^{G_C - G}, what a unit of T's, k's and q's operands is worth,
+    // and the first row whose k, g or beta is no finite number (64: none).
+    float* fac;
     int slot0, slot1;   // the chunks' slots that the workspace holds now
     int T, B, Hk, Hv, rep, Dv, dt;
     int nshort;  // sequences of up to this many tokens are gla_step_kernel's
@@ -179,6 +181,7 @@ __device__ inline float to_top(uint32_t bits) {
 __device__ inline float inverse_pow2(float p) { return bits_f((254u << 23) - f_bits(p)); }
 
 __device__ inline uint32_t abs_bits(float x) { return f_bits(x) & 0x7FFFFFFFu; }
+constexpr uint32_t kInfBits = 0x7F800000u;  // and above: NaN
 
 __device__ inline f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ inline f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -239,6 +242,7 @@ __global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
     __shared__ double sg[kChunk];
     __shared__ __align__(16) float sbeta[kChunk];
     __shared__ uint32_t stop[2][4];
+    __shared__ int sbad[4];
     _Float16* const in = reinterpret_cast<_Float16*>(lds);  // k hi, k lo, q hi, q lo
     _Float16* const sk = in;
     _Float16* const sq = in + NT * kChunk * KS;
@@ -262,16 +266,28 @@ __global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
         kx[i] = load4(a.k, DT, at * a.k_token + hk * a.k_head + d);
         qx[i] = load4(a.q, DT, at * a.q_token + hk * a.q_head + d);
     }
+    // A k that is no finite number enters no product, whose zeros it would spoil for the rows
+    // before it: its row and those after it are made NaN at the end.  A q spoils its own row only.
+    int bad = kChunk;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        if ((tid + 256 * i) / L >= n) kx[i] = qx[i] = (f4){0, 0, 0, 0};
+        const int row = (tid + 256 * i) / L;
+        if (row >= n) kx[i] = qx[i] = (f4){0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t x = abs_bits(kx[i][j]), y = abs_bits(qx[i][j]);
-            kt = max(kt, x < 0x7F800000u ? x : 0u);
-            qt = max(qt, y < 0x7F800000u ? y : 0u);
+            if (x >= kInfBits) {
+                kx[i][j] = 0.0f;
+                bad = min(bad, row);
+            } else {
+                kt = max(kt, x);
+            }
+            qt = max(qt, y < kInfBits ? y : 0u);
         }
     }
+    if (__any(bad < kChunk))
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2) bad = min(bad, __shfl_xor(bad, s));
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) {
         kt = max(kt, (uint32_t)__shfl_xor((int)kt, s));
@@ -280,12 +296,14 @@ __global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
     if (lane == 0) {
         stop[0][wave] = kt;
         stop[1][wave] = qt;
+        sbad[wave] = bad;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         kt = max(kt, stop[0][w]);
         qt = max(qt, stop[1][w]);
+        bad = min(bad, sbad[w]);
     }
     const float kup = to_top<3>(kt), qup = to_top<3>(qt), kunit = inverse_pow2(kup), qunit = inverse_pow2(qup);
     const int64_t ck = (int64_t)slot * a.Hk + hk;
@@ -351,9 +369,13 @@ __global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
         float* fac = a.fac + cv * kFac;
         if (wave == 0) {
             const bool is = lane < n;
-            double G = is ? (double)clean_g(a.g[(int64_t)(tok + lane) * a.g_token + hv]) : 0.0;
-            float be = 0.0f;
+            float gv = is ? clean_g(a.g[(int64_t)(tok + lane) * a.g_token + hv]) : 0.0f, be = 0.0f;
             if constexpr (DELTA) be = is ? a.beta[(int64_t)(tok + lane) * a.beta_token + hv] : 0.0f;
+            const uint64_t spoilt = __ballot(abs_bits(gv) >= kInfBits || abs_bits(be) >= kInfBits);
+            if (abs_bits(gv) >= kInfBits) gv = 0.0f;
+            if (abs_bits(be) >= kInfBits) be = 0.0f;
+            if (lane == 0) fac[2 * kChunk + 3] = (float)min(bad, spoilt ? __builtin_ctzll(spoilt) : kChunk);
+            double G = gv;
 #pragma unroll
             for (int s = 1; s < 64; s *= 2) {
                 const double up = __shfl_up(G, s);
@@ -491,15 +513,20 @@ __global__ __launch_bounds__(256, 2) void gla_intra_kernel(GlaArgs a) {
 
 // ------------------------------------------------------------------ from chunk to chunk
 
-// The largest magnitude of a column that four lanes hold (rows 16 t + 4 c + e).
-template <int N>
+// The largest magnitude of a column that four lanes hold (rows 16 t + 4 c + e); of
+// its numbers, or (ANY) NaN where it holds one.
+template <int N, bool ANY = false>
 __device__ inline float column_top(const f4* x) {
+    const auto larger = [](float a, float b) { return ANY ? __builtin_elementwise_maximum(a, b) : fmaxf(a, b); };
     float top = 0.0f;
 #pragma unroll
     for (int t = 0; t < N; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) top = fmaxf(fmaxf(top, __builtin_fabsf(x[t][e])), __builtin_fabsf(x[t][e + 1]));
-    return max_halves(max_rows16(top));
+        for (int e = 0; e < 4; e += 2) top = larger(larger(top, __builtin_fabsf(x[t][e])), __builtin_fabsf(x[t][e + 1]));
+    const auto a = __builtin_amdgcn_permlane16_swap(f_bits(top), f_bits(top), false, false);
+    top = larger(bits_f(a[0]), bits_f(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(f_bits(top), f_bits(top), false, false);
+    return larger(bits_f(b[0]), bits_f(b[1]));
 }
 
 // x p and y q as two fp16 terms: each is one instruction, which multiplies,
@@ -585,6 +612,7 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
     __shared__ __align__(1024) uint8_t su[2][NO * 2 * 1024];
     __shared__ __align__(1024) float sf[2][kFac];
     __shared__ float sunits[2][2][16];  // what a unit of those is worth, for each column
+    __shared__ int sbad[2][16];         // a column's first row whose k, v, g or beta is no finite number
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int pair = wave & 1, r16 = lane & 15, c = lane >> 4;
@@ -695,6 +723,13 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[t][e] = __builtin_fmaf(acc[t][e], w3, qs[t][e]);
+            const int bad = sbad[pair][r16];
+            if (__any(bad < kChunk))
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * t + 4 * c + e >= bad) y[t][e] = __builtin_nanf("");
             // The stores come last and stay on their way; the loads before them are waited for.
             if (ch + 1 < nchunk) {
                 if (mine) {
@@ -778,6 +813,7 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
         const uint8_t* const kb = skq[ch & 1];
         const float* const fac = sf[ch & 1];
         const float kunit = fac[2 * kChunk + 1];
+        const int kgb_bad = (int)fac[2 * kChunk + 3];
         f4 u[4];  // U is u times uworth
         float uworth = 1.0f;
         f4 x[4];
@@ -820,16 +856,38 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[t][e] = __builtin_fmaf(eg[t][e] * w, ks[t][e], x[t][e]);
+        }
+        // What is no finite number stays out of the products, whose zeros it would spoil for the
+        // column's earlier rows: its row and those after it are made NaN at the end.
+        float xtop = column_top<4, true>(x), utop;
+        int bad = kChunk;
+        if (__builtin_expect(__any(!(xtop < INFINITY)), 0)) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (abs_bits(x[t][e]) >= kInfBits) {
+                        x[t][e] = 0.0f;
+                        bad = min(bad, 16 * t + 4 * c + e);
+                    }
+            bad = min(bad, __shfl_xor(bad, 16));
+            bad = min(bad, __shfl_xor(bad, 32));
+            xtop = column_top<4>(x);
+        }
+        if constexpr (DELTA) {
             h8 xh[2], xl[2];
-            const float xup = to_top<12>(f_bits(column_top<4>(x)));
+            const float xup = to_top<12>(f_bits(xtop));
             to_operand<4>(x, xup, nullptr, c, xh, xl);
             tri_product<true>(th, tl, xh, xl, u);
             uworth = fac[2 * kChunk] * inverse_pow2(xup);
+            utop = column_top<4>(u);
         } else {
 #pragma unroll
             for (int t = 0; t < 4; ++t) u[t] = x[t];
+            utop = xtop;
         }
-        const float uup = to_top<12>(f_bits(column_top<4>(u))), uunit = inverse_pow2(uup) * uworth;
+        bad = min(bad, kgb_bad);
+        const float uup = to_top<12>(f_bits(utop)), uunit = inverse_pow2(uup) * uworth;
         h8 uh[2], ul[2];
         to_operand<4>(u, uup, nullptr, c, uh, ul);
 #pragma unroll
@@ -837,7 +895,10 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
             *reinterpret_cast<h8*>(su[pair] + 1024 * s + 16 * lane) = uh[s];
             if constexpr (TWO) *reinterpret_cast<h8*>(su[pair] + 1024 * (2 + s) + 16 * lane) = ul[s];
         }
-        if (c == 0) sunits[1][pair][r16] = uunit;
+        if (c == 0) {
+            sunits[1][pair][r16] = uunit;
+            sbad[pair][r16] = bad;
+        }
         __syncthreads();
         if (ch + 1 < nchunk) {
             load_v(ch + 1);
@@ -887,6 +948,11 @@ __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if (__any(bad < kChunk))
+#pragma unroll
+            for (int t = 0; t < ST; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[t][e] = bad < kChunk ? __builtin_nanf("") : S[t][e];
         if (ch + 1 < nchunk) hand_over();
         __syncthreads();
     }
