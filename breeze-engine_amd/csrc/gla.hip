@@ -229,7 +229,7 @@ constexpr int tm_bytes(bool delta) { return (delta ? 4 : 2) * kTriBytes; }
 
 // One workgroup for a chunk and a key head: the products k_i . k_j and
 // q_i . k_j once, then T and M for each of its value heads.  64 chunks of 16 key
-// and 48 value heads, fp32: 59 us, of which 28 for the operands of k and q (134
+// and 48 value heads, fp32: 60 us, of which 28 for the operands of k and q (134
 // MB in and out) and 10 for each value head's T and M (25 KB a chunk and head
 // out, and a chain of small triangular products).
 template <int DK, int DT, bool DELTA>
@@ -595,10 +595,12 @@ __device__ inline void tri_product(const h8* hi, const h8* lo, const h8* xh, con
 //
 // Bound by the chain through the state: per chunk 114 matrix instructions
 // (1,824 cycles of fp32 calls) and about as much in conversions, exchanges of
-// column maxima and LDS reads between them; 3.0 us a chunk, of which the
+// column maxima and LDS reads between them; 3.2 us a chunk, of which the
 // update's products take 0.6 and the hand-over 0.4 (64 chunks of 48 heads of
-// 128 x 128, 192 workgroups: 195 us).  All products in one wave and 64 columns
-// a workgroup took 5.0 (the LDS reads of four waves, 480 KB, alone 1.6).
+// 128 x 128, 192 workgroups: fp32 202 us, fp16 166, bf16 160).  All products in one
+// wave and 64 columns a workgroup took 5.0 (the LDS reads of four waves, 480 KB,
+// alone 1.6).  fp16's second terms for the rows of O leave one workgroup a unit: where
+// there are many (6 sequences of 32 heads), 69 us against 54 with one term.
 template <int DK, int DT, bool DELTA>
 __global__ __launch_bounds__(256, DT == kF32 || (DT == kF16 && DK == 128) ? 1 : 2) void gla_inter_kernel(GlaArgs a) {
     constexpr bool LO = DT == kF32;      // two terms of q and k

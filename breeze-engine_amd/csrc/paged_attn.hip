@@ -8,11 +8,14 @@
 // Numerics.  A page's INT8 or e4m3 values are exact in fp16, so both products
 // run on the fp16 matrix instructions with exact cache operands and fp32 sums.
 // q is scaled by a power of two for each row (its largest magnitude lands in
-// [2^13, 2^14)), which bf16 and fp16 queries survive exactly; fp32 queries are
-// split into two fp16 terms (22 bits), as are their probabilities.  bf16 calls
-// round the probabilities once to fp16's 11 bits, three more than their output
-// keeps.  For fp16 that is as many, and a second term costs half as many matrix
-// instructions again: few rows, and rows of few keys, take it, the others not.
+// [2^13, 2^14)), which bf16 and fp16 queries survive exactly down to 2^-27 of that (an
+// element errs by 2^-25 at most); fp32 queries are split into two fp16 terms (22
+// bits), as are their probabilities.  bf16 calls round the probabilities once to
+// fp16's 11 bits, three more than their output keeps: against 64 bits their outputs
+// are as near as those of fp32 sums (1.7e-3, the output's own rounding), and a second
+// term would take 2% of a batch of single tokens, 27% of a prompt.  For fp16 that is as
+// many as the output keeps: few rows, and rows of few keys, take the second term, the
+// others not (a 4096-token prompt 2.4e-4 off, where one rounding leaves 2.0e-4).
 // The key scales multiply the scores and the value scales the probabilities; the
 // latter are held relative to a power of two `nu` near the largest value scale
 // that the row sees in the tile (a later token's values, however large, take no
@@ -173,10 +176,11 @@ __device__ inline h8 round8(const float* w) {
 // keys; its four waves take tiles of 32 keys in turn.  Bound by HBM: the next tile's
 // keys and values are on their way while this one is computed, 16 KB a wave
 // (D = 256), and no wave waits for another before the end.  64 single tokens
-// over 100 to 16000 keys of 8 heads of 128 (537 MB): 126 us, 4.3 TB/s, and the
-// join 5.3.  One token over 4101 keys of 4 heads of 256: 11 us in 64 splits
-// of 64 keys, 14.6 in 32 of 128, and the join 7.4; latency, of the table, the
-// keys and one tile's chain of products.
+// over 100 to 16000 keys of 8 heads of 128 (537 MB): 125 us, 4.3 TB/s, and the
+// join 5.6; over 4 heads of 256 141 (bf16) and 163 (fp32), and 5.8.  One token over
+// 4101 keys of 4 heads of 256, 129 tiles: of 64 splits 43 have three tiles each
+// and the others none, 10.6 us and the join 7.2; of 32 26 have five, 13.2 and 5.2.
+// Latency, of the table, the keys and one tile's chain of products.
 
 // LDS row of a key's values: the transposed reads' four rows fall on unlike banks.
 constexpr int keys_row(int D) { return D + 16; }
@@ -411,15 +415,15 @@ __device__ __forceinline__ void attend_keys(const AttnArgs& a, int block, uint8_
     }
 }
 
-// Workgroups a compute unit.  fp32 with heads of 256 spills 54 registers a lane at
+// Workgroups a compute unit.  fp32 with heads of 256 spills 49 to 57 registers a lane at
 // two, whose traffic weighs where a workgroup has few rows and waits for HBM: 32
-// single tokens over up to 8000 keys of 4 heads 100 us at two, 54 at one; 12 tokens
-// over 6000 keys, 72 rows, 50 and 56.  Half types with heads of 128 spill 3 at three
-// (INT8: 64 tokens over 100 to 16000 keys 148 us, at two 140), which many rows beside
-// chunks are faster at.
+// single tokens over up to 8000 keys of 4 heads 91 us at two, 51 at one, 64 over 100 to
+// 16000 keys 224 and 162; 12 tokens over 6000 keys, 72 rows, 48 and 56.  Half types
+// with heads of 128 spill nothing at three (INT8: 64 tokens over 100 to 16000 keys 130
+// us, at two 133).
 constexpr int keys_per_unit(int D, int DT, bool lone) {
     if (D == 256 && DT == kF32) return lone ? 1 : 2;
-    return D == 256 || DT == kF32 || (D == 128 && lone) ? 2 : 3;
+    return D == 256 || DT == kF32 ? 2 : 3;
 }
 
 template <int D, int KIND, int DT, bool LONE>
@@ -800,7 +804,7 @@ __global__ __launch_bounds__(256) void attn_unpack_kernel(AttnArgs a) {
 
 // Both, where a call has few rows of some sequences and many of others: the first
 // `keys` workgroups are attn_keys_kernel's.  Each waits on memory most of its time:
-// 31 us together, 26 and 13 one after the other (8 sequences of 1 to 700 tokens behind
+// 27 us together, 20 and 13 one after the other (8 sequences of 1 to 700 tokens behind
 // up to 5000, 32/8 heads of 128, bf16, INT8).
 template <int D, int KIND, int DT>
 __global__ __launch_bounds__(256, keys_per_unit(D, DT, false)) void attn_keys_unpack_kernel(AttnArgs a, unsigned keys) {
@@ -819,7 +823,7 @@ __global__ __launch_bounds__(256, keys_per_unit(D, DT, false)) void attn_keys_un
 // prompt of 32/8 heads of 128 (fp16, 137 GFLOP, 175 to 220 us) they were busy 41%
 // and 54% of the cycles, one beside the other hardly ever, whatever the waves'
 // priorities and the order of the code.  1024 tokens behind 31744, 24/4 heads
-// of 256, fp32 (812 GFLOP, twice that in two-term products): 1.63 ms, 995
+// of 256, fp32 (812 GFLOP, twice that in two-term products): 1.66 ms, 980
 // TFLOP/s of matrix instructions against 1160 of a large library product.
 template <int D, int DT>
 __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) void attn_tiles_kernel(AttnArgs a) {
@@ -960,7 +964,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
             };
             // Rarely a row's units change, its reference with them; here, since a branch behind
             // the next scores' matrix instructions would keep the softmax from running beside them.
-            if (__any(!(vmax <= nu * 8.0f && vmax > nu * 0x1p-4f))) {
+            if (__any(vmax > nu * 8.0f || (vmax > 0.0f && vmax <= nu * 0x1p-4f))) {
                 const float f = move();
                 l *= f;
                 peak *= f;
@@ -1045,17 +1049,18 @@ __global__ __launch_bounds__(256, D == 256 || (D == 128 && DT == kF32) ? 1 : 2) 
         }
 }
 
-// Splits.  Single tokens: a split's keys cost a workgroup no more than its
-// start does while they are few, and one long sequence among short ones must
-// not be one workgroup's; so as many as bring a workgroup's keys down to
-// kSplitMin while compute units are idle, and to kSplitKeys at least.  Chunks:
-// the number that wastes the least of the last round of workgroups, each split
-// of at least kSplitRows keys.
 // Rows up to which 16 a workgroup over the same keys are faster than 128 (us over
-// 16000 keys, INT8, bf16: 8 / 16 / 32 tokens of 4 heads of 128 to a key head
-// 30 / 47 / - against 50 / 52 / 55; 8 / 16 tokens of 6 heads of 256 39 / 59 against 105 / 93).
+// 16000 keys, INT8, bf16: 8 / 16 tokens of 4 heads of 128 to a key head 29 / 42
+// against 51 / 53; 8 / 16 tokens of 6 heads of 256 39 / 59 against 85 / 96).
 constexpr int few_rows(int D) { return D == 256 ? 128 : 64; }
 constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer than 2^32
+
+// Splits, by the keys that the table has room for.  Single tokens: a split's keys cost
+// a workgroup no more than its start does while they are few, and one long sequence
+// among short ones must not be one workgroup's; so as many as bring a workgroup's keys
+// down to kSplitMin while compute units are idle, and to kSplitKeys at least.  Chunks:
+// the number that wastes the least of the last round of workgroups, each split
+// of at least kSplitRows keys.
 constexpr int kSplitMin = 64, kSplitMixed = 1024, kSplitKeys = 2048, kSplitRows = 512, kSplitMost = 64;
 
 // The splits of a row joined: D/4 lanes a split and NG splits of a row at a
@@ -1147,9 +1152,10 @@ struct AttnPlan {
     size_t copy, kpart, rpart, bytes;  // of the copies, of the two kinds' sums (without maxima), of the workspace
 };
 
-// Copies are made for calls of kUnpackRows rows or more (heads of 256, whose sums
-// leave attn_rows_kernel no registers for the unpacking: 120 -> 73 us at 768 rows,
-// 95 -> 63 at 96; heads of 128 are even there): of every sequence where
+// Copies are made for calls of kUnpackRows rows or more (heads of 256, whose sums in
+// fp32 leave attn_rows_kernel no registers for the unpacking, of kUnpackRows256: over
+// 2000 keys 109 -> 72 us at 768 rows, 95 -> 62 at 192, bf16 60 -> 58 and 52 -> 51;
+// heads of 128 are even at 512): of every sequence where
 // they have kUnpackMean rows on average, else of those of kBigRows or more; at
 // most kUnpackMost bytes.
 constexpr int kUnpackRows = 512, kUnpackRows256 = 64, kUnpackMean = 64;
@@ -1299,7 +1305,8 @@ bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, boo
                      c->kv_heads, T, B, heads, table_w);
         return false;
     }
-    // A launch has fewer than 2^24 workgroups (eight a sequence and head at most here), and keys are counted in 32 bits with some room.
+    // A launch has fewer than 2^24 workgroups (eight a sequence and head at most here), and keys are counted in 32
+    // bits with some room.
     if ((int64_t)T * heads > (1 << 28) || (int64_t)B * c->kv_heads > kMostBlocks / 8 || table_w > ((1 << 30) >> s)) {
         bq_set_error("paged_attention: %d tokens of %d heads in %d sequences of up to %d pages are too much for one call", T,
                      heads, B, table_w);

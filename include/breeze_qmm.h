@@ -234,8 +234,8 @@ typedef struct {
 int i4_kv_write_dev(const i4_kv_cache* cache, const void* dK, const void* dV, int64_t k_token, int64_t k_head,
                     int64_t v_token, int64_t v_head, int T, int dtype, const int32_t* dSlots, void* stream);
 
-/* Reads T slots back: dK, dV [T, kv_heads, head_dim] contiguous, value times
- * scale, rounded once to the type.  Zeros where a slot is not the cache's. */
+/* Reads T slots back: dK, dV [T, kv_heads, head_dim] contiguous, the fp32 product
+ * of value and scale rounded to the type.  Zeros where a slot is not the cache's. */
 int i4_kv_read_dev(const i4_kv_cache* cache, void* dK, void* dV, int T, int dtype, const int32_t* dSlots,
                    void* stream);
 
@@ -245,11 +245,12 @@ int i4_kv_read_dev(const i4_kv_cache* cache, void* dK, void* dV, int T, int dtyp
  * i reads key-value head i / (heads / kv_heads).  dTable [B, table_w] (int32,
  * row stride table_row) holds its pages in order, dKvLens[b] its keys, the new
  * ones included: new token i of q_len sees the keys up to dKvLens[b] - q_len +
- * i.  A row that sees no key gets zeros; keys in pages outside the cache and
- * past the table are not seen; rows outside every sequence are left as they
- * were.  scale > 0.  dOut [T, heads, head_dim] of dQ's type, strides as dQ's.
+ * i.  A row that sees no key gets zeros; keys in pages outside the cache are not
+ * seen; lengths past the table's columns are cut to them; rows outside every
+ * sequence are left as they were.  scale > 0.  dOut [T, heads, head_dim] of dQ's type, strides as dQ's.
  * dWork: as many bytes as i4_paged_attention_workspace says for the same
- * shapes (0: may be NULL), 16-byte aligned. */
+ * shapes (0: may be NULL; 5 GiB at most, by the table's columns), 16-byte
+ * aligned. */
 int64_t i4_paged_attention_workspace(int kv_heads, int page_size, int head_dim, int T, int B, int heads, int dtype,
                                      int table_w, int has_cu);
 int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
@@ -272,7 +273,7 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
  * without tokens keeps its state.  k_dim 64 or 128, v_dim a multiple of 16 up
  * to 1024.  Rows outside every sequence are left as they were.  dWork: as many
  * bytes as i4_gated_linear_attention_workspace says for the same shapes (0: may
- * be NULL), 256-byte aligned. */
+ * be NULL; 1 GiB at most, but for heads by the thousand), 256-byte aligned. */
 int64_t i4_gated_linear_attention_workspace(int T, int B, int k_heads, int v_heads, int k_dim, int v_dim, int dtype,
                                             int has_cu, int has_beta);
 int i4_gated_linear_attention_dev(const void* dQ, int64_t q_token, int64_t q_head, const void* dK, int64_t k_token,
