@@ -356,7 +356,9 @@ def gated_linear_attention(q, k, v, g, beta=None, state=None, cu_seqlens=None, s
     bits of every operand, of q and k down to 2^-28 of the largest in their chunk
     of 64 tokens and head, of v and the state down to 2^-37 of the largest in their
     column there.  With bf16 the state and u have 11 bits in the products that make
-    rows of o, three more than those keep.
+    rows of o, three more than those keep.  With beta, those bounds are for what the
+    delta rule is stable for, beta |k|^2 up to 2: past that u grows from token to token,
+    and a chunk's earlier rows lose bits to its largest u.
 
     A NaN in k, v, g or beta reaches its token's row and those after it (from v: in its
     column), one in q its own row; no earlier ones.  Sequences of more than 16

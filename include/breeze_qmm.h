@@ -266,7 +266,8 @@ int i4_paged_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_t
  * dQ, dK [T, k_heads, k_dim], dV, dOut [T, v_heads, v_dim] of one type (element
  * strides per token and head, multiples of four; last dimension contiguous;
  * 16-byte aligned); dG (logarithms of the decays, at most 0; -infinity drops
- * a finite state), dBeta: fp32 [T, v_heads], strides per token.  A NaN in k, v, g or beta
+ * a finite state), dBeta: fp32 [T, v_heads], strides per token; beta |k|^2 up to 2, else a
+ * chunk's earlier rows lose bits to the later ones, which grow.  A NaN in k, v, g or beta
  * reaches its token's row and later ones, no earlier one.  Sequence b's tokens
  * are dCu[b] .. dCu[b + 1] - 1 (dCu NULL: token b).  dStateIn (NULL: zeros),
  * dStateOut (may be dStateIn): fp32 [B, v_heads, k_dim, v_dim]; a sequence
