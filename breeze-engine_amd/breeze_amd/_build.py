@@ -13,8 +13,12 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(PKG), "csrc")
 # Host code and small kernels; the decode and prefill kernels, one unit per
 # (bits, activation mode) so the device passes run side by side.
-# Then the token mixers (the paged cache, attention over it, gated linear attention).
-SOURCES = ["qmm.hip", "pf16_w4.hip", "pf16_w8.hip", "pf_w4_i8.hip", "kv_cache.hip", "paged_attn.hip", "gla.hip"] + [f"{k}_w{b}_{m}.hip" for k in ("dec", "pf") for b in (4, 8) for m in ("hp", "lp")]
+# Then the token mixers (the paged cache, attention over it, gated linear attention),
+# and what a step with drafted tokens adds (positions, page tables, trees, verification).
+SOURCES = [
+    "qmm.hip", "pf16_w4.hip", "pf16_w8.hip", "pf_w4_i8.hip", "kv_cache.hip", "paged_attn.hip", "gla.hip", "rotary.hip",
+    "pages.hip", "tree_attn.hip", "verify.hip",
+] + [f"{k}_w{b}_{m}.hip" for k in ("dec", "pf") for b in (4, 8) for m in ("hp", "lp")]
 LIB_NAME = "libbreeze_qmm.so"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -50,6 +54,7 @@ DEVICE_FLAGS = [
 # Attention's 128-row workgroups hold more than 256 registers a lane: their
 # accumulators take the accumulation registers.
 ATTN_FLAGS = DEVICE_FLAGS[:4]
+ATTN_SOURCES = ("paged_attn.hip", "tree_attn.hip")
 
 
 def lib_path():
@@ -83,7 +88,7 @@ def build(verbose=False):
         objs = [os.path.join(work, f"{i}.o") for i in range(len(srcs))]
         try:
             running = [(_run([HIPCC, "-x", "hip", *FLAGS,
-                              *(ATTN_FLAGS if os.path.basename(s) == "paged_attn.hip" else DEVICE_FLAGS),
+                              *(ATTN_FLAGS if os.path.basename(s) in ATTN_SOURCES else DEVICE_FLAGS),
                               "--offload-device-only", "-c", s, "-o", fb], verbose), s) for s, fb in zip(srcs, fatbins)]
             finish(running, "device pass")
             running = [(_run([HIPCC, "-x", "hip", *FLAGS, "--offload-host-only", "-Xclang",

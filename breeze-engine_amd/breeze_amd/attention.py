@@ -10,6 +10,9 @@ quantized projections (``hip_backend``).
 - ``gated_linear_attention``: the linear-attention layers' recurrence
   (kernel/qwen35_decoder.cpp:46-121), one token at a time from a kept state or
   whole prompts in chunks.
+- ``Rotary`` and ``rotary``: positions of queries and keys ahead of the cache
+  (the decoder's rope, kernel/qwen35_decoder.cpp:218-428).
+- ``PageTable``: which pages sequences hold, and new tokens' slots and positions.
 
 Tensors are fp32, bf16 or fp16 on one gfx950 GPU.  Calls are asynchronous on
 the current stream, own no memory between calls (a workspace comes from
@@ -19,6 +22,7 @@ offsets, page and slot numbers) is checked by the kernels, which skip what is
 out of range.  Outputs carry no gradient.  There is no CPU fallback.
 """
 import ctypes
+import math
 
 from . import hip_backend as hb
 
@@ -82,9 +86,7 @@ def _workspace(shape, kind, device):
     key = (kind, device.index, shape)
     n = _needs.get(key)
     if n is None:
-        query = (hb._lib.i4_paged_attention_workspace if kind == "paged"
-                 else hb._lib.i4_gated_linear_attention_workspace)
-        n = query(*shape)
+        n = getattr(hb._lib, _queries[kind])(*shape)
         if n < 0:
             raise ValueError(hb.last_error())
         if len(_needs) >= 4096:
@@ -94,6 +96,8 @@ def _workspace(shape, kind, device):
 
 
 _needs = {}
+_queries = {"paged": "i4_paged_attention_workspace", "gla": "i4_gated_linear_attention_workspace",
+            "tree": "i4_tree_attention_workspace", "verify": "i4_verify_workspace"}
 
 
 class KVCache:
@@ -207,6 +211,252 @@ def kv_read(cache, slots, dtype):
         if rc:
             hb._check_rc(rc, "i4_kv_read_dev")
     return k, v
+
+
+class Rotary:
+    """The angles of ``rotary``: of pair i of a head's first ``dim`` values,
+    position times f_i radians, f_i = base ** (-2 i / dim).
+
+    ``layout``: "half" (values i and i + dim / 2 are a pair) or "interleaved" (2 i
+    and 2 i + 1).  ``scaling`` for contexts ``factor`` times as long:
+
+    - "linear": all f_i divided by the factor;
+    - "base": the base times factor ** (dim / (dim - 2)), so that the slowest f_i
+      is divided by the factor and the fastest stays;
+    - "parts": a pair that turns more than ``fast`` times in the ``original``
+      context keeps its f_i, one that turns less than ``slow`` times has it divided,
+      those in between are mixed linearly in the turns; sine and cosine are
+      multiplied by 0.1 ln(factor) + 1 (or ``amplitude``).
+
+    ``freqs``: f_i themselves (dim / 2 numbers), in place of all that.  They are kept
+    in 64 bits on ``device``, as quarter turns."""
+
+    def __init__(self, dim, base=10000.0, layout="half", scaling=None, factor=1.0, original=None, slow=1.0, fast=32.0,
+                 amplitude=None, freqs=None, device="cuda"):
+        torch = _torch()
+        if dim < 2 or dim % 2 or dim > 4096:
+            raise ValueError(f"dim must be even, from 2 to 4096, got {dim}")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+        if scaling not in (None, "linear", "base", "parts"):
+            raise ValueError(f"scaling must be None, 'linear', 'base' or 'parts', got {scaling!r}")
+        if not 0 < base < math.inf or not 0 < factor < math.inf:
+            raise ValueError(f"base and factor must be positive and finite, got {base} and {factor}")
+        if freqs is not None:
+            f = [float(x) for x in freqs]
+            if len(f) != dim // 2 or scaling is not None:
+                raise ValueError(f"freqs must be {dim // 2} numbers, without scaling, got {len(f)}")
+        else:
+            if scaling == "base" and dim > 2:
+                base = base * factor ** (dim / (dim - 2))
+            f = [base ** (-2 * i / dim) for i in range(dim // 2)]
+            if scaling == "linear":
+                f = [x / factor for x in f]
+            elif scaling == "parts":
+                if not original or original < 1 or not 0 <= slow < fast:
+                    raise ValueError(f"'parts' needs the original context and slow < fast, got {original}, {slow}, {fast}")
+                for i, x in enumerate(f):
+                    keep = min(max((original * x / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0)
+                    f[i] = x * (keep + (1 - keep) / factor)
+                if amplitude is None:
+                    amplitude = 0.1 * math.log(factor) + 1
+        if not all(math.isfinite(x) for x in f):
+            raise ValueError("freqs must be finite")
+        self.dim, self.layout, self.amplitude = dim, layout, 1.0 if amplitude is None else float(amplitude)
+        self._turns = torch.tensor([x * (2 / math.pi) for x in f], dtype=torch.float64, device=device)
+        self.device, self._index = self._turns.device, self._turns.get_device()
+        self._p, self._inter = self._turns.data_ptr(), int(layout == "interleaved")
+
+
+def _heads(t, T, D, what):
+    """`t` [T, heads, D] with a contiguous last dimension: itself, or a copy."""
+    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D:
+        raise ValueError(f"{what} must be [{T}, heads, {D}], got {tuple(t.shape)}")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _turned(out, like, what):
+    torch = hb._torch
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    T, H, D = like.shape
+    st = out.stride()
+    if out.dtype is not like.dtype or out.shape != like.shape or out.device != like.device:
+        raise ValueError(f"{what} must be {like.dtype} {tuple(like.shape)} on {like.device}, got {out.dtype} "
+                         f"{tuple(out.shape)} on {out.device}")
+    if st[2] != 1 or (H > 1 and st[1] < D) or (T > 1 and st[0] < (H - 1) * st[1] + D):
+        raise ValueError(f"{what} needs a contiguous last dimension and rows that do not overlap, got strides {st}")
+    return out
+
+
+def _disjoint(a, b):
+    """No row of a lies on one of b: they are apart, or other columns of one projection."""
+    x, y = _span(a), _span(b)
+    if x[0] >= y[1] or y[0] >= x[1]:
+        return True
+    step = a.stride(0) * a.element_size()
+    if a.stride(0) != b.stride(0) or a.dtype is not b.dtype or step == 0:
+        return False
+    # Columns of each token, from the first one's start on, modulo the step.
+    wide = [((t.shape[1] - 1) * t.stride(1) + t.shape[2]) * t.element_size() for t in (a, b)]
+    apart = (y[0] - x[0]) % step
+    return wide[0] <= apart and apart + wide[1] <= step
+
+
+def rotary(rope, q, k, positions, out=None):
+    """Rotary positions of queries and keys; ``(q, k)``, turned.
+
+    ``q``: ``[T, heads, head_dim]``; ``k``: ``[T, kv_heads, head_dim]`` of q's type,
+    or None; ``positions``: int32 ``[T]``, each token's (``PageTable.extend`` gives
+    them).  The first ``rope.dim`` values of a head are turned, in fp32 with angles
+    from 64 bits, at whatever position; the others are copied.
+
+    Views are read in place.  ``out``: (q, k) to write to, each the input itself
+    (only what is turned is written then) or apart from both inputs."""
+    torch = _torch()
+    T, _, D = q.shape if q.dim() == 3 else (0, 0, 0)
+    dt = _type(q, "q")
+    q = _heads(q, T, D, "q")
+    if D % 2 or D < rope.dim or D > 4096:
+        raise ValueError(f"head_dim must be even, from the rotary's {rope.dim} to 4096, got {D} (q: {tuple(q.shape)})")
+    if k is not None:
+        k = _heads(k, T, D, "k")
+        if k.dtype is not q.dtype:
+            raise ValueError(f"q and k must have one type, got {q.dtype} and {k.dtype}")
+    _ints(positions, (T,), "positions")
+    _same_device(rope._index, q, k, positions)
+    if out is None:
+        qo, ko = _turned(None, q, "q"), None if k is None else _turned(None, k, "k")
+    else:
+        qo, ko = out
+        if qo is None or (ko is None) != (k is None):
+            raise ValueError("out must be (q, k), with None where k is None")
+        qo = _turned(qo, q, "out's q")
+        ko = None if k is None else _turned(ko, k, "out's k")
+        if T:
+            for o, own, other, there in ((qo, q, k, ko), (ko, k, q, qo)):
+                if o is None:
+                    continue
+                if not (o.data_ptr() == own.data_ptr() and o.stride() == own.stride()) and not _disjoint(o, own):
+                    raise ValueError("out overlaps its input: it may be the input itself, or apart from it")
+                if other is not None and not (_disjoint(o, other) and _disjoint(o, there)):
+                    raise ValueError("out's q and k lie on one another, or on the other's input")
+    if T == 0:
+        return qo, ko
+    if rope._index != _current():
+        with torch.cuda.device(rope.device):
+            return rotary(rope, q, k, positions, (qo, ko))
+    qs, os = q.stride(), qo.stride()
+    if k is None:
+        kp, ks, kn, kop, kos = None, (0, 0), 0, None, (0, 0)
+    else:
+        kp, ks, kn, kop, kos = k.data_ptr(), k.stride(), k.shape[1], ko.data_ptr(), ko.stride()
+    rc = hb._lib.i4_rotary_dev(q.data_ptr(), qs[0], qs[1], q.shape[1], kp, ks[0], ks[1], kn, T, D, rope.dim, rope._inter,
+                               dt, positions.data_ptr(), rope._p, rope.amplitude, qo.data_ptr(), os[0], os[1], kop,
+                               kos[0], kos[1], hb._torch_stream(q))
+    if rc:
+        hb._check_rc(rc, "i4_rotary_dev")
+    return qo, ko
+
+
+class PageTable:
+    """Which pages of a cache a batch's sequences hold, on the GPU.
+
+    ``table``: int32 ``[B, columns]``, each sequence's pages in order (the
+    ``block_table`` of attention), of which it holds the first ``held`` (int32
+    ``[B]``); ``free``: int32 ``[pages]``, the first ``count`` (int32 ``[1]``) of which
+    are the free pages, a stack.  The tensors are kept as given and changed in
+    place, in the order of the stream's calls; the host reads none of them."""
+
+    def __init__(self, table, held, free, count, page_size):
+        torch = _torch()
+        if page_size & (page_size - 1) or not 16 <= page_size <= 1024:
+            raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+        if table.dim() != 2 or free.dim() != 1 or not free.shape[0]:
+            raise ValueError(f"table must be [B, columns] and free [pages], got {tuple(table.shape)} and "
+                             f"{tuple(free.shape)}")
+        B, cols = table.shape
+        if B > 1 << 20 or B * cols >= 1 << 31 or cols * page_size > 1 << 30 or free.shape[0] * page_size >= 1 << 31:
+            raise ValueError(f"a table has up to 2^20 sequences, fewer than 2^31 entries and up to 2^30 keys a sequence, a "
+                             f"cache fewer than 2^31 slots, got {B}, {cols} columns and {free.shape[0]} pages of {page_size}")
+        for t, shape, what in ((table, (B, cols), "table"), (held, (B,), "held"), (free, tuple(free.shape), "free"),
+                               (count, (1,), "count")):
+            if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"{what} must be contiguous int32 {shape}, got {t.dtype} {tuple(t.shape)}")
+            if t.device != table.device:
+                raise ValueError(f"the page table's tensors lie on {t.device} and {table.device}")
+        self.table, self.held, self.free, self.count, self.page_size = table, held, free, count, page_size
+        self.device, self._index = table.device, table.get_device()
+        self._args = (table.data_ptr(), held.data_ptr(), free.data_ptr(), count.data_ptr(), free.shape[0], page_size, B,
+                      cols)
+
+    @classmethod
+    def empty(cls, num_pages, page_size, batch, columns, device="cuda"):
+        """A table of ``batch`` sequences that hold nothing; all pages are free."""
+        torch = _torch()
+        new = lambda *shape, **kw: torch.full(shape, dtype=torch.int32, device=device, **kw)  # noqa: E731
+        free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        return cls(new(batch, columns, fill_value=-1), new(batch, fill_value=0), free, new(1, fill_value=num_pages),
+                   page_size)
+
+    def extend(self, lens, cu=None, tokens=None, parents=None):
+        """Room for new tokens; ``(slots, positions, kv_lens)``.
+
+        ``lens``: int32 ``[B]``, each sequence's tokens in the cache.  ``cu``: int32
+        ``[B + 1]``, where each sequence's new tokens begin and the last one's end, of
+        ``tokens`` in all; None: one each.  ``parents``: int32 ``[tokens]``, the new
+        tokens being trees (``drafts.tree_attention``).
+
+        Pages come off the stack for the sequences in order.  ``slots`` are
+        ``kv_write``'s, ``positions`` the tokens' own: lens + the token's number, or
+        its depth in the tree; ``kv_lens`` the lengths with the new tokens.  Where the
+        pages do not suffice, that sequence and every later one that needs pages get
+        none; those, sequences past the table's columns or of a negative length, and
+        trees past 1024 nodes, have a kv_len and slots of -1: no call writes or sees
+        anything of them.  Tokens outside every sequence have slot -1."""
+        torch = _torch()
+        B = self._args[6]
+        _ints(lens, (B,), "lens")
+        if cu is None:
+            T = B
+            if tokens not in (None, B):
+                raise ValueError(f"{tokens} tokens in {B} sequences: cu says where each begins")
+        else:
+            _ints(cu, (B + 1,), "cu")
+            if tokens is None and parents is not None:
+                tokens = parents.shape[0]
+            if tokens is None or tokens < 0:
+                raise ValueError(f"with cu, tokens says how many there are in all, got {tokens}")
+            T = int(tokens)
+        if parents is not None:
+            _ints(parents, (T,), "parents")
+        _same_device(self._index, lens, cu, parents)
+        if self._index != _current():
+            with torch.cuda.device(self.device):
+                return self.extend(lens, cu, T, parents)
+        # One allocation: the host part is most of a small call.
+        new = torch.empty((2 * T + B,), dtype=torch.int32, device=self.device)
+        p = new.data_ptr()
+        rc = hb._lib.i4_pages_extend_dev(*self._args, lens.data_ptr(), None if cu is None else cu.data_ptr(), T,
+                                         None if parents is None else parents.data_ptr(), p, p + 4 * T, p + 8 * T,
+                                         hb._torch_stream(lens))
+        if rc:
+            hb._check_rc(rc, "i4_pages_extend_dev")
+        return new.split((T, T, B))
+
+    def trim(self, lens):
+        """Pages past ``lens`` (int32 ``[B]``) tokens of each sequence go back to the
+        stack: 0 gives all of a sequence's, a negative length none.  Table entries that
+        go become -1."""
+        torch = _torch()
+        _ints(lens, (self._args[6],), "lens")
+        _same_device(self._index, lens)
+        if self._index != _current():
+            with torch.cuda.device(self.device):
+                return self.trim(lens)
+        rc = hb._lib.i4_pages_trim_dev(*self._args, lens.data_ptr(), hb._torch_stream(lens))
+        if rc:
+            hb._check_rc(rc, "i4_pages_trim_dev")
 
 
 def _output(out, like, shape, what):

@@ -111,6 +111,25 @@ try:
     _lib.i4_gated_linear_attention_dev.restype = _i
     _lib.i4_gated_linear_attention_dev.argtypes = [_vp, _i64, _i64] * 3 + [_vp, _i64] * 2 + [_i] * 6 + [
         _vp, _i, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp]
+    _lib.i4_rotary_dev.restype = _i
+    _lib.i4_rotary_dev.argtypes = [_vp, _i64, _i64, _i] * 2 + [_i] * 5 + [_vp, _vp, ctypes.c_float] + [
+        _vp, _i64, _i64] * 2 + [_vp]
+    _lib.i4_pages_extend_dev.restype = _i
+    _lib.i4_pages_extend_dev.argtypes = [_vp] * 4 + [_i] * 4 + [_vp, _vp, _i] + [_vp] * 5
+    _lib.i4_pages_trim_dev.restype = _i
+    _lib.i4_pages_trim_dev.argtypes = [_vp] * 4 + [_i] * 4 + [_vp] * 2
+    _lib.i4_tree_attention_workspace.restype = _i64
+    _lib.i4_tree_attention_workspace.argtypes = [_i] * 9
+    _lib.i4_tree_attention_dev.restype = _i
+    _lib.i4_tree_attention_dev.argtypes = [_vp, _vp, _i64, _i64, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _vp,
+                                           ctypes.c_float, _vp, _i64, _i64, _vp, _i64, _vp]
+    _lib.i4_verify_workspace.restype = _i64
+    _lib.i4_verify_workspace.argtypes = [_i] * 5
+    _lib.i4_verify_dev.restype = _i
+    _lib.i4_verify_dev.argtypes = [_vp, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, ctypes.c_float, _vp, _i64, _vp,
+                                   _vp, _vp, _vp, _i64, _vp]
+    _lib.i4_kv_compact_dev.restype = _i
+    _lib.i4_kv_compact_dev.argtypes = [_vp, _i, _vp, _i64, _i, _vp, _vp, _i, _i] + [_vp] * 4
 except (OSError, AttributeError):
     _lib = None
 

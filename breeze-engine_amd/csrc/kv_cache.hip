@@ -1,4 +1,5 @@
-// Keys and values quantized into the pages of a cache, and read back.
+// Keys and values quantized into the pages of a cache, and read back; rows moved
+// within their sequence.
 //
 // A row is one token's D values of one key-value head.  INT8: the scale is
 // s = max|x| / 127 (one fp32 division) and a value the whole number nearest to
@@ -15,6 +16,8 @@
 // heads of 256, fp32, INT8: write 20.0 us (84 MB, 4.2 TB/s), read 14.4 us (5.8
 // TB/s, part of it from the caches); one token 3.2 and 2.5 us, the launch.
 #include "mix_common.h"
+
+#include <algorithm>
 
 #include "../../include/breeze_qmm.h"
 
@@ -168,6 +171,65 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a) {
     }
 }
 
+// Rows of accepted tokens moved together: in every layer, place ctx + path[i] of a
+// sequence to ctx + i, for i below its count, ctx being its keys before the new
+// ones.  A path's numbers grow, so path[i] >= i, and what a step of rows in
+// order overwrites no later step reads; the rows of one step are all read before
+// any is written.  A wave for each sequence, layer, head, and keys or values: a few
+// rows, whose four dependent reads (lengths, path, page, row) are what it costs.
+constexpr int kLayers = 32;  // of one launch: their pointers are kernel arguments
+
+struct CompactArgs {
+    struct {
+        uint8_t* page[2];  // keys, values
+        float* scale[2];
+    } layer[kLayers];
+    const int32_t* table;
+    const int32_t* kv_lens;
+    const int32_t* cu;  // null: one node a sequence
+    const int32_t* path;
+    const int32_t* counts;
+    int32_t* lens;  // null: another launch writes them
+    int64_t table_row, capacity;
+    int T, B, H, P, pshift;
+};
+
+template <int D>
+__global__ __launch_bounds__(64) void kv_compact_kernel(CompactArgs a) {
+    constexpr int L = D / 16, R = 64 / L;  // lanes a row, rows a step
+    const int b = blockIdx.x, h = blockIdx.y, val = blockIdx.z & 1, lane = threadIdx.x % L;
+    const int q0 = a.cu ? min(max(a.cu[b], 0), a.T) : b, n = a.cu ? min(max(a.cu[b + 1], q0), a.T) - q0 : 1;
+    const int kv = a.kv_lens[b], ctx = kv - n, keep = min(max(a.counts[b], 0), n);
+    if (a.lens && h == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.lens[b] = kv < 0 ? -1 : ctx + keep;
+    if (kv < 0) return;
+    uint8_t* const pages = a.layer[blockIdx.z >> 1].page[val];
+    float* const scales = a.layer[blockIdx.z >> 1].scale[val];
+    const auto row_of = [&](int place) -> int64_t {
+        if (place < 0 || place >= a.capacity) return -1;
+        const int page = a.table[b * a.table_row + (place >> a.pshift)];
+        if (page < 0 || page >= a.P) return -1;
+        return (((int64_t)page * a.H + h) << a.pshift) + (place & ((1 << a.pshift) - 1));
+    };
+    for (int i0 = 0; i0 < keep; i0 += R) {
+        const int i = i0 + threadIdx.x / L, from = i < keep ? a.path[q0 + i] : -1;
+        const bool moves = from > i && from < n;
+        const int64_t src = moves ? row_of(ctx + from) : -1, dst = moves ? row_of(ctx + i) : -1;
+        const bool is = src >= 0 && dst >= 0;
+        u4 w = {0, 0, 0, 0};
+        float s = 0.0f;
+        if (is) {
+            w = *reinterpret_cast<const u4*>(pages + src * D + 16 * lane);
+            s = scales[src];
+        }
+        wait_loads<0>();  // no row is written before all of this step are read
+        if (is) {
+            *reinterpret_cast<u4*>(pages + dst * D + 16 * lane) = w;
+            if (lane == 0) scales[dst] = s;
+        }
+        wait_loads<0>();
+    }
+}
+
 template <int D, int KIND, int DT>
 void launch3(const KvArgs& a, bool write, hipStream_t st) {
     constexpr int per = 256 / (D / 4) * kUnroll;
@@ -265,6 +327,82 @@ int i4_kv_read_dev(const i4_kv_cache* cache, void* dK, void* dV, int T, int dtyp
     a.vo = dV;
     a.slots = dSlots;
     return kv_call(cache, a, T, dtype, false, stream, "kv_read");
+}
+
+int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_t* dTable, int64_t table_row,
+                      int table_w, const int32_t* dKvLens, const int32_t* dCu, int T, int B, const int32_t* dPath,
+                      const int32_t* dCounts, int32_t* dLens, void* stream) {
+    if (!caches || layers < 1 || layers > 4096 || T < 0 || B < 0 || B > (1 << 23)) {
+        bq_set_error("kv_compact: needs 1 to 4096 caches, T >= 0 and 0 to 2^23 sequences (got %d, %d, %d)", layers, T, B);
+        return -2;
+    }
+    for (int i = 0; i < layers; ++i) {
+        const i4_kv_cache* c = caches[i];
+        if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) {
+            bq_set_error("kv_compact: null cache pointer");
+            return -2;
+        }
+        if (c->head_dim != caches[0]->head_dim || c->page_size != caches[0]->page_size ||
+            c->num_pages != caches[0]->num_pages || c->kv_heads != caches[0]->kv_heads) {
+            bq_set_error("kv_compact: the caches differ in pages, heads or sizes");
+            return -2;
+        }
+    }
+    const i4_kv_cache* c = caches[0];
+    int pshift = 4;
+    while (pshift < 10 && (1 << pshift) != c->page_size) ++pshift;
+    if ((c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) || (1 << pshift) != c->page_size ||
+        c->num_pages < 1 || c->kv_heads < 1 || c->kv_heads > 4096 || c->num_pages > (INT32_MAX >> pshift) ||
+        table_w < 0 || table_w > ((1 << 30) >> pshift)) {
+        bq_set_error("kv_compact: needs heads of 64, 128 or 256, a page size of 16 to 1024 that is a power of two, 1 to "
+                     "4096 heads, fewer than 2^31 slots and tables of up to 2^30 keys (got %d, %d, %d, %d pages, %d "
+                     "columns)",
+                     c->head_dim, c->page_size, c->kv_heads, c->num_pages, table_w);
+        return -2;
+    }
+    if (B == 0) return 0;
+    if (!dCu && T != B) {
+        bq_set_error("kv_compact: needs one node a sequence where no offsets are given (got %d, %d sequences)", T, B);
+        return -2;
+    }
+    if (!dKvLens || !dCounts || !dLens || (T > 0 && !dPath) || (table_w > 0 && !dTable)) {
+        bq_set_error("kv_compact: null device pointer");
+        return -2;
+    }
+    if (dLens == dKvLens) {
+        bq_set_error("kv_compact: the new lengths need a place of their own");
+        return -2;
+    }
+    CompactArgs a{};
+    a.table = dTable;
+    a.kv_lens = dKvLens;
+    a.cu = dCu;
+    a.path = dPath;
+    a.counts = dCounts;
+    a.table_row = table_row;
+    a.capacity = (int64_t)table_w << pshift;
+    a.T = T;
+    a.B = B;
+    a.H = c->kv_heads;
+    a.P = c->num_pages;
+    a.pshift = pshift;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    (void)hipGetLastError();
+    for (int l0 = 0; l0 < layers; l0 += kLayers) {
+        const int n = std::min(layers - l0, kLayers);
+        for (int i = 0; i < n; ++i) {
+            a.layer[i].page[0] = static_cast<uint8_t*>(caches[l0 + i]->k);
+            a.layer[i].page[1] = static_cast<uint8_t*>(caches[l0 + i]->v);
+            a.layer[i].scale[0] = caches[l0 + i]->k_scale;
+            a.layer[i].scale[1] = caches[l0 + i]->v_scale;
+        }
+        a.lens = l0 == 0 ? dLens : nullptr;
+        const dim3 grid((unsigned)B, (unsigned)a.H, (unsigned)(2 * n));
+        if (c->head_dim == 64) kv_compact_kernel<64><<<grid, 64, 0, st>>>(a);
+        else if (c->head_dim == 128) kv_compact_kernel<128><<<grid, 64, 0, st>>>(a);
+        else kv_compact_kernel<256><<<grid, 64, 0, st>>>(a);
+    }
+    return launched("kv_compact") ? 0 : -5;
 }
 
 }  // extern "C"

@@ -284,6 +284,92 @@ int i4_gated_linear_attention_dev(const void* dQ, int64_t q_token, int64_t q_hea
                                   const float* dStateIn, float* dStateOut, void* dOut, int64_t o_token, int64_t o_head,
                                   void* dWork, int64_t work_bytes, void* stream);
 
+/* ---- a step with drafted tokens ----------------------------------------
+ *
+ * Under the token mixers' conventions.  A tree of drafted tokens packs its nodes
+ * like a sequence's new tokens: node 0 is the last token that was decided, the
+ * others are drafted, parents[i] is node i's parent by its number in its tree, a
+ * parent before its children (anything else counts as none).  A tree has at most
+ * 1024 nodes. */
+
+/* Turns pairs of the first `rot` values of each of T tokens' q and k heads by
+ * dPositions[t] times dFreqs[i] quarter turns (fp64, [rot / 2]):
+ *   (a, b) -> amplitude (a cos - b sin, b cos + a sin),
+ * pair i being values i and i + rot / 2, or with `interleaved` 2 i and 2 i + 1.
+ * The other values are copied.  dQ, dQo [T, q_heads, head_dim], dK, dKo
+ * [T, k_heads, head_dim] of one type (element strides per token and head; any
+ * alignment of the type, 16 bytes is faster); an output is its input, or apart
+ * from all.  Without q or k: 0 heads.  head_dim and rot are even, rot <= head_dim <=
+ * 4096, T up to 2^23. */
+int i4_rotary_dev(const void* dQ, int64_t q_token, int64_t q_head, int q_heads, const void* dK, int64_t k_token,
+                  int64_t k_head, int k_heads, int T, int head_dim, int rot, int interleaved, int dtype,
+                  const int32_t* dPositions, const double* dFreqs, float amplitude, void* dQo, int64_t qo_token,
+                  int64_t qo_head, void* dKo, int64_t ko_token, int64_t ko_head, void* stream);
+
+/* A batch's page table: dTable [B, cols] holds each sequence's dHeld[b] pages in
+ * order, dFree[0 .. dCount[0] - 1] the free pages of num_pages.
+ *
+ * extend: sequence b, of dLens[b] tokens, gets pages for the new ones dCu[b] ..
+ * dCu[b + 1] - 1 of T (dCu NULL: token b), off the free stack's top, sequences in
+ * order.  dKvLens[b]: its length with them.  dSlots[t]: page * page_size + place;
+ * dPositions[t]: dLens[b] + t's number in the sequence, or with dParents its depth
+ * in the tree.  Where the pages do not suffice the sequence and every later one
+ * that needs pages get none; those, sequences that pass the table's columns, trees
+ * past 1024 nodes and sequences of a negative length have dKvLens[b] = -1 and
+ * slots of -1.  Tokens outside every sequence: slot -1, position 0.
+ *
+ * trim: pages past dLens[b] tokens go back (a negative length: none do), their
+ * table entries become -1.  What one call gives back comes out again in the same
+ * order. */
+int i4_pages_extend_dev(int32_t* dTable, int32_t* dHeld, int32_t* dFree, int32_t* dCount, int num_pages, int page_size,
+                        int B, int cols, const int32_t* dLens, const int32_t* dCu, int T, const int32_t* dParents,
+                        int32_t* dSlots, int32_t* dPositions, int32_t* dKvLens, void* stream);
+int i4_pages_trim_dev(int32_t* dTable, int32_t* dHeld, int32_t* dFree, int32_t* dCount, int num_pages, int page_size,
+                      int B, int cols, const int32_t* dLens, void* stream);
+
+/* Attention of the sequences' trees over the cache, which holds the nodes' keys and
+ * values already, as the last of dKvLens[b].  As i4_paged_attention_dev, but node i
+ * sees the keys before the tree, its ancestors and itself.  Rows of a tree past
+ * 1024 nodes are NaN. */
+int64_t i4_tree_attention_workspace(int kv_heads, int page_size, int head_dim, int T, int B, int heads, int dtype,
+                                    int table_w, int has_cu);
+int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
+                          int dtype, const int32_t* dTable, int64_t table_row, int table_w, const int32_t* dKvLens,
+                          const int32_t* dCu, int B, const int32_t* dParents, float scale, void* dOut, int64_t o_token,
+                          int64_t o_head, void* dWork, int64_t work_bytes, void* stream);
+
+/* The drafted tokens dTokens[T] against the target's scores dLogits [T, V] (element
+ * stride `row`; any alignment of the type), which at a node are of the token after
+ * it.  Per sequence (dCu [B + 1], dCu NULL: node b) from node 0 on: with p =
+ * softmax(scores / temperature) and the node's children in order, child c is taken
+ * where dUniforms[c] q(c) < r(c); r is p at first, q is 1 (dDraft NULL) or
+ * dDraft[node, c] over what dDraft[node] leaves without the earlier children; a
+ * child that is not taken leaves r = max(r - q, 0) without it, normalized.  Where
+ * none is taken the next token is drawn from r: the first whose running sum passes
+ * dUniforms of node 0.  Temperature 0: the largest score, the first of equal ones.
+ * dDraft: fp32 [T, V], stride draft_row.  dTemps: fp32 [B], or NULL: `temperature`.
+ * dCounts[b]: the nodes on the path, 1 or more (0 for no node, or more than 1024);
+ * dPath, dOut [T], packed like the nodes: the path's node numbers, and the new tokens,
+ * as many: the accepted ones, then the drawn one.  The rest is -1, and so is a token
+ * that no distribution gives (scores with a NaN, +infinity or nothing finite, a
+ * temperature below 0, a draft's NaN).  Children whose token is outside the
+ * vocabulary, or an earlier sibling's, are passed over.  V up to 2^21; dWork: as many bytes as
+ * i4_verify_workspace says, 16-byte aligned. */
+int64_t i4_verify_workspace(int T, int V, int B, int has_cu, int has_draft);
+int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, const int32_t* dTokens,
+                  const int32_t* dParents, const float* dUniforms, const int32_t* dCu, int B, const float* dTemps,
+                  float temperature, const float* dDraft, int64_t draft_row, int32_t* dOut, int32_t* dPath,
+                  int32_t* dCounts, void* dWork, int64_t work_bytes, void* stream);
+
+/* Cache rows of the nodes on a path moved together, in `layers` caches of one
+ * geometry: place ctx + dPath[dCu[b] + i] to ctx + i for i < dCounts[b], ctx =
+ * dKvLens[b] - the sequence's nodes.  dLens[b] (apart from dKvLens) = ctx +
+ * dCounts[b]; a negative dKvLens[b] stays.  A path's numbers grow, as
+ * i4_verify_dev's do; entries that do not pass their own place move nothing. */
+int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_t* dTable, int64_t table_row,
+                      int table_w, const int32_t* dKvLens, const int32_t* dCu, int T, int B, const int32_t* dPath,
+                      const int32_t* dCounts, int32_t* dLens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
