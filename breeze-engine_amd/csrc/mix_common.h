@@ -74,6 +74,22 @@ __device__ inline void store4(void* p, int dt, int64_t i, f4 v) {
     }
 }
 
+// Two values to bf16, by the instruction.
+__device__ inline uint32_t pack_bf16(float a, float b) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
+}
+
+// store4 of a type known at compile time.
+template <int DT>
+__device__ inline void put4(void* p, int64_t i, f4 v) {
+    if constexpr (DT == kBF16) {
+        *reinterpret_cast<u2*>(static_cast<uint16_t*>(p) + i) = (u2){pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)};
+    } else {
+        store4(p, DT, i, v);
+    }
+}
+
 // Two of the four 8-bit values of w as fp16, exactly.  INT8: the byte plus 128
 // becomes the low mantissa of 1024 (one byte permute for two values), and
 // 1152 comes off again.

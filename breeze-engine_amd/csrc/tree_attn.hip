@@ -18,6 +18,11 @@
 // end).  Tiles go from the last keys to the first, so that the tree comes first and
 // a lane follows its node's parents down once: a tile's mask is the 32 bits that
 // it passes.  Tiles before the tree have no mask.
+//
+// The tiles of all units (a sequence, a key-value head, up to 128 rows), one unit
+// after another, are cut into equal shares, one a workgroup, whatever the sequences'
+// lengths, which the host does not read; each workgroup sums up the lengths for
+// itself.  A unit that is cut leaves its parts' sums to tree_join_kernel.
 #include "attn_common.h"
 
 #include <algorithm>
@@ -27,6 +32,8 @@
 using namespace mx;
 
 namespace {
+
+typedef int i2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTreeNodes = 1024;
 
@@ -42,10 +49,11 @@ struct TreeArgs {
     const int32_t* kv_lens;
     const int32_t* cu;  // null: one node a sequence
     const int32_t* parents;
-    float* part;        // [splits][T * Hq][D] where keys are split
-    f2* ml;             // [splits][T * Hq]: maximum and sum
+    float* part;        // [2 shares][rows a unit][D]: sums of cut units, a share's first and last one
+    f2* ml;             // [2 shares][rows a unit]: maximum and sum
+    i2* shares;         // [slots][H]: a unit's first and last share
     int64_t table_row;
-    int T, B, Hq, H, G, P, pshift, table_w, nslots, splits, chunk;  // chunk: keys a split
+    int T, B, Hq, H, G, P, pshift, table_w, nslots, grid;  // grid: shares
     float scale;  // softmax scale * log2(e)
 };
 
@@ -66,8 +74,564 @@ __device__ inline Seq sequence(const TreeArgs& a, int b) {
     return s;
 }
 
+// A value that all lanes have alike, as the scalar unit's.
+__device__ inline int64_t uniform(int64_t x) {
+    const int lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+    return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+
+// x / y of whole numbers up to 2^53: the fp64 quotient is rounded to a whole number
+// only where it is one.  A tenth of the instructions of a division in 64-bit integers.
+__device__ inline int64_t over(int64_t x, int64_t y) { return (int64_t)((double)x / (double)y); }
+
+// Tiles of a sequence's keys; one where it has none, or where its tree is too large, which says so.
+__device__ inline int tiles_of(const Seq& sq, int KT) {
+    return sq.n > kTreeNodes ? 1 : max((sq.kv + KT - 1) / KT, 1);
+}
+
+// R rows a wave: 32 on the 32x32x16 instructions, 16 on the 16x16x32 ones.  A lane's
+// row is its number modulo R, its part `c` the rest: 64 / R parts hold 8 values each
+// of a slab of an operand, and quads of a result, keys or values QS q + 4 c + 0..3.
+template <int R>
+struct Shape;
+template <>
+struct Shape<32> {
+    typedef f16 Acc;
+    static constexpr int kSlab = 16, kQuads = 4, kStep = 8;  // an operand's depth; a result's quads, their step
+    static __device__ inline f16 mfma(h8 a, h8 b, f16 c) { return mfma32(a, b, c); }
+};
+template <>
+struct Shape<16> {
+    typedef f4 Acc;
+    static constexpr int kSlab = 32, kQuads = 1, kStep = 16;
+    static __device__ inline f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <int R>
+__device__ inline float max_parts(float x) { return R == 32 ? max_halves(x) : max_halves(max_rows16(x)); }
+template <int R>
+__device__ inline float sum_parts(float x) { return R == 32 ? sum_halves(x) : sum_halves(sum_rows16(x)); }
+
+// A row's queries as they lie in memory: values kSlab s + 8 c + 0..7 for slab s, from
+// element `at` on.
+template <int D, int DT, int R>
+struct RawQueries {
+    static constexpr int kSlab = Shape<R>::kSlab, N = D / kSlab;
+    u4 w[N][DT == kF32 ? 2 : 1];
+    __device__ inline void load(const void* q, int64_t at) {
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+            if constexpr (DT == kF32) {
+                const u4* const p = reinterpret_cast<const u4*>(static_cast<const float*>(q) + at + kSlab * s);
+                w[s][0] = p[0];
+                w[s][1] = p[1];
+            } else {  // rows are 8-byte aligned
+                const u2* const p = reinterpret_cast<const u2*>(static_cast<const uint16_t*>(q) + at + kSlab * s);
+                const u2 x = p[0], y = p[1];
+                w[s][0] = (u4){x.x, x.y, y.x, y.y};
+            }
+        }
+    }
+    // As operands, scaled; returns what a score is worth in log2.
+    __device__ inline float operands(float scale, h8* hi, h8* lo) const {
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < N; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (DT == kF32) {
+                    top = max(max(top, w[s][0][j] & 0x7FFFFFFFu), w[s][1][j] & 0x7FFFFFFFu);
+                } else {
+                    top = max(max(top, w[s][0][j] << 16 & 0x7FFF0000u), w[s][0][j] & 0x7FFF0000u);
+                }
+            }
+        top = lane_max_u32(top, 32);
+        if constexpr (R == 16) top = lane_max_u32(top, 16);
+        if constexpr (DT == kF16) {  // halves order like their magnitudes
+            const uint16_t bits = (uint16_t)(top >> 16);
+            top = f_bits((float)__builtin_bit_cast(_Float16, bits));
+        }
+        const float up = row_scale(top);
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (DT == kF32) {
+                    x[j] = bits_f(w[s][0][j]) * up;
+                    x[4 + j] = bits_f(w[s][1][j]) * up;
+                } else {
+                    const uint32_t b = w[s][0][j];
+                    const h2 h = __builtin_bit_cast(h2, b);
+                    x[2 * j] = (DT == kBF16 ? bf_lo(b) : (float)h[0]) * up;
+                    x[2 * j + 1] = (DT == kBF16 ? bf_hi(b) : (float)h[1]) * up;
+                }
+            }
+            if constexpr (DT == kF32) split8(x, hi[s], lo[s]);
+            else hi[s] = round8(x);
+        }
+        return score_worth(scale, up);
+    }
+};
+
+// How a kernel's waves share out rows and keys: W waves, WR of them along the rows,
+// RT rows a unit, W / WR along a tile's keys, KT keys a tile, 32 or more a wave.
+template <int D, int WR>
+struct Tiling {
+    static constexpr int R = D == 256 ? 16 : 32, W = D == 256 ? 8 : 4, WK = W / WR, RT = R * WR;
+    static constexpr int KT = WK == 4 ? 128 : 64, KW = KT / WK;
+    static constexpr int KS = D + 8, VS = D + 16;  // LDS rows of a key and of its values: reads of one instruction fall on unlike banks
+};
+// Workgroups a compute unit.
+constexpr int per_unit(int D) { return D == 256 ? 1 : 2; }
+
+constexpr int kLeastTiles = 2;  // a share's: less is not worth a workgroup's start
+
+// The share that this wave's workgroup has of all units' tiles: tiles [pos, end), the
+// first in sequence b, whose first tile is `base`; `per` tiles a share.  Every wave
+// sums up all sequences' tiles for itself, 256 a round.
+struct Share {
+    int64_t pos, end, per, base;
+    int b;
+    Seq sq;
+};
+template <int RT, int KT>
+__device__ inline Share share_of(const TreeArgs& a, int id) {
+    constexpr int N = 4;  // sequences a lane and round
+    const int lane = threadIdx.x & 63;
+    Seq s[N];
+    int64_t n[N], upto, all;
+    const auto round = [&](int b0) {
+        int64_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) s[j] = sequence(a, min(b0 + N * lane + j, a.B - 1));
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int tiles = b0 + N * lane + j < a.B ? tiles_of(s[j], KT) : 0;
+            n[j] = (int64_t)((uint32_t)(s[j].n * a.G + RT - 1) / RT * a.H) * tiles;
+            mine += n[j];
+        }
+        upto = mine;
+#pragma unroll
+        for (int st = 1; st < 64; st *= 2) {
+            const int64_t y = __shfl_up(upto, st);
+            if (lane >= st) upto += y;
+        }
+        all = uniform(__shfl(upto, 63));
+        upto -= mine;  // before this lane's
+    };
+    Share w;
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64 * N) {
+        round(b0);
+        total += all;
+    }
+    w.per = max(over(total + a.grid - 1, a.grid), (int64_t)kLeastTiles);
+    w.pos = id * w.per;
+    w.end = min(w.pos + w.per, total);
+    if (w.pos >= w.end) return w;
+    int64_t before = 0;
+    for (int b0 = 0;; b0 += 64 * N) {
+        if (a.B > 64 * N) round(b0);
+        upto += before;
+        before += all;
+        if (w.pos < before) {
+            bool is = false;
+            int64_t first = 0;
+            int b = 0, q0 = 0, rows = 0, kv = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (w.pos >= upto && w.pos < upto + n[j]) {
+                    is = true;
+                    first = upto;
+                    b = b0 + N * lane + j;
+                    q0 = s[j].q0;
+                    rows = s[j].n;
+                    kv = s[j].kv;
+                }
+                upto += n[j];
+            }
+            const int who = __builtin_ctzll(__ballot(is));
+            w.base = uniform(__shfl(first, who));
+            w.b = __builtin_amdgcn_readlane(b, who);
+            w.sq = {__builtin_amdgcn_readlane(q0, who), __builtin_amdgcn_readlane(rows, who), __builtin_amdgcn_readlane(kv, who)};
+            return w;
+        }
+    }
+}
+
+template <int D, int KIND, int DT, int WR>
+__global__ __launch_bounds__((64 * Tiling<D, WR>::W), (per_unit(D) * Tiling<D, WR>::W / 4)) void tree_keys_kernel(TreeArgs a) {
+    typedef Tiling<D, WR> T;
+    constexpr bool SPLIT = DT == kF32, PSPLIT = DT != kBF16;  // two terms of the queries, and of the weights
+    constexpr int R = T::R, W = T::W, WK = T::WK, RT = T::RT, KT = T::KT, KW = T::KW, KS = T::KS, VS = T::VS;
+    constexpr int THREADS = 64 * W, U = KW / 32;    // blocks of 32 keys a wave
+    constexpr int NC = KT * D / (16 * THREADS);     // 16-byte chunks a thread loads of a tile's keys (and of its values)
+    constexpr int NG = KT / 16;                     // groups of 16 keys, each in one page
+    constexpr int per_row = D / 16;
+    constexpr int SL = D / Shape<R>::kSlab, NA = D / R, NQ = Shape<R>::kQuads, QS = Shape<R>::kStep;
+    constexpr int J = R / 2;                        // scores a lane has of 32 keys
+    constexpr int kBytes = std::max(KT * (KS + VS) * 2, (WK - 1) * WR * R * D * 4);
+    typedef typename Shape<R>::Acc Acc;
+    __shared__ __align__(16) uint8_t lds[kBytes];
+    __shared__ __align__(16) float sks[KT], svs[KT];
+    __shared__ float smax[KT / 32], sm[W][R], sl[W][R], sf[W][R];
+    __shared__ uint32_t svalid[KT / 32];
+    __shared__ int16_t up[kTreeNodes];
+    _Float16 *const sk = reinterpret_cast<_Float16*>(lds), *const sv = sk + KT * KS;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & (R - 1), c = lane / R, rg = wave % WR, kg = wave / WR, r16 = lane & 15;
+    // Neighbouring shares lie on one XCD each, whose cache has a unit's keys for its next rows.
+    const int id = (blockIdx.x & 7) * (a.grid >> 3) + (blockIdx.x >> 3);
+    Share w = share_of<RT, KT>(a, id);
+
+    while (w.pos < w.end) {
+        // A unit: rows of one key-value head; its tiles [t0, t1) are this share's.
+        const Seq sq = w.sq;
+        const int ntile = tiles_of(sq, KT), nrow = (uint32_t)(sq.n * a.G + RT - 1) / RT;
+        const int its = (int)over(w.pos - w.base, ntile), h = its / nrow, first = (its - h * nrow) * RT;
+        const int64_t began = w.base + (int64_t)its * ntile;
+        const int t0 = (int)(w.pos - began), t1 = (int)min((int64_t)ntile, t0 + (w.end - w.pos));
+        const bool whole = t0 == 0 && t1 == ntile, spoilt = sq.n > kTreeNodes;
+        const int rows = min(sq.n * a.G, first + RT), row = first + R * rg + r;
+        const bool has_row = row < rows;
+        const int node = has_row ? row / a.G : 0, tok = sq.q0 + node, head = h * a.G + (has_row ? row % a.G : 0);
+        const int ctx = sq.kv - sq.n;  // place of node 0; below zero where the cache lacks the first nodes
+        const int32_t* const table = a.table + w.b * a.table_row;
+        int t = spoilt || sq.kv == 0 ? t0 - 1 : t1 - 1;
+
+        // The pages of a tile's groups of 16 keys, one a lane; -1 where the sequence has no
+        // key or the cache no such page.
+        const auto pages_of = [&](int tile) {
+            const int key = KT * tile + 16 * (lane & (NG - 1));
+            int page = -1;
+            if (tile >= t0 && key < sq.kv) page = table[key >> a.pshift];
+            return page < a.P ? page : -1;
+        };
+        int pages = pages_of(t), pages_now = pages;
+        RawQueries<D, DT, R> raw;
+        raw.load(a.q, tok * a.q_token + head * a.q_head + 8 * c);
+
+        u4 kraw[NC], vraw[NC];
+        float ksc = 0.0f, vsc = 0.0f;
+        bool sc_bad = true;
+        const auto load = [&](int tile, int pages) {
+            const auto row_of = [&](int page, int key) {  // cache row of a group's first key
+                return (((int64_t)max(page, 0) * a.H + h) << a.pshift) + (key & ((1 << a.pshift) - 1));
+            };
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int g = (wave * 64 + THREADS * i) / per_row >> 4;  // the wave's group of this pass
+                const int64_t at = row_of(__builtin_amdgcn_readlane(pages, g), KT * tile + 16 * g) +
+                                   ((tid + THREADS * i) / per_row & 15);
+                kraw[i] = *reinterpret_cast<const u4*>(a.kp + at * D + 16 * (tid % per_row));
+                vraw[i] = *reinterpret_cast<const u4*>(a.vp + at * D + 16 * (tid % per_row));
+            }
+            if (tid < KT) {
+                const int page = __shfl(pages, tid >> 4 & (NG - 1));
+                sc_bad = page < 0 || KT * tile + tid >= sq.kv;
+                const int64_t at = row_of(page, KT * tile + (tid & ~15)) + (tid & 15);
+                ksc = a.ks[at];
+                vsc = a.vs[at];
+            }
+        };
+        if (t >= t0) load(t, pages);
+        pages = pages_of(t - 1);
+        if (t0 == 0 && tid == 0) {
+            const int slot = (a.cu ? (int)((int64_t)sq.q0 * a.G / RT) + w.b : w.b * nrow) + first / RT;
+            a.shares[(int64_t)slot * a.H + h] = (i2){id, (int)over(began + ntile - 1, w.per)};
+        }
+        __syncthreads();  // the last unit's reads are over
+        if (t1 * KT > ctx)
+            for (int i = tid; i < min(sq.n, kTreeNodes); i += THREADS) {
+                const int p = a.parents[sq.q0 + i];
+                up[i] = (int16_t)(p >= 0 && p < i ? p : -1);
+            }
+
+        h8 qh[SL], ql[SPLIT ? SL : 1];
+        const float rowf = raw.operands(a.scale, qh, ql);
+
+        Acc o[NA];
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+#pragma unroll
+            for (int j = 0; j < 4 * NQ; ++j) o[i][j] = 0.0f;
+        // A tile's weights are computed in units in which a probability of 1 is 2^9 / nu, at
+        // most 2^119 of those eight, so that a lane's add up to less than fp32 holds.
+        constexpr float least = 0x1p-110f;
+        float m = -INFINITY, l = 0.0f, nu = least, peak = 0.0f, unit = __builtin_log2f(kPScale / least);
+        int at_node = has_row ? node : -1;  // the next of the row's node and its ancestors
+        const bool wave_rows = first + R * rg < rows;
+
+        for (; t >= t0; --t) {
+            const int key0 = KT * t;
+            __syncthreads();  // the last tile's reads are over
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int kr = (tid + THREADS * i) / per_row, col = 16 * (tid % per_row);
+                u4 kw = kraw[i], vw = vraw[i];
+                if constexpr (KIND == kFp8) {  // bytes of rows that no key is in may be NaN
+                    const int page = __builtin_amdgcn_readlane(pages_now, (wave * 64 + THREADS * i) / per_row >> 4);
+                    if (page < 0 || key0 + kr >= sq.kv) kw = vw = (u4){0, 0, 0, 0};
+                }
+                h8* kd = reinterpret_cast<h8*>(sk + kr * KS + col);
+                h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
+                kd[0] = unpack8<KIND>(kw.x, kw.y);
+                kd[1] = unpack8<KIND>(kw.z, kw.w);
+                vd[0] = unpack8<KIND>(vw.x, vw.y);
+                vd[1] = unpack8<KIND>(vw.z, vw.w);
+            }
+            if (tid < KT) {
+                // A value scale of NaN goes with the key's, whose score a row that does
+                // not see the key leaves out; times a probability of zero it would not.
+                const bool nan = vsc != vsc;
+                const float v = sc_bad || nan ? 0.0f : vsc;
+                sks[tid] = sc_bad ? 0.0f : nan ? vsc : ksc;
+                svs[tid] = v;
+                float vmax = v;
+#pragma unroll
+                for (int st = 1; st < 32; st *= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, st));
+                const uint64_t valid = __ballot(!sc_bad);
+                if ((lane & 31) == 0) {
+                    smax[tid >> 5] = vmax;
+                    svalid[tid >> 5] = (uint32_t)(valid >> (lane & 32));
+                }
+            }
+            __syncthreads();
+            pages_now = pages;
+            if (t > t0) load(t - 1, pages);
+            pages = pages_of(t - 2);
+            if (!wave_rows) continue;
+
+            // Scores: a lane's j-th of a block of 32 keys is key QS (j / 4) + 4 c + j % 4.
+            float x[U][J];
+            if constexpr (R == 32) {
+                f16 s[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < SL; ++i)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const h8 k = *reinterpret_cast<const h8*>(sk + (KW * kg + 32 * u + r) * KS + 8 * c + 16 * i);
+                        s[u] = mfma32(k, qh[i], s[u]);
+                        if constexpr (SPLIT) s[u] = mfma32(k, ql[i], s[u]);
+                    }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[u][j] = s[u][j];
+            } else {
+                f4 s[2 * U];
+#pragma unroll
+                for (int v = 0; v < 2 * U; ++v) s[v] = (f4){0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < SL; ++i)
+#pragma unroll
+                    for (int v = 0; v < 2 * U; ++v) {
+                        const h8 k = *reinterpret_cast<const h8*>(sk + (KW * kg + 16 * v + r) * KS + 8 * c + 32 * i);
+                        s[v] = Shape<16>::mfma(k, qh[i], s[v]);
+                        if constexpr (SPLIT) s[v] = Shape<16>::mfma(k, ql[i], s[v]);
+                    }
+#pragma unroll
+                for (int v = 0; v < 2 * U; ++v)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[v / 2][4 * (v % 2) + j] = s[v][j];
+            }
+            // Times the key scales.
+            float vmax = 0.0f;
+            bool all = key0 + KT <= ctx;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                vmax = fmaxf(vmax, smax[U * kg + u]);
+                all = all && svalid[U * kg + u] == 0xFFFFFFFFu;
+#pragma unroll
+                for (int j = 0; j < J; j += 4) {
+                    const f4 sc = *reinterpret_cast<const f4*>(sks + KW * kg + 32 * u + QS * (j / 4) + 4 * c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][j + e] *= sc[e];
+                }
+            }
+            if (!all) {
+                vmax = 0.0f;
+#pragma unroll
+                for (int u = U - 1; u >= 0; --u) {
+                    // The keys of these 32 that the row sees: those before the tree, and the nodes that
+                    // its path to the root passes.
+                    const int n0 = key0 + KW * kg + 32 * u - ctx;  // the first one's node
+                    uint32_t bits = n0 <= -32 ? 0xFFFFFFFFu : n0 < 0 ? (1u << -n0) - 1 : 0u;
+                    if (n0 + 32 > 0) {
+                        while (at_node >= n0 + 32) at_node = up[at_node];
+                        while (at_node >= max(n0, 0)) {
+                            bits |= 1u << (at_node - n0);
+                            at_node = up[at_node];
+                        }
+                    }
+                    bits &= has_row ? svalid[U * kg + u] : 0u;
+                    bits >>= 4 * c;
+#pragma unroll
+                    for (int j = 0; j < J; j += 4) {
+                        const f4 vs = *reinterpret_cast<const f4*>(svs + KW * kg + 32 * u + QS * (j / 4) + 4 * c);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool out = !(bits >> (QS * (j / 4) + e) & 1);
+                            x[u][j + e] = out ? -INFINITY : x[u][j + e];
+                            vmax = fmaxf(vmax, out ? 0.0f : vs[e]);
+                        }
+                    }
+                }
+                vmax = max_parts<R>(vmax);
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < J; j += 2) top = fmaxf(fmaxf(top, x[u][j]), x[u][j + 1]);
+            top = max_parts<R>(top);
+            // The reference moves only once a row's scores pass it by kSlack, its units where the
+            // values' size leaves their range.
+            const bool moves = (top - m) * rowf > kSlack;
+            const bool other = vmax > nu * 8.0f || (vmax > 0.0f && vmax <= nu * 0x1p-4f);
+            if (__any(moves || other)) {
+                float f = moves ? fast_exp2((m - top) * rowf) : 1.0f;
+                m = moves ? top : m;
+                l *= f;
+                peak *= f;
+                const float now = next_nu(nu, vmax, peak, least);
+                f *= nu / now;
+                unit = __builtin_log2f(kPScale / now);
+                nu = now;
+#pragma unroll
+                for (int i = 0; i < NA; ++i) o[i] *= f;
+            }
+            peak = fmaxf(peak, nu);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float bias = __builtin_fmaf(-ref, rowf, unit);
+            // m rowf is rounded once here, by less than half while it is below 2^22; past that
+            // the difference is taken first, else the largest weight would be 2 to that error.
+            if (__any(__builtin_fabsf(ref) * rowf > 0x1p22f)) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) x[u][j] -= ref;
+                bias = unit;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int g = 0; g < J / 8; ++g) {  // eight of a lane's scores make an operand
+                    float y[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        y[j] = fast_exp2(__builtin_fmaf(x[u][8 * g + j], rowf, bias));
+                        sum += y[j];
+                    }
+                    const int k0 = KW * kg + 32 * u + 16 * g + 4 * c;  // of the first quad; the second QS on
+                    const f4 s0 = *reinterpret_cast<const f4*>(svs + k0), s1 = *reinterpret_cast<const f4*>(svs + k0 + QS);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        y[j] *= s0[j];
+                        y[4 + j] *= s1[j];
+                    }
+                    h8 ph, pl;
+                    if constexpr (PSPLIT) split8(y, ph, pl);
+                    else ph = round8(y);
+                    const _Float16* p = sv + (k0 + (r16 >> 2)) * VS + 16 * (r >> 4) + 4 * (r16 & 3);
+#pragma unroll
+                    for (int i = 0; i < NA; ++i) {
+                        const h8 v = mx::join(read_tr(p + R * i), read_tr(p + R * i + QS * VS));
+                        o[i] = Shape<R>::mfma(v, ph, o[i]);
+                        if constexpr (PSPLIT) o[i] = Shape<R>::mfma(v, pl, o[i]);
+                    }
+                }
+            l = __builtin_fmaf(sum, nu * (1.0f / kPScale), l);
+        }
+
+        l = sum_parts<R>(l);
+        float f = nu * (1.0f / kPScale), mlog = m * rowf;
+        if constexpr (WK > 1) {
+            // The groups' sums, joined in their order.
+            __syncthreads();
+            f4* const so = reinterpret_cast<f4*>(lds);
+            if (c == 0) {
+                sm[wave][r] = mlog;
+                sl[wave][r] = l;
+                sf[wave][r] = f;
+            }
+            if (kg > 0) {
+                f4* const mine = so + ((kg - 1) * WR + rg) * NA * NQ * 64 + lane;
+#pragma unroll
+                for (int i = 0; i < NA; ++i)
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+                        mine[64 * (i * NQ + q)] = (f4){o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]};
+            }
+            __syncthreads();
+            float top = mlog;
+#pragma unroll
+            for (int g = 1; g < WK; ++g) top = fmaxf(top, sm[g * WR + rg][r]);
+            const float safe = top == -INFINITY ? 0.0f : top;
+            const float f0 = fast_exp2(mlog - safe);
+            l *= f0;
+            f *= f0;
+            if (kg == 0) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) o[i] *= f;
+#pragma unroll
+                for (int g = 1; g < WK; ++g) {
+                    const float e = fast_exp2(sm[g * WR + rg][r] - safe), by = e * sf[g * WR + rg][r];
+                    l += e * sl[g * WR + rg][r];
+                    const f4* const from = so + ((g - 1) * WR + rg) * NA * NQ * 64 + lane;
+#pragma unroll
+                    for (int i = 0; i < NA; ++i)
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) {
+                            const f4 v = from[64 * (i * NQ + q)] * by;
+#pragma unroll
+                            for (int e4 = 0; e4 < 4; ++e4) o[i][4 * q + e4] += v[e4];
+                        }
+                }
+            }
+            f = 1.0f;
+            mlog = top;
+        }
+        if (wave_rows && kg == 0) {
+            if (!whole) {
+                // A share's first unit may have begun in an earlier one; its last may go on.  A part is kept
+                // in the lanes' order, 1 KB an instruction.
+                const int64_t part = 2 * id + (t0 == 0);
+                if (c == 0) a.ml[part * RT + R * rg + r] = (f2){mlog, l};
+                f4* const to = reinterpret_cast<f4*>(a.part + part * RT * D) + rg * NA * NQ * 64 + lane;
+#pragma unroll
+                for (int i = 0; i < NA; ++i)
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+                        to[64 * (i * NQ + q)] = (f4){o[i][4 * q] * f, o[i][4 * q + 1] * f, o[i][4 * q + 2] * f, o[i][4 * q + 3] * f};
+            } else if (has_row) {
+                f *= spoilt ? __builtin_nanf("") : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+#pragma unroll
+                for (int i = 0; i < NA; ++i)
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+                        put4<DT>(a.out, tok * a.o_token + head * a.o_head + R * i + 8 * q + 4 * c,
+                                 (f4){o[i][4 * q] * f, o[i][4 * q + 1] * f, o[i][4 * q + 2] * f, o[i][4 * q + 3] * f});
+            }
+        }
+        w.pos += t1 - t0;
+        if (w.pos < w.end && w.pos >= w.base + (int64_t)nrow * a.H * ntile) {  // on to the next sequence that has rows
+            w.base = w.pos;
+            do {
+                w.sq = sequence(a, ++w.b);
+            } while (w.sq.n == 0);
+        }
+    }
+}
+
 // The RT rows of a slot: their sequence (-1: none) and the first of them.  Sequence b's
-// tiles take the slots from cu[b] * G / RT + b on, which leaves room for all
+// units take the slots from cu[b] * G / RT + b on, which leaves room for all
 // without a pass over the lengths.
 template <int RT>
 __device__ inline int rows_of_slot(const TreeArgs& a, int slot, Seq& sq, int& first) {
@@ -91,425 +655,106 @@ __device__ inline int rows_of_slot(const TreeArgs& a, int slot, Seq& sq, int& fi
     return at < 0 || at >= rows ? -1 : b;
 }
 
-// Splits of a sequence: a tree that is too large has one, which says so.
-__device__ inline int splits_of(const TreeArgs& a, const Seq& sq) {
-    return sq.n > kTreeNodes ? 1 : max((sq.kv + a.chunk - 1) / a.chunk, 1);
-}
-
-// A row's queries as operands (values 16 s + 8 (lane / 32) + 0..7 for slab s,
-// from element `at` on), scaled; returns what a score is worth in log2.
-template <int D, int DT>
-__device__ inline float load_queries(const TreeArgs& a, int64_t at, h8* hi, h8* lo) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-            const f4 v = load4(a.q, DT, at + 16 * s + j);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, f_bits(v[e]) & 0x7FFFFFFFu);
-        }
-    top = lane_max_u32(top, 32);
-    const float up = row_scale(top);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-        float w[8];
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-            const f4 v = load4(a.q, DT, at + 16 * s + j);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[j + e] = v[e] * up;
-        }
-        if constexpr (DT == kF32) split8(w, hi[s], lo[s]);
-        else hi[s] = round8(w);
-    }
-    return score_worth(a.scale, up);
-}
-
-// Keys of a tile: 32 a wave where the waves share them out, else 64.
-constexpr int tile_keys(int WR) { return WR == 1 ? 128 : 64; }
-constexpr int row_k(int D) { return D + 8; }   // LDS rows of a key and of its values: reads of one
-constexpr int row_v(int D) { return D + 16; }  // instruction fall on unlike banks
-constexpr int per_unit(int D, int DT) { return D == 256 ? 1 : D == 128 && DT == kF32 ? 1 : 2; }
-
-template <int D, int KIND, int DT, int WR>
-__global__ __launch_bounds__(256, per_unit(D, DT)) void tree_keys_kernel(TreeArgs a) {
-    constexpr bool SPLIT = DT == kF32, PSPLIT = DT != kBF16;  // two terms of the queries, and of the weights
-    constexpr int WK = 4 / WR, RT = 32 * WR, KT = tile_keys(WR), KW = KT / WK, U = KW / 32;
-    constexpr int KS = row_k(D), VS = row_v(D);
-    constexpr int NC = KT * D / 4096;  // 16-byte chunks a thread loads of a tile's keys (and of its values)
-    constexpr int per_row = D / 16;
-    constexpr int kBytes = std::max(KT * (KS + VS) * 2, (WK - 1) * WR * D * 128);
-    __shared__ __align__(16) uint8_t lds[kBytes];
-    __shared__ __align__(16) float sks[KT], svs[KT];
-    __shared__ float smax[KT / 32], sm[4][32], sl[4][32], sf[4][32];
-    __shared__ uint32_t svalid[KT / 32];
-    __shared__ int16_t up[kTreeNodes];
-    _Float16 *const sk = reinterpret_cast<_Float16*>(lds), *const sv = sk + KT * KS;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r32 = lane & 31, hf = lane >> 5, rg = wave % WR, kg = wave / WR;
-    const int h = blockIdx.x % a.H, ss = blockIdx.x / a.H, split = ss % a.splits, slot = ss / a.splits;
+// The parts of a unit that was cut joined, in their order.  A wave takes one quad of
+// the values of R rows, which a part has in 1 KB; where there are few units, the
+// four waves of a workgroup take a quarter of the parts each.
+template <int D, int DT, int WR, bool FEW>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
+    typedef Tiling<D, WR> T;
+    constexpr int R = T::R, RT = T::RT, NQ = Shape<R>::kQuads, N = D / R * NQ, NG = FEW ? 4 : 1;
+    __shared__ __align__(16) f4 sv[FEW ? 192 : 1];
+    __shared__ float ssum[FEW ? 192 : 1], stop[FEW ? 256 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & (R - 1), c = lane / R, slot = blockIdx.x / a.H, h = blockIdx.x - slot * a.H;
+    const int item = FEW ? blockIdx.y : 4 * blockIdx.y + wave, rg = item / N, quad = item % N;
     Seq sq;
     int first;
-    const int b = rows_of_slot<RT>(a, slot, sq, first);
-    if (b < 0) return;
-    const int nsplit = splits_of(a, sq);
-    if (split >= nsplit) return;
-    const int rows = (int)min((int64_t)sq.n * a.G, (int64_t)first + RT);
-    const int row = first + 32 * rg + r32;
-    const bool has_row = row < rows, spoilt = sq.n > kTreeNodes;
-    const int node = has_row ? row / a.G : 0, tok = sq.q0 + node, head = h * a.G + (has_row ? row % a.G : 0);
-    const int ctx = sq.kv - sq.n;  // place of node 0; below zero where the cache lacks the first nodes
-
-    const int k0 = split * a.chunk, k1 = spoilt ? 0 : min(k0 + a.chunk, sq.kv);
-    const int t0 = k0 / KT, t1 = (k1 + KT - 1) / KT;
-    int t = t1 - 1;
-    const int32_t* table = a.table + b * a.table_row;
-
-    u4 kraw[NC], vraw[NC];
-    int64_t grow[NC];
-    float ksc = 0.0f, vsc = 0.0f;
-    bool sc_bad = true;
-    // Cache row of the 16 keys from `key` on; -1 where the sequence or its table has none.
-    const auto group_row = [&](int key) -> int64_t {
-        const int page = table[min(key, sq.kv - 1) >> a.pshift];
-        const bool is = key < sq.kv && page >= 0 && page < a.P;
-        return is ? (((int64_t)page * a.H + h) << a.pshift) + (key & ((1 << a.pshift) - 1)) : -1;
-    };
-    const auto load = [&](int tile) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int kr = (wave * 64 + 256 * i) / per_row;  // the wave's first row of this pass
-            grow[i] = group_row(KT * tile + (kr & ~15));
-            const int64_t at = (grow[i] < 0 ? 0 : grow[i]) + ((tid + 256 * i) / per_row & 15);
-            kraw[i] = *reinterpret_cast<const u4*>(a.kp + at * D + 16 * (tid % per_row));
-            vraw[i] = *reinterpret_cast<const u4*>(a.vp + at * D + 16 * (tid % per_row));
-        }
-        if (tid < KT) {
-            const int64_t at = group_row(KT * tile + (tid & ~15));
-            sc_bad = at < 0 || KT * tile + tid >= sq.kv;
-            ksc = sc_bad ? 0.0f : a.ks[at + (tid & 15)];
-            vsc = sc_bad ? 0.0f : a.vs[at + (tid & 15)];
-        }
-    };
-    if (t >= t0) load(t);
-    if (k1 > ctx)
-        for (int i = tid; i < min(sq.n, kTreeNodes); i += 256) {
-            const int p = a.parents[sq.q0 + i];
-            up[i] = (int16_t)(p >= 0 && p < i ? p : -1);
-        }
-
-    h8 qh[D / 16], ql[SPLIT ? D / 16 : 1];
-    const float rowf = load_queries<D, DT>(a, tok * a.q_token + head * a.q_head + 8 * hf, qh, ql);
-
-    f16 o[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-    // A tile's weights are computed in units in which a probability of 1 is 2^9 / nu, at
-    // most 2^119 of those eight, so that a lane's add up to less than fp32 holds.
-    constexpr float least = 0x1p-110f;
-    float m = -INFINITY, l = 0.0f, nu = least, peak = 0.0f, unit = __builtin_log2f(kPScale / least);
-    int at_node = has_row ? node : -1;  // the next of the row's node and its ancestors
-
-    for (; t >= t0; --t) {
-        const int key0 = KT * t;
-        __syncthreads();  // the last tile's reads are over
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int kr = (tid + 256 * i) / per_row, col = 16 * (tid % per_row);
-            u4 kw = kraw[i], vw = vraw[i];
-            if (KIND == kFp8 && (grow[i] < 0 || key0 + kr >= sq.kv)) kw = vw = (u4){0, 0, 0, 0};
-            h8* kd = reinterpret_cast<h8*>(sk + kr * KS + col);
-            h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
-            kd[0] = unpack8<KIND>(kw.x, kw.y);
-            kd[1] = unpack8<KIND>(kw.z, kw.w);
-            vd[0] = unpack8<KIND>(vw.x, vw.y);
-            vd[1] = unpack8<KIND>(vw.z, vw.w);
-        }
-        if (tid < KT) {
-            // A value scale of NaN goes with the key's, whose score a row that does
-            // not see the key leaves out; times a probability of zero it would not.
-            const bool nan = vsc != vsc;
-            sks[tid] = nan ? vsc : ksc;
-            svs[tid] = nan ? 0.0f : vsc;
-            float vmax = nan ? 0.0f : vsc;
-#pragma unroll
-            for (int st = 1; st < 32; st *= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, st));
-            const uint64_t valid = __ballot(!sc_bad);
-            if ((lane & 31) == 0) {
-                smax[tid >> 5] = vmax;
-                svalid[tid >> 5] = (uint32_t)(valid >> (lane & 32));
-            }
-        }
-        __syncthreads();
-        if (t > t0) load(t - 1);
-
-        f16 s[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
-            const _Float16* p = sk + (KW * kg + 32 * u + r32) * KS + 8 * hf;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                const h8 k = *reinterpret_cast<const h8*>(p + 16 * i);
-                s[u] = mfma32(k, qh[i], s[u]);
-                if constexpr (SPLIT) s[u] = mfma32(k, ql[i], s[u]);
-            }
-        }
-        // Scores times the key scales; result register j holds key 8 (j / 4) + 4 hf + j % 4.
-        float vmax = 0.0f;
-        bool all = key0 + KT <= ctx;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            vmax = fmaxf(vmax, smax[U * kg + u]);
-            all = all && svalid[U * kg + u] == 0xFFFFFFFFu;
-#pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const f4 sc = *reinterpret_cast<const f4*>(sks + KW * kg + 32 * u + 2 * j + 4 * hf);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[u][j + e] *= sc[e];
-            }
-        }
-        if (!all) {
-            vmax = 0.0f;
-#pragma unroll
-            for (int u = U - 1; u >= 0; --u) {
-                // The keys of these 32 that the row sees: those before the tree, and the nodes that
-                // its path to the root passes.
-                const int n0 = key0 + KW * kg + 32 * u - ctx;  // the first one's node
-                uint32_t bits = n0 <= -32 ? 0xFFFFFFFFu : n0 < 0 ? (1u << -n0) - 1 : 0u;
-                if (n0 + 32 > 0) {
-                    while (at_node >= n0 + 32) at_node = up[at_node];
-                    while (at_node >= max(n0, 0)) {
-                        bits |= 1u << (at_node - n0);
-                        at_node = up[at_node];
-                    }
-                }
-                bits &= has_row ? svalid[U * kg + u] : 0u;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int k = 8 * (j / 4) + 4 * hf + j % 4;
-                    const bool out = !(bits >> k & 1);
-                    s[u][j] = out ? -INFINITY : s[u][j];
-                    vmax = fmaxf(vmax, out ? 0.0f : svs[KW * kg + 32 * u + k]);
-                }
-            }
-            vmax = max_halves(vmax);
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(top, s[u][j]), s[u][j + 1]);
-        top = max_halves(top);
-        // The reference moves only once a row's scores pass it by kSlack, its units where the
-        // values' size leaves their range.
-        const bool moves = (top - m) * rowf > kSlack;
-        float f = moves ? fast_exp2((m - top) * rowf) : 1.0f;
-        m = moves ? top : m;
-        l *= f;
-        peak *= f;
-        if (__any(vmax > nu * 8.0f || (vmax > 0.0f && vmax <= nu * 0x1p-4f))) {
-            const float now = next_nu(nu, vmax, peak, least);
-            f *= nu / now;
-            unit = __builtin_log2f(kPScale / now);
-            nu = now;
-        }
-        peak = fmaxf(peak, nu);
-        if (__any(f != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) o[i] *= f;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float bias = __builtin_fmaf(-ref, rowf, unit);
-        // m rowf is rounded once here, by less than half while it is below 2^22; past that
-        // the difference is taken first, else the largest weight would be 2 to that error.
-        if (__any(__builtin_fabsf(ref) * rowf > 0x1p22f)) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) s[u][j] -= ref;
-            bias = unit;
-        }
-        float sum = 0.0f;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {  // 16 keys
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    w[j] = fast_exp2(__builtin_fmaf(s[u][8 * g + j], rowf, bias));
-                    sum += w[j];
-                }
-                const float* const vp = svs + KW * kg + 32 * u + 16 * g + 4 * hf;
-                const f4 s0 = *reinterpret_cast<const f4*>(vp), s1 = *reinterpret_cast<const f4*>(vp + 8);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    w[j] *= s0[j];
-                    w[4 + j] *= s1[j];
-                }
-                h8 ph, pl;
-                if constexpr (PSPLIT) split8(w, ph, pl);
-                else ph = round8(w);
-                const int i16 = lane & 15;
-                const _Float16* p =
-                    sv + (KW * kg + 32 * u + 16 * g + 4 * hf + (i16 >> 2)) * VS + 16 * (r32 >> 4) + 4 * (i16 & 3);
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const h8 v = mx::join(read_tr(p + 32 * i), read_tr(p + 32 * i + 8 * VS));
-                    o[i] = mfma32(v, ph, o[i]);
-                    if constexpr (PSPLIT) o[i] = mfma32(v, pl, o[i]);
-                }
-            }
-        l = __builtin_fmaf(sum, nu * (1.0f / kPScale), l);
-    }
-
-    l = sum_halves(l);
-    float f = nu * (1.0f / kPScale), mlog = m * rowf;
-    if constexpr (WK > 1) {
-        // The groups' sums, joined in their order.
-        __syncthreads();
-        float* const so = reinterpret_cast<float*>(lds);
-        constexpr int N = D / 2;  // a lane's sums
-        if (hf == 0) {
-            sm[wave][r32] = mlog;
-            sl[wave][r32] = l;
-            sf[wave][r32] = f;
-        }
-        if (kg > 0) {
-            float* const mine = so + ((kg - 1) * WR + rg) * N * 64 + lane;
-#pragma unroll
-            for (int i = 0; i < N; ++i) mine[64 * i] = o[i / 16][i % 16];
-        }
-        __syncthreads();
-        if (kg > 0) return;
-        float top = mlog;
-#pragma unroll
-        for (int g = 1; g < WK; ++g) top = fmaxf(top, sm[g * WR + rg][r32]);
-        const float safe = top == -INFINITY ? 0.0f : top;
-        const float f0 = fast_exp2(mlog - safe);
-        l *= f0;
-        f *= f0;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] *= f;
-        f = 1.0f;
-#pragma unroll
-        for (int g = 1; g < WK; ++g) {
-            const float e = fast_exp2(sm[g * WR + rg][r32] - safe), w = e * sf[g * WR + rg][r32];
-            l += e * sl[g * WR + rg][r32];
-            const float* const its = so + ((g - 1) * WR + rg) * N * 64 + lane;
-#pragma unroll
-            for (int i = 0; i < N; ++i) o[i / 16][i % 16] += w * its[64 * i];
-        }
-        mlog = top;
-    }
-    if (!has_row) return;
-    const int64_t orow = (int64_t)tok * a.Hq + head, prow = (int64_t)split * a.T * a.Hq + orow;
-    if (nsplit > 1) {
-        if (hf == 0) a.ml[prow] = (f2){mlog, l};
-    } else {
-        f *= spoilt ? __builtin_nanf("") : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const int d = 32 * i + 2 * j + 4 * hf;
-            const f4 v = {o[i][j] * f, o[i][j + 1] * f, o[i][j + 2] * f, o[i][j + 3] * f};
-            if (nsplit > 1) *reinterpret_cast<f4*>(a.part + prow * D + d) = v;
-            else store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
-        }
-}
-
-// The splits of a row joined, in their order: a wave a row.
-template <int D, int DT>
-__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
-    constexpr int L = D / 4, NG = 64 / L;  // lanes a split, splits at a time
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * 4 + wave, n = (int64_t)a.T * a.Hq;
-    if (row >= n) return;
-    const int tok = (int)(row / a.Hq), head = (int)(row - (int64_t)tok * a.Hq);
-    int b = tok;
-    if (a.cu) {
-        int hi = a.B;
-        b = 0;
-        while (hi - b > 1) {
-            const int mid = (b + hi) >> 1;
-            if (a.cu[mid] <= tok) b = mid;
-            else hi = mid;
-        }
-    }
-    const Seq sq = sequence(a, b);
-    const int nsplit = splits_of(a, sq);
-    if (tok < sq.q0 || tok >= sq.q0 + sq.n || nsplit == 1) return;
+    if (rows_of_slot<RT>(a, slot, sq, first) < 0) return;
+    const i2 share = a.shares[blockIdx.x];
+    const int rows = sq.n * a.G, row = first + R * rg + r;
+    if (share[1] <= share[0] || first + R * rg >= rows) return;
+    const auto part_of = [&](int s) { return (int64_t)(2 * s + (s == share[0])); };
+    const auto ml_of = [&](int s) { return a.ml[part_of(s) * RT + R * rg + r]; };
+    const int s0 = share[0] + (FEW ? wave : 0);
     float top = -INFINITY;
-    for (int s = lane; s < nsplit; s += 64) top = fmaxf(top, a.ml[s * n + row].x);
-    top = max_wave(top);
+#pragma unroll 4
+    for (int s = s0; s <= share[1]; s += NG) top = fmaxf(top, ml_of(s).x);
+    if constexpr (FEW) {
+        stop[threadIdx.x] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, stop[64 * i + lane]);
+    }
     const float safe = top == -INFINITY ? 0.0f : top;
     f4 v = {0, 0, 0, 0};
     float sum = 0.0f;
-    const int g = lane / L, d = 4 * (lane % L);
-#pragma unroll 4
-    for (int s = g; s < nsplit; s += NG) {
-        const f2 x = a.ml[s * n + row];
-        const f4 y = *reinterpret_cast<const f4*>(a.part + (s * n + row) * D + d);
-        const bool none = x.y == 0.0f && x.x == -INFINITY;
-        const float f = none ? 0.0f : fast_exp2(x.x - safe);
-        sum += none ? 0.0f : f * x.y;
-        v += none ? (f4){0, 0, 0, 0} : y * f;
+#pragma unroll 8
+    for (int s = s0; s <= share[1]; s += NG) {
+        const f2 x = ml_of(s);
+        const f4 y = reinterpret_cast<const f4*>(a.part + part_of(s) * RT * D)[(rg * N + quad) * 64 + lane];
+        const float f = fast_exp2(x.x - safe);  // a part that saw nothing: zeros times 0
+        sum += f * x.y;
+        v += y * f;
     }
+    if constexpr (FEW) {
+        if (wave > 0) {
+            sv[threadIdx.x - 64] = v;
+            ssum[threadIdx.x - 64] = sum;
+        }
+        __syncthreads();
+        if (wave > 0) return;
 #pragma unroll
-    for (int st = L; st < 64; st *= 2) {
-        sum += __shfl_xor(sum, st);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], st);
+        for (int i = 0; i < 3; ++i) {
+            v += sv[64 * i + lane];
+            sum += ssum[64 * i + lane];
+        }
     }
-    if (g > 0) return;
+    if (row >= rows) return;
     v *= sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-    store4(a.out, DT, tok * a.o_token + head * a.o_head + d, v);
+    const int tok = sq.q0 + row / a.G, head = h * a.G + row % a.G;
+    put4<DT>(a.out, tok * a.o_token + head * a.o_head + R * (quad / NQ) + 8 * (quad % NQ) + 4 * c, v);
 }
 
 // ------------------------------------------------------------------ host
 
 constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer than 2^32
-constexpr size_t kPartMost = (size_t)512 << 20;
-constexpr int kMostSplits = 1 << 16;
 
 struct Plan {
-    int wr, nslots, splits, chunk;
-    size_t part, bytes;
+    int wr, nslots, grid;
+    size_t ml, shares, bytes;  // offsets of the maxima and of the shares, and the whole
 };
 
-// Rows a workgroup by the mean tree; keys a split so that there are a few workgroups
-// for each place on the units while a split has its start's worth of keys.
-Plan plan_tree(int T, int B, int Hq, int H, int D, bool cu, int64_t capacity, int dtype, int n_cu) {
+// Rows a unit by the mean tree; a share for each place on the units, fewer where the
+// table has fewer tiles.
+template <int D, int WR>
+void plan_rows(Plan& p, int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
+    typedef Tiling<D, WR> L;
+    p.nslots = (int)(cu ? (int64_t)T * G / L::RT + B : (int64_t)B * ((G + L::RT - 1) / L::RT));
+    const int64_t tiles = (int64_t)p.nslots * H * std::max<int64_t>(1, (capacity + L::KT - 1) / L::KT);
+    const int64_t room = (int64_t)n_cu * per_unit(D);
+    p.grid = (int)((std::min(room, (tiles + kLeastTiles - 1) / kLeastTiles) + 7) / 8 * 8);
+    p.ml = (size_t)p.grid * 2 * L::RT * D * 4;
+    p.shares = p.ml + (size_t)p.grid * 2 * L::RT * 8;
+    p.bytes = p.shares + (size_t)p.nslots * H * 8;
+}
+
+template <int D>
+Plan plan_tree(int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
+    constexpr int S = D == 256 ? 2 : 1;  // row groups of 32 rows
     Plan p{};
-    const int G = Hq / H;
     const int64_t mean = (((int64_t)T + B - 1) / B) * G;
-    p.wr = mean <= 32 ? 1 : mean <= 64 ? 2 : 4;
-    const int RT = 32 * p.wr, KT = tile_keys(p.wr);
-    p.nslots = (int)(cu ? (int64_t)T * G / RT + B : (int64_t)B * ((G + RT - 1) / RT));
-    const int64_t tiles = (int64_t)B * ((mean + RT - 1) / RT) * H, room = (int64_t)n_cu * per_unit(D, dtype);
-    int64_t splits = std::max<int64_t>(1, (4 * room + tiles - 1) / tiles);
-    int64_t chunk = (capacity + splits - 1) / splits;
-    chunk = std::max<int64_t>(chunk, 128);
-    const int64_t row_bytes = (int64_t)T * Hq * (D * 4 + 8);
-    const int64_t most = std::max<int64_t>(
-        1, std::min<int64_t>({(int64_t)kPartMost / row_bytes, kMostBlocks / ((int64_t)p.nslots * H), (int64_t)kMostSplits}));
-    chunk = std::max(chunk, (capacity + most - 1) / most);
-    chunk = (chunk + KT - 1) / KT * KT;
-    p.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
-    p.splits = (int)std::max<int64_t>(1, (capacity + p.chunk - 1) / p.chunk);
-    if (p.splits > 1) {
-        p.part = (size_t)p.splits * T * Hq * D * 4;
-        p.bytes = p.part + (size_t)p.splits * T * Hq * 8;
-    }
+    p.wr = mean <= 32 ? S : mean <= 64 ? 2 * S : 4 * S;
+    if (p.wr == S) plan_rows<D, S>(p, T, B, H, G, cu, capacity, n_cu);
+    else if (p.wr == 2 * S) plan_rows<D, 2 * S>(p, T, B, H, G, cu, capacity, n_cu);
+    else plan_rows<D, 4 * S>(p, T, B, H, G, cu, capacity, n_cu);
     return p;
+}
+
+Plan plan_of(int T, int B, int heads, int H, int D, bool cu, int64_t capacity, int n_cu) {
+    const int G = heads / H;
+    return D == 64    ? plan_tree<64>(T, B, H, G, cu, capacity, n_cu)
+           : D == 128 ? plan_tree<128>(T, B, H, G, cu, capacity, n_cu)
+                      : plan_tree<256>(T, B, H, G, cu, capacity, n_cu);
 }
 
 int cu_count() {
@@ -523,13 +768,23 @@ int cu_count() {
     return n[dev];
 }
 
+template <int D, int KIND, int DT, int WR>
+void launch4(const TreeArgs& a, hipStream_t st) {
+    typedef Tiling<D, WR> L;
+    tree_keys_kernel<D, KIND, DT, WR><<<(unsigned)a.grid, 64 * L::W, 0, st>>>(a);
+    // At one tile a sequence nothing is cut.
+    if (((int64_t)a.table_w << a.pshift) <= L::KT) return;
+    const unsigned units = (unsigned)a.nslots * a.H, items = WR * D / 4 * L::R / 64;
+    if (units <= 32) tree_join_kernel<D, DT, WR, true><<<dim3(units, items), 256, 0, st>>>(a);
+    else tree_join_kernel<D, DT, WR, false><<<dim3(units, items / 4), 256, 0, st>>>(a);
+}
+
 template <int D, int KIND, int DT>
 void launch3(const TreeArgs& a, const Plan& p, hipStream_t st) {
-    const unsigned blocks = (unsigned)((int64_t)a.nslots * a.H * a.splits);
-    if (p.wr == 1) tree_keys_kernel<D, KIND, DT, 1><<<blocks, 256, 0, st>>>(a);
-    else if (p.wr == 2) tree_keys_kernel<D, KIND, DT, 2><<<blocks, 256, 0, st>>>(a);
-    else tree_keys_kernel<D, KIND, DT, 4><<<blocks, 256, 0, st>>>(a);
-    if (a.splits > 1) tree_join_kernel<D, DT><<<(unsigned)(((int64_t)a.T * a.Hq + 3) / 4), 256, 0, st>>>(a);
+    constexpr int S = D == 256 ? 2 : 1;
+    if (p.wr == S) launch4<D, KIND, DT, S>(a, st);
+    else if (p.wr == 2 * S) launch4<D, KIND, DT, 2 * S>(a, st);
+    else launch4<D, KIND, DT, 4 * S>(a, st);
 }
 
 template <int D, int KIND>
@@ -594,7 +849,7 @@ int64_t i4_tree_attention_workspace(int kv_heads, int page_size, int head_dim, i
     int ps = 0;
     if (!check_shape(&c, T, B, heads, table_w, has_cu != 0, &ps)) return -2;
     if (T == 0 || B == 0) return 0;
-    return (int64_t)plan_tree(T, B, heads, kv_heads, head_dim, has_cu != 0, (int64_t)table_w << ps, dtype, cu_count()).bytes;
+    return (int64_t)plan_of(T, B, heads, kv_heads, head_dim, has_cu != 0, (int64_t)table_w << ps, cu_count()).bytes;
 }
 
 int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
@@ -638,16 +893,16 @@ int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_to
     a.P = cache->num_pages;
     a.pshift = ps;
     a.scale = scale * kLog2e;
-    const Plan p = plan_tree(T, B, heads, a.H, cache->head_dim, dCu != nullptr, (int64_t)table_w << ps, dtype, cu_count());
+    const Plan p = plan_of(T, B, heads, a.H, cache->head_dim, dCu != nullptr, (int64_t)table_w << ps, cu_count());
     if (p.bytes > 0 && (!dWork || work_bytes < (int64_t)p.bytes)) {
         bq_set_error("tree_attention: needs a workspace of %zu bytes, got %lld", p.bytes, (long long)work_bytes);
         return -4;
     }
     a.nslots = p.nslots;
-    a.splits = p.splits;
-    a.chunk = p.chunk;
+    a.grid = p.grid;
     a.part = static_cast<float*>(dWork);
-    a.ml = reinterpret_cast<f2*>(static_cast<uint8_t*>(dWork) + p.part);
+    a.ml = reinterpret_cast<f2*>(static_cast<uint8_t*>(dWork) + p.ml);
+    a.shares = reinterpret_cast<i2*>(static_cast<uint8_t*>(dWork) + p.shares);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     if (cache->head_dim == 64) launch1<64>(a, p, cache->kind, dtype, st);
