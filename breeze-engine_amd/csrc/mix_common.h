@@ -130,17 +130,18 @@ __device__ inline float sum_rows16(float x) {
     return bits_f(r[0]) + bits_f(r[1]);
 }
 
-// The max over a wave, in all lanes.
-__device__ inline float max_wave(float x) {
+// The max over 16 neighbouring lanes, in all of them.
+__device__ inline float max_16(float x) {
     const auto turned = [](float v, auto n) {
         return bits_f((uint32_t)__builtin_amdgcn_mov_dpp((int)f_bits(v), 0x120 + decltype(n)::value, 0xF, 0xF, true));
     };
     x = fmaxf(x, turned(x, std::integral_constant<int, 1>()));  // row_ror:1, 2, 4, 8 within 16 lanes
     x = fmaxf(x, turned(x, std::integral_constant<int, 2>()));
     x = fmaxf(x, turned(x, std::integral_constant<int, 4>()));
-    x = fmaxf(x, turned(x, std::integral_constant<int, 8>()));
-    return max_halves(max_rows16(x));
+    return fmaxf(x, turned(x, std::integral_constant<int, 8>()));
 }
+// The max over a wave, in all lanes.
+__device__ inline float max_wave(float x) { return max_halves(max_rows16(max_16(x))); }
 
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

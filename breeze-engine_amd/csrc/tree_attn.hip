@@ -74,10 +74,25 @@ __device__ inline Seq sequence(const TreeArgs& a, int b) {
     return s;
 }
 
-// A value that all lanes have alike, as the scalar unit's.
-__device__ inline int64_t uniform(int64_t x) {
-    const int lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+// Lane `who`'s value, as the scalar unit's.
+__device__ inline int64_t lane_of(int64_t x, int who) {
+    const int lo = __builtin_amdgcn_readlane((int)x, who), hi = __builtin_amdgcn_readlane((int)(x >> 32), who);
     return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+// The sum over a wave's lanes up to this one.
+__device__ inline int64_t scan_wave(int64_t x) {
+    const auto step = [&](auto control, auto rows) {  // adds the lane's below, or a row's last one's; 0 where there is none
+        const int lo = __builtin_amdgcn_update_dpp(0, (int)x, decltype(control)::value, decltype(rows)::value, 0xF, true);
+        const int hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), decltype(control)::value, decltype(rows)::value, 0xF, true);
+        x += (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+    };
+    step(std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xF>());  // row_shr:1, 2, 4, 8 within 16 lanes
+    step(std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xF>());
+    step(std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xF>());
+    step(std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xF>());
+    step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xA>());  // row_bcast:15 to rows 1 and 3
+    step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xC>());  // row_bcast:31 to rows 2 and 3
+    return x;
 }
 
 // x / y of whole numbers up to 2^53: the fp64 quotient is rounded to a whole number
@@ -175,14 +190,28 @@ struct RawQueries {
 
 // How a kernel's waves share out rows and keys: W waves, WR of them along the rows,
 // RT rows a unit, W / WR along a tile's keys, KT keys a tile, 32 or more a wave.
+// Where eight waves make a workgroup it has a compute unit to itself and two tiles in
+// LDS: one barrier a tile, and one tile is unpacked while the other is computed.
+template <int D>
+constexpr int rows_a_wave() { return D == 256 ? 16 : 32; }
 template <int D, int WR>
 struct Tiling {
-    static constexpr int R = D == 256 ? 16 : 32, W = D == 256 ? 8 : 4, WK = W / WR, RT = R * WR;
+    static constexpr int R = rows_a_wave<D>(), RT = R * WR;
+    static constexpr bool kTwo = false;  // tiles in LDS
+    static constexpr int W = R == 16 ? 8 : 4, WK = W / WR;
     static constexpr int KT = WK == 4 ? 128 : 64, KW = KT / WK;
     static constexpr int KS = D + 8, VS = D + 16;  // LDS rows of a key and of its values: reads of one instruction fall on unlike banks
+    static constexpr int kUnit = D == 256 ? 1 : 2;   // workgroups a compute unit
 };
-// Workgroups a compute unit.
-constexpr int per_unit(int D) { return D == 256 ? 1 : 2; }
+
+// The order of a stretch of code: `n` instructions of a kind next.  Left to itself the
+// compiler reads each operand from LDS right before its matrix instruction, and
+// every one waits out the read.
+template <int KIND, int N>
+__device__ __forceinline__ void next_are() {
+    if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(KIND, N, 0);
+}
+constexpr int kValu = 2, kMatrix = 8, kLdsRead = 0x100;
 
 constexpr int kLeastTiles = 2;  // a share's: less is not worth a workgroup's start
 
@@ -210,13 +239,8 @@ __device__ inline Share share_of(const TreeArgs& a, int id) {
             n[j] = (int64_t)((uint32_t)(s[j].n * a.G + RT - 1) / RT * a.H) * tiles;
             mine += n[j];
         }
-        upto = mine;
-#pragma unroll
-        for (int st = 1; st < 64; st *= 2) {
-            const int64_t y = __shfl_up(upto, st);
-            if (lane >= st) upto += y;
-        }
-        all = uniform(__shfl(upto, 63));
+        upto = scan_wave(mine);
+        all = lane_of(upto, 63);
         upto -= mine;  // before this lane's
     };
     Share w;
@@ -251,7 +275,7 @@ __device__ inline Share share_of(const TreeArgs& a, int id) {
                 upto += n[j];
             }
             const int who = __builtin_ctzll(__ballot(is));
-            w.base = uniform(__shfl(first, who));
+            w.base = lane_of(first, who);
             w.b = __builtin_amdgcn_readlane(b, who);
             w.sq = {__builtin_amdgcn_readlane(q0, who), __builtin_amdgcn_readlane(rows, who), __builtin_amdgcn_readlane(kv, who)};
             return w;
@@ -260,7 +284,7 @@ __device__ inline Share share_of(const TreeArgs& a, int id) {
 }
 
 template <int D, int KIND, int DT, int WR>
-__global__ __launch_bounds__((64 * Tiling<D, WR>::W), (per_unit(D) * Tiling<D, WR>::W / 4)) void tree_keys_kernel(TreeArgs a) {
+__global__ __launch_bounds__((64 * Tiling<D, WR>::W), (Tiling<D, WR>::kUnit * Tiling<D, WR>::W / 4)) void tree_keys_kernel(TreeArgs a) {
     typedef Tiling<D, WR> T;
     constexpr bool SPLIT = DT == kF32, PSPLIT = DT != kBF16;  // two terms of the queries, and of the weights
     constexpr int R = T::R, W = T::W, WK = T::WK, RT = T::RT, KT = T::KT, KW = T::KW, KS = T::KS, VS = T::VS;
@@ -270,14 +294,14 @@ __global__ __launch_bounds__((64 * Tiling<D, WR>::W), (per_unit(D) * Tiling<D, W
     constexpr int per_row = D / 16;
     constexpr int SL = D / Shape<R>::kSlab, NA = D / R, NQ = Shape<R>::kQuads, QS = Shape<R>::kStep;
     constexpr int J = R / 2;                        // scores a lane has of 32 keys
-    constexpr int kBytes = std::max(KT * (KS + VS) * 2, (WK - 1) * WR * R * D * 4);
+    constexpr int NB = T::kTwo ? 2 : 1;
+    constexpr int kTile = KT * (KS + VS) * 2, kBytes = std::max(NB * kTile, (WK - 1) * WR * R * D * 4);
     typedef typename Shape<R>::Acc Acc;
     __shared__ __align__(16) uint8_t lds[kBytes];
-    __shared__ __align__(16) float sks[KT], svs[KT];
-    __shared__ float smax[KT / 32], sm[W][R], sl[W][R], sf[W][R];
-    __shared__ uint32_t svalid[KT / 32];
+    __shared__ __align__(16) float sks_[NB][KT], svs_[NB][KT];
+    __shared__ float smax_[NB][KT / 32], sm[W][R], sl[W][R], sf[W][R];
+    __shared__ uint32_t svalid_[NB][KT / 32];
     __shared__ int16_t up[kTreeNodes];
-    _Float16 *const sk = reinterpret_cast<_Float16*>(lds), *const sv = sk + KT * KS;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & (R - 1), c = lane / R, rg = wave % WR, kg = wave / WR, r16 = lane & 15;
@@ -300,43 +324,44 @@ __global__ __launch_bounds__((64 * Tiling<D, WR>::W), (per_unit(D) * Tiling<D, W
         const int32_t* const table = a.table + w.b * a.table_row;
         int t = spoilt || sq.kv == 0 ? t0 - 1 : t1 - 1;
 
-        // The pages of a tile's groups of 16 keys, one a lane; -1 where the sequence has no
-        // key or the cache no such page.
+        // The pages of a tile's groups of 16 keys, one a lane, as the table has them: nothing
+        // waits for them here.
         const auto pages_of = [&](int tile) {
-            const int key = KT * tile + 16 * (lane & (NG - 1));
-            int page = -1;
-            if (tile >= t0 && key < sq.kv) page = table[key >> a.pshift];
-            return page < a.P ? page : -1;
+            return table[min(max(KT * tile + 16 * (lane / (64 / NG)), 0), sq.kv - 1) >> a.pshift];
         };
-        int pages = pages_of(t), pages_now = pages;
+        int pages = 0, pages_in = 0;  // of the tile that is loaded next, of the one in registers
+        if (t >= t0) pages = pages_of(t);
         RawQueries<D, DT, R> raw;
+        const bool wave_rows = first + R * rg < rows;
         raw.load(a.q, tok * a.q_token + head * a.q_head + 8 * c);
 
         u4 kraw[NC], vraw[NC];
         float ksc = 0.0f, vsc = 0.0f;
         bool sc_bad = true;
-        const auto load = [&](int tile, int pages) {
+        const auto load = [&](int tile) {
+            // -1 where the sequence has no key or the cache no such page.
+            pages_in = KT * tile + 16 * (lane / (64 / NG)) < sq.kv && (uint32_t)pages < (uint32_t)a.P ? pages : -1;
             const auto row_of = [&](int page, int key) {  // cache row of a group's first key
                 return (((int64_t)max(page, 0) * a.H + h) << a.pshift) + (key & ((1 << a.pshift) - 1));
             };
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 const int g = (wave * 64 + THREADS * i) / per_row >> 4;  // the wave's group of this pass
-                const int64_t at = row_of(__builtin_amdgcn_readlane(pages, g), KT * tile + 16 * g) +
+                const int64_t at = row_of(__builtin_amdgcn_readlane(pages_in, 64 / NG * g), KT * tile + 16 * g) +
                                    ((tid + THREADS * i) / per_row & 15);
                 kraw[i] = *reinterpret_cast<const u4*>(a.kp + at * D + 16 * (tid % per_row));
                 vraw[i] = *reinterpret_cast<const u4*>(a.vp + at * D + 16 * (tid % per_row));
             }
             if (tid < KT) {
-                const int page = __shfl(pages, tid >> 4 & (NG - 1));
+                const int page = KT == 64 ? pages_in : __shfl(pages_in, 64 / NG * (tid >> 4));
                 sc_bad = page < 0 || KT * tile + tid >= sq.kv;
                 const int64_t at = row_of(page, KT * tile + (tid & ~15)) + (tid & 15);
                 ksc = a.ks[at];
                 vsc = a.vs[at];
             }
+            pages = pages_of(tile - 1);
         };
-        if (t >= t0) load(t, pages);
-        pages = pages_of(t - 1);
+        if (t >= t0) load(t);
         if (t0 == 0 && tid == 0) {
             const int slot = (a.cu ? (int)((int64_t)sq.q0 * a.G / RT) + w.b : w.b * nrow) + first / RT;
             a.shares[(int64_t)slot * a.H + h] = (i2){id, (int)over(began + ntile - 1, w.per)};
@@ -361,98 +386,109 @@ __global__ __launch_bounds__((64 * Tiling<D, WR>::W), (per_unit(D) * Tiling<D, W
         constexpr float least = 0x1p-110f;
         float m = -INFINITY, l = 0.0f, nu = least, peak = 0.0f, unit = __builtin_log2f(kPScale / least);
         int at_node = has_row ? node : -1;  // the next of the row's node and its ancestors
-        const bool wave_rows = first + R * rg < rows;
 
-        for (; t >= t0; --t) {
-            const int key0 = KT * t;
-            __syncthreads();  // the last tile's reads are over
+        // The tile in registers to LDS.
+        const auto unpack = [&](int tile, int buf) {
+            const int key0 = KT * tile;
+            _Float16 *const sk = reinterpret_cast<_Float16*>(lds + buf * kTile), *const sv = sk + KT * KS;
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 const int kr = (tid + THREADS * i) / per_row, col = 16 * (tid % per_row);
                 u4 kw = kraw[i], vw = vraw[i];
                 if constexpr (KIND == kFp8) {  // bytes of rows that no key is in may be NaN
-                    const int page = __builtin_amdgcn_readlane(pages_now, (wave * 64 + THREADS * i) / per_row >> 4);
+                    const int page = __builtin_amdgcn_readlane(pages_in, 64 / NG * ((wave * 64 + THREADS * i) / per_row >> 4));
                     if (page < 0 || key0 + kr >= sq.kv) kw = vw = (u4){0, 0, 0, 0};
                 }
                 h8* kd = reinterpret_cast<h8*>(sk + kr * KS + col);
                 h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
-                kd[0] = unpack8<KIND>(kw.x, kw.y);
-                kd[1] = unpack8<KIND>(kw.z, kw.w);
-                vd[0] = unpack8<KIND>(vw.x, vw.y);
-                vd[1] = unpack8<KIND>(vw.z, vw.w);
+                // Eight lanes of sixteen write their second half first: all at once they fall on unlike banks.
+                const int one = lane >> 3 & 1;
+                kd[one] = unpack8<KIND>(one ? kw.z : kw.x, one ? kw.w : kw.y);
+                kd[1 - one] = unpack8<KIND>(one ? kw.x : kw.z, one ? kw.y : kw.w);
+                vd[one] = unpack8<KIND>(one ? vw.z : vw.x, one ? vw.w : vw.y);
+                vd[1 - one] = unpack8<KIND>(one ? vw.x : vw.z, one ? vw.y : vw.w);
             }
             if (tid < KT) {
                 // A value scale of NaN goes with the key's, whose score a row that does
                 // not see the key leaves out; times a probability of zero it would not.
                 const bool nan = vsc != vsc;
                 const float v = sc_bad || nan ? 0.0f : vsc;
-                sks[tid] = sc_bad ? 0.0f : nan ? vsc : ksc;
-                svs[tid] = v;
-                float vmax = v;
-#pragma unroll
-                for (int st = 1; st < 32; st *= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, st));
+                sks_[buf][tid] = sc_bad ? 0.0f : nan ? vsc : ksc;
+                svs_[buf][tid] = v;
+                const float vmax = max_rows16(max_16(v));  // of 32 keys
                 const uint64_t valid = __ballot(!sc_bad);
                 if ((lane & 31) == 0) {
-                    smax[tid >> 5] = vmax;
-                    svalid[tid >> 5] = (uint32_t)(valid >> (lane & 32));
+                    smax_[buf][tid >> 5] = vmax;
+                    svalid_[buf][tid >> 5] = (uint32_t)(valid >> (lane & 32));
                 }
             }
-            __syncthreads();
-            pages_now = pages;
-            if (t > t0) load(t - 1, pages);
-            pages = pages_of(t - 2);
+        };
+        if constexpr (NB == 2) {
+            if (t >= t0) unpack(t, 0);
+            if (t > t0) load(t - 1);
+        }
+        for (int buf = 0; t >= t0; --t, buf ^= NB - 1) {
+            const int key0 = KT * t;
+            __syncthreads();  // NB 1: the last tile's reads are over; 2: this tile is there as well
+            if constexpr (NB == 2) {
+                if (t > t0) unpack(t - 1, buf ^ 1);
+                if (t - 1 > t0) load(t - 2);
+            } else {
+                unpack(t, 0);
+                __syncthreads();
+                if (t > t0) load(t - 1);
+            }
             if (!wave_rows) continue;
+            const _Float16 *const sk = reinterpret_cast<const _Float16*>(lds + buf * kTile), *const sv = sk + KT * KS;
+            const float *const sks = sks_[buf], *const svs = svs_[buf], *const smax = smax_[buf];
+            const uint32_t* const svalid = svalid_[buf];
 
             // Scores: a lane's j-th of a block of 32 keys is key QS (j / 4) + 4 c + j % 4.
+            constexpr int KB = KW / R, NK = SL * KB, TERMS = SPLIT ? 2 : 1;  // blocks of R keys, operands of K
             float x[U][J];
-            if constexpr (R == 32) {
-                f16 s[U];
+            {
+                Acc s[KB];
+                h8 k[NK];
+#pragma unroll
+                for (int n = 0; n < NK; ++n)
+                    k[n] = *reinterpret_cast<const h8*>(sk + (KW * kg + R * (n % KB) + r) * KS + 8 * c + Shape<R>::kSlab * (n / KB));
+                f4 sc[U * J / 4];
+#pragma unroll
+                for (int n = 0; n < U * J / 4; ++n)
+                    sc[n] = *reinterpret_cast<const f4*>(sks + KW * kg + 32 * (n / (J / 4)) + QS * (n % (J / 4)) + 4 * c);
+#pragma unroll
+                for (int v = 0; v < KB; ++v)
+#pragma unroll
+                    for (int j = 0; j < 4 * NQ; ++j) s[v][j] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    s[n % KB] = Shape<R>::mfma(k[n], qh[n / KB], s[n % KB]);
+                    if constexpr (SPLIT) s[n % KB] = Shape<R>::mfma(k[n], ql[n / KB], s[n % KB]);
+                }
+                // Times the key scales.
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
+                    for (int j = 0; j < J; ++j) x[u][j] = s[(J * u + j) / (4 * NQ)][j % (4 * NQ)] * sc[(J * u + j) / 4][j % 4];
+                constexpr int AHEAD = 6, NS = U * J / 4;
+                next_are<kLdsRead, AHEAD>();
 #pragma unroll
-                for (int i = 0; i < SL; ++i)
+                for (int n = 0; n < NK - AHEAD; ++n) {
+                    next_are<kMatrix, TERMS>();
+                    next_are<kLdsRead, 1>();
+                }
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const h8 k = *reinterpret_cast<const h8*>(sk + (KW * kg + 32 * u + r) * KS + 8 * c + 16 * i);
-                        s[u] = mfma32(k, qh[i], s[u]);
-                        if constexpr (SPLIT) s[u] = mfma32(k, ql[i], s[u]);
-                    }
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) x[u][j] = s[u][j];
-            } else {
-                f4 s[2 * U];
-#pragma unroll
-                for (int v = 0; v < 2 * U; ++v) s[v] = (f4){0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < SL; ++i)
-#pragma unroll
-                    for (int v = 0; v < 2 * U; ++v) {
-                        const h8 k = *reinterpret_cast<const h8*>(sk + (KW * kg + 16 * v + r) * KS + 8 * c + 32 * i);
-                        s[v] = Shape<16>::mfma(k, qh[i], s[v]);
-                        if constexpr (SPLIT) s[v] = Shape<16>::mfma(k, ql[i], s[v]);
-                    }
-#pragma unroll
-                for (int v = 0; v < 2 * U; ++v)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[v / 2][4 * (v % 2) + j] = s[v][j];
+                for (int n = 0; n < AHEAD; ++n) {
+                    next_are<kMatrix, TERMS>();
+                    next_are<kLdsRead, (NS + AHEAD - 1) / AHEAD>();
+                }
             }
-            // Times the key scales.
             float vmax = 0.0f;
             bool all = key0 + KT <= ctx;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 vmax = fmaxf(vmax, smax[U * kg + u]);
                 all = all && svalid[U * kg + u] == 0xFFFFFFFFu;
-#pragma unroll
-                for (int j = 0; j < J; j += 4) {
-                    const f4 sc = *reinterpret_cast<const f4*>(sks + KW * kg + 32 * u + QS * (j / 4) + 4 * c);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][j + e] *= sc[e];
-                }
             }
             if (!all) {
                 vmax = 0.0f;
@@ -519,34 +555,49 @@ __global__ __launch_bounds__((64 * Tiling<D, WR>::W), (per_unit(D) * Tiling<D, W
                 bias = unit;
             }
             float sum = 0.0f;
+            // Eight of a lane's scores make an operand of the weights, for a group of 512 / R keys.
+            constexpr int GS = U * J / 8, NV = GS * NA;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int g = 0; g < GS; ++g) {
+                const int k0 = KW * kg + (512 / R) * g + 4 * c;  // of the first quad; the second QS on
+                const f4 s0 = *reinterpret_cast<const f4*>(svs + k0), s1 = *reinterpret_cast<const f4*>(svs + k0 + QS);
+                const _Float16* p = sv + (k0 + (r16 >> 2)) * VS + 16 * (r >> 4) + 4 * (r16 & 3);
+                h8 v[NA];
 #pragma unroll
-                for (int g = 0; g < J / 8; ++g) {  // eight of a lane's scores make an operand
-                    float y[8];
+                for (int i = 0; i < NA; ++i) v[i] = mx::join(read_tr(p + R * i), read_tr(p + R * i + QS * VS));
+                float y[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        y[j] = fast_exp2(__builtin_fmaf(x[u][8 * g + j], rowf, bias));
-                        sum += y[j];
-                    }
-                    const int k0 = KW * kg + 32 * u + 16 * g + 4 * c;  // of the first quad; the second QS on
-                    const f4 s0 = *reinterpret_cast<const f4*>(svs + k0), s1 = *reinterpret_cast<const f4*>(svs + k0 + QS);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        y[j] *= s0[j];
-                        y[4 + j] *= s1[j];
-                    }
-                    h8 ph, pl;
-                    if constexpr (PSPLIT) split8(y, ph, pl);
-                    else ph = round8(y);
-                    const _Float16* p = sv + (k0 + (r16 >> 2)) * VS + 16 * (r >> 4) + 4 * (r16 & 3);
-#pragma unroll
-                    for (int i = 0; i < NA; ++i) {
-                        const h8 v = mx::join(read_tr(p + R * i), read_tr(p + R * i + QS * VS));
-                        o[i] = Shape<R>::mfma(v, ph, o[i]);
-                        if constexpr (PSPLIT) o[i] = Shape<R>::mfma(v, pl, o[i]);
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    y[j] = fast_exp2(__builtin_fmaf(x[8 * g / J][8 * g % J + j], rowf, bias));
+                    sum += y[j];
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] *= s0[j];
+                    y[4 + j] *= s1[j];
+                }
+                h8 ph, pl;
+                if constexpr (PSPLIT) split8(y, ph, pl);
+                else ph = round8(y);
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    o[i] = Shape<R>::mfma(v[i], ph, o[i]);
+                    if constexpr (PSPLIT) o[i] = Shape<R>::mfma(v[i], pl, o[i]);
+                }
+            }
+            {
+                // The values' operands some instructions ahead; a group's weights beside the matrix
+                // instructions of the one before.
+                constexpr int AHEAD = 4, VALU = PSPLIT ? 60 : 40, PT = PSPLIT ? 2 : 1;
+                next_are<kLdsRead, 2 * AHEAD + 2>();
+                next_are<kValu, VALU>();
+#pragma unroll
+                for (int n = 0; n < NV; ++n) {
+                    next_are<kMatrix, PT>();
+                    next_are<kLdsRead, 2>();
+                    next_are<kValu, (VALU + NA - 1) / NA>();
+                }
+            }
             l = __builtin_fmaf(sum, nu * (1.0f / kPScale), l);
         }
 
@@ -731,7 +782,7 @@ void plan_rows(Plan& p, int T, int B, int H, int G, bool cu, int64_t capacity, i
     typedef Tiling<D, WR> L;
     p.nslots = (int)(cu ? (int64_t)T * G / L::RT + B : (int64_t)B * ((G + L::RT - 1) / L::RT));
     const int64_t tiles = (int64_t)p.nslots * H * std::max<int64_t>(1, (capacity + L::KT - 1) / L::KT);
-    const int64_t room = (int64_t)n_cu * per_unit(D);
+    const int64_t room = (int64_t)n_cu * L::kUnit;
     p.grid = (int)((std::min(room, (tiles + kLeastTiles - 1) / kLeastTiles) + 7) / 8 * 8);
     p.ml = (size_t)p.grid * 2 * L::RT * D * 4;
     p.shares = p.ml + (size_t)p.grid * 2 * L::RT * 8;
@@ -740,7 +791,7 @@ void plan_rows(Plan& p, int T, int B, int H, int G, bool cu, int64_t capacity, i
 
 template <int D>
 Plan plan_tree(int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
-    constexpr int S = D == 256 ? 2 : 1;  // row groups of 32 rows
+    constexpr int S = 32 / rows_a_wave<D>();
     Plan p{};
     const int64_t mean = (((int64_t)T + B - 1) / B) * G;
     p.wr = mean <= 32 ? S : mean <= 64 ? 2 * S : 4 * S;
@@ -781,7 +832,7 @@ void launch4(const TreeArgs& a, hipStream_t st) {
 
 template <int D, int KIND, int DT>
 void launch3(const TreeArgs& a, const Plan& p, hipStream_t st) {
-    constexpr int S = D == 256 ? 2 : 1;
+    constexpr int S = 32 / rows_a_wave<D>();
     if (p.wr == S) launch4<D, KIND, DT, S>(a, st);
     else if (p.wr == 2 * S) launch4<D, KIND, DT, 2 * S>(a, st);
     else launch4<D, KIND, DT, 4 * S>(a, st);
