@@ -188,20 +188,18 @@ struct RawQueries {
     }
 };
 
-// How a kernel's waves share out rows and keys: W waves, WR of them along the rows,
-// RT rows a unit, W / WR along a tile's keys, KT keys a tile, 32 or more a wave.
-// Where eight waves make a workgroup it has a compute unit to itself and two tiles in
-// LDS: one barrier a tile, and one tile is unpacked while the other is computed.
-template <int D>
-constexpr int rows_a_wave() { return D == 256 ? 16 : 32; }
-template <int D, int WR>
+// How a workgroup of W waves takes a unit of RT rows: R rows a wave, W / (RT / R) waves
+// along the KT keys of a tile; kUnit workgroups a compute unit.  Heads of 256: a wave's
+// sums of 32 rows would leave no registers for a second wave.  Up to 32 rows
+// HBM bounds it: many small workgroups, whose loads are on their way at once.
+template <int D, int RT>
 struct Tiling {
-    static constexpr int R = rows_a_wave<D>(), RT = R * WR;
-    static constexpr bool kTwo = false;  // tiles in LDS
-    static constexpr int W = R == 16 ? 8 : 4, WK = W / WR;
-    static constexpr int KT = WK == 4 ? 128 : 64, KW = KT / WK;
+    static constexpr int R = D == 256 || RT == 32 ? 16 : 32, WR = RT / R;
+    static constexpr int W = D == 256 && RT > 32 ? 8 : 4, WK = W / WR;
+    static constexpr int KT = 64, KW = KT / WK;
     static constexpr int KS = D + 8, VS = D + 16;  // LDS rows of a key and of its values: reads of one instruction fall on unlike banks
-    static constexpr int kUnit = D == 256 ? 1 : 2;   // workgroups a compute unit
+    static constexpr int kUnit = W == 8 ? 1 : D == 256 || RT > 32 ? 2 : 3;
+    static_assert(KW >= 32, "a wave takes blocks of 32 keys");
 };
 
 // The order of a stretch of code: `n` instructions of a kind next.  Left to itself the
@@ -283,25 +281,25 @@ __device__ inline Share share_of(const TreeArgs& a, int id) {
     }
 }
 
-template <int D, int KIND, int DT, int WR>
-__global__ __launch_bounds__((64 * Tiling<D, WR>::W), (Tiling<D, WR>::kUnit * Tiling<D, WR>::W / 4)) void tree_keys_kernel(TreeArgs a) {
-    typedef Tiling<D, WR> T;
+template <int D, int KIND, int DT, int RT>
+__global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Tiling<D, RT>::W / 4)) void tree_keys_kernel(TreeArgs a) {
+    typedef Tiling<D, RT> T;
     constexpr bool SPLIT = DT == kF32, PSPLIT = DT != kBF16;  // two terms of the queries, and of the weights
-    constexpr int R = T::R, W = T::W, WK = T::WK, RT = T::RT, KT = T::KT, KW = T::KW, KS = T::KS, VS = T::VS;
+    constexpr int R = T::R, W = T::W, WR = T::WR, WK = T::WK, KT = T::KT, KW = T::KW, KS = T::KS, VS = T::VS;
     constexpr int THREADS = 64 * W, U = KW / 32;    // blocks of 32 keys a wave
     constexpr int NC = KT * D / (16 * THREADS);     // 16-byte chunks a thread loads of a tile's keys (and of its values)
     constexpr int NG = KT / 16;                     // groups of 16 keys, each in one page
     constexpr int per_row = D / 16;
     constexpr int SL = D / Shape<R>::kSlab, NA = D / R, NQ = Shape<R>::kQuads, QS = Shape<R>::kStep;
     constexpr int J = R / 2;                        // scores a lane has of 32 keys
-    constexpr int NB = T::kTwo ? 2 : 1;
-    constexpr int kTile = KT * (KS + VS) * 2, kBytes = std::max(NB * kTile, (WK - 1) * WR * R * D * 4);
+    constexpr int kBytes = std::max(KT * (KS + VS) * 2, (WK - 1) * RT * D * 4);
     typedef typename Shape<R>::Acc Acc;
     __shared__ __align__(16) uint8_t lds[kBytes];
-    __shared__ __align__(16) float sks_[NB][KT], svs_[NB][KT];
-    __shared__ float smax_[NB][KT / 32], sm[W][R], sl[W][R], sf[W][R];
-    __shared__ uint32_t svalid_[NB][KT / 32];
+    __shared__ __align__(16) float sks[KT], svs[KT];
+    __shared__ float smax[KT / 32], sm[W][R], sl[W][R], sf[W][R];
+    __shared__ uint32_t svalid[KT / 32];
     __shared__ int16_t up[kTreeNodes];
+    _Float16 *const sk = reinterpret_cast<_Float16*>(lds), *const sv = sk + KT * KS;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & (R - 1), c = lane / R, rg = wave % WR, kg = wave / WR, r16 = lane & 15;
@@ -388,9 +386,7 @@ __global__ __launch_bounds__((64 * Tiling<D, WR>::W), (Tiling<D, WR>::kUnit * Ti
         int at_node = has_row ? node : -1;  // the next of the row's node and its ancestors
 
         // The tile in registers to LDS.
-        const auto unpack = [&](int tile, int buf) {
-            const int key0 = KT * tile;
-            _Float16 *const sk = reinterpret_cast<_Float16*>(lds + buf * kTile), *const sv = sk + KT * KS;
+        const auto unpack = [&](int key0) {
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 const int kr = (tid + THREADS * i) / per_row, col = 16 * (tid % per_row);
@@ -413,35 +409,23 @@ __global__ __launch_bounds__((64 * Tiling<D, WR>::W), (Tiling<D, WR>::kUnit * Ti
                 // not see the key leaves out; times a probability of zero it would not.
                 const bool nan = vsc != vsc;
                 const float v = sc_bad || nan ? 0.0f : vsc;
-                sks_[buf][tid] = sc_bad ? 0.0f : nan ? vsc : ksc;
-                svs_[buf][tid] = v;
+                sks[tid] = sc_bad ? 0.0f : nan ? vsc : ksc;
+                svs[tid] = v;
                 const float vmax = max_rows16(max_16(v));  // of 32 keys
                 const uint64_t valid = __ballot(!sc_bad);
                 if ((lane & 31) == 0) {
-                    smax_[buf][tid >> 5] = vmax;
-                    svalid_[buf][tid >> 5] = (uint32_t)(valid >> (lane & 32));
+                    smax[tid >> 5] = vmax;
+                    svalid[tid >> 5] = (uint32_t)(valid >> (lane & 32));
                 }
             }
         };
-        if constexpr (NB == 2) {
-            if (t >= t0) unpack(t, 0);
-            if (t > t0) load(t - 1);
-        }
-        for (int buf = 0; t >= t0; --t, buf ^= NB - 1) {
+        for (; t >= t0; --t) {
             const int key0 = KT * t;
-            __syncthreads();  // NB 1: the last tile's reads are over; 2: this tile is there as well
-            if constexpr (NB == 2) {
-                if (t > t0) unpack(t - 1, buf ^ 1);
-                if (t - 1 > t0) load(t - 2);
-            } else {
-                unpack(t, 0);
-                __syncthreads();
-                if (t > t0) load(t - 1);
-            }
+            __syncthreads();  // the last tile's reads are over
+            unpack(key0);
+            __syncthreads();
+            if (t > t0) load(t - 1);
             if (!wave_rows) continue;
-            const _Float16 *const sk = reinterpret_cast<const _Float16*>(lds + buf * kTile), *const sv = sk + KT * KS;
-            const float *const sks = sks_[buf], *const svs = svs_[buf], *const smax = smax_[buf];
-            const uint32_t* const svalid = svalid_[buf];
 
             // Scores: a lane's j-th of a block of 32 keys is key QS (j / 4) + 4 c + j % 4.
             constexpr int KB = KW / R, NK = SL * KB, TERMS = SPLIT ? 2 : 1;  // blocks of R keys, operands of K
@@ -706,18 +690,18 @@ __device__ inline int rows_of_slot(const TreeArgs& a, int slot, Seq& sq, int& fi
     return at < 0 || at >= rows ? -1 : b;
 }
 
-// The parts of a unit that was cut joined, in their order.  A wave takes one quad of
-// the values of R rows, which a part has in 1 KB; where there are few units, the
-// four waves of a workgroup take a quarter of the parts each.
-template <int D, int DT, int WR, bool FEW>
+// The parts of a unit that was cut joined, in their order.  A wave takes QN quads of
+// the values of R rows, each of which a part has in 1 KB; where there are few units,
+// one quad, and the four waves of a workgroup a quarter of its parts each.
+template <int D, int DT, int RT, bool FEW>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
-    typedef Tiling<D, WR> T;
-    constexpr int R = T::R, RT = T::RT, NQ = Shape<R>::kQuads, N = D / R * NQ, NG = FEW ? 4 : 1;
+    typedef Tiling<D, RT> T;
+    constexpr int R = T::R, NQ = Shape<R>::kQuads, N = D / R * NQ, NG = FEW ? 4 : 1, QN = FEW ? 1 : 2;
     __shared__ __align__(16) f4 sv[FEW ? 192 : 1];
     __shared__ float ssum[FEW ? 192 : 1], stop[FEW ? 256 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & (R - 1), c = lane / R, slot = blockIdx.x / a.H, h = blockIdx.x - slot * a.H;
-    const int item = FEW ? blockIdx.y : 4 * blockIdx.y + wave, rg = item / N, quad = item % N;
+    const int item = (FEW ? blockIdx.y : 4 * blockIdx.y + wave) * QN, rg = item / N, quad = item % N;
     Seq sq;
     int first;
     if (rows_of_slot<RT>(a, slot, sq, first) < 0) return;
@@ -725,45 +709,72 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
     const int rows = sq.n * a.G, row = first + R * rg + r;
     if (share[1] <= share[0] || first + R * rg >= rows) return;
     const auto part_of = [&](int s) { return (int64_t)(2 * s + (s == share[0])); };
-    const auto ml_of = [&](int s) { return a.ml[part_of(s) * RT + R * rg + r]; };
-    const int s0 = share[0] + (FEW ? wave : 0);
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int s = s0; s <= share[1]; s += NG) top = fmaxf(top, ml_of(s).x);
-    if constexpr (FEW) {
+    float top = -INFINITY, sum = 0.0f;
+    f4 v[QN];
+#pragma unroll
+    for (int i = 0; i < QN; ++i) v[i] = (f4){0, 0, 0, 0};
+    constexpr int AT = 8;  // parts whose reads are on their way at once
+    for (int s0 = share[0] + (FEW ? wave : 0); s0 <= share[1]; s0 += AT * NG) {
+        f2 x[AT];
+        f4 y[AT][QN];
+#pragma unroll
+        for (int j = 0; j < AT; ++j) {
+            const int s = s0 + j * NG;
+            x[j] = (f2){-INFINITY, 0.0f};
+#pragma unroll
+            for (int i = 0; i < QN; ++i) y[j][i] = (f4){0, 0, 0, 0};
+            if (s > share[1]) continue;
+            const int64_t part = part_of(s);
+            x[j] = a.ml[part * RT + R * rg + r];
+#pragma unroll
+            for (int i = 0; i < QN; ++i)
+                y[j][i] = reinterpret_cast<const f4*>(a.part + part * RT * D)[(rg * N + quad + i) * 64 + lane];
+        }
+        float now = top;
+#pragma unroll
+        for (int j = 0; j < AT; ++j) now = fmaxf(now, x[j].x);
+        const float safe = now == -INFINITY ? 0.0f : now, old = fast_exp2(top - safe);
+        top = now;
+        sum *= old;
+#pragma unroll
+        for (int i = 0; i < QN; ++i) v[i] *= old;
+#pragma unroll
+        for (int j = 0; j < AT; ++j) {
+            const float f = fast_exp2(x[j].x - safe);  // a part that saw nothing: zeros times 0
+            sum += f * x[j].y;
+#pragma unroll
+            for (int i = 0; i < QN; ++i) v[i] += y[j][i] * f;
+        }
+    }
+    if constexpr (FEW) {  // the four waves' parts relative to one maximum
         stop[threadIdx.x] = top;
         __syncthreads();
+        float all = top;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, stop[64 * i + lane]);
-    }
-    const float safe = top == -INFINITY ? 0.0f : top;
-    f4 v = {0, 0, 0, 0};
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int s = s0; s <= share[1]; s += NG) {
-        const f2 x = ml_of(s);
-        const f4 y = reinterpret_cast<const f4*>(a.part + part_of(s) * RT * D)[(rg * N + quad) * 64 + lane];
-        const float f = fast_exp2(x.x - safe);  // a part that saw nothing: zeros times 0
-        sum += f * x.y;
-        v += y * f;
+        for (int i = 0; i < 4; ++i) all = fmaxf(all, stop[64 * i + lane]);
+        const float f = fast_exp2(top - (all == -INFINITY ? 0.0f : all));
+        sum *= f;
+        v[0] *= f;
     }
     if constexpr (FEW) {
         if (wave > 0) {
-            sv[threadIdx.x - 64] = v;
+            sv[threadIdx.x - 64] = v[0];
             ssum[threadIdx.x - 64] = sum;
         }
         __syncthreads();
         if (wave > 0) return;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-            v += sv[64 * i + lane];
+            v[0] += sv[64 * i + lane];
             sum += ssum[64 * i + lane];
         }
     }
     if (row >= rows) return;
-    v *= sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    const float f = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
     const int tok = sq.q0 + row / a.G, head = h * a.G + row % a.G;
-    put4<DT>(a.out, tok * a.o_token + head * a.o_head + R * (quad / NQ) + 8 * (quad % NQ) + 4 * c, v);
+#pragma unroll
+    for (int i = 0; i < QN; ++i)
+        put4<DT>(a.out, tok * a.o_token + head * a.o_head + R * ((quad + i) / NQ) + 8 * ((quad + i) % NQ) + 4 * c, v[i] * f);
 }
 
 // ------------------------------------------------------------------ host
@@ -771,34 +782,33 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
 constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer than 2^32
 
 struct Plan {
-    int wr, nslots, grid;
+    int rt, nslots, grid;
     size_t ml, shares, bytes;  // offsets of the maxima and of the shares, and the whole
 };
 
-// Rows a unit by the mean tree; a share for each place on the units, fewer where the
-// table has fewer tiles.
-template <int D, int WR>
-void plan_rows(Plan& p, int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
-    typedef Tiling<D, WR> L;
-    p.nslots = (int)(cu ? (int64_t)T * G / L::RT + B : (int64_t)B * ((G + L::RT - 1) / L::RT));
+// A share for each place on the units, fewer where the table has fewer tiles.
+template <int D, int RT>
+Plan plan_rows(int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
+    typedef Tiling<D, RT> L;
+    Plan p{};
+    p.rt = RT;
+    p.nslots = (int)(cu ? (int64_t)T * G / RT + B : (int64_t)B * ((G + RT - 1) / RT));
     const int64_t tiles = (int64_t)p.nslots * H * std::max<int64_t>(1, (capacity + L::KT - 1) / L::KT);
     const int64_t room = (int64_t)n_cu * L::kUnit;
     p.grid = (int)((std::min(room, (tiles + kLeastTiles - 1) / kLeastTiles) + 7) / 8 * 8);
-    p.ml = (size_t)p.grid * 2 * L::RT * D * 4;
-    p.shares = p.ml + (size_t)p.grid * 2 * L::RT * 8;
+    p.ml = (size_t)p.grid * 2 * RT * D * 4;
+    p.shares = p.ml + (size_t)p.grid * 2 * RT * 8;
     p.bytes = p.shares + (size_t)p.nslots * H * 8;
+    return p;
 }
 
+// Rows a unit by the mean tree.
 template <int D>
 Plan plan_tree(int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
-    constexpr int S = 32 / rows_a_wave<D>();
-    Plan p{};
     const int64_t mean = (((int64_t)T + B - 1) / B) * G;
-    p.wr = mean <= 32 ? S : mean <= 64 ? 2 * S : 4 * S;
-    if (p.wr == S) plan_rows<D, S>(p, T, B, H, G, cu, capacity, n_cu);
-    else if (p.wr == 2 * S) plan_rows<D, 2 * S>(p, T, B, H, G, cu, capacity, n_cu);
-    else plan_rows<D, 4 * S>(p, T, B, H, G, cu, capacity, n_cu);
-    return p;
+    if (mean <= 32) return plan_rows<D, 32>(T, B, H, G, cu, capacity, n_cu);
+    if (mean <= 64) return plan_rows<D, 64>(T, B, H, G, cu, capacity, n_cu);
+    return plan_rows<D, 128>(T, B, H, G, cu, capacity, n_cu);
 }
 
 Plan plan_of(int T, int B, int heads, int H, int D, bool cu, int64_t capacity, int n_cu) {
@@ -819,23 +829,24 @@ int cu_count() {
     return n[dev];
 }
 
-template <int D, int KIND, int DT, int WR>
+template <int D, int KIND, int DT, int RT>
 void launch4(const TreeArgs& a, hipStream_t st) {
-    typedef Tiling<D, WR> L;
-    tree_keys_kernel<D, KIND, DT, WR><<<(unsigned)a.grid, 64 * L::W, 0, st>>>(a);
+    typedef Tiling<D, RT> L;
+    tree_keys_kernel<D, KIND, DT, RT><<<(unsigned)a.grid, 64 * L::W, 0, st>>>(a);
     // At one tile a sequence nothing is cut.
     if (((int64_t)a.table_w << a.pshift) <= L::KT) return;
-    const unsigned units = (unsigned)a.nslots * a.H, items = WR * D / 4 * L::R / 64;
-    if (units <= 32) tree_join_kernel<D, DT, WR, true><<<dim3(units, items), 256, 0, st>>>(a);
-    else tree_join_kernel<D, DT, WR, false><<<dim3(units, items / 4), 256, 0, st>>>(a);
+    constexpr unsigned items = RT * D / 256;  // quads of a wave's rows
+    static_assert(items % 8 == 0, "a workgroup of the join takes eight");
+    const unsigned units = (unsigned)a.nslots * a.H;
+    if (units <= 32) tree_join_kernel<D, DT, RT, true><<<dim3(units, items), 256, 0, st>>>(a);
+    else tree_join_kernel<D, DT, RT, false><<<dim3(units, items / 8), 256, 0, st>>>(a);
 }
 
 template <int D, int KIND, int DT>
 void launch3(const TreeArgs& a, const Plan& p, hipStream_t st) {
-    constexpr int S = 32 / rows_a_wave<D>();
-    if (p.wr == S) launch4<D, KIND, DT, S>(a, st);
-    else if (p.wr == 2 * S) launch4<D, KIND, DT, 2 * S>(a, st);
-    else launch4<D, KIND, DT, 4 * S>(a, st);
+    if (p.rt == 32) launch4<D, KIND, DT, 32>(a, st);
+    else if (p.rt == 64) launch4<D, KIND, DT, 64>(a, st);
+    else launch4<D, KIND, DT, 128>(a, st);
 }
 
 template <int D, int KIND>
