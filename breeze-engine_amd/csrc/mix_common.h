@@ -143,6 +143,23 @@ __device__ inline float max_16(float x) {
 // The max over a wave, in all lanes.
 __device__ inline float max_wave(float x) { return max_halves(max_rows16(max_16(x))); }
 
+// The last of n (1 or more) whole numbers from 0 on that `is` holds for, given that it holds
+// for 0 and for all before one that it holds for: 64 at a time, one a lane, so that a search
+// of up to 4096 waits for memory twice.
+template <typename F>
+__device__ inline int last_of(int n, F is) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (;;) {
+        const int step = (n + 63) >> 6;
+        const uint64_t yes = __ballot(lane * step < n && is(base + lane * step));
+        const int last = yes ? 63 - __builtin_clzll(yes) : 0;
+        base += last * step;
+        if (step == 1) return base;
+        n = min(step, n - last * step);
+    }
+}
+
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 16 bytes a lane from `src` to LDS at `lds` + 16 * lane.  The compiler does not

@@ -20,8 +20,9 @@
 //
 // verify_rows_kernel takes one pass over all rows, for each of their pieces of 2048
 // scores the largest and the sum of exponentials relative to it: HBM, and fp64
-// vector work of the same time.  verify_walk_kernel goes down, one workgroup a
-// sequence, from what the pieces hold; to draw it reads one piece again.  The first
+// vector work of nearly the same time.  verify_walk_kernel goes down, one workgroup a
+// sequence: first what every node's pieces add up to, a node a wave, and every child's
+// score, then the walk itself in LDS; to draw it reads one piece again.  The first
 // residual of each sequence, a pass over the row that stands alone on its path, is
 // spread over all units (verify_rest_kernel), between the two halves of the walk.
 #include "mix_common.h"
@@ -36,8 +37,7 @@ namespace {
 
 constexpr int kPiece = 2048, kPieces = 1024;  // scores a piece; pieces of a row at most
 constexpr int kTreeNodes = 1024;
-constexpr int kWalk = 256;                    // threads of a walk; of one with residuals
-constexpr int kWalkDraft = 1024;
+constexpr int kWalk = 512;                    // threads of a walk
 
 struct Piece {
     double sum;
@@ -66,6 +66,7 @@ struct VerArgs {
     int32_t* path;
     int32_t* counts;
     Piece* pieces;  // [T][np]
+    f2* own;        // [T]: each node's own score, and the draft's probability, at its parent
     Walk* walks;    // [B], with a draft
     double* rest;   // [B][np], with a draft
     int T, V, B, np;
@@ -83,47 +84,89 @@ __device__ inline float score(const void* p, int64_t i) {
     return DT == kBF16 ? bf_lo(w) : (float)__builtin_bit_cast(_Float16, w);
 }
 
-// A lane's scores of a piece: load v holds scores (64 v + lane) * VEC on.  Rows
+// A lane's scores of a piece, N at a time: the v-th are scores (64 v + lane) * N on.  Rows
 // lie at any address of their type's alignment.  Past the row's end: -infinity.
-template <int DT>
+template <int DT, int N = vec<DT>()>
 __device__ inline void load_piece(const void* logits, int64_t row, int V, int piece, int lane, float* x) {
-    constexpr int N = vec<DT>(), L = kPiece / 64 / N;
+    constexpr int L = kPiece / 64 / N, PER = vec<DT>();  // of 16 bytes
 #pragma unroll
-    for (int v = 0; v < L; ++v) {
-        const int i = piece * kPiece + (64 * v + lane) * N;
-        if (i + N <= V) {
-            const u4a w = *reinterpret_cast<const u4a*>(static_cast<const uint8_t*>(logits) + (row + i) * (DT == kF32 ? 4 : 2));
+    for (int v = 0; v < L; ++v)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (DT == kF32) {
-                    x[N * v + j] = bits_f(w[j]);
-                } else {
+        for (int k = 0; k < N; k += PER) {
+            const int i = piece * kPiece + (64 * v + lane) * N + k;
+            if (i + PER <= V) {
+                const u4a w =
+                    *reinterpret_cast<const u4a*>(static_cast<const uint8_t*>(logits) + (row + i) * (DT == kF32 ? 4 : 2));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
                     const uint32_t b = w[j];  // bit_cast of a vector's element itself would take its first
-                    const h2 h = __builtin_bit_cast(h2, b);
-                    x[N * v + 2 * j] = DT == kBF16 ? bf_lo(w[j]) : (float)h[0];
-                    x[N * v + 2 * j + 1] = DT == kBF16 ? bf_hi(w[j]) : (float)h[1];
+                    if constexpr (DT == kF32) {
+                        x[N * v + k + j] = bits_f(b);
+                    } else {
+                        const h2 h = __builtin_bit_cast(h2, b);
+                        x[N * v + k + 2 * j] = DT == kBF16 ? bf_lo(b) : (float)h[0];
+                        x[N * v + k + 2 * j + 1] = DT == kBF16 ? bf_hi(b) : (float)h[1];
+                    }
                 }
-            }
-        } else {
+            } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[N * v + j] = i + j < V ? score<DT>(logits, row + i + j) : -INFINITY;
+                for (int j = 0; j < PER; ++j) x[N * v + k + j] = i + j < V ? score<DT>(logits, row + i + j) : -INFINITY;
+            }
         }
-    }
 }
 
-__device__ inline double sum_wave(double x) {
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) x += __shfl_xor(x, s);
+// A lane's value as DPP control CONTROL moves it, 0 where nothing comes.
+template <int CONTROL, int ROWS>
+__device__ inline double moved(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CONTROL, ROWS, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CONTROL, ROWS, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+// The sum over a wave's lanes up to this one.
+__device__ inline double scan_wave(double x) {
+    x += moved<0x111, 0xF>(x);  // row_shr:1, 2, 4, 8 within 16 lanes
+    x += moved<0x112, 0xF>(x);
+    x += moved<0x114, 0xF>(x);
+    x += moved<0x118, 0xF>(x);
+    x += moved<0x142, 0xA>(x);  // row_bcast:15 to rows 1 and 3
+    x += moved<0x143, 0xC>(x);  // row_bcast:31 to rows 2 and 3
     return x;
 }
+__device__ inline double of_lane(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ inline double sum_wave(double x) { return of_lane(scan_wave(x), 63); }
 __device__ inline int min_wave(int x) {
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) x = min(x, __shfl_xor(x, s));
     return x;
 }
 
-// exp((x - top) / temperature); zero for -infinity.
-__device__ inline double weight(float x, double top, double inv) { return exp(((double)x - top) * inv); }
+// exp((x - top) / temperature) with scale = log2(e) / temperature: 2^t, t = (x - top)
+// scale, at most 0, as 2^n times 2^r with n the nearest whole number and |r| at most a
+// half, whose Taylor series in r ln(2) is taken up to the eleventh power (7e-15 is left
+// out).  -infinity gives zero, and so does all that is below fp64's range.  Two thirds of
+// a general exponential's instructions.
+__device__ inline double weight(float x, double top, double scale) {
+    const double t = __builtin_fmax(((double)x - top) * scale, -1080.0), n = __builtin_rint(t), r = t - n;
+    double p = 4.4455382718708115e-10;  // ln(2)^11 / 11!, and so on down
+    p = __builtin_fma(p, r, 7.0549116208011233e-9);
+    p = __builtin_fma(p, r, 1.0178086009239699e-7);
+    p = __builtin_fma(p, r, 1.3215486790144309e-6);
+    p = __builtin_fma(p, r, 1.5252733804059840e-5);
+    p = __builtin_fma(p, r, 1.5403530393381609e-4);
+    p = __builtin_fma(p, r, 1.3333558146428443e-3);
+    p = __builtin_fma(p, r, 9.6181291076284772e-3);
+    p = __builtin_fma(p, r, 5.5504108664821580e-2);
+    p = __builtin_fma(p, r, 2.4022650695910071e-1);
+    p = __builtin_fma(p, r, 6.9314718055994531e-1);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n);
+}
+constexpr double kLog2e64 = 1.4426950408889634;
 
 struct Seq {
     int q0, n;
@@ -143,17 +186,14 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerArgs a) {
     if (piece >= a.np) return;
     float x[E];
     load_piece<DT>(a.logits, t * a.row, a.V, piece, lane, x);
-    int b = t;
-    if (a.cu) {
-        int hi = a.B;
-        b = 0;
-        while (hi - b > 1) {
-            const int mid = (b + hi) >> 1;
-            if (a.cu[mid] <= t) b = mid;
-            else hi = mid;
-        }
-    }
+    const int b = a.cu ? last_of(a.B, [&](int i) { return a.cu[i] <= t; }) : t;
     const float temp = temperature(a, b);
+    if (piece == 0 && lane == 0 && a.parents) {  // what the walk will ask of this node, while the scores are read anyway
+        const int q0 = a.cu ? min(max(a.cu[b], 0), a.T) : t, up = a.parents[t], token = a.tokens[t];
+        if (up >= 0 && up < t - q0 && token >= 0 && token < a.V)
+            a.own[t] = (f2){score<DT>(a.logits, (q0 + up) * a.row + token),
+                            a.draft ? a.draft[(q0 + up) * a.draft_row + token] : 1.0f};
+    }
     float top = -INFINITY;
     bool bad = false;
 #pragma unroll
@@ -167,9 +207,9 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerArgs a) {
     double sum = 0.0;
     if (temp > 0.0f) {
         if (top > -INFINITY) {
-            const double inv = 1.0 / (double)temp;
+            const double scale = kLog2e64 / (double)temp;
 #pragma unroll
-            for (int i = 0; i < E; ++i) sum += weight(x[i], top, inv);
+            for (int i = 0; i < E; ++i) sum += weight(x[i], top, scale);
         }
         sum = sum_wave(sum);
     } else {
@@ -183,32 +223,47 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerArgs a) {
 
 // One row's weights: G of a node.
 struct Row {
-    double top, inv, one, A;  // one: 1 / the sum of exponentials
+    double top, scale, one, A;  // one: 1 / the sum of exponentials
 };
 
-template <int DT, bool DRAFT>
-__device__ inline double share(const VerArgs& a, const Row& r, float x, const float* q) {
-    const double p = weight(x, r.top, r.inv) * r.one;
+// G of a token of score x that the draft gives q.
+template <bool DRAFT>
+__device__ inline double share(const Row& r, float x, float q) {
+    const double p = weight(x, r.top, r.scale) * r.one;
     if (!DRAFT || r.A == 0.0) return p;
-    const double d = p - r.A * (double)*q;
+    const double d = p - r.A * (double)q;
     return d > 0.0 ? d : d * 0.0;  // a draft's NaN or infinity shows
 }
 
-// A lane's weights of a piece of node t's row without the tokens in `gone`
-// (a bit each; null: none), in load_piece's order.
-template <int DT, bool DRAFT>
-__device__ inline void weights_of(const VerArgs& a, const Row& r, int t, int piece, int lane, const uint32_t* gone,
-                                  double* g) {
+// A lane's weights of a piece of node t's row without the tokens in `gone` (a bit each):
+// f(v, g) with those of scores (64 v + lane) * N on, for one v after another.
+template <int DT, bool DRAFT, typename F>
+__device__ inline void weights_of(const VerArgs& a, const Row& r, int t, int piece, int lane, const uint32_t* gone, F f) {
     constexpr int N = vec<DT>(), E = kPiece / 64;
-    float x[E];
+    float x[E], q[DRAFT ? E : 1];
     load_piece<DT>(a.logits, t * a.row, a.V, piece, lane, x);
-    const float* const q = DRAFT ? a.draft + t * a.draft_row : nullptr;
+    if (DRAFT && r.A != 0.0) load_piece<kF32, N>(a.draft, t * a.draft_row, a.V, piece, lane, q);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int in = (64 * (i / N) + lane) * N + i % N, at = piece * kPiece + in;
-        const bool is = at < a.V && !(gone && (gone[in >> 5] >> (in & 31) & 1));
-        g[i] = is ? share<DT, DRAFT>(a, r, x[i], DRAFT ? q + at : nullptr) : 0.0;
+    for (int v = 0; v < E / N; ++v) {
+        double g[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int in = (64 * v + lane) * N + j, at = piece * kPiece + in;
+            const bool is = at < a.V && !(gone[in >> 5] >> (in & 31) & 1);
+            g[j] = is ? share<DRAFT>(r, x[N * v + j], DRAFT ? q[N * v + j] : 0.0f) : 0.0;
+        }
+        f(v, g);
     }
+}
+// Their sum over the piece.
+template <int DT, bool DRAFT>
+__device__ inline double weight_of(const VerArgs& a, const Row& r, int t, int piece, int lane, const uint32_t* gone) {
+    double sum = 0.0;
+    weights_of<DT, DRAFT>(a, r, t, piece, lane, gone, [&](int, const double* g) {
+#pragma unroll
+        for (int j = 0; j < vec<DT>(); ++j) sum += g[j];
+    });
+    return sum_wave(sum);
 }
 
 // The sequences whose walk stands before its first residual, all pieces.
@@ -224,26 +279,34 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerArgs a) {
     gone[wave][lane] = in >= 0 && in < kPiece && in >> 5 == lane ? 1u << (in & 31) : 0;
     __syncthreads();
     if (piece >= a.np) return;
-    const Row r = {w.top, 1.0 / (double)temperature(a, b), w.one, w.A};
-    double g[kPiece / 64], sum = 0.0;
-    weights_of<DT, true>(a, r, s.q0 + w.node, piece, lane, gone[wave], g);
-#pragma unroll
-    for (int i = 0; i < kPiece / 64; ++i) sum += g[i];
-    sum = sum_wave(sum);
+    const Row r = {w.top, kLog2e64 / (double)temperature(a, b), w.one, w.A};
+    const double sum = weight_of<DT, true>(a, r, s.q0 + w.node, piece, lane, gone[wave]);
     if (lane == 0) a.rest[(int64_t)b * a.np + piece] = sum;
 }
 
-template <int DT, bool DRAFT, bool RESUME, int THREADS>
-__global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerArgs a) {
-    constexpr int W = THREADS / 64, N = vec<DT>(), E = kPiece / 64;
+// What a node's pieces add up to.
+struct Node {
+    double one;  // 1 / the sum of exponentials
+    float top;   // NaN: no distribution
+    int best;    // the largest score's token, at temperature 0
+};
+
+template <int DT, bool DRAFT, bool RESUME>
+__global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
+    constexpr int W = kWalk / 64, N = vec<DT>(), AT = 2;
+    struct Child {
+        int token;
+        float u, score, q;  // its random number; its score, and the draft's probability, at its parent
+    };
+    __shared__ Node nodes[kTreeNodes];
+    __shared__ Child children[kTreeNodes];
     __shared__ int parents[kTreeNodes], removed[kTreeNodes];
-    __shared__ double mass[kPieces];  // G's sums of the node's pieces
-    __shared__ double sums[W];
-    __shared__ float tops[W];
-    __shared__ int ats[W], bads[W];
+    __shared__ double removed_g[DRAFT ? 1 : kTreeNodes];  // what each had
+    __shared__ double mass[kPieces], sums[W];             // G's sums of the node's pieces
     __shared__ uint32_t gone[W][kPiece / 32];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Seq s = sequence(a, b);
+    const float temp = temperature(a, b);
     Walk k = {0.0, 1.0, 0.0, 1.0, 0, 1, 0, 0};
     if constexpr (RESUME) {
         k = a.walks[b];
@@ -251,40 +314,91 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerArgs a) {
     } else {
         // Rows outside every sequence, and what this one's walk leaves: -1.
         const int from = b == 0 ? 0 : s.q0, to = b == a.B - 1 ? a.T : s.q0 + s.n;
-        for (int i = from + tid; i < to; i += THREADS) a.out[i] = a.path[i] = -1;
+        for (int i = from + tid; i < to; i += kWalk) a.out[i] = a.path[i] = -1;
         if (DRAFT && tid == 0) a.walks[b].going = 0;
         if (s.n == 0 || s.n > kTreeNodes) {
             if (tid == 0) a.counts[b] = 0;
             return;
         }
     }
-    for (int i = tid; i < s.n; i += THREADS) parents[i] = a.parents ? a.parents[s.q0 + i] : -1;
-    __syncthreads();
-    if (!RESUME && tid == 0) a.path[s.q0] = 0;
-    const float temp = temperature(a, b);
-    const bool greedy = temp == 0.0f;
-    const double inv = 1.0 / (double)temp;
-
-    int node = k.node, m = k.m, cursor = k.node, nremoved = 0, best = -1;
-    double S = 1.0, Q = 1.0, base = 1.0;
-    Row r = {0.0, inv, 1.0, 0.0};
-    bool fresh = true, bad = !(temp >= 0.0f) || temp > 3e38f;
-
-    const auto block_sum = [&](double x) {
-        x = sum_wave(x);
-        __syncthreads();
-        if (lane == 0) sums[wave] = x;
-        __syncthreads();
-        double all = 0.0;
+    const bool greedy = temp == 0.0f, cold = !(temp >= 0.0f) || temp > 3e38f;
+    const double scale = kLog2e64 / (double)temp;
+    for (int i = tid; i < s.n; i += kWalk) {
+        const int up = a.parents ? a.parents[s.q0 + i] : -1;
+        const f2 own = a.own[s.q0 + i];  // not a number where there is no parent: not read then
+        parents[i] = up >= 0 && up < i ? up : -1;
+        children[i] = Child{a.tokens[s.q0 + i], a.uniforms[s.q0 + i], own.x, own.y};
+    }
+    for (int i0 = wave * AT; i0 < s.n; i0 += W * AT) {  // AT nodes' first 128 pieces are on their way at once
+        Piece p[AT][2];
 #pragma unroll
-        for (int w = 0; w < W; ++w) all += sums[w];
-        return all;
+        for (int n = 0; n < AT; ++n) {
+            const Piece* const own = a.pieces + (int64_t)(s.q0 + min(i0 + n, s.n - 1)) * a.np;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) p[n][j] = own[min(lane + 64 * j, a.np - 1)];
+        }
+#pragma unroll
+        for (int n = 0; n < AT; ++n) {
+            const int i = i0 + n;
+            if (i >= s.n) continue;
+            const Piece* const own = a.pieces + (int64_t)(s.q0 + i) * a.np;
+            float top = -INFINITY;
+            bool nan = false;
+            const auto look = [&](const Piece& q) {
+                top = fmaxf(top, q.top);
+                nan |= q.top != q.top;
+            };
+            look(p[n][0]);
+            look(p[n][1]);
+            for (int j = lane + 128; j < a.np; j += 64) look(own[j]);
+            top = max_wave(top);
+            nan = cold || __any(nan) || !(top > -INFINITY);
+            int best = INT32_MAX;
+            double z = 0.0;
+            const auto add = [&](const Piece& q) {
+                if (greedy) best = q.top == top ? min(best, q.at) : best;
+                else if (q.top > -INFINITY) z += q.sum * weight(q.top, top, scale);
+            };
+            if (!nan) {
+                if (lane < a.np) add(p[n][0]);
+                if (lane + 64 < a.np) add(p[n][1]);
+                for (int j = lane + 128; j < a.np; j += 64) add(own[j]);
+                if (greedy) best = min_wave(best);
+                else z = sum_wave(z);
+            }
+            if (lane == 0) nodes[i] = Node{1.0 / z, nan ? __builtin_nanf("") : top, best};
+        }
+    }
+    __syncthreads();
+    // The walk is one wave's, but for residuals, which all take part in.
+    constexpr int STEP = RESUME ? kWalk : 64;
+    if (!RESUME && wave > 0) return;
+    const auto sync = [] {
+        if constexpr (RESUME) __syncthreads();
+        else __builtin_amdgcn_wave_barrier();
     };
+    if (!RESUME && lane == 0) a.path[s.q0] = 0;
+
+    int node = k.node, m = k.m, cursor = k.node, nremoved = 0;
+    double S = 1.0, Q = 1.0, base = 1.0;
+    Row r = {0.0, scale, 1.0, 0.0};
+    Node at = {1.0, 0.0f, 0};
+    bool fresh = true, bad = false;
+
     const auto mass_sum = [&] {
         double x = 0.0;
-        __syncthreads();
-        for (int i = tid; i < a.np; i += THREADS) x += mass[i];
-        return block_sum(x);
+        sync();
+        for (int i = tid; i < a.np; i += STEP) x += mass[i];
+        x = sum_wave(x);
+        if constexpr (RESUME) {
+            __syncthreads();
+            if (lane == 0) sums[wave] = x;
+            __syncthreads();
+            x = 0.0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) x += sums[w];
+        }
+        return x;
     };
     // The bits of the removed tokens in a piece.
     const auto mark = [&](int piece) {
@@ -297,82 +411,55 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerArgs a) {
         __builtin_amdgcn_wave_barrier();
     };
     const auto piece_mass = [&](int piece) {
-        double g[E], x = 0.0;
         mark(piece);
-        weights_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[wave], g);
-#pragma unroll
-        for (int i = 0; i < E; ++i) x += g[i];
-        x = sum_wave(x);
+        const double x = weight_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[wave]);
         if (lane == 0) mass[piece] = x;
     };
-    // The sums of the pieces that removed tokens are in, without them.
-    const auto remove = [&] {
-        __syncthreads();
-        for (int i = wave; i < nremoved; i += W) piece_mass(removed[i] / kPiece);
-        return mass_sum();
+    // All pieces' masses at a node without a draft's part.  A removed token's share is taken
+    // off its piece's; where less than 2^-10 is left the difference has lost its last bits,
+    // and the piece is summed up anew.
+    const auto masses = [&] {
+        const Piece* const own = a.pieces + (int64_t)(s.q0 + node) * a.np;
+        sync();
+        for (int i = tid; i < a.np; i += STEP) {
+            const Piece p = own[i];
+            mass[i] = p.top > -INFINITY ? p.sum * weight(p.top, r.top, scale) * r.one : 0.0;
+        }
+        sync();
+        if constexpr (!DRAFT) {
+            for (int i = 0; i < nremoved; ++i) {
+                const int piece = removed[i] / kPiece;
+                const double was = mass[piece], now = was - removed_g[i];
+                sync();
+                if (lane == 0 && was >= 0.0) mass[piece] = now < was * 0x1p-10 ? -1.0 : now;
+                sync();
+            }
+            for (int i = 0; i < nremoved; ++i) {
+                const int piece = removed[i] / kPiece;
+                if (mass[piece] < 0.0) piece_mass(piece);
+                sync();
+            }
+        }
     };
 
     if constexpr (RESUME) {
         cursor = k.child;
-        r = {k.top, inv, k.one, k.A};
+        r = {k.top, scale, k.one, k.A};
         Q = k.Q;
-        for (int i = tid; i < a.np; i += THREADS) mass[i] = a.rest[(int64_t)b * a.np + i];
-        if (tid == 0) removed[0] = a.tokens[s.q0 + k.child];
-        const int gone0 = a.tokens[s.q0 + k.child];
-        nremoved = gone0 >= 0 && gone0 < a.V;
-        __syncthreads();
-        S = base = mass_sum();
+        for (int i = tid; i < a.np; i += STEP) mass[i] = a.rest[(int64_t)b * a.np + i];
+        if (tid == 0) removed[0] = children[k.child].token;
+        nremoved = 1;
+        S = mass_sum();
         fresh = false;
     }
-    for (;;) {
+    for (;;) {  // every wave alike
         if (fresh) {
-            // The node's own probabilities.
-            const Piece* const own = a.pieces + (int64_t)(s.q0 + node) * a.np;
-            float top = -INFINITY;
-            int at = INT32_MAX;
-            bool nan = false;
-            for (int i = tid; i < a.np; i += THREADS) {
-                const Piece p = own[i];
-                nan |= p.top != p.top;
-                if (p.top > top) {  // pieces come in order: the first of equal ones stays
-                    top = p.top;
-                    at = p.at;
-                }
-            }
-            const float wave_top = max_wave(top);
-            at = min_wave(top == wave_top ? at : INT32_MAX);
-            nan = __any(nan);
-            __syncthreads();
-            if (lane == 0) {
-                tops[wave] = wave_top;
-                ats[wave] = at;
-                bads[wave] = nan;
-            }
-            __syncthreads();
-            top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                top = fmaxf(top, tops[w]);
-                bad |= bads[w] != 0;
-            }
-            best = INT32_MAX;
-#pragma unroll
-            for (int w = 0; w < W; ++w) best = tops[w] == top ? min(best, ats[w]) : best;
-            bad |= !(top > -INFINITY);
+            at = nodes[node];
+            bad = at.top != at.top;
             if (bad) break;
-            r = {(double)top, inv, 1.0, 0.0};
+            r = {(double)at.top, scale, at.one, 0.0};
             nremoved = 0;
-            if (!greedy) {
-                double z = 0.0;
-                for (int i = tid; i < a.np; i += THREADS) {
-                    const Piece p = own[i];
-                    mass[i] = p.top > -INFINITY ? p.sum * weight(p.top, r.top, inv) : 0.0;
-                    z += mass[i];
-                }
-                r.one = 1.0 / block_sum(z);
-                for (int i = tid; i < a.np; i += THREADS) mass[i] *= r.one;
-                S = Q = base = 1.0;
-            }
+            S = Q = base = 1.0;
             cursor = node;
             fresh = false;
         }
@@ -387,33 +474,37 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerArgs a) {
         }
         if (child < 0) break;
         cursor = child;
-        const int token = a.tokens[s.q0 + child];
-        const bool real = token >= 0 && token < a.V;
+        const Child c = children[child];
         bool take = false;
         if (greedy) {
-            take = token == best;
+            take = c.token == at.best;
         } else {
             // A token that no vocabulary has, or an earlier sibling had, is passed over, and
             // so is one that the draft's probabilities have nothing left for.
-            bool there = real && Q > 0.0;
-            for (int i = 0; i < nremoved && there; ++i) there = removed[i] != token;
+            bool there = c.token >= 0 && c.token < a.V && Q > 0.0;
+            for (int i = 0; i < nremoved && there; ++i) there = removed[i] != c.token;
             if (there) {
-                const int64_t t = s.q0 + node;
-                const float x = score<DT>(a.logits, t * a.row + token), q = DRAFT ? a.draft[t * a.draft_row + token] : 1.0f;
-                const double g = share<DT, DRAFT>(a, r, x, &q);
-                take = (double)a.uniforms[s.q0 + child] * (DRAFT ? (double)q / Q : 1.0) * S < g;
+                const double g = share<DRAFT>(r, c.score, c.q);
+                take = (double)c.u * (DRAFT ? (double)c.q / Q : 1.0) * S < g;
                 if (!take) {
-                    if (tid == 0) removed[nremoved] = token;
+                    sync();
+                    if (tid == 0) {
+                        removed[nremoved] = c.token;
+                        if constexpr (!DRAFT) removed_g[nremoved] = g;
+                    }
                     ++nremoved;
-                    __syncthreads();
+                    sync();
                     if constexpr (!DRAFT) {
                         S -= g;
-                        if (S < base * 0x1p-10) S = base = remove();  // the difference has lost its last bits
+                        if (S < base * 0x1p-10) {
+                            masses();
+                            S = base = mass_sum();
+                        }
                     } else {
                         r.A += S / Q;
-                        Q -= (double)q;
+                        Q -= (double)c.q;
                         if constexpr (!RESUME) {
-                            if (tid == 0) {
+                            if (lane == 0) {
                                 a.walks[b] = Walk{r.A, Q, r.top, r.one, node, m, child, 1};
                                 a.counts[b] = m;
                             }
@@ -428,7 +519,7 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerArgs a) {
         }
         if (take) {
             if (tid == 0) {
-                a.out[s.q0 + m - 1] = token;
+                a.out[s.q0 + m - 1] = c.token;
                 a.path[s.q0 + m] = child;
             }
             node = child;
@@ -438,24 +529,18 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerArgs a) {
     }
     if (tid == 0) a.counts[b] = m;
     if (bad || greedy) {
-        if (tid == 0) a.out[s.q0 + m - 1] = bad ? -1 : best;
+        if (tid == 0) a.out[s.q0 + m - 1] = bad ? -1 : at.best;
         return;
     }
-    if (!DRAFT && nremoved > 0) remove();
-    __syncthreads();
+    if (r.A == 0.0) masses();
+    sync();
     if (wave > 0) return;
     // The piece that the running sum passes the random number in: each lane takes
     // consecutive ones.
     const int per = (a.np + 63) / 64, first = lane * per, last = min(first + per, a.np);
     double x = 0.0;
     for (int i = first; i < last; ++i) x += mass[i];
-    double until = x;
-#pragma unroll
-    for (int st = 1; st < 64; st *= 2) {
-        const double y = __shfl_up(until, st);
-        if (lane >= st) until += y;
-    }
-    const double total = __shfl(until, 63), goal = (double)a.uniforms[s.q0] * total;
+    const double until = scan_wave(x), total = of_lane(until, 63), goal = (double)children[0].u * total;
     double before = __shfl_up(until, 1);
     if (lane == 0) before = 0.0;
     int piece = -1;
@@ -469,35 +554,27 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerArgs a) {
         return;
     }
     const int who = __builtin_ctzll(has);
-    piece = __shfl(piece, who);
-    before = __shfl(before, who);
+    piece = __builtin_amdgcn_readlane(piece, who);
+    before = of_lane(before, who);
     mark(piece);
-    double g[E];
-    weights_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[0], g);
     int drawn = INT32_MAX, final = -1;  // and the last token that has any weight
-#pragma unroll
-    for (int v = 0; v < E / N; ++v) {
+    weights_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[0], [&](int v, const double* g) {
         double own = 0.0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) own += g[N * v + j];
-        double upto = own;
-#pragma unroll
-        for (int st = 1; st < 64; st *= 2) {
-            const double y = __shfl_up(upto, st);
-            if (lane >= st) upto += y;
-        }
+        for (int j = 0; j < N; ++j) own += g[j];
+        const double upto = scan_wave(own);
         double run = before + (upto - own);
-        before += __shfl(upto, 63);
+        before += of_lane(upto, 63);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int at = piece * kPiece + (64 * v + lane) * N + j;
-            run += g[N * v + j];
-            if (g[N * v + j] > 0.0) {
+            run += g[j];
+            if (g[j] > 0.0) {
                 if (run > goal) drawn = min(drawn, at);
                 final = at;
             }
         }
-    }
+    });
     drawn = min_wave(drawn);
     final = -min_wave(-final);
     if (lane == 0) a.out[s.q0 + m - 1] = drawn < INT32_MAX ? drawn : final;
@@ -508,12 +585,12 @@ void launch(const VerArgs& a, hipStream_t st) {
     const unsigned blocks = (unsigned)((a.np + 3) / 4);
     if (a.T > 0) verify_rows_kernel<DT><<<(unsigned)a.T * blocks, 256, 0, st>>>(a);
     if (!a.draft) {
-        verify_walk_kernel<DT, false, false, kWalk><<<a.B, kWalk, 0, st>>>(a);
+        verify_walk_kernel<DT, false, false><<<a.B, kWalk, 0, st>>>(a);
         return;
     }
-    verify_walk_kernel<DT, true, false, kWalk><<<a.B, kWalk, 0, st>>>(a);
+    verify_walk_kernel<DT, true, false><<<a.B, kWalk, 0, st>>>(a);
     verify_rest_kernel<DT><<<(unsigned)a.B * blocks, 256, 0, st>>>(a);
-    verify_walk_kernel<DT, true, true, kWalkDraft><<<a.B, kWalkDraft, 0, st>>>(a);
+    verify_walk_kernel<DT, true, true><<<a.B, kWalk, 0, st>>>(a);
 }
 
 bool check(int T, int V, int B, bool has_cu) {
@@ -528,11 +605,18 @@ bool check(int T, int V, int B, bool has_cu) {
     return true;
 }
 
-int64_t sizes(int T, int V, int B, bool draft, int64_t* walks, int64_t* rest) {
+// The workspace's parts: where those after the pieces begin, and its end.
+struct Parts {
+    int64_t own, walks, rest, end;
+};
+Parts parts_of(int T, int V, int B, bool draft) {
     const int64_t np = (V + kPiece - 1) / kPiece;
-    *walks = T * np * (int64_t)sizeof(Piece);
-    *rest = *walks + (draft ? B * (int64_t)sizeof(Walk) : 0);
-    return *rest + (draft ? B * np * 8 : 0);
+    Parts p;
+    p.own = T * np * (int64_t)sizeof(Piece);
+    p.walks = p.own + T * (int64_t)sizeof(f2);
+    p.rest = p.walks + (draft ? B * (int64_t)sizeof(Walk) : 0);
+    p.end = p.rest + (draft ? B * np * 8 : 0);
+    return p;
 }
 
 }  // namespace
@@ -541,8 +625,7 @@ extern "C" {
 
 int64_t i4_verify_workspace(int T, int V, int B, int has_cu, int has_draft) {
     if (!check(T, V, B, has_cu != 0)) return -2;
-    int64_t walks, rest;
-    return sizes(T, V, B, has_draft != 0, &walks, &rest);
+    return parts_of(T, V, B, has_draft != 0).end;
 }
 
 int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, const int32_t* dTokens,
@@ -560,10 +643,9 @@ int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, con
         return -2;
     }
     VerArgs a{};
-    int64_t walks, rest;
-    const int64_t need = sizes(T, V, B, dDraft != nullptr, &walks, &rest);
-    if (need > 0 && (!dWork || work_bytes < need)) {
-        bq_set_error("verify: needs a workspace of %lld bytes, got %lld", (long long)need, (long long)work_bytes);
+    const Parts at = parts_of(T, V, B, dDraft != nullptr);
+    if (at.end > 0 && (!dWork || work_bytes < at.end)) {
+        bq_set_error("verify: needs a workspace of %lld bytes, got %lld", (long long)at.end, (long long)work_bytes);
         return -4;
     }
     a.logits = dLogits;
@@ -580,8 +662,9 @@ int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, con
     a.path = dPath;
     a.counts = dCounts;
     a.pieces = static_cast<Piece*>(dWork);
-    a.walks = reinterpret_cast<Walk*>(static_cast<uint8_t*>(dWork) + walks);
-    a.rest = reinterpret_cast<double*>(static_cast<uint8_t*>(dWork) + rest);
+    a.own = reinterpret_cast<f2*>(static_cast<uint8_t*>(dWork) + at.own);
+    a.walks = reinterpret_cast<Walk*>(static_cast<uint8_t*>(dWork) + at.walks);
+    a.rest = reinterpret_cast<double*>(static_cast<uint8_t*>(dWork) + at.rest);
     a.T = T;
     a.V = V;
     a.B = B;

@@ -232,7 +232,7 @@ def test_c_verify():
         assert call(**kw) == -2, kw
     assert call(B=0, T=0) == 0
     assert call() == -4 and "workspace" in hb.last_error()
-    assert hb._lib.i4_verify_workspace(4, 100, 2, 1, 0) == 4 * 16
+    assert hb._lib.i4_verify_workspace(4, 100, 2, 1, 0) == 4 * (16 + 8)
     assert hb._lib.i4_verify_workspace(4, 0, 2, 1, 0) == -2
 
 
