@@ -137,6 +137,7 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = P, H, page, D
         self.device, self._index = k.device, k.get_device()
+        self._geometry = (P, H, page, D, self._index)
         self._c = _CCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, H, page, D,
                           kinds[k.dtype])
         self._p = ctypes.addressof(self._c)
@@ -276,9 +277,8 @@ def _heads(t, T, D, what):
 
 
 def _turned(out, like, what):
-    torch = hb._torch
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(like.shape)
     T, H, D = like.shape
     st = out.stride()
     if out.dtype is not like.dtype or out.shape != like.shape or out.device != like.device:
@@ -435,7 +435,7 @@ class PageTable:
             with torch.cuda.device(self.device):
                 return self.extend(lens, cu, T, parents)
         # One allocation: the host part is most of a small call.
-        new = torch.empty((2 * T + B,), dtype=torch.int32, device=self.device)
+        new = lens.new_empty((2 * T + B,))
         p = new.data_ptr()
         rc = hb._lib.i4_pages_extend_dev(*self._args, lens.data_ptr(), None if cu is None else cu.data_ptr(), T,
                                          None if parents is None else parents.data_ptr(), p, p + 4 * T, p + 8 * T,

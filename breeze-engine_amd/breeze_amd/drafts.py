@@ -17,7 +17,7 @@ The conventions are ``attention``'s: asynchronous calls on the current stream
 that own no memory, shapes, types and strides checked here (``ValueError``), what
 lies on the GPU bounded by the kernels, no gradients, no CPU fallback.
 """
-import ctypes
+import array
 
 from . import attention as att
 from . import hip_backend as hb
@@ -58,7 +58,7 @@ def tree_attention(q, cache, block_table, kv_lens, parents, cu_q=None, scale=Non
         raise ValueError(f"scale must be positive and finite, got {scale}")
     att._same_device(cache._index, q, block_table, kv_lens, parents, cu_q, out)
     given = out is not None
-    out = att._output(out, q, (T, heads, D), "out")
+    out = att._output(out, q, (T, heads, D), "out") if given else q.new_empty((T, heads, D))
     if T == 0 or B == 0:
         return out
     if cache._index != att._current():
@@ -154,7 +154,7 @@ def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=No
     if B == 0:
         none = torch.full((2 * T,), -1, dtype=torch.int32, device=logits.device)
         return none[:T], none[T:], none[:0]
-    new = torch.empty((2 * T + B,), dtype=torch.int32, device=logits.device)
+    new = tokens.new_empty((2 * T + B,))
     work, n = att._workspace((T, V, B, cu is not None, draft is not None), "verify", logits.device)
     p = new.data_ptr()
     rc = hb._lib.i4_verify_dev(
@@ -182,8 +182,7 @@ def kv_compact(caches, block_table, kv_lens, cu_q, path, counts):
         raise ValueError(f"needs 1 to 4096 caches, got {len(caches)}")
     first = caches[0]
     for c in caches:
-        if (c.num_pages, c.kv_heads, c.page_size, c.head_dim, c._index) != (
-                first.num_pages, first.kv_heads, first.page_size, first.head_dim, first._index):
+        if c._geometry != first._geometry:
             raise ValueError("the caches differ in pages, heads, sizes or device")
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [B, columns], got {tuple(block_table.shape)}")
@@ -201,10 +200,10 @@ def kv_compact(caches, block_table, kv_lens, cu_q, path, counts):
     if first._index != att._current():
         with torch.cuda.device(first.device):
             return kv_compact(caches, block_table, kv_lens, cu_q, path, counts)
-    lens = torch.empty((B,), dtype=torch.int32, device=first.device)
+    lens = kv_lens.new_empty((B,))
     if B:
-        pointers = (ctypes.c_void_p * len(caches))(*[c._p for c in caches])
-        rc = hb._lib.i4_kv_compact_dev(pointers, len(caches), block_table.data_ptr(), block_table.stride(0), cols,
+        pointers = array.array("Q", [c._p for c in caches])  # the C structs' addresses; a ctypes array takes longer to fill
+        rc = hb._lib.i4_kv_compact_dev(pointers.buffer_info()[0], len(caches), block_table.data_ptr(), block_table.stride(0), cols,
                                        kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), T, B,
                                        path.data_ptr(), counts.data_ptr(), lens.data_ptr(), hb._torch_stream(lens))
         if rc:

@@ -82,51 +82,34 @@ __device__ inline int owner(const int* until, int k) {
     return lo;
 }
 
-// The sequence that token t belongs to; -1: none.
-__device__ inline int sequence_of(const PageArgs& a, int t) {
-    if (!a.cu) return t;
-    if (a.B == 0) return -1;
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= t) lo = mid;
-        else hi = mid;
+// A node's depth in its tree; up(i) gives node i's parent, if it comes before.
+template <typename F>
+__device__ inline int depth_of(int node, F up) {
+    int depth = 0;
+    for (;;) {
+        const int p = up(node);
+        if (p < 0 || p >= node) return depth;
+        node = p;
+        ++depth;
     }
-    const New s = new_tokens(a, lo);
-    return t >= s.q0 && t < s.q0 + s.n ? lo : -1;
+}
+// The slot of a sequence's place.
+__device__ inline int slot_of(const PageArgs& a, int b, int place) {
+    const int page = a.table[(int64_t)b * a.cols + (place >> a.pshift)];
+    return page >= 0 && page < a.P ? (page << a.pshift) + (place & ((1 << a.pshift) - 1)) : -1;
 }
 
-// A token's slot and position, once its sequence has its pages.
-__device__ inline void place_token(const PageArgs& a, int t) {
-    const int b = sequence_of(a, t);
-    int slot = -1, position = 0;
-    if (b >= 0) {
-        const New s = new_tokens(a, b);
-        const int len = a.lens[b], i = t - s.q0, place = len + i;
-        int depth = i;
-        if (a.parents && s.n <= kTreeNodes) {
-            depth = 0;
-            for (int at = i;;) {
-                const int up = a.parents[s.q0 + at];
-                if (up < 0 || up >= at) break;
-                at = up;
-                ++depth;
-            }
-        }
-        position = len + depth;
-        if (a.kv_lens[b] >= 0) {
-            const int page = a.table[(int64_t)b * a.cols + (place >> a.pshift)];
-            if (page >= 0 && page < a.P) slot = (page << a.pshift) + (place & ((1 << a.pshift) - 1));
-        }
-    }
-    a.slots[t] = slot;
-    a.positions[t] = position;
-}
+// Tokens up to which the workgroup that sums places them too, and sequences: their
+// offsets, lengths and parents are in LDS then, where a token finds its sequence
+// and its depth.
+constexpr int kHere = 2048;
 
-// `here`: the tokens' slots in this launch too.
 __global__ __launch_bounds__(kScan) void pages_extend_kernel(PageArgs a, bool here) {
     __shared__ int64_t wide[kScan / 64];
     __shared__ int lds[kScan / 64], until[kScan], from[kScan];
+    __shared__ int first[kScan], count[kScan], lens[kScan], grown[kScan], parents[kHere];  // of all sequences, where they are `here`
+    if (here && a.parents)
+        for (int t = threadIdx.x; t < a.T; t += kScan) parents[t] = a.parents[t];
     const int have = min(max(a.count[0], 0), a.P);
     int64_t asked = 0;
     int taken = 0;
@@ -138,6 +121,9 @@ __global__ __launch_bounds__(kScan) void pages_extend_kernel(PageArgs a, bool he
         if (b < a.B) {
             const New s = new_tokens(a, b);
             const int len = a.lens[b];
+            first[threadIdx.x] = s.q0;
+            count[threadIdx.x] = s.n;
+            lens[threadIdx.x] = len;
             held = min(max(a.held[b], 0), a.cols);
             end = (int64_t)len + s.n;
             const int64_t want = (end + (1 << a.pshift) - 1) >> a.pshift;
@@ -155,6 +141,7 @@ __global__ __launch_bounds__(kScan) void pages_extend_kernel(PageArgs a, bool he
         if (b < a.B) {
             if (ok && need > 0) a.held[b] = held + need;
             a.kv_lens[b] = ok ? (int)end : -1;
+            grown[threadIdx.x] = ok;
         }
         __syncthreads();
         for (int k = threadIdx.x; k < got; k += kScan) {
@@ -167,12 +154,43 @@ __global__ __launch_bounds__(kScan) void pages_extend_kernel(PageArgs a, bool he
     if (!here) return;
     __threadfence_block();
     __syncthreads();
-    for (int t = threadIdx.x; t < a.T; t += kScan) place_token(a, t);
+    for (int t = threadIdx.x; t < a.T; t += kScan) {
+        int lo = 0, hi = a.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        const int i = t - first[lo];
+        int slot = -1, position = 0;
+        if (i >= 0 && i < count[lo]) {
+            const int q0 = first[lo];
+            position = lens[lo] + (a.parents && count[lo] <= kTreeNodes ? depth_of(i, [&](int n) { return parents[q0 + n]; }) : i);
+            if (grown[lo]) slot = slot_of(a, lo, lens[lo] + i);
+        }
+        a.slots[t] = slot;
+        a.positions[t] = position;
+    }
 }
 
+// 256 tokens a workgroup, each wave's found by its first one.
 __global__ __launch_bounds__(256) void pages_slots_kernel(PageArgs a) {
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t < a.T) place_token(a, t);
+    const int t = blockIdx.x * 256 + threadIdx.x, t0 = t & ~63;
+    if (t0 >= a.T) return;
+    int b = a.cu ? a.B > 0 ? last_of(a.B, [&](int i) { return a.cu[i] <= t0; }) : -1 : t;
+    if (t >= a.T) return;
+    int slot = -1, position = 0;
+    if (b >= 0) {
+        while (a.cu && b + 1 < a.B && a.cu[b + 1] <= t) ++b;  // the wave's later tokens may be later sequences'
+        const New s = new_tokens(a, b);
+        const int len = a.lens[b], i = t - s.q0;
+        if (i >= 0 && i < s.n) {
+            position = len + (a.parents && s.n <= kTreeNodes ? depth_of(i, [&](int n) { return a.parents[s.q0 + n]; }) : i);
+            if (a.kv_lens[b] >= 0) slot = slot_of(a, b, len + i);
+        }
+    }
+    a.slots[t] = slot;
+    a.positions[t] = position;
 }
 
 __global__ __launch_bounds__(kScan) void pages_trim_kernel(PageArgs a) {
@@ -237,9 +255,6 @@ bool check_pages(const char* what, PageArgs& a, int num_pages, int page_size, in
     return true;
 }
 
-// Tokens up to which the workgroup that sums places them too.
-constexpr int kHere = 2048;
-
 }  // namespace
 
 extern "C" {
@@ -269,8 +284,9 @@ int i4_pages_extend_dev(int32_t* dTable, int32_t* dHeld, int32_t* dFree, int32_t
     a.kv_lens = dKvLens;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    if (B > 0) pages_extend_kernel<<<1, kScan, 0, st>>>(a, T <= kHere);
-    if (T > 0 && (T > kHere || B == 0)) pages_slots_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(a);
+    const bool here = T <= kHere && B <= kScan;
+    if (B > 0) pages_extend_kernel<<<1, kScan, 0, st>>>(a, here);
+    if (T > 0 && (!here || B == 0)) pages_slots_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(a);
     return launched("pages_extend") ? 0 : -5;
 }
 
