@@ -210,6 +210,8 @@ __device__ __forceinline__ void next_are() {
     if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(KIND, N, 0);
 }
 constexpr int kValu = 2, kMatrix = 8, kLdsRead = 0x100;
+// Keeps what a branch hardly ever does from being done, and left unused, every time.
+__device__ __forceinline__ void stay_branch() { asm volatile(""); }
 
 constexpr int kLeastTiles = 2;  // a share's: less is not worth a workgroup's start
 
@@ -387,14 +389,18 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
 
         // The tile in registers to LDS.
         const auto unpack = [&](int key0) {
+            if (KIND == kFp8 && (key0 + KT > sq.kv || __any(pages_in < 0))) {  // bytes of rows that no key is in may be NaN
+                stay_branch();
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    const int page = __builtin_amdgcn_readlane(pages_in, 64 / NG * ((wave * 64 + THREADS * i) / per_row >> 4));
+                    if (page < 0 || key0 + (tid + THREADS * i) / per_row >= sq.kv) kraw[i] = vraw[i] = (u4){0, 0, 0, 0};
+                }
+            }
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 const int kr = (tid + THREADS * i) / per_row, col = 16 * (tid % per_row);
-                u4 kw = kraw[i], vw = vraw[i];
-                if constexpr (KIND == kFp8) {  // bytes of rows that no key is in may be NaN
-                    const int page = __builtin_amdgcn_readlane(pages_in, 64 / NG * ((wave * 64 + THREADS * i) / per_row >> 4));
-                    if (page < 0 || key0 + kr >= sq.kv) kw = vw = (u4){0, 0, 0, 0};
-                }
+                const u4 kw = kraw[i], vw = vraw[i];
                 h8* kd = reinterpret_cast<h8*>(sk + kr * KS + col);
                 h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
                 // Eight lanes of sixteen write their second half first: all at once they fall on unlike banks.
@@ -532,6 +538,7 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
             // m rowf is rounded once here, by less than half while it is below 2^22; past that
             // the difference is taken first, else the largest weight would be 2 to that error.
             if (__any(__builtin_fabsf(ref) * rowf > 0x1p22f)) {
+                stay_branch();
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
