@@ -137,8 +137,8 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = P, H, page, D
         self.device, self._index = k.device, k.get_device()
-        self._geometry = (P, H, page, D, self._index)
-        self._c = _CCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, H, page, D,
+        self._geometry, self._k = (P, H, page, D, self._index), k.data_ptr()
+        self._c = _CCache(self._k, v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, H, page, D,
                           kinds[k.dtype])
         self._p = ctypes.addressof(self._c)
 
@@ -261,9 +261,9 @@ class Rotary:
                     f[i] = x * (keep + (1 - keep) / factor)
                 if amplitude is None:
                     amplitude = 0.1 * math.log(factor) + 1
-        if not all(math.isfinite(x) for x in f):
-            raise ValueError("freqs must be finite")
         self.dim, self.layout, self.amplitude = dim, layout, 1.0 if amplitude is None else float(amplitude)
+        if not all(math.isfinite(x) for x in (*f, self.amplitude)):
+            raise ValueError("freqs and amplitude must be finite")
         self._turns = torch.tensor([x * (2 / math.pi) for x in f], dtype=torch.float64, device=device)
         self.device, self._index = self._turns.device, self._turns.get_device()
         self._p, self._inter = self._turns.data_ptr(), int(layout == "interleaved")
@@ -424,7 +424,7 @@ class PageTable:
         else:
             _ints(cu, (B + 1,), "cu")
             if tokens is None and parents is not None:
-                tokens = parents.shape[0]
+                tokens = parents.numel()
             if tokens is None or tokens < 0:
                 raise ValueError(f"with cu, tokens says how many there are in all, got {tokens}")
             T = int(tokens)

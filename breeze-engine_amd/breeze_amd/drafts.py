@@ -184,6 +184,8 @@ def kv_compact(caches, block_table, kv_lens, cu_q, path, counts):
     for c in caches:
         if c._geometry != first._geometry:
             raise ValueError("the caches differ in pages, heads, sizes or device")
+    if len({c._k for c in caches}) < len(caches):
+        raise ValueError("a cache is given twice: its rows would move twice")
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [B, columns], got {tuple(block_table.shape)}")
     B, cols = block_table.shape

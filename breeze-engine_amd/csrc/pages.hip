@@ -220,13 +220,13 @@ __global__ __launch_bounds__(kScan) void pages_trim_kernel(PageArgs a) {
         for (int k = threadIdx.x; k < total; k += kScan) {
             const int i = owner(until, k), j = k - (i > 0 ? until[i - 1] : 0);
             int32_t* const at = a.table + (int64_t)(b0 + i) * a.cols + from[i] + j;
-            const int to = have + R - 1 - before - k;
+            const int64_t to = (int64_t)have + R - 1 - before - k;
             if (to < a.P) a.free[to] = *at;
             *at = -1;
         }
         before += total;
     }
-    if (threadIdx.x == 0) a.count[0] = min(have + R, a.P);
+    if (threadIdx.x == 0) a.count[0] = (int)min((int64_t)have + R, (int64_t)a.P);
 }
 
 int page_shift(int page) {

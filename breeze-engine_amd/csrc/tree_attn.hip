@@ -319,7 +319,9 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
         const bool whole = t0 == 0 && t1 == ntile, spoilt = sq.n > kTreeNodes;
         const int rows = min(sq.n * a.G, first + RT), row = first + R * rg + r;
         const bool has_row = row < rows;
-        const int node = has_row ? row / a.G : 0, tok = sq.q0 + node, head = h * a.G + (has_row ? row % a.G : 0);
+        // Lanes past the rows repeat the unit's first: no other workgroup writes that one meanwhile,
+        // where the output is q.
+        const int like = has_row ? row : first, node = like / a.G, tok = sq.q0 + node, head = h * a.G + like % a.G;
         const int ctx = sq.kv - sq.n;  // place of node 0; below zero where the cache lacks the first nodes
         const int32_t* const table = a.table + w.b * a.table_row;
         int t = spoilt || sq.kv == 0 ? t0 - 1 : t1 - 1;

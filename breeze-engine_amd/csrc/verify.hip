@@ -166,6 +166,12 @@ __device__ inline double weight(float x, double top, double scale) {
     p = __builtin_fma(p, r, 1.0);
     return __builtin_ldexp(p, (int)n);
 }
+// What the wave's lanes wrote to LDS is there for all of them.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
 constexpr double kLog2e64 = 1.4426950408889634;
 
 struct Seq {
@@ -321,7 +327,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
             return;
         }
     }
-    const bool greedy = temp == 0.0f, cold = !(temp >= 0.0f) || temp > 3e38f;
+    const bool greedy = temp == 0.0f, cold = !(temp >= 0.0f && temp < INFINITY);
     const double scale = kLog2e64 / (double)temp;
     for (int i = tid; i < s.n; i += kWalk) {
         const int up = a.parents ? a.parents[s.q0 + i] : -1;
@@ -375,7 +381,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     if (!RESUME && wave > 0) return;
     const auto sync = [] {
         if constexpr (RESUME) __syncthreads();
-        else __builtin_amdgcn_wave_barrier();
+        else wave_sync();
     };
     if (!RESUME && lane == 0) a.path[s.q0] = 0;
 
@@ -403,12 +409,12 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     // The bits of the removed tokens in a piece.
     const auto mark = [&](int piece) {
         gone[wave][lane] = 0;
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         for (int i = lane; i < nremoved; i += 64) {
             const int in = removed[i] - piece * kPiece;
             if (in >= 0 && in < kPiece) atomicOr(&gone[wave][in >> 5], 1u << (in & 31));
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
     };
     const auto piece_mass = [&](int piece) {
         mark(piece);
@@ -593,12 +599,13 @@ void launch(const VerArgs& a, hipStream_t st) {
     verify_walk_kernel<DT, true, true><<<a.B, kWalk, 0, st>>>(a);
 }
 
+// A launch has fewer than 2^32 threads in a dimension: 64 a piece of a row, 512 a sequence.
 bool check(int T, int V, int B, bool has_cu) {
     const int64_t np = ((int64_t)V + kPiece - 1) / kPiece;
     if (T < 0 || B < 0 || V < 1 || V > kPiece * kPieces || (!has_cu && T != B) || T * np > (1 << 23) ||
-        B * np > (1 << 23)) {
+        B * np > (1 << 22)) {
         bq_set_error("verify: needs 1 to 2^21 scores a row, one node a sequence where no offsets are given, and no more "
-                     "than 2^23 pieces of 2048 scores (got %d rows of %d, %d sequences)",
+                     "than 2^23 pieces of 2048 scores, half of them of sequences (got %d rows of %d, %d sequences)",
                      T, V, B);
         return false;
     }

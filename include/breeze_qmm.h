@@ -361,7 +361,7 @@ int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, con
                   float temperature, const float* dDraft, int64_t draft_row, int32_t* dOut, int32_t* dPath,
                   int32_t* dCounts, void* dWork, int64_t work_bytes, void* stream);
 
-/* Cache rows of the nodes on a path moved together, in `layers` caches of one
+/* Cache rows of the nodes on a path moved together, in `layers` caches, none twice, of one
  * geometry: place ctx + dPath[dCu[b] + i] to ctx + i for i < dCounts[b], ctx =
  * dKvLens[b] - the sequence's nodes.  dLens[b] (apart from dKvLens) = ctx +
  * dCounts[b]; a negative dKvLens[b] stays.  A path's numbers grow, as

@@ -32,7 +32,8 @@ def _raises(f, calls, **known):
                                 dict(base=0.0), dict(base=float("inf")), dict(factor=0.0), dict(factor=float("nan")),
                                 dict(scaling="parts"), dict(scaling="parts", original=100, slow=40.0),
                                 dict(freqs=[1.0]), dict(freqs=[1.0] * 32, scaling="linear"),
-                                dict(freqs=[float("nan")] * 32)])
+                                dict(freqs=[float("nan")] * 32), dict(amplitude=float("nan")),
+                                dict(amplitude=float("inf"))])
 def test_rotary_objects(kw):
     with pytest.raises(ValueError):
         att.Rotary(**dict(dict(dim=64, device="cpu"), **kw))
@@ -88,7 +89,8 @@ def test_page_tables():
     _raises(pt.extend, [((_ints(3),), {}), ((_ints(2).long(),), {}), ((_ints(2),), dict(tokens=3)),
                         ((_ints(2), _ints(3)), {}), ((_ints(2), _ints(2), 4), {}), ((_ints(2), _ints(3), -1), {}),
                         ((_ints(2), _ints(3).long(), 4), {}), ((_ints(2), _ints(3), 4, _ints(5)), {}),
-                        ((_ints(2), _ints(3), 4, _ints(4).long()), {})])
+                        ((_ints(2), _ints(3), 4, _ints(4).long()), {}),
+                        ((_ints(2), _ints(3), None, _ints(1)[0]), {})])
     _raises(pt.trim, [((_ints(3),), {}), ((torch.zeros(2),), {})])
 
 
@@ -131,7 +133,12 @@ def test_kv_compact(cache):
     with pytest.raises(ValueError, match="GPU"):
         drafts.kv_compact(cache, table, lens, cu, path, counts)
     other = att.KVCache.empty(4, 16, 2, 64, device="cpu")
-    ok = ([cache, cache], table, lens, cu, path, counts)
+    ok = ([cache, att.KVCache.empty(3, 16, 2, 64, device="cpu")], table, lens, cu, path, counts)
+    with pytest.raises(ValueError, match="GPU"):
+        drafts.kv_compact(*ok)
+    for twice in (cache, att.KVCache(cache.k, cache.v, cache.k_scale, cache.v_scale)):
+        with pytest.raises(ValueError, match="twice"):
+            drafts.kv_compact([cache, twice], *ok[1:])
     swap = lambda i, y: tuple(y if j == i else z for j, z in enumerate(ok))  # noqa: E731
     _raises(drafts.kv_compact, [
         (swap(0, []), {}), (swap(0, [cache, other]), {}), (swap(0, [cache] * 4097), {}), (swap(1, table[0]), {}),
@@ -228,7 +235,7 @@ def test_c_verify():
 
     for kw in (dict(x=None), dict(tokens=None), dict(u=None), dict(out=None), dict(path=None), dict(counts=None), dict(T=-1),
                dict(B=-1), dict(V=0), dict(V=(1 << 21) + 1), dict(dt=3), dict(cu=None), dict(t=-1.0), dict(t=float("nan")),
-               dict(t=1e31), dict(T=1 << 23, V=4000)):
+               dict(t=1e31), dict(T=1 << 23, V=4000), dict(T=1 << 23, B=(1 << 22) + 1)):
         assert call(**kw) == -2, kw
     assert call(B=0, T=0) == 0
     assert call() == -4 and "workspace" in hb.last_error()

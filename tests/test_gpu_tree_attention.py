@@ -258,3 +258,19 @@ def test_graph_and_streams(mods):
             outs.append(drafts.tree_attention(q, cache, table, lens, parents, cu))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_in_place_is_the_same(mods):
+    """Units whose rows do not fill their waves, many sequences: what lies past them is no one's."""
+    att, drafts = mods
+    gen = torch.Generator().manual_seed(14)
+    lens = [int(n) for n in torch.randint(1, 12, (96,), generator=gen)]
+    kv_lens = [n + int(k) for n, k in zip(lens, torch.randint(0, 200, (96,), generator=gen))]
+    cache, table = _cache(att, gen, kv_lens, 2, 64, 16, "fp8")
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    q = torch.randn((sum(lens), 6, 64), generator=gen).cuda() * 3
+    args = (cache, table.cuda(), torch.tensor(kv_lens, dtype=torch.int32).cuda(), _flat([tree(n, gen) for n in lens]).cuda(), cu)
+    want = drafts.tree_attention(q, *args)
+    for _ in range(4):
+        own = q.clone()
+        assert torch.equal(drafts.tree_attention(own, *args, out=own), want)
