@@ -197,7 +197,7 @@ struct Tiling {
     static constexpr int R = D == 256 || RT == 32 ? 16 : 32, WR = RT / R;
     static constexpr int W = D == 256 && RT > 32 ? 8 : 4, WK = W / WR;
     static constexpr int KT = 64, KW = KT / WK;
-    static constexpr int KS = D + 8, VS = D + 16;  // LDS rows of a key and of its values: reads of one instruction fall on unlike banks
+    static constexpr int KS = D + 8, VS = D + (R == 32 ? 32 : 16);  // LDS rows of a key and of its values: reads of one instruction fall on unlike banks
     static constexpr int kUnit = W == 8 ? 1 : D == 256 || RT > 32 ? 2 : 3;
     static_assert(KW >= 32, "a wave takes blocks of 32 keys");
 };
@@ -298,8 +298,9 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
     typedef typename Shape<R>::Acc Acc;
     __shared__ __align__(16) uint8_t lds[kBytes];
     __shared__ __align__(16) float sks[KT], svs[KT];
-    __shared__ float smax[KT / 32], sm[W][R], sl[W][R], sf[W][R];
-    __shared__ uint32_t svalid[KT / 32];
+    __shared__ float sm[W][R], sl[W][R], sf[W][R];
+    __shared__ __align__(16) float smax[KT / 32];      // of each 32 keys' value scales
+    __shared__ __align__(16) uint32_t svalid[KT / 32];  // the keys that are there, a bit each
     __shared__ int16_t up[kTreeNodes];
     _Float16 *const sk = reinterpret_cast<_Float16*>(lds), *const sv = sk + KT * KS;
 
@@ -337,6 +338,9 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
         const bool wave_rows = first + R * rg < rows;
         raw.load(a.q, tok * a.q_token + head * a.q_head + 8 * c);
 
+        // A lane's place in the 16 keys that a wave's pass begins with, the same in all passes.
+        static_assert(THREADS / per_row % 16 == 0 && KT == 64, "passes of whole groups; a key a lane");
+        const uint32_t own = (tid / per_row & 15) * D + 16 * (tid % per_row);
         u4 kraw[NC], vraw[NC];
         float ksc = 0.0f, vsc = 0.0f;
         bool sc_bad = true;
@@ -349,17 +353,17 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 const int g = (wave * 64 + THREADS * i) / per_row >> 4;  // the wave's group of this pass
-                const int64_t at = row_of(__builtin_amdgcn_readlane(pages_in, 64 / NG * g), KT * tile + 16 * g) +
-                                   ((tid + THREADS * i) / per_row & 15);
-                kraw[i] = *reinterpret_cast<const u4*>(a.kp + at * D + 16 * (tid % per_row));
-                vraw[i] = *reinterpret_cast<const u4*>(a.vp + at * D + 16 * (tid % per_row));
+                const int64_t at = row_of(__builtin_amdgcn_readlane(pages_in, 64 / NG * g), KT * tile + 16 * g) * D;
+                kraw[i] = *reinterpret_cast<const u4*>(a.kp + at + own);
+                vraw[i] = *reinterpret_cast<const u4*>(a.vp + at + own);
             }
-            if (tid < KT) {
-                const int page = KT == 64 ? pages_in : __shfl(pages_in, 64 / NG * (tid >> 4));
-                sc_bad = page < 0 || KT * tile + tid >= sq.kv;
-                const int64_t at = row_of(page, KT * tile + (tid & ~15)) + (tid & 15);
-                ksc = a.ks[at];
-                vsc = a.vs[at];
+            if (wave < 3) {  // a key a lane: its key's scale, its value's, whether it is there
+                sc_bad = pages_in < 0 || KT * tile + lane >= sq.kv;
+                if (wave < 2) {
+                    const int64_t at = row_of(pages_in, KT * tile + (lane & ~15)) + (lane & 15);
+                    if (wave == 0) ksc = a.ks[at];
+                    vsc = a.vs[at];
+                }
             }
             pages = pages_of(tile - 1);
         };
@@ -405,26 +409,28 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
                 const u4 kw = kraw[i], vw = vraw[i];
                 h8* kd = reinterpret_cast<h8*>(sk + kr * KS + col);
                 h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
-                // Eight lanes of sixteen write their second half first: all at once they fall on unlike banks.
-                const int one = lane >> 3 & 1;
-                kd[one] = unpack8<KIND>(one ? kw.z : kw.x, one ? kw.w : kw.y);
-                kd[1 - one] = unpack8<KIND>(one ? kw.x : kw.z, one ? kw.y : kw.w);
+                // Eight lanes of sixteen write their second half first: all at once they fall on unlike
+                // banks.  Keys of 128 values do so as they are, two rows of KS.
+                const int one = lane >> 3 & 1, kone = D == 128 ? 0 : one;
+                kd[kone] = unpack8<KIND>(kone ? kw.z : kw.x, kone ? kw.w : kw.y);
+                kd[1 - kone] = unpack8<KIND>(kone ? kw.x : kw.z, kone ? kw.y : kw.w);
                 vd[one] = unpack8<KIND>(one ? vw.z : vw.x, one ? vw.w : vw.y);
                 vd[1 - one] = unpack8<KIND>(one ? vw.x : vw.z, one ? vw.y : vw.w);
             }
-            if (tid < KT) {
-                // A value scale of NaN goes with the key's, whose score a row that does
-                // not see the key leaves out; times a probability of zero it would not.
-                const bool nan = vsc != vsc;
+            // A wave each for the keys' scales, the values' and what is there: all wait for the last.
+            // A value scale of NaN goes with the key's, whose score a row that does
+            // not see the key leaves out; times a probability of zero it would not.
+            const bool nan = vsc != vsc;
+            if (wave == 0) {
+                sks[lane] = sc_bad ? 0.0f : nan ? vsc : ksc;
+            } else if (wave == 1) {
                 const float v = sc_bad || nan ? 0.0f : vsc;
-                sks[tid] = sc_bad ? 0.0f : nan ? vsc : ksc;
-                svs[tid] = v;
+                svs[lane] = v;
                 const float vmax = max_rows16(max_16(v));  // of 32 keys
+                if ((lane & 31) == 0) smax[lane >> 5] = vmax;
+            } else if (wave == 2) {
                 const uint64_t valid = __ballot(!sc_bad);
-                if ((lane & 31) == 0) {
-                    smax[tid >> 5] = vmax;
-                    svalid[tid >> 5] = (uint32_t)(valid >> (lane & 32));
-                }
+                if ((lane & 31) == 0) svalid[lane >> 5] = (uint32_t)(valid >> (lane & 32));
             }
         };
         for (; t >= t0; --t) {
@@ -437,7 +443,14 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
 
             // Scores: a lane's j-th of a block of 32 keys is key QS (j / 4) + 4 c + j % 4.
             constexpr int KB = KW / R, NK = SL * KB, TERMS = SPLIT ? 2 : 1;  // blocks of R keys, operands of K
-            float x[U][J];
+            float x[U][J], vmax = 0.0f;
+            uint32_t valid[U], every = ~0u;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                vmax = fmaxf(vmax, smax[U * kg + u]);
+                valid[u] = svalid[U * kg + u];
+                every &= valid[u];
+            }
             {
                 Acc s[KB];
                 h8 k[NK];
@@ -463,7 +476,7 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
 #pragma unroll
                     for (int j = 0; j < J; ++j) x[u][j] = s[(J * u + j) / (4 * NQ)][j % (4 * NQ)] * sc[(J * u + j) / 4][j % 4];
                 constexpr int AHEAD = 6, NS = U * J / 4;
-                next_are<kLdsRead, AHEAD>();
+                next_are<kLdsRead, 2 + AHEAD>();
 #pragma unroll
                 for (int n = 0; n < NK - AHEAD; ++n) {
                     next_are<kMatrix, TERMS>();
@@ -475,14 +488,7 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
                     next_are<kLdsRead, (NS + AHEAD - 1) / AHEAD>();
                 }
             }
-            float vmax = 0.0f;
-            bool all = key0 + KT <= ctx;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                vmax = fmaxf(vmax, smax[U * kg + u]);
-                all = all && svalid[U * kg + u] == 0xFFFFFFFFu;
-            }
-            if (!all) {
+            if (key0 + KT > ctx || __builtin_amdgcn_readfirstlane(every) != ~0u) {
                 vmax = 0.0f;
 #pragma unroll
                 for (int u = U - 1; u >= 0; --u) {
@@ -497,7 +503,7 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
                             at_node = up[at_node];
                         }
                     }
-                    bits &= has_row ? svalid[U * kg + u] : 0u;
+                    bits &= has_row ? valid[u] : 0u;
                     bits >>= 4 * c;
 #pragma unroll
                     for (int j = 0; j < J; j += 4) {
@@ -547,6 +553,7 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
                     for (int j = 0; j < J; ++j) x[u][j] -= ref;
                 bias = unit;
             }
+            __builtin_amdgcn_s_setprio(1);
             float sum = 0.0f;
             // Eight of a lane's scores make an operand of the weights, for a group of 512 / R keys.
             constexpr int GS = U * J / 8, NV = GS * NA;
@@ -591,6 +598,7 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
                     next_are<kValu, (VALU + NA - 1) / NA>();
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
             l = __builtin_fmaf(sum, nu * (1.0f / kPScale), l);
         }
 
