@@ -410,10 +410,10 @@ __global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Ti
                 h8* kd = reinterpret_cast<h8*>(sk + kr * KS + col);
                 h8* vd = reinterpret_cast<h8*>(sv + kr * VS + col);
                 // Eight lanes of sixteen write their second half first: all at once they fall on unlike
-                // banks.  Keys of 128 values do so as they are, two rows of KS.
-                const int one = lane >> 3 & 1, kone = D == 128 ? 0 : one;
-                kd[kone] = unpack8<KIND>(kone ? kw.z : kw.x, kone ? kw.w : kw.y);
-                kd[1 - kone] = unpack8<KIND>(kone ? kw.x : kw.z, kone ? kw.y : kw.w);
+                // banks.  Rows of 128 values do not need it (keys), or lose less to the banks (values).
+                const int one = D == 128 ? 0 : lane >> 3 & 1;
+                kd[one] = unpack8<KIND>(one ? kw.z : kw.x, one ? kw.w : kw.y);
+                kd[1 - one] = unpack8<KIND>(one ? kw.x : kw.z, one ? kw.y : kw.w);
                 vd[one] = unpack8<KIND>(one ? vw.z : vw.x, one ? vw.w : vw.y);
                 vd[1 - one] = unpack8<KIND>(one ? vw.x : vw.z, one ? vw.y : vw.w);
             }
