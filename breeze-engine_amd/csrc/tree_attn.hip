@@ -11,18 +11,27 @@
 // partial sums are fp32.
 //
 // A tree has tens of rows a key-value head (nodes times the query heads of one),
-// which all see the same keys but for the tree itself.  So a workgroup takes up
-// to 128 rows and a share of the keys: each key is loaded and unpacked once for
-// all of them.  WR of its four waves take 32 rows each, and where the rows are
-// fewer the waves share out a tile's keys instead (4 / WR groups, joined at the
-// end).  Tiles go from the last keys to the first, so that the tree comes first and
-// a lane follows its node's parents down once: a tile's mask is the 32 bits that
-// it passes.  Tiles before the tree have no mask.
+// which all see the same keys but for the tree itself.  So a workgroup takes 32, 64 or
+// 128 rows and a share of the keys: each key is loaded and unpacked once for
+// all of them.  A wave takes 16 or 32 of the rows, and where that leaves waves over
+// they share out a tile's keys, joined at the end.  Tiles go from the last keys to the
+// first, so that the tree comes first and a lane follows its node's parents down once: a
+// tile's mask is the 32 bits that it passes.  Tiles before the tree have no mask.
 //
 // The tiles of all units (a sequence, a key-value head, up to 128 rows), one unit
 // after another, are cut into equal shares, one a workgroup, whatever the sequences'
 // lengths, which the host does not read; each workgroup sums up the lengths for
 // itself.  A unit that is cut leaves its parts' sums to tree_join_kernel.
+//
+// What bounds it.  Few rows of many sequences: HBM, less what unpacking does not hide (8
+// nodes of each of 64 sequences behind 100 to 16000 keys, 32/8 heads of 128, e4m3, bf16:
+// 151 us, 0.7 of a copy's rate).  From about 64 rows on, issue: of a compute unit's cycles
+// (32 nodes of 16 sequences, 51 us, of which the join is 12) vector instructions take
+// half, matrix instructions 0.29, LDS 0.4, and a wave waits a third of its time, at two
+// waves a SIMD, which is what the registers hold.  Tried there and no faster: two LDS
+// buffers and one barrier a tile, the next tile's loads among the products, waves started
+// half a tile apart.  One sequence: latency (12 nodes behind 4100 keys 26 us: two
+// launches, five dependent reads, 82 KB of sums a share written and read).
 #include "attn_common.h"
 
 #include <algorithm>
@@ -189,18 +198,27 @@ struct RawQueries {
 };
 
 // How a workgroup of W waves takes a unit of RT rows: R rows a wave, W / (RT / R) waves
-// along the KT keys of a tile; kUnit workgroups a compute unit.  Heads of 256: a wave's
-// sums of 32 rows would leave no registers for a second wave.  Up to 32 rows
-// HBM bounds it: many small workgroups, whose loads are on their way at once.
+// along the KT keys of a tile.
+//
+// Rows of 16: a wave's sums and queries are half as large, and three workgroups share
+// a compute unit, whose loads hide one another's waits.  Rows of 32 read a key from LDS half as
+// often; they are for 128 rows of 64 and 128 values (32 nodes of 16 sequences, bf16: 51 us; 57 with
+// 16 rows a wave, 70 with eight waves of 32).  Units of 64 rows were so once (10 nodes of
+// 64 sequences, bf16: 207 us, 162 now).  With heads of 256 a wave's sums of 32 rows would
+// leave no registers for a second wave.
 template <int D, int RT>
 struct Tiling {
-    static constexpr int R = D == 256 || RT == 32 ? 16 : 32, WR = RT / R;
+    static constexpr int R = D == 256 || RT <= 64 ? 16 : 32, WR = RT / R;
     static constexpr int W = D == 256 && RT > 32 ? 8 : 4, WK = W / WR;
     static constexpr int KT = 64, KW = KT / WK;
     static constexpr int KS = D + 8, VS = D + (R == 32 ? 32 : 16);  // LDS rows of a key and of its values: reads of one instruction fall on unlike banks
-    static constexpr int kUnit = W == 8 ? 1 : D == 256 || RT > 32 ? 2 : 3;
     static_assert(KW >= 32, "a wave takes blocks of 32 keys");
 };
+// Workgroups a compute unit.  Heads of 128, 64 rows: fp32 spills 28 registers a lane at three
+// (10 nodes of 64 sequences 226 us, 198 at two), bf16 7 (162, 181).  32 rows: fp32 11
+// (8 nodes of 64 sequences 175, 191 at two), bf16 2 (151, 173).
+template <int D, int RT, int DT>
+constexpr int per_unit() { return D == 256 ? RT > 32 ? 1 : 2 : RT > 64 || (DT == kF32 && RT > 32) ? 2 : 3; }
 
 // The order of a stretch of code: `n` instructions of a kind next.  Left to itself the
 // compiler reads each operand from LDS right before its matrix instruction, and
@@ -213,7 +231,9 @@ constexpr int kValu = 2, kMatrix = 8, kLdsRead = 0x100;
 // Keeps what a branch hardly ever does from being done, and left unused, every time.
 __device__ __forceinline__ void stay_branch() { asm volatile(""); }
 
-constexpr int kLeastTiles = 2;  // a share's: less is not worth a workgroup's start
+// Tiles a share at least: each share of a cut unit has its sums to write and to join.  12 nodes
+// behind 4100 keys, heads of 256, fp32: 26.4 us; with one 27.4, three 28.2, four 31.5.
+constexpr int kLeastTiles = 2;
 
 // The share that this wave's workgroup has of all units' tiles: tiles [pos, end), the
 // first in sequence b, whose first tile is `base`; `per` tiles a share.  Every wave
@@ -284,7 +304,7 @@ __device__ inline Share share_of(const TreeArgs& a, int id) {
 }
 
 template <int D, int KIND, int DT, int RT>
-__global__ __launch_bounds__((64 * Tiling<D, RT>::W), (Tiling<D, RT>::kUnit * Tiling<D, RT>::W / 4)) void tree_keys_kernel(TreeArgs a) {
+__global__ __launch_bounds__((64 * Tiling<D, RT>::W), (per_unit<D, RT, DT>() * Tiling<D, RT>::W / 4)) void tree_keys_kernel(TreeArgs a) {
     typedef Tiling<D, RT> T;
     constexpr bool SPLIT = DT == kF32, PSPLIT = DT != kBF16;  // two terms of the queries, and of the weights
     constexpr int R = T::R, W = T::W, WR = T::WR, WK = T::WK, KT = T::KT, KW = T::KW, KS = T::KS, VS = T::VS;
@@ -805,13 +825,13 @@ struct Plan {
 
 // A share for each place on the units, fewer where the table has fewer tiles.
 template <int D, int RT>
-Plan plan_rows(int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
+Plan plan_rows(int T, int B, int H, int G, int dt, bool cu, int64_t capacity, int n_cu) {
     typedef Tiling<D, RT> L;
     Plan p{};
     p.rt = RT;
     p.nslots = (int)(cu ? (int64_t)T * G / RT + B : (int64_t)B * ((G + RT - 1) / RT));
     const int64_t tiles = (int64_t)p.nslots * H * std::max<int64_t>(1, (capacity + L::KT - 1) / L::KT);
-    const int64_t room = (int64_t)n_cu * L::kUnit;
+    const int64_t room = (int64_t)n_cu * (dt == kF32 ? per_unit<D, RT, kF32>() : per_unit<D, RT, kBF16>());
     p.grid = (int)((std::min(room, (tiles + kLeastTiles - 1) / kLeastTiles) + 7) / 8 * 8);
     p.ml = (size_t)p.grid * 2 * RT * D * 4;
     p.shares = p.ml + (size_t)p.grid * 2 * RT * 8;
@@ -819,20 +839,26 @@ Plan plan_rows(int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) 
     return p;
 }
 
-// Rows a unit by the mean tree.
+// Rows a unit by the mean tree: the fewest that hold it, as what a unit lacks of rows is worked out
+// all the same, and a tree of two units has its keys loaded and unpacked twice.  us with one step
+// more and one less: 32 rows (8 nodes of 64 sequences, heads of 128, bf16) 151, 195 by units of
+// 64; 64 rows (16 of 16) 43, 43 by 128; 40 rows (10 of 64) 162, 215 by 128, 235 by 32; 128 rows (32 of 16) 52, 61 by 64.
+// Heads of 256 have no units of 64: 48 rows (8 of 64) 202 by 128, 218 by 64, 241 by 32.
 template <int D>
-Plan plan_tree(int T, int B, int H, int G, bool cu, int64_t capacity, int n_cu) {
+Plan plan_tree(int T, int B, int H, int G, int dt, bool cu, int64_t capacity, int n_cu) {
     const int64_t mean = (((int64_t)T + B - 1) / B) * G;
-    if (mean <= 32) return plan_rows<D, 32>(T, B, H, G, cu, capacity, n_cu);
-    if (mean <= 64) return plan_rows<D, 64>(T, B, H, G, cu, capacity, n_cu);
-    return plan_rows<D, 128>(T, B, H, G, cu, capacity, n_cu);
+    if (mean <= 32) return plan_rows<D, 32>(T, B, H, G, dt, cu, capacity, n_cu);
+    if constexpr (D < 256) {
+        if (mean <= 64) return plan_rows<D, 64>(T, B, H, G, dt, cu, capacity, n_cu);
+    }
+    return plan_rows<D, 128>(T, B, H, G, dt, cu, capacity, n_cu);
 }
 
-Plan plan_of(int T, int B, int heads, int H, int D, bool cu, int64_t capacity, int n_cu) {
+Plan plan_of(int T, int B, int heads, int H, int D, int dt, bool cu, int64_t capacity, int n_cu) {
     const int G = heads / H;
-    return D == 64    ? plan_tree<64>(T, B, H, G, cu, capacity, n_cu)
-           : D == 128 ? plan_tree<128>(T, B, H, G, cu, capacity, n_cu)
-                      : plan_tree<256>(T, B, H, G, cu, capacity, n_cu);
+    return D == 64    ? plan_tree<64>(T, B, H, G, dt, cu, capacity, n_cu)
+           : D == 128 ? plan_tree<128>(T, B, H, G, dt, cu, capacity, n_cu)
+                      : plan_tree<256>(T, B, H, G, dt, cu, capacity, n_cu);
 }
 
 int cu_count() {
@@ -855,14 +881,17 @@ void launch4(const TreeArgs& a, hipStream_t st) {
     constexpr unsigned items = RT * D / 256;  // quads of a wave's rows
     static_assert(items % 8 == 0, "a workgroup of the join takes eight");
     const unsigned units = (unsigned)a.nslots * a.H;
+    // 12 nodes behind 4100 keys (4 units): 26.4 us, 29.6 by the other; 10 nodes of 16 sequences (128): 34, 35.
     if (units <= 32) tree_join_kernel<D, DT, RT, true><<<dim3(units, items), 256, 0, st>>>(a);
     else tree_join_kernel<D, DT, RT, false><<<dim3(units, items / 8), 256, 0, st>>>(a);
 }
 
 template <int D, int KIND, int DT>
 void launch3(const TreeArgs& a, const Plan& p, hipStream_t st) {
+    if constexpr (D < 256) {
+        if (p.rt == 64) return launch4<D, KIND, DT, 64>(a, st);
+    }
     if (p.rt == 32) launch4<D, KIND, DT, 32>(a, st);
-    else if (p.rt == 64) launch4<D, KIND, DT, 64>(a, st);
     else launch4<D, KIND, DT, 128>(a, st);
 }
 
@@ -928,7 +957,7 @@ int64_t i4_tree_attention_workspace(int kv_heads, int page_size, int head_dim, i
     int ps = 0;
     if (!check_shape(&c, T, B, heads, table_w, has_cu != 0, &ps)) return -2;
     if (T == 0 || B == 0) return 0;
-    return (int64_t)plan_of(T, B, heads, kv_heads, head_dim, has_cu != 0, (int64_t)table_w << ps, cu_count()).bytes;
+    return (int64_t)plan_of(T, B, heads, kv_heads, head_dim, dtype, has_cu != 0, (int64_t)table_w << ps, cu_count()).bytes;
 }
 
 int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
@@ -972,7 +1001,7 @@ int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_to
     a.P = cache->num_pages;
     a.pshift = ps;
     a.scale = scale * kLog2e;
-    const Plan p = plan_of(T, B, heads, a.H, cache->head_dim, dCu != nullptr, (int64_t)table_w << ps, cu_count());
+    const Plan p = plan_of(T, B, heads, a.H, cache->head_dim, dtype, dCu != nullptr, (int64_t)table_w << ps, cu_count());
     if (p.bytes > 0 && (!dWork || work_bytes < (int64_t)p.bytes)) {
         bq_set_error("tree_attention: needs a workspace of %zu bytes, got %lld", p.bytes, (long long)work_bytes);
         return -4;
