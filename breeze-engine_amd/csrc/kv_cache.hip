@@ -176,7 +176,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a) {
 // ones.  A path's numbers grow, so path[i] >= i, and what a step of rows in
 // order overwrites no later step reads; the rows of one step are all read before
 // any is written.  A wave for each sequence, layer, head, and keys or values: a few
-// rows, whose four dependent reads (lengths, path, page, row) are what it costs.
+// rows, whose four dependent reads (lengths, path, page, row) are what it costs: 2.7 us
+// for one sequence in 16 layers of 4 heads of 256, 4.8 for 48 sequences in 8 layers of 8 of 128
+// (4.9 MB); with the host's part 11 and 10.5.
 constexpr int kLayers = 32;  // of one launch: their pointers are kernel arguments
 
 struct CompactArgs {
