@@ -362,6 +362,12 @@ int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_
                      c->head_dim, c->page_size, c->kv_heads, c->num_pages, table_w);
         return -2;
     }
+    // A launch has up to 2^24 workgroups.
+    const int64_t rows = (int64_t)B * c->kv_heads;
+    if (rows > (1 << 23)) {
+        bq_set_error("kv_compact: %d sequences of %d heads are too many for one call", B, c->kv_heads);
+        return -2;
+    }
     if (B == 0) return 0;
     if (!dCu && T != B) {
         bq_set_error("kv_compact: needs one node a sequence where no offsets are given (got %d, %d sequences)", T, B);
@@ -390,8 +396,9 @@ int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_
     a.pshift = pshift;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    for (int l0 = 0; l0 < layers; l0 += kLayers) {
-        const int n = std::min(layers - l0, kLayers);
+    const int most = (int)std::min<int64_t>(kLayers, (1 << 23) / rows);  // layers a launch
+    for (int l0 = 0; l0 < layers; l0 += most) {
+        const int n = std::min(layers - l0, most);
         for (int i = 0; i < n; ++i) {
             a.layer[i].page[0] = static_cast<uint8_t*>(caches[l0 + i]->k);
             a.layer[i].page[1] = static_cast<uint8_t*>(caches[l0 + i]->v);

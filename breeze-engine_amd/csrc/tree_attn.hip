@@ -816,8 +816,6 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
 
 // ------------------------------------------------------------------ host
 
-constexpr int64_t kMostBlocks = 1 << 23;  // of 256 threads: a grid has fewer than 2^32
-
 struct Plan {
     int rt, nslots, grid;
     size_t ml, shares, bytes;  // offsets of the maxima and of the shares, and the whole
@@ -934,8 +932,9 @@ bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, boo
                      c->kv_heads, T, B, heads, table_w);
         return false;
     }
-    // A launch has fewer than 2^24 workgroups: one for each 32 rows, and one a sequence and head.
-    if ((int64_t)T * heads > (1 << 26) || (int64_t)B * c->kv_heads > kMostBlocks / 4) {
+    // A launch has fewer than 2^24 workgroups.  The join's are the most: 16 a unit of 128 rows, of which a sequence
+    // and head may leave one unfilled (but has more than 32 rows on the mean); 4 a unit of 64 or 32.
+    if ((int64_t)T * heads > (1 << 24) || (int64_t)B * c->kv_heads > (1 << 20)) {
         bq_set_error("tree_attention: %d nodes of %d heads in %d sequences are too much for one call", T, heads, B);
         return false;
     }

@@ -212,6 +212,7 @@ def test_c_tree_attention():
     need = hb._lib.i4_tree_attention_workspace
     assert need(2, 16, 64, 4, 2, 4, 0, 4096, 1) > 0 and need(2, 16, 64, 4, 2, 3, 0, 4096, 1) == -2
     assert need(2, 16, 64, 0, 2, 4, 0, 4096, 1) == 0
+    assert need(2, 16, 64, (1 << 22) + 1, 2, 4, 0, 4096, 1) == -2 and need(2, 16, 64, 1 << 20, (1 << 19) + 1, 4, 0, 4096, 1) == -2
 
 
 def test_workspaces_have_a_bound():
@@ -252,7 +253,7 @@ def test_c_compact():
 
     for kw in (dict(caches=None), dict(layers=0), dict(layers=4097), dict(table=None), dict(kv=None), dict(path=None),
                dict(counts=None), dict(lens=None), dict(lens=4096), dict(cu=None), dict(T=-1), dict(B=-1), dict(cols=-1),
-               dict(cols=1 << 28)):
+               dict(cols=1 << 28), dict(B=(1 << 22) + 1)):
         assert call(**kw) == -2 and "kv_compact" in hb.last_error(), kw
     d = _c_cache(num_pages=3)
     assert call(caches=(ctypes.c_void_p * 2)(ctypes.addressof(c), ctypes.addressof(d))) == -2
