@@ -93,6 +93,14 @@ def test_trees(mods, page, kind, dtype, heads, H, D):
     _run(mods, 2, kind, dtype, heads, H, D, page, [13, 64, 1, 33, 20, 0, 90, 31], [100, 33, 64, 0, 500, 3, 191, 1])
 
 
+@pytest.mark.parametrize("heads,H,D", [(8, 1, 64), (12, 2, 128), (12, 2, 256)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("page,kind", [(16, "int8"), (64, "fp8")])
+def test_some_nodes(mods, page, kind, dtype, heads, H, D):
+    """33 to 64 rows a key head on the mean, some trees of fewer and some of several units."""
+    _run(mods, 8, kind, dtype, heads, H, D, page, [6, 13, 1, 0, 9, 17, 2, 4], [700, 3, 64, 5, 1999, 130, 63, 0])
+
+
 @pytest.mark.parametrize("chain,roots", [(True, 1), (False, 1), (False, 5)])
 @pytest.mark.parametrize("heads,H,D", HEADS)
 def test_large_trees(mods, heads, H, D, chain, roots):
@@ -274,3 +282,14 @@ def test_in_place_is_the_same(mods):
     for _ in range(4):
         own = q.clone()
         assert torch.equal(drafts.tree_attention(own, *args, out=own), want)
+
+
+@pytest.mark.parametrize("dtype,kind", [("bf16", "fp8"), ("fp32", "int8")])
+def test_many_sequences(mods, dtype, kind):
+    """More sequences than a wave looks through at once, some without nodes, some without keys before them."""
+    gen = torch.Generator().manual_seed(15)
+    lens = [int(n) for n in torch.randint(0, 6, (700,), generator=gen)]
+    ctx = [int(n) for n in torch.randint(0, 90, (700,), generator=gen)]
+    for b in (0, 255, 256, 400, 511, 512, 699):
+        lens[b], ctx[b] = [(0, 30), (3, 0), (0, 0), (2, 700), (5, 64), (1, 1), (0, 5)][b % 7]
+    _run(mods, 16, kind, dtype, 4, 2, 64, 16, lens, ctx)

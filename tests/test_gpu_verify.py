@@ -343,3 +343,14 @@ def test_graph_and_streams(drafts, draft):
             outs.append(call(held_in))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_many_sequences(drafts, draft):
+    """More sequences than a wave looks through at once, many of them without nodes."""
+    gen = torch.Generator().manual_seed(11)
+    sizes = [int(n) for n in torch.randint(-2, 5, (5000,), generator=gen).clamp_min(0)]
+    sizes[0] = sizes[63] = sizes[4096] = sizes[-1] = 0
+    trees = [tree(n, gen) for n in sizes]
+    logits, tokens, uniforms, q = _inputs(gen, trees, 100, "fp16", draft)
+    _check(drafts, logits, tokens, trees, uniforms, 0.9, q)
