@@ -314,6 +314,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     __shared__ Child children[kTreeNodes];
     __shared__ int parents[kTreeNodes], removed[kTreeNodes];
     __shared__ double removed_g[DRAFT ? 1 : kTreeNodes];  // what each had
+    __shared__ double full[DRAFT ? 1 : kPieces];          // the pieces' sums with them
     __shared__ double mass[kPieces], sums[W];             // G's sums of the node's pieces
     __shared__ uint32_t gone[W][kPiece / 32];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -427,15 +428,17 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
         const double x = weight_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[wave]);
         if (lane == 0) mass[piece] = x;
     };
-    // All pieces' masses at a node without a draft's part.  A removed token's share is taken
-    // off its piece's; where less than 2^-10 is left the difference has lost its last bits,
-    // and the piece is summed up anew.
+    // All pieces' masses at a node without a draft's part.  The removed tokens' shares are
+    // taken off their piece's; where they leave less than 2^-10 of all that it had, however
+    // many steps it took, the difference has lost its last bits, and the piece is summed up
+    // anew.
     const auto masses = [&] {
         const Piece* const own = a.pieces + (int64_t)(s.q0 + node) * a.np;
         sync();
         for (int i = tid; i < a.np; i += STEP) {
             const Piece p = own[i];
             mass[i] = p.top > -INFINITY ? p.sum * weight(p.top, r.top, scale) * r.one : 0.0;
+            if constexpr (!DRAFT) full[i] = mass[i];
         }
         sync();
         if constexpr (!DRAFT) {
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
                 const int piece = removed[i] / kPiece;
                 const double was = mass[piece], now = was - removed_g[i];
                 sync();
-                if (lane == 0 && was >= 0.0) mass[piece] = now < was * 0x1p-10 ? -1.0 : now;
+                if (lane == 0 && was >= 0.0) mass[piece] = now < full[piece] * 0x1p-10 ? -1.0 : now;
                 sync();
             }
             for (int i = 0; i < nremoved; ++i) {
