@@ -6,10 +6,12 @@
 // and S = 1 at first.  Child c is taken where
 //   u_c q(c) / Q < G(c) / S;
 // else G(c) becomes zero and, where the draft's probabilities q are given,
-//   A += S / Q,   G = max(p - A q, 0) but for the rejected,   Q -= q(c),   S = sum G.
+//   A += S / Q,   G = max(p - A q, 0),   S = sum G,   Q = sum q,   but for the rejected.
 // That is the rejection rule's residual max(R - q / Q, 0) / sum, sibling by sibling:
 // every step takes a multiple of the same q off, so p and one number A are all it
-// needs.  Without q a child is the draft's whole chance (q(c) / Q = 1) and only the
+// needs.  Q, 1 at first, is summed up along with G: 1 less the rejected tokens' q would be
+// what fp32 left of the row's sum, where the draft gave them nearly everything (1 - 10^-7 to
+// one token: 19% off).  Without q a child is the draft's whole chance (q(c) / Q = 1) and only the
 // rejected ones leave.  Where no child is taken, or there is none, the first token
 // whose running sum of G passes u_0 S is drawn.  Then every token is distributed as
 // the target's own.
@@ -53,8 +55,13 @@ struct Piece {
 
 // Where a walk stands before its first residual.
 struct Walk {
-    double A, Q, top, one;
+    double A, top, one;
     int node, m, child, going;
+};
+
+// G, and the draft's q, of the tokens that are left, summed up.
+struct Left {
+    double g, q;
 };
 
 struct VerArgs {
@@ -74,7 +81,7 @@ struct VerArgs {
     Piece* pieces;  // [T][np]
     f2* own;        // [T]: each node's own score, and the draft's probability, at its parent
     Walk* walks;    // [B], with a draft
-    double* rest;   // [B][np], with a draft
+    Left* rest;     // [B][np], with a draft
     int T, V, B, np;
 };
 
@@ -248,7 +255,8 @@ __device__ inline double share(const Row& r, float x, float q) {
 }
 
 // A lane's weights of a piece of node t's row without the tokens in `gone` (a bit each):
-// f(v, g) with those of scores (64 v + lane) * N on, for one v after another.
+// f(v, g, q) with those of scores (64 v + lane) * N on, for one v after another, and the
+// draft's q, where it has taken a part off the row.
 template <int DT, bool DRAFT, typename F>
 __device__ inline void weights_of(const VerArgs& a, const Row& r, int t, int piece, int lane, const uint32_t* gone, F f) {
     constexpr int N = vec<DT>(), E = kPiece / 64;
@@ -257,25 +265,31 @@ __device__ inline void weights_of(const VerArgs& a, const Row& r, int t, int pie
     if (DRAFT && r.A != 0.0) load_piece<kF32, N>(a.draft, t * a.draft_row, a.V, piece, lane, q);
 #pragma unroll
     for (int v = 0; v < E / N; ++v) {
-        double g[N];
+        double g[N], left[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int in = (64 * v + lane) * N + j, at = piece * kPiece + in;
             const bool is = at < a.V && !(gone[in >> 5] >> (in & 31) & 1);
             g[j] = is ? share<DRAFT>(r, x[N * v + j], DRAFT ? q[N * v + j] : 0.0f) : 0.0;
+            left[j] = is && DRAFT ? (double)q[N * v + j] : 0.0;
         }
-        f(v, g);
+        f(v, g, left);
     }
 }
-// Their sum over the piece.
+// Their sums over the piece.
 template <int DT, bool DRAFT>
-__device__ inline double weight_of(const VerArgs& a, const Row& r, int t, int piece, int lane, const uint32_t* gone) {
-    double sum = 0.0;
-    weights_of<DT, DRAFT>(a, r, t, piece, lane, gone, [&](int, const double* g) {
+__device__ inline Left left_of(const VerArgs& a, const Row& r, int t, int piece, int lane, const uint32_t* gone) {
+    Left sum = {0.0, 0.0};
+    weights_of<DT, DRAFT>(a, r, t, piece, lane, gone, [&](int, const double* g, const double* q) {
 #pragma unroll
-        for (int j = 0; j < vec<DT>(); ++j) sum += g[j];
+        for (int j = 0; j < vec<DT>(); ++j) {
+            sum.g += g[j];
+            if constexpr (DRAFT) sum.q += q[j];
+        }
     });
-    return sum_wave(sum);
+    sum.g = sum_wave(sum.g);
+    if constexpr (DRAFT) sum.q = sum_wave(sum.q);
+    return sum;
 }
 
 // The sequences whose walk stands before its first residual, all pieces.
@@ -292,7 +306,7 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerArgs a) {
     __syncthreads();
     if (piece >= a.np) return;
     const Row r = {w.top, kLog2e64 / (double)temperature(a, b), w.one, w.A};
-    const double sum = weight_of<DT, true>(a, r, s.q0 + w.node, piece, lane, gone[wave]);
+    const Left sum = left_of<DT, true>(a, r, s.q0 + w.node, piece, lane, gone[wave]);
     if (lane == 0) a.rest[(int64_t)b * a.np + piece] = sum;
 }
 
@@ -316,11 +330,12 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     __shared__ double removed_g[DRAFT ? 1 : kTreeNodes];  // what each had
     __shared__ double full[DRAFT ? 1 : kPieces];          // the pieces' sums with them
     __shared__ double mass[kPieces], sums[W];             // G's sums of the node's pieces
+    __shared__ double draft_left[RESUME ? kPieces : 1];   // and q's
     __shared__ uint32_t gone[W][kPiece / 32];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Seq s = sequence(a, b);
     const float temp = temperature(a, b);
-    Walk k = {0.0, 1.0, 0.0, 1.0, 0, 1, 0, 0};
+    Walk k = {0.0, 0.0, 1.0, 0, 1, 0, 0};
     if constexpr (RESUME) {
         k = a.walks[b];
         if (!k.going) return;
@@ -398,10 +413,11 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     Node at = {1.0, 0.0f, 0};
     bool fresh = true, bad = false;
 
-    const auto mass_sum = [&] {
+    // Over all pieces.
+    const auto sum_of = [&](const double* of) {
         double x = 0.0;
         sync();
-        for (int i = tid; i < a.np; i += STEP) x += mass[i];
+        for (int i = tid; i < a.np; i += STEP) x += of[i];
         x = sum_wave(x);
         if constexpr (RESUME) {
             __syncthreads();
@@ -425,8 +441,11 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     };
     const auto piece_mass = [&](int piece) {
         mark(piece);
-        const double x = weight_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[wave]);
-        if (lane == 0) mass[piece] = x;
+        const Left x = left_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[wave]);
+        if (lane == 0) {
+            mass[piece] = x.g;
+            if constexpr (RESUME) draft_left[piece] = x.q;
+        }
     };
     // All pieces' masses at a node without a draft's part.  The removed tokens' shares are
     // taken off their piece's; where they leave less than 2^-10 of all that it had, however
@@ -460,11 +479,15 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     if constexpr (RESUME) {
         cursor = k.child;
         r = {k.top, scale, k.one, k.A};
-        Q = k.Q;
-        for (int i = tid; i < a.np; i += STEP) mass[i] = a.rest[(int64_t)b * a.np + i];
+        for (int i = tid; i < a.np; i += STEP) {
+            const Left x = a.rest[(int64_t)b * a.np + i];
+            mass[i] = x.g;
+            draft_left[i] = x.q;
+        }
         if (tid == 0) removed[0] = children[k.child].token;
         nremoved = 1;
-        S = mass_sum();
+        S = sum_of(mass);
+        Q = sum_of(draft_left);
         fresh = false;
     }
     for (;;) {  // every wave alike
@@ -513,20 +536,20 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
                         S -= g;
                         if (S < base * 0x1p-10) {
                             masses();
-                            S = base = mass_sum();
+                            S = base = sum_of(mass);
                         }
                     } else {
                         r.A += S / Q;
-                        Q -= (double)c.q;
                         if constexpr (!RESUME) {
                             if (lane == 0) {
-                                a.walks[b] = Walk{r.A, Q, r.top, r.one, node, m, child, 1};
+                                a.walks[b] = Walk{r.A, r.top, r.one, node, m, child, 1};
                                 a.counts[b] = m;
                             }
                             return;
                         } else {
                             for (int i = wave; i < a.np; i += W) piece_mass(i);
-                            S = mass_sum();
+                            S = sum_of(mass);
+                            Q = sum_of(draft_left);
                         }
                     }
                 }
@@ -573,7 +596,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
     before = of_lane(before, who);
     mark(piece);
     int drawn = INT32_MAX, final = -1;  // and the last token that has any weight
-    weights_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[0], [&](int v, const double* g) {
+    weights_of<DT, DRAFT>(a, r, s.q0 + node, piece, lane, gone[0], [&](int v, const double* g, const double*) {
         double own = 0.0;
 #pragma unroll
         for (int j = 0; j < N; ++j) own += g[j];
@@ -631,7 +654,7 @@ Parts parts_of(int T, int V, int B, bool draft) {
     p.own = T * np * (int64_t)sizeof(Piece);
     p.walks = p.own + T * (int64_t)sizeof(f2);
     p.rest = p.walks + (draft ? B * (int64_t)sizeof(Walk) : 0);
-    p.end = p.rest + (draft ? B * np * 8 : 0);
+    p.end = p.rest + (draft ? B * np * (int64_t)sizeof(Left) : 0);
     return p;
 }
 
@@ -680,7 +703,7 @@ int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, con
     a.pieces = static_cast<Piece*>(dWork);
     a.own = reinterpret_cast<f2*>(static_cast<uint8_t*>(dWork) + at.own);
     a.walks = reinterpret_cast<Walk*>(static_cast<uint8_t*>(dWork) + at.walks);
-    a.rest = reinterpret_cast<double*>(static_cast<uint8_t*>(dWork) + at.rest);
+    a.rest = reinterpret_cast<Left*>(static_cast<uint8_t*>(dWork) + at.rest);
     a.T = T;
     a.V = V;
     a.B = B;

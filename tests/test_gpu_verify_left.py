@@ -66,3 +66,81 @@ def test_siblings_that_each_leave_a_little(drafts, k, gap):
         lo, hi = _drawn(r if m == 1 else whole, float(x[0]), k)
         assert lo <= want[-1] <= hi and lo <= new[b][m - 1] <= hi, (b, float(x[0]), want, new[b][:m])
         assert hi - lo <= 1  # no more than a border's two sides
+
+
+def _told(row, tokens, u, q):
+    """A root's children by the rule as it is told, in 64 bits: what a draft leaves is the sum
+    over the tokens that are left."""
+    r = torch.softmax(row[0].double(), 0)
+    q, left = q[0].double().clone(), 1.0
+    for i, x in enumerate(tokens):
+        if left != left:
+            return [-1], [0]
+        if not left > 0:
+            continue
+        if not 0 <= float(q[x]) < float("inf"):
+            return [-1], [0]
+        if float(u[1 + i]) * float(q[x]) / left < float(r[x]):
+            return [x], [0, 1 + i]
+        r = (r - q / left).clamp_min(0)
+        r[x] = q[x] = 0.0
+        r, left = r / r.sum(), float(q.sum())
+    total = torch.cumsum(r, 0)
+    return [int((total > float(u[0]) * total[-1]).nonzero()[0])], [0]
+
+
+def _confident(V, gen, rest):
+    """A draft that gives its first token all but `rest`, and a target that does not."""
+    q = torch.rand((1, V), generator=gen)
+    top = torch.randperm(V, generator=gen)[:4]
+    q[0, top] = 0.0
+    q *= 0.3 * rest / q.sum()
+    q[0, top[1:]] = rest * torch.tensor([0.4, 0.2, 0.1])
+    q[0, top[0]] = 1.0 - rest
+    row = torch.randn((1, V), generator=gen)
+    row[0, top] = torch.log(torch.exp(row).sum()) + torch.tensor([-1.0, -1.5, -2.0, -2.5])
+    return row, q, top.tolist()
+
+
+@pytest.mark.parametrize("V", [300, 5000, 32003])
+@pytest.mark.parametrize("rest", [1e-3, 1e-6, 1e-7, 2.0 ** -24])
+def test_confident_drafts(drafts, rest, V):
+    """The first child is rejected; the others, drawn from next to nothing, go by their share of it."""
+    gen = torch.Generator().manual_seed(V)
+    row, q, top = _confident(V, gen, rest)
+    r, left = torch.softmax(row[0].double(), 0), q[0].double()
+    r = (r - left).clamp_min(0)
+    left[top[0]] = r[top[0]] = 0.0
+    border = float(r[top[1]] / r.sum() / (left[top[1]] / left.sum()))
+    assert 0.1 < border < 0.9
+    u = torch.rand((64, 5), generator=gen)
+    u[:, 1] = LAST
+    u[:8, 2] = border * (1 - 1e-4)
+    u[8:16, 2] = border * (1 + 1e-4)
+    u[16:40, 2:] = LAST
+    want = [_told(row, top, x, q) for x in u]
+    taken = [len(nodes) > 1 for _, nodes in want]
+    assert all(taken[:8]) and not any(taken[16:40])
+    got = _root(drafts, row, top, u, q=q)
+    for b, (tokens, nodes) in enumerate(want):
+        m = len(nodes)
+        # The child's own row gives the token after it: not looked at here.
+        assert got[2][b] == [m] and got[1][b][:m] == nodes and got[0][b][0] == tokens[0], (b, u[b].tolist(), tokens, got[0][b])
+
+
+def test_tokens_of_a_confident_draft_are_distributed_as_the_target(drafts):
+    """40000 sequences, three children drawn from the draft without replacement: each token's
+    frequency lies within five deviations of its chance."""
+    gen = torch.Generator().manual_seed(3)
+    B, V = 40000, 12
+    q = torch.full((1, V), 1e-8)
+    q[0, 5], q[0, 2], q[0, 7] = 1.0 - 1e-7, 6e-8, 3e-8
+    row = 0.3 * torch.randn((1, V), generator=gen)
+    p = torch.softmax(row[0].double(), 0)
+    drawn = torch.multinomial(q.double().expand(B, V), 3, generator=gen)
+    tokens = torch.cat([torch.zeros((B, 1), dtype=torch.int64), drawn], 1).to(torch.int32).reshape(-1)
+    got = drafts.verify(row.cuda().expand(4 * B, V), tokens.cuda(),
+                        torch.tensor([-1, 0, 0, 0] * B, dtype=torch.int32).cuda(),
+                        torch.rand((4 * B,), generator=gen).cuda(), cu_of([4] * B).cuda(), 1.0, q.cuda().expand(4 * B, V))
+    freq = torch.bincount(got[0].cpu().view(B, 4)[:, 0].long(), minlength=V).double() / B
+    assert ((freq - p).abs() <= 5 * (p * (1 - p) / B).sqrt()).all(), (freq, p)
