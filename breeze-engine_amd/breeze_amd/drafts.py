@@ -110,10 +110,11 @@ def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=No
     tokens: the accepted ones and then the drawn one.  ``path`` and ``new_tokens``: int32
     ``[T]``, packed like the nodes, -1 after the path's end.  A token that no
     distribution gives is -1 (a row with a NaN, +inf or nothing finite, a temperature
-    below 0 or not finite, a draft's NaN); no node, or more than 1024, have the count
-    0.  A child whose token is not in the vocabulary, or an earlier sibling's, is passed
-    over, and so is one that ``draft`` has nothing left for.  Only rows of ``draft`` of
-    nodes with children are read."""
+    below 0 or not finite, a draft that gives a child that it comes to NaN, infinity or
+    less than 0, or NaN or infinity to any token after a rejected child); no node, or more
+    than 1024, have the count 0.  A child whose token is not in the vocabulary, or an
+    earlier sibling's, is passed over, and so is one that ``draft`` has nothing left for.
+    Only rows of ``draft`` of nodes with children are read."""
     torch = att._torch()
     T, V = logits.shape if logits.dim() == 2 else (0, 0)
     if not 1 <= V <= 1 << 21:

@@ -521,6 +521,9 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
             // so is one that the draft's probabilities have nothing left for.
             bool there = c.token >= 0 && c.token < a.V && Q > 0.0;
             for (int i = 0; i < nremoved && there; ++i) there = removed[i] != c.token;
+            // A draft that gave the child no probability: nothing says what chance it had.
+            bad = DRAFT && there && !(c.q >= 0.0f && c.q < INFINITY);
+            if (bad) break;
             if (there) {
                 const double g = share<DRAFT>(r, c.score, c.q);
                 take = (double)c.u * (DRAFT ? (double)c.q / Q : 1.0) * S < g;

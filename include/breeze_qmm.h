@@ -352,7 +352,8 @@ int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_to
  * dPath, dOut [T], packed like the nodes: the path's node numbers, and the new tokens,
  * as many: the accepted ones, then the drawn one.  The rest is -1, and so is a token
  * that no distribution gives (scores with a NaN, +infinity or nothing finite, a
- * temperature below 0, a draft's NaN).  Children whose token is outside the
+ * temperature below 0, a draft that gives a child that it comes to NaN, infinity or less
+ * than 0, or NaN or infinity to any token after a rejected child).  Children whose token is outside the
  * vocabulary, or an earlier sibling's, are passed over.  V up to 2^21; dWork: as many bytes as
  * i4_verify_workspace says, 16-byte aligned. */
 int64_t i4_verify_workspace(int T, int V, int B, int has_cu, int has_draft);

@@ -144,3 +144,28 @@ def test_tokens_of_a_confident_draft_are_distributed_as_the_target(drafts):
                         torch.rand((4 * B,), generator=gen).cuda(), cu_of([4] * B).cuda(), 1.0, q.cuda().expand(4 * B, V))
     freq = torch.bincount(got[0].cpu().view(B, 4)[:, 0].long(), minlength=V).double() / B
     assert ((freq - p).abs() <= 5 * (p * (1 - p) / B).sqrt()).all(), (freq, p)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -0.25])
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_a_child_whose_own_probability_is_none(drafts, at, bad):
+    """The sequence ends there with -1, whatever siblings follow; one that takes an earlier child
+    does not see it."""
+    gen = torch.Generator().manual_seed(at)
+    V = 3000
+    row, top = torch.randn((1, V), generator=gen), [7, 2900, 1500]
+    q = torch.softmax(row + torch.randn((1, V), generator=gen), -1)
+    q[0, top[:at]] = 0.2  # more than the target gives: rejected by the largest random number, taken by 0
+    q[0, top[at]] = bad
+    u = torch.full((2, 4), LAST)
+    u[:, 0] = 0.4
+    u[1, 1] = 0.0
+    for k in range(at + 1, 4):  # the child alone or the last, and with later siblings
+        got = _root(drafts, row, top[:k], u[:, :k + 1], q=q)
+        want = [_told(row, top[:k], x, q) for x in u]
+        assert want[0] == ([-1], [0])
+        assert got[2][0] == [1] and got[0][0] == [-1] * (k + 1) and got[1][0] == [0] + [-1] * k
+        if at:
+            assert got[2][1] == [2] and got[0][1][0] == top[0] and got[0][1][1] >= 0
+        else:
+            assert got[0][1] == [-1] * (k + 1)
