@@ -413,7 +413,8 @@ class PageTable:
         pages do not suffice, that sequence and every later one that needs pages get
         none; those, sequences past the table's columns or of a negative length, and
         trees past 1024 nodes, have a kv_len and slots of -1: no call writes or sees
-        anything of them.  Tokens outside every sequence have slot -1."""
+        anything of them, and ``drafts.verify`` and ``kv_compact`` take kv_lens and lens, so
+        that they get no token and keep their length and pages for a later step.  Tokens outside every sequence have slot -1."""
         torch = _torch()
         B = self._args[6]
         _ints(lens, (B,), "lens")

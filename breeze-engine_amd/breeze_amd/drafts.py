@@ -85,7 +85,7 @@ def _scores(t, T, V, what):
     return t if t.stride(1) == 1 or V == 1 else t.contiguous()
 
 
-def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=None):
+def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=None, kv_lens=None):
     """Drafted tokens checked against the target, and the next one drawn;
     ``(new_tokens, path, counts)``.
 
@@ -97,6 +97,9 @@ def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=No
     the largest score, the first of equal ones.  ``draft``: fp32 ``[T, V]``, at each
     node the probabilities that its children were drawn with, one after another without
     the earlier ones; None: children that the draft did not draw (its best ones, say).
+    ``kv_lens``: int32 ``[B]``, as ``tree_attention`` had them: a negative one's sequence
+    had no place in the cache (``PageTable.extend``), its scores mean nothing, and it gets
+    no token, the count 0.
 
     From node 0 on, with r = softmax(logits / temperature) of the node, its children
     go in order: child c is taken where ``uniforms[c] * q(c) < r(c)``, q being 1
@@ -133,6 +136,8 @@ def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=No
         att._ints(parents, (T,), "parents")
     elif cu is not None:
         raise ValueError("with cu, parents says how the nodes hang together")
+    if kv_lens is not None:
+        att._ints(kv_lens, (B,), "kv_lens")
     if uniforms.dtype is not torch.float32 or uniforms.shape != (T,) or (T > 1 and uniforms.stride(0) != 1):
         raise ValueError(f"uniforms must be contiguous float32 {(T,)}, got {uniforms.dtype} {tuple(uniforms.shape)}")
     temps = None
@@ -148,35 +153,39 @@ def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=No
             raise ValueError(f"draft must be float32, got {draft.dtype}")
         draft = _scores(draft, T, V, "draft")
     index = logits.get_device()
-    att._same_device(index, tokens, parents, uniforms, cu, temps, draft)
+    att._same_device(index, tokens, parents, uniforms, cu, temps, draft, kv_lens)
     if index != att._current():
         with torch.cuda.device(logits.device):
-            return verify(logits, tokens, parents, uniforms, cu, temperature if temps is None else temps, draft)
+            return verify(logits, tokens, parents, uniforms, cu, temperature if temps is None else temps, draft, kv_lens)
     if B == 0:
         none = torch.full((2 * T,), -1, dtype=torch.int32, device=logits.device)
         return none[:T], none[T:], none[:0]
     new = tokens.new_empty((2 * T + B,))
     work, n = att._workspace((T, V, B, cu is not None, draft is not None), "verify", logits.device)
     p = new.data_ptr()
-    rc = hb._lib.i4_verify_dev(
+    rc = hb._lib.i4_verify_lens_dev(
         logits.data_ptr(), logits.stride(0), T, V, dt, tokens.data_ptr(), None if parents is None else parents.data_ptr(),
-        uniforms.data_ptr(), None if cu is None else cu.data_ptr(), B, None if temps is None else temps.data_ptr(),
-        temperature, None if draft is None else draft.data_ptr(), 0 if draft is None else draft.stride(0), p, p + 4 * T,
+        uniforms.data_ptr(), None if cu is None else cu.data_ptr(), B, None if kv_lens is None else kv_lens.data_ptr(),
+        None if temps is None else temps.data_ptr(), temperature, None if draft is None else draft.data_ptr(), 0 if draft is None else draft.stride(0), p, p + 4 * T,
         p + 8 * T, None if work is None else work.data_ptr(), n, hb._torch_stream(logits))
     if rc:
-        hb._check_rc(rc, "i4_verify_dev")
+        hb._check_rc(rc, "i4_verify_lens_dev")
     return new.split((T, T, B))
 
 
-def kv_compact(caches, block_table, kv_lens, cu_q, path, counts):
+def kv_compact(caches, block_table, kv_lens, cu_q, path, counts, lens=None):
     """The accepted nodes' cache rows moved together; the new lengths, int32 ``[B]``.
 
     ``caches``: a ``KVCache``, or a list of them (the layers'; of one geometry, with one
     ``block_table``), changed in place.  ``kv_lens``, ``cu_q``: as ``tree_attention``
     had them; ``path``, ``counts``: as ``verify`` gave them.  The row of node ``path[i]``
     goes to the place of node i, for the first ``counts`` of each sequence, and a
-    sequence's length becomes the keys before its tree and those; a negative length
-    stays -1.  Rows past it keep what they hold."""
+    sequence's length becomes the keys before its tree and those.  Rows past it keep what
+    they hold.
+
+    ``lens``: int32 ``[B]``, the lengths before the step (``PageTable.extend``'s): where
+    kv_lens is negative nothing moves, and the sequence keeps that length, so that a
+    later step can go on with it.  Without them its length becomes -1."""
     torch = att._torch()
     caches = [caches] if isinstance(caches, att.KVCache) else list(caches)
     if not 1 <= len(caches) <= 4096:
@@ -199,16 +208,19 @@ def kv_compact(caches, block_table, kv_lens, cu_q, path, counts):
         att._ints(cu_q, (B + 1,), "cu_q")
     elif T != B:
         raise ValueError(f"{T} nodes in {B} sequences: cu_q says where each begins")
-    att._same_device(first._index, block_table, kv_lens, cu_q, path, counts)
+    if lens is not None:
+        att._ints(lens, (B,), "lens")
+    att._same_device(first._index, block_table, kv_lens, cu_q, path, counts, lens)
     if first._index != att._current():
         with torch.cuda.device(first.device):
-            return kv_compact(caches, block_table, kv_lens, cu_q, path, counts)
-    lens = kv_lens.new_empty((B,))
+            return kv_compact(caches, block_table, kv_lens, cu_q, path, counts, lens)
+    after = kv_lens.new_empty((B,))
     if B:
         pointers = array.array("Q", [c._p for c in caches])  # the C structs' addresses; a ctypes array takes longer to fill
-        rc = hb._lib.i4_kv_compact_dev(pointers.buffer_info()[0], len(caches), block_table.data_ptr(), block_table.stride(0), cols,
-                                       kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), T, B,
-                                       path.data_ptr(), counts.data_ptr(), lens.data_ptr(), hb._torch_stream(lens))
+        rc = hb._lib.i4_kv_compact_lens_dev(
+            pointers.buffer_info()[0], len(caches), block_table.data_ptr(), block_table.stride(0), cols, kv_lens.data_ptr(),
+            None if lens is None else lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), T, B, path.data_ptr(),
+            counts.data_ptr(), after.data_ptr(), hb._torch_stream(after))
         if rc:
-            hb._check_rc(rc, "i4_kv_compact_dev")
-    return lens
+            hb._check_rc(rc, "i4_kv_compact_lens_dev")
+    return after

@@ -128,8 +128,13 @@ try:
     _lib.i4_verify_dev.restype = _i
     _lib.i4_verify_dev.argtypes = [_vp, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, ctypes.c_float, _vp, _i64, _vp,
                                    _vp, _vp, _vp, _i64, _vp]
+    _lib.i4_verify_lens_dev.restype = _i
+    _lib.i4_verify_lens_dev.argtypes = [_vp, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, ctypes.c_float, _vp, _i64,
+                                        _vp, _vp, _vp, _vp, _i64, _vp]
     _lib.i4_kv_compact_dev.restype = _i
     _lib.i4_kv_compact_dev.argtypes = [_vp, _i, _vp, _i64, _i, _vp, _vp, _i, _i] + [_vp] * 4
+    _lib.i4_kv_compact_lens_dev.restype = _i
+    _lib.i4_kv_compact_lens_dev.argtypes = [_vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _i, _i] + [_vp] * 4
 except (OSError, AttributeError):
     _lib = None
 

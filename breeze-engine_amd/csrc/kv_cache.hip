@@ -188,6 +188,7 @@ struct CompactArgs {
     } layer[kLayers];
     const int32_t* table;
     const int32_t* kv_lens;
+    const int32_t* before;  // lengths before the step, or null
     const int32_t* cu;  // null: one node a sequence
     const int32_t* path;
     const int32_t* counts;
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(64) void kv_compact_kernel(CompactArgs a) {
     const int b = blockIdx.x, h = blockIdx.y, val = blockIdx.z & 1, lane = threadIdx.x % L;
     const int q0 = a.cu ? min(max(a.cu[b], 0), a.T) : b, n = a.cu ? min(max(a.cu[b + 1], q0), a.T) - q0 : 1;
     const int kv = a.kv_lens[b], ctx = kv - n, keep = min(max(a.counts[b], 0), n);
-    if (a.lens && h == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.lens[b] = kv < 0 ? -1 : ctx + keep;
+    if (a.lens && h == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.lens[b] = kv >= 0 ? ctx + keep : a.before ? a.before[b] : -1;
     if (kv < 0) return;
     uint8_t* const pages = a.layer[blockIdx.z >> 1].page[val];
     float* const scales = a.layer[blockIdx.z >> 1].scale[val];
@@ -331,9 +332,9 @@ int i4_kv_read_dev(const i4_kv_cache* cache, void* dK, void* dV, int T, int dtyp
     return kv_call(cache, a, T, dtype, false, stream, "kv_read");
 }
 
-int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_t* dTable, int64_t table_row,
-                      int table_w, const int32_t* dKvLens, const int32_t* dCu, int T, int B, const int32_t* dPath,
-                      const int32_t* dCounts, int32_t* dLens, void* stream) {
+int i4_kv_compact_lens_dev(const i4_kv_cache* const* caches, int layers, const int32_t* dTable, int64_t table_row,
+                           int table_w, const int32_t* dKvLens, const int32_t* dBefore, const int32_t* dCu, int T,
+                           int B, const int32_t* dPath, const int32_t* dCounts, int32_t* dLens, void* stream) {
     if (!caches || layers < 1 || layers > 4096 || T < 0 || B < 0 || B > (1 << 23)) {
         bq_set_error("kv_compact: needs 1 to 4096 caches, T >= 0 and 0 to 2^23 sequences (got %d, %d, %d)", layers, T, B);
         return -2;
@@ -384,6 +385,7 @@ int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_
     CompactArgs a{};
     a.table = dTable;
     a.kv_lens = dKvLens;
+    a.before = dBefore;
     a.cu = dCu;
     a.path = dPath;
     a.counts = dCounts;
@@ -412,6 +414,13 @@ int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_
         else kv_compact_kernel<256><<<grid, 64, 0, st>>>(a);
     }
     return launched("kv_compact") ? 0 : -5;
+}
+
+int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_t* dTable, int64_t table_row,
+                      int table_w, const int32_t* dKvLens, const int32_t* dCu, int T, int B, const int32_t* dPath,
+                      const int32_t* dCounts, int32_t* dLens, void* stream) {
+    return i4_kv_compact_lens_dev(caches, layers, dTable, table_row, table_w, dKvLens, nullptr, dCu, T, B, dPath,
+                                  dCounts, dLens, stream);
 }
 
 }  // extern "C"

@@ -73,6 +73,7 @@ struct VerArgs {
     const int32_t* parents;
     const float* uniforms;
     const int32_t* cu;  // null: one node a sequence
+    const int32_t* kv_lens;  // null: all sequences take part
     const float* temps; // null: `temp` for all
     float temp;
     int32_t* out;
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(kWalk) void verify_walk_kernel(VerArgs a) {
         const int from = b == 0 ? 0 : s.q0, to = b == a.B - 1 ? a.T : s.q0 + s.n;
         for (int i = from + tid; i < to; i += kWalk) a.out[i] = a.path[i] = -1;
         if (DRAFT && tid == 0) a.walks[b].going = 0;
-        if (s.n == 0 || s.n > kTreeNodes) {
+        if (s.n == 0 || s.n > kTreeNodes || (a.kv_lens && a.kv_lens[b] < 0)) {
             if (tid == 0) a.counts[b] = 0;
             return;
         }
@@ -670,10 +671,11 @@ int64_t i4_verify_workspace(int T, int V, int B, int has_cu, int has_draft) {
     return parts_of(T, V, B, has_draft != 0).end;
 }
 
-int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, const int32_t* dTokens,
-                  const int32_t* dParents, const float* dUniforms, const int32_t* dCu, int B, const float* dTemps,
-                  float temperature, const float* dDraft, int64_t draft_row, int32_t* dOut, int32_t* dPath,
-                  int32_t* dCounts, void* dWork, int64_t work_bytes, void* stream) {
+int i4_verify_lens_dev(const void* dLogits, int64_t row, int T, int V, int dtype, const int32_t* dTokens,
+                       const int32_t* dParents, const float* dUniforms, const int32_t* dCu, int B,
+                       const int32_t* dKvLens, const float* dTemps, float temperature, const float* dDraft,
+                       int64_t draft_row, int32_t* dOut, int32_t* dPath, int32_t* dCounts, void* dWork,
+                       int64_t work_bytes, void* stream) {
     if (!check(T, V, B, dCu != nullptr)) return -2;
     if (dtype < kF32 || dtype > kF16 || (!dTemps && !(temperature >= 0.0f && temperature < 1e30f))) {
         bq_set_error("verify: needs a type of 0 to 2 and a temperature of zero or more (got %d, %g)", dtype, temperature);
@@ -698,6 +700,7 @@ int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, con
     a.parents = dParents;
     a.uniforms = dUniforms;
     a.cu = dCu;
+    a.kv_lens = dKvLens;
     a.temps = dTemps;
     a.temp = temperature;
     a.out = dOut;
@@ -717,6 +720,14 @@ int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, con
     else if (dtype == kBF16) launch<kBF16>(a, st);
     else launch<kF16>(a, st);
     return launched("verify") ? 0 : -5;
+}
+
+int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, const int32_t* dTokens,
+                  const int32_t* dParents, const float* dUniforms, const int32_t* dCu, int B, const float* dTemps,
+                  float temperature, const float* dDraft, int64_t draft_row, int32_t* dOut, int32_t* dPath,
+                  int32_t* dCounts, void* dWork, int64_t work_bytes, void* stream) {
+    return i4_verify_lens_dev(dLogits, row, T, V, dtype, dTokens, dParents, dUniforms, dCu, B, nullptr, dTemps,
+                              temperature, dDraft, draft_row, dOut, dPath, dCounts, dWork, work_bytes, stream);
 }
 
 }  // extern "C"

@@ -361,15 +361,27 @@ int i4_verify_dev(const void* dLogits, int64_t row, int T, int V, int dtype, con
                   const int32_t* dParents, const float* dUniforms, const int32_t* dCu, int B, const float* dTemps,
                   float temperature, const float* dDraft, int64_t draft_row, int32_t* dOut, int32_t* dPath,
                   int32_t* dCounts, void* dWork, int64_t work_bytes, void* stream);
+/* The same, but a sequence that has no place in the cache gets no token: where dKvLens[b]
+ * (i4_pages_extend_dev's; NULL: nowhere) is negative, dCounts[b] is 0. */
+int i4_verify_lens_dev(const void* dLogits, int64_t row, int T, int V, int dtype, const int32_t* dTokens,
+                       const int32_t* dParents, const float* dUniforms, const int32_t* dCu, int B,
+                       const int32_t* dKvLens, const float* dTemps, float temperature, const float* dDraft,
+                       int64_t draft_row, int32_t* dOut, int32_t* dPath, int32_t* dCounts, void* dWork,
+                       int64_t work_bytes, void* stream);
 
 /* Cache rows of the nodes on a path moved together, in `layers` caches, none twice, of one
  * geometry: place ctx + dPath[dCu[b] + i] to ctx + i for i < dCounts[b], ctx =
  * dKvLens[b] - the sequence's nodes.  dLens[b] (apart from dKvLens) = ctx +
- * dCounts[b]; a negative dKvLens[b] stays.  A path's numbers grow, as
+ * dCounts[b], or -1 for a negative dKvLens[b].  A path's numbers grow, as
  * i4_verify_dev's do; entries that do not pass their own place move nothing. */
 int i4_kv_compact_dev(const i4_kv_cache* const* caches, int layers, const int32_t* dTable, int64_t table_row,
                       int table_w, const int32_t* dKvLens, const int32_t* dCu, int T, int B, const int32_t* dPath,
                       const int32_t* dCounts, int32_t* dLens, void* stream);
+/* The same, but a sequence with a negative dKvLens[b] keeps the length that it had before
+ * the step, dBefore[b] (NULL: -1). */
+int i4_kv_compact_lens_dev(const i4_kv_cache* const* caches, int layers, const int32_t* dTable, int64_t table_row,
+                           int table_w, const int32_t* dKvLens, const int32_t* dBefore, const int32_t* dCu, int T,
+                           int B, const int32_t* dPath, const int32_t* dCounts, int32_t* dLens, void* stream);
 
 #ifdef __cplusplus
 }
