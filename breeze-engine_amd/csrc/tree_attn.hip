@@ -818,8 +818,20 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
 
 struct Plan {
     int rt, nslots, grid;
+    int64_t join;              // workgroups of the join, 0: nothing is cut
     size_t ml, shares, bytes;  // offsets of the maxima and of the shares, and the whole
 };
+
+// The join's grid.  At one tile a sequence there is none.  12 nodes behind 4100 keys (4 units): 26.4 us, 29.6 by
+// the other; 10 nodes of 16 sequences (128): 34, 35.
+constexpr int kFewUnits = 32;
+template <int D, int RT>
+dim3 join_grid(int64_t units, int64_t capacity) {
+    constexpr unsigned items = RT * D / 256;  // quads of a wave's rows
+    static_assert(items % 8 == 0, "a workgroup of the join takes eight");
+    if (capacity <= Tiling<D, RT>::KT) return dim3(0, 0);
+    return dim3((unsigned)units, units <= kFewUnits ? items : items / 8);
+}
 
 // A share for each place on the units, fewer where the table has fewer tiles.
 template <int D, int RT>
@@ -828,6 +840,8 @@ Plan plan_rows(int T, int B, int H, int G, int dt, bool cu, int64_t capacity, in
     Plan p{};
     p.rt = RT;
     p.nslots = (int)(cu ? (int64_t)T * G / RT + B : (int64_t)B * ((G + RT - 1) / RT));
+    const dim3 join = join_grid<D, RT>((int64_t)p.nslots * H, capacity);
+    p.join = (int64_t)join.x * join.y;
     const int64_t tiles = (int64_t)p.nslots * H * std::max<int64_t>(1, (capacity + L::KT - 1) / L::KT);
     const int64_t room = (int64_t)n_cu * (dt == kF32 ? per_unit<D, RT, kF32>() : per_unit<D, RT, kBF16>());
     p.grid = (int)((std::min(room, (tiles + kLeastTiles - 1) / kLeastTiles) + 7) / 8 * 8);
@@ -874,14 +888,10 @@ template <int D, int KIND, int DT, int RT>
 void launch4(const TreeArgs& a, hipStream_t st) {
     typedef Tiling<D, RT> L;
     tree_keys_kernel<D, KIND, DT, RT><<<(unsigned)a.grid, 64 * L::W, 0, st>>>(a);
-    // At one tile a sequence nothing is cut.
-    if (((int64_t)a.table_w << a.pshift) <= L::KT) return;
-    constexpr unsigned items = RT * D / 256;  // quads of a wave's rows
-    static_assert(items % 8 == 0, "a workgroup of the join takes eight");
-    const unsigned units = (unsigned)a.nslots * a.H;
-    // 12 nodes behind 4100 keys (4 units): 26.4 us, 29.6 by the other; 10 nodes of 16 sequences (128): 34, 35.
-    if (units <= 32) tree_join_kernel<D, DT, RT, true><<<dim3(units, items), 256, 0, st>>>(a);
-    else tree_join_kernel<D, DT, RT, false><<<dim3(units, items / 8), 256, 0, st>>>(a);
+    const dim3 join = join_grid<D, RT>((int64_t)a.nslots * a.H, (int64_t)a.table_w << a.pshift);
+    if (join.x == 0) return;
+    if (join.x <= kFewUnits) tree_join_kernel<D, DT, RT, true><<<join, 256, 0, st>>>(a);
+    else tree_join_kernel<D, DT, RT, false><<<join, 256, 0, st>>>(a);
 }
 
 template <int D, int KIND, int DT>
@@ -932,14 +942,21 @@ bool check_shape(const i4_kv_cache* c, int T, int B, int heads, int table_w, boo
                      c->kv_heads, T, B, heads, table_w);
         return false;
     }
-    // A launch has fewer than 2^24 workgroups.  The join's are the most: 16 a unit of 128 rows, of which a sequence
-    // and head may leave one unfilled (but has more than 32 rows on the mean); 4 a unit of 64 or 32.
+    // Rows and units are counted in 32 bits.
     if ((int64_t)T * heads > (1 << 24) || (int64_t)B * c->kv_heads > (1 << 20)) {
         bq_set_error("tree_attention: %d nodes of %d heads in %d sequences are too much for one call", T, heads, B);
         return false;
     }
     *pshift = s;
     return true;
+}
+
+// A launch has fewer than 2^24 workgroups.  The join's are the most, up to 16 a unit.
+bool check_launch(const Plan& p, int T, int B, int heads) {
+    if (p.join < (1 << 24)) return true;
+    bq_set_error("tree_attention: %d nodes of %d heads in %d sequences are too much for one call (%lld workgroups)", T, heads,
+                 B, (long long)p.join);
+    return false;
 }
 
 }  // namespace
@@ -956,7 +973,8 @@ int64_t i4_tree_attention_workspace(int kv_heads, int page_size, int head_dim, i
     int ps = 0;
     if (!check_shape(&c, T, B, heads, table_w, has_cu != 0, &ps)) return -2;
     if (T == 0 || B == 0) return 0;
-    return (int64_t)plan_of(T, B, heads, kv_heads, head_dim, dtype, has_cu != 0, (int64_t)table_w << ps, cu_count()).bytes;
+    const Plan p = plan_of(T, B, heads, kv_heads, head_dim, dtype, has_cu != 0, (int64_t)table_w << ps, cu_count());
+    return check_launch(p, T, B, heads) ? (int64_t)p.bytes : -2;
 }
 
 int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_token, int64_t q_head, int T, int heads,
@@ -1001,6 +1019,7 @@ int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_to
     a.pshift = ps;
     a.scale = scale * kLog2e;
     const Plan p = plan_of(T, B, heads, a.H, cache->head_dim, dtype, dCu != nullptr, (int64_t)table_w << ps, cu_count());
+    if (!check_launch(p, T, B, heads)) return -2;
     if (p.bytes > 0 && (!dWork || work_bytes < (int64_t)p.bytes)) {
         bq_set_error("tree_attention: needs a workspace of %zu bytes, got %lld", p.bytes, (long long)work_bytes);
         return -4;
