@@ -289,18 +289,32 @@ def _turned(out, like, what):
     return out
 
 
+def _same_rows(a, b):
+    """a and b, of one shape and type, are the same rows at the same places."""
+    return a.data_ptr() == b.data_ptr() and all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
+
+
 def _disjoint(a, b):
-    """No row of a lies on one of b: they are apart, or other columns of one projection."""
+    """No row of a lies on one of b: they are apart, or other columns of one projection, of
+    its tokens or of its heads."""
     x, y = _span(a), _span(b)
     if x[0] >= y[1] or y[0] >= x[1]:
         return True
-    step = a.stride(0) * a.element_size()
-    if a.stride(0) != b.stride(0) or a.dtype is not b.dtype or step == 0:
+    if a.dtype is not b.dtype:
         return False
-    # Columns of each token, from the first one's start on, modulo the step.
-    wide = [((t.shape[1] - 1) * t.stride(1) + t.shape[2]) * t.element_size() for t in (a, b)]
-    apart = (y[0] - x[0]) % step
-    return wide[0] <= apart and apart + wide[1] <= step
+    size = a.element_size()
+    for t, d in ((a, 0), (b, 0), (a, 1), (b, 1)):
+        step = t.stride(d) * size
+        if t.shape[d] < 2 or step == 0:
+            continue
+        # The bytes of each, from the first row's on, modulo the step: a dimension that goes on by
+        # whole steps adds none.
+        wide = [sum((t.shape[i] - 1) * t.stride(i) * size for i in (0, 1) if t.stride(i) * size % step) + t.shape[2] * size
+                for t in (a, b)]
+        apart = (y[0] - x[0]) % step
+        if wide[0] <= apart and apart + wide[1] <= step:
+            return True
+    return False
 
 
 def rotary(rope, q, k, positions, out=None):
@@ -337,7 +351,7 @@ def rotary(rope, q, k, positions, out=None):
             for o, own, other, there in ((qo, q, k, ko), (ko, k, q, qo)):
                 if o is None:
                     continue
-                if not (o.data_ptr() == own.data_ptr() and o.stride() == own.stride()) and not _disjoint(o, own):
+                if not _same_rows(o, own) and not _disjoint(o, own):
                     raise ValueError("out overlaps its input: it may be the input itself, or apart from it")
                 if other is not None and not (_disjoint(o, other) and _disjoint(o, there)):
                     raise ValueError("out's q and k lie on one another, or on the other's input")
