@@ -229,8 +229,10 @@ class Rotary:
       those in between are mixed linearly in the turns; sine and cosine are
       multiplied by 0.1 ln(factor) + 1 (or ``amplitude``).
 
-    ``freqs``: f_i themselves (dim / 2 numbers), in place of all that.  They are kept
-    in 64 bits on ``device``, as quarter turns."""
+    ``freqs``: f_i themselves (dim / 2 numbers), in place of all that, for other
+    scalings: one that goes from kept to divided along the pairs' numbers i, say,
+    where "parts" goes by their turns.  They are kept in 64 bits on ``device``, as
+    quarter turns."""
 
     def __init__(self, dim, base=10000.0, layout="half", scaling=None, factor=1.0, original=None, slow=1.0, fast=32.0,
                  amplitude=None, freqs=None, device="cuda"):
@@ -326,7 +328,8 @@ def rotary(rope, q, k, positions, out=None):
     from 64 bits, at whatever position; the others are copied.
 
     Views are read in place.  ``out``: (q, k) to write to, each the input itself
-    (only what is turned is written then) or apart from both inputs."""
+    or apart from both inputs (other columns of one projection, or of its heads, are).
+    Where all are the inputs themselves only what is turned is written."""
     torch = _torch()
     T, _, D = q.shape if q.dim() == 3 else (0, 0, 0)
     dt = _type(q, "q")

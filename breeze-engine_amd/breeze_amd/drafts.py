@@ -95,11 +95,11 @@ def verify(logits, tokens, parents, uniforms, cu=None, temperature=1.0, draft=No
     1]``, where each sequence's nodes begin and the last one's end; None: one node a
     sequence, whose token is drawn.  ``temperature``: a number, or fp32 ``[B]``; 0 takes
     the largest score, the first of equal ones.  ``draft``: fp32 ``[T, V]``, at each
-    node the probabilities that its children were drawn with, one after another without
-    the earlier ones; None: children that the draft did not draw (its best ones, say).
-    ``kv_lens``: int32 ``[B]``, as ``tree_attention`` had them: a negative one's sequence
-    had no place in the cache (``PageTable.extend``), its scores mean nothing, and it gets
-    no token, the count 0.
+    node the probabilities (a row sums to 1) that its children were drawn with, one after
+    another without the earlier ones; None: children that the draft did not draw (its
+    best ones, say).  ``kv_lens``: int32 ``[B]``, as ``tree_attention`` had them: a negative
+    one's sequence had no place in the cache (``PageTable.extend``), its scores mean
+    nothing, and it gets no token, the count 0.
 
     From node 0 on, with r = softmax(logits / temperature) of the node, its children
     go in order: child c is taken where ``uniforms[c] * q(c) < r(c)``, q being 1

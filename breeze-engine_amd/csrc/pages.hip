@@ -1,6 +1,6 @@
 // A batch's page table on the GPU: pages of a free stack given to sequences that
 // grow, and taken back from those that shrink; new tokens' slots, positions and
-// lengths; and cache rows of accepted tokens moved together.
+// lengths.
 //
 // extend: sequence b has n_b new tokens behind len_b and needs
 //   need_b = max(ceil((len_b + n_b) / page) - held_b, 0)

@@ -62,7 +62,7 @@ struct TreeArgs {
     f2* ml;             // [2 shares][rows a unit]: maximum and sum
     i2* shares;         // [slots][H]: a unit's first and last share
     int64_t table_row;
-    int T, B, Hq, H, G, P, pshift, table_w, nslots, grid;  // grid: shares
+    int T, B, H, G, P, pshift, table_w, nslots, grid;  // grid: shares
     float scale;  // softmax scale * log2(e)
 };
 
@@ -200,8 +200,8 @@ struct RawQueries {
 // How a workgroup of W waves takes a unit of RT rows: R rows a wave, W / (RT / R) waves
 // along the KT keys of a tile.
 //
-// Rows of 16: a wave's sums and queries are half as large, and three workgroups share
-// a compute unit, whose loads hide one another's waits.  Rows of 32 read a key from LDS half as
+// Rows of 16: a wave's sums and queries are half as large, and up to three workgroups share
+// a compute unit (per_unit), whose loads hide one another's waits.  Rows of 32 read a key from LDS half as
 // often; they are for 128 rows of 64 and 128 values (32 nodes of 16 sequences, bf16: 51 us; 57 with
 // 16 rows a wave, 70 with eight waves of 32).  Units of 64 rows were so once (10 nodes of
 // 64 sequences, bf16: 207 us, 162 now).  With heads of 256 a wave's sums of 32 rows would
@@ -214,7 +214,8 @@ struct Tiling {
     static constexpr int KS = D + 8, VS = D + (R == 32 ? 32 : 16);  // LDS rows of a key and of its values: reads of one instruction fall on unlike banks
     static_assert(KW >= 32, "a wave takes blocks of 32 keys");
 };
-// Workgroups a compute unit.  Heads of 128, 64 rows: fp32 spills 28 registers a lane at three
+// Workgroups a compute unit: three where the registers hold them, two of 128 rows or of fp32's
+// 64, with heads of 256 two of 32 rows and one of 128.  Heads of 128, 64 rows: fp32 spills 28 registers a lane at three
 // (10 nodes of 64 sequences 226 us, 198 at two), bf16 7 (162, 181).  32 rows: fp32 11
 // (8 nodes of 64 sequences 175, 191 at two), bf16 2 (151, 173).
 template <int D, int RT, int DT>
@@ -1012,7 +1013,6 @@ int i4_tree_attention_dev(const i4_kv_cache* cache, const void* dQ, int64_t q_to
     a.parents = dParents;
     a.T = T;
     a.B = B;
-    a.Hq = heads;
     a.H = cache->kv_heads;
     a.G = heads / cache->kv_heads;
     a.P = cache->num_pages;
