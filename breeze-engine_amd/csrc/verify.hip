@@ -29,8 +29,8 @@
 // spread over all units (verify_rest_kernel), between the two halves of the walk; any
 // further one of a tree is its workgroup's alone.
 //
-// 640 nodes over 151936 tokens, fp32: rows 87 to 94 us (389 MB, 4.1 to 4.5 TB/s; a sum of a
-// GiB reads 4.0), walk of 16 sequences of 40 nodes 18; 12 nodes: 5.7 and 12.  A walk is latency:
+// 640 nodes over 151936 tokens, fp32: rows 87 to 97 us (389 MB, 4.0 to 4.5 TB/s; a sum of a
+// GiB reads 4.0), bf16 92; walk of 16 sequences of 40 nodes 18; 12 nodes: 5.7 and 12.  A walk is latency:
 // five dependent reads of memory, a fp64 exponential and sum over a node's pieces, a few
 // LDS reads a child.  24 sequences of 3 to 9 nodes over 32003 tokens with a draft, bf16: rows 9,
 // walk 12, residual 9, walk 12, each a launch.  16 trees of 32 nodes, four children a node, over
